@@ -40,6 +40,8 @@ enum {
     MYNAH_B200_GGML_Q4_K = 112,
     MYNAH_B200_GGML_Q6_K = 114
 };
+/* formats of the rows of a paged cache beside MYNAH_B200_F32 (100 + ggml type id; no weights) */
+enum { MYNAH_B200_F16 = 101, MYNAH_B200_BF16 = 130 };
 
 /* qmat_mul flags */
 enum {
@@ -309,6 +311,76 @@ int mynah_b200_stream_step_decode(mynah_b200_stream_group *g, const float *mel, 
 /* the same with device buffers on both sides (asynchronous on the model's stream) */
 int mynah_b200_stream_step_device(mynah_b200_stream_group *g, const float *mel_dev, int n_mel, int is_last,
                                   float *out_dev);
+
+/* ---- paged key/value cache of a decoder layer ------------------------------------- */
+/* No counterpart in the reference, whose attention decoder keeps one run of keys per utterance inside the call
+ * (src/decoder_aed.c). For a host that runs the layers of a text decoder itself on resident linears
+ * (mynah_b200_qmat_mul_device): the keys and values of many sequences in pages of one pool, their rows put there with
+ * the norm of every head and the rotation by the position on the way, and attention over them. One handle is one
+ * layer; the tables may be shared by all layers.
+ *
+ * Types: fmt is that of the rows (queries, keys, values, results): F32, F16 or BF16. The cache holds 16 bits a value:
+ * bf16 for BF16 rows, else f16. Queries, probabilities and results of F16 / BF16 rows pass through 16 bits, too; for
+ * F32 rows they keep f32 accuracy (relative to the stored keys and values).
+ * Layout: the pools are [n_pages][n_kv_heads][page_size][head_dim]; head h of a row is its values
+ * [h head_dim, (h + 1) head_dim); query head h looks at kv head h / (n_heads / n_kv_heads). */
+typedef struct {
+    int n_heads, n_kv_heads, head_dim;   /* n_heads a multiple (1 to 64 times) of n_kv_heads; head_dim a multiple of 16 up to 128 */
+    int page_size, n_pages;              /* slots per page: a power of two from 8 to 256 */
+    int fmt;                             /* MYNAH_B200_F32, _F16 or _BF16 */
+    int rotary_dim;                      /* the first rotary_dim values of a q or k head turn (a multiple of 8, 0: none) */
+    int rotary_interleaved;              /* pairs are (2i, 2i + 1) instead of (i, i + rotary_dim / 2) */
+    double rope_theta;                   /* pair i turns by theta^(-2i / rotary_dim) per position, */
+    const double *inv_freq;              /* or by inv_freq[i] where given [rotary_dim / 2] */
+    const float *q_norm, *k_norm;        /* [head_dim] weights of a root-mean-square norm of every q / k head; NULL: none */
+    float norm_eps;
+    int window, n_sinks;                 /* window > 0: a row at position p sees the keys j with p - window < j <= p, and j < n_sinks */
+    float scale;                         /* of the scores; 0: 1 / sqrt(head_dim) */
+} mynah_b200_kv_config;
+void mynah_b200_kv_config_default(mynah_b200_kv_config *cfg);     /* zeros, pages of 16, theta 10000, eps 1e-6 */
+
+/* Allocates the pools (zeroed) on the current device; the arrays that cfg names are copied. NULL on error. */
+typedef struct mynah_b200_kv mynah_b200_kv;
+mynah_b200_kv *mynah_b200_kv_create(const mynah_b200_kv_config *cfg);
+/* waits for the handle's work; graphs that hold its calls must not be launched afterwards */
+void mynah_b200_kv_free(mynah_b200_kv *h);
+/* The pools' device addresses, for copying pages out and in. Values written into them this way have to be finite. */
+int mynah_b200_kv_pages(const mynah_b200_kv *h, void **k, void **v);
+
+/* Where the rows of a call belong. The tables are DEVICE memory and are read when the work runs, so a captured graph may
+ * be launched again with other contents. Sequence s has kv_len[s] keys, those of this call included; its rows
+ * [row_off[s], row_off[s + 1]) stand at its last positions. row_off NULL: one row per sequence (row s, at position
+ * kv_len[s] - 1). Position p lies in slot p % page_size of page page_table[s][p / page_size]; entries that no visible key
+ * and no new row needs may hold anything. kv_len[s] = 0 (one row per sequence) is an empty place: nothing is stored, its
+ * result is 0. Rows behind the last sequence are left as they are. */
+typedef struct {
+    int n_seq, n_rows;                   /* n_rows: rows that the buffers hold */
+    const int *row_off;                  /* [n_seq + 1], not decreasing, or NULL */
+    const int *kv_len;                   /* [n_seq] */
+    const int *page_table;               /* [n_seq][max_pages] */
+    int max_pages;
+} mynah_b200_kv_batch;
+
+/* Both calls below: rows of n_heads (n_kv_heads) x head_dim values on the handle's device, ld* the stride from row to row
+ * in values; addresses and strides are multiples of 16 bytes. ASYNCHRONOUS on `stream`, a cudaStream_t of the handle's
+ * device (cudaStreamLegacy for the legacy default stream), or on the handle's own non-blocking stream where NULL. They
+ * allocate nothing, use no workspace and can be captured; calls of one handle may overlap on the GPU as long as none
+ * writes a slot that another reads or writes. 0, or -1 with mynah_b200_last_error and nothing launched. What only the
+ * tables show (a page or length out of range: skipped, or read as page 0) and values that do not fit 16 bits (stored as
+ * 0) are reported by mynah_b200_kv_sync.
+ *
+ * append: norm and rotation of q into q_out (which may be q itself with the same stride), of k into the cache, v into the
+ * cache as it is. Rows whose position is below 0 (more rows than keys) are skipped. A slot that two rows of a call name
+ * ends up with a mix of the two. */
+int mynah_b200_kv_append(mynah_b200_kv *h, const mynah_b200_kv_batch *b, const void *q, long long ldq, const void *k, long long ldk,
+                         const void *v, long long ldv, void *q_out, long long ldqo, void *stream);
+/* attend: out = softmax over the visible keys of scale q . k, times their values; 0 for a row that sees none. q as
+ * append left it in q_out. */
+int mynah_b200_kv_attend(mynah_b200_kv *h, const mynah_b200_kv_batch *b, const void *q, long long ldq, void *out, long long ldo,
+                         void *stream);
+/* waits for `stream` (NULL: the handle's own) and reports, once, what the handle's calls have found since the last sync:
+ * 0, or -1. Not to be called while the stream is being captured. */
+int mynah_b200_kv_sync(mynah_b200_kv *h, void *stream);
 
 /* ---- whole path, resident ------------------------------------------------------- */
 /* audio in, token ids out: log-mel -> encoder (packed batch) -> greedy decoder, with only the

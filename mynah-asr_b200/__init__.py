@@ -22,6 +22,7 @@ LIB_PATH = os.path.join(_HERE, "libmynah_b200.so")
 
 F32, MYNAH_Q8, MYNAH_Q4 = 0, 1, 2
 GGML_Q4_0, GGML_Q8_0, GGML_Q4_K, GGML_Q6_K = 102, 108, 112, 114
+F16, BF16 = 101, 130                                     # rows of a KvCache beside F32
 A16, A8, FAST, SCALAR, MMA_SYNC, FEW_ROWS = 0, 1, 2, 4, 8, 16
 
 c_fp = C.POINTER(C.c_float)
@@ -42,6 +43,18 @@ class VadConfig(C.Structure):
                 ("enc_channels", C.c_int * 8), ("enc_kernels", C.c_int * 8), ("enc_strides", C.c_int * 8),
                 ("enc_pads", C.c_int * 16), ("threshold", C.c_double), ("neg_threshold", C.c_double),
                 ("min_speech_ms", C.c_int), ("min_silence_ms", C.c_int), ("speech_pad_ms", C.c_int)]
+
+
+class KvConfig(C.Structure):
+    _fields_ = [("n_heads", C.c_int), ("n_kv_heads", C.c_int), ("head_dim", C.c_int), ("page_size", C.c_int), ("n_pages", C.c_int),
+                ("fmt", C.c_int), ("rotary_dim", C.c_int), ("rotary_interleaved", C.c_int), ("rope_theta", C.c_double),
+                ("inv_freq", C.POINTER(C.c_double)), ("q_norm", c_fp), ("k_norm", c_fp), ("norm_eps", C.c_float), ("window", C.c_int),
+                ("n_sinks", C.c_int), ("scale", C.c_float)]
+
+
+class KvBatchStruct(C.Structure):
+    _fields_ = [("n_seq", C.c_int), ("n_rows", C.c_int), ("row_off", C.c_void_p), ("kv_len", C.c_void_p), ("page_table", C.c_void_p),
+                ("max_pages", C.c_int)]
 
 
 class BackendError(RuntimeError):
@@ -196,6 +209,17 @@ def lib():
     L.mynah_b200_vad_probs.argtypes = [vp, c_fp, C.c_size_t, c_fp, ci]
     L.mynah_b200_vad_speech_spans.argtypes = [vp, c_fp, C.c_size_t, C.POINTER(C.c_longlong), ci]
     L.mynah_b200_plan_segments.argtypes = [vp, c_fp, C.c_size_t, ci, C.c_double, C.POINTER(C.c_longlong), ci]
+    cl = C.c_longlong
+    L.mynah_b200_kv_config_default.argtypes = [C.POINTER(KvConfig)]
+    L.mynah_b200_kv_config_default.restype = None
+    L.mynah_b200_kv_create.restype = vp
+    L.mynah_b200_kv_create.argtypes = [C.POINTER(KvConfig)]
+    L.mynah_b200_kv_free.argtypes = [vp]
+    L.mynah_b200_kv_free.restype = None
+    L.mynah_b200_kv_pages.argtypes = [vp, C.POINTER(vp), C.POINTER(vp)]
+    L.mynah_b200_kv_append.argtypes = [vp, vp, vp, cl, vp, cl, vp, cl, vp, cl, vp]
+    L.mynah_b200_kv_attend.argtypes = [vp, vp, vp, cl, vp, cl, vp]
+    L.mynah_b200_kv_sync.argtypes = [vp, vp]
     L.mynah_b200_batch_upload.restype = vp
     L.mynah_b200_batch_upload.argtypes = [vp, C.POINTER(c_fp), C.POINTER(C.c_size_t), ci]
     L.mynah_b200_batch_run.argtypes = [vp, vp, ci]
@@ -370,6 +394,109 @@ def plan_segments(samples, sample_rate, seg_sec, vad=None):
     if k < 0:
         raise BackendError("plan_segments: " + _err())
     return [(int(buf[2 * i]), int(buf[2 * i + 1])) for i in range(k)]
+
+
+class _Pool:
+    """One of a cache's pools as device memory that other array libraries can wrap; the cache lives as long as it does."""
+
+    def __init__(self, cache, ptr, shape, typestr):
+        self._cache = cache
+        self.__cuda_array_interface__ = {"shape": shape, "typestr": typestr, "data": (ptr, False), "version": 3}
+
+
+class KvBatch:
+    """Where the rows of a call belong (mynah_b200_kv_batch): device tables that a captured graph reads anew at each launch."""
+
+    def __init__(self, kv_len, page_table, row_off, n_rows):
+        for t in (kv_len, page_table) + (() if row_off is None else (row_off,)):
+            if str(t.dtype) != "torch.int32" or not t.is_contiguous() or not t.is_cuda:
+                raise ValueError("the tables of a batch are contiguous int32 tensors on the GPU")
+        n_seq = kv_len.shape[0]
+        if kv_len.dim() != 1 or page_table.dim() != 2 or page_table.shape[0] != n_seq or (row_off is not None and tuple(row_off.shape) != (n_seq + 1,)):
+            raise ValueError("a batch has kv_len [n_seq], page_table [n_seq, max_pages] and row_off [n_seq + 1] or None")
+        if row_off is not None and n_rows is None:
+            raise ValueError("n_rows has to be given where row_off is")
+        self.n_rows = n_seq if n_rows is None else int(n_rows)
+        self._keep = (kv_len, page_table, row_off)
+        self.device = kv_len.device
+        if page_table.device != self.device or (row_off is not None and row_off.device != self.device):
+            raise ValueError("the tables of a batch are on one device")
+        self._c = KvBatchStruct(n_seq, self.n_rows, None if row_off is None else row_off.data_ptr(), kv_len.data_ptr(),
+                                page_table.data_ptr(), page_table.shape[1])
+        self.at = C.addressof(self._c)
+
+
+class KvCache:
+    """Paged key/value cache of one decoder layer on the current device (mynah_b200_kv). Tensors are anything with torch's
+    data_ptr, shape, stride, dtype and device; row tensors are [rows, heads * head_dim], a row's values side by side."""
+
+    def __init__(self, n_heads, n_kv_heads, head_dim, page_size, n_pages, fmt=F32, rotary_dim=0, interleaved=False, rope_theta=10000.0,
+                 inv_freq=None, q_norm=None, k_norm=None, norm_eps=1e-6, window=0, n_sinks=0, scale=0.0):
+        self.h = None
+        c = KvConfig(n_heads, n_kv_heads, head_dim, page_size, n_pages, fmt, rotary_dim, int(interleaved), rope_theta, None, None, None,
+                     norm_eps, window, n_sinks, scale)
+        keep = []
+        for name, given, kind, n in (("inv_freq", inv_freq, np.float64, rotary_dim // 2), ("q_norm", q_norm, np.float32, head_dim),
+                                     ("k_norm", k_norm, np.float32, head_dim)):
+            if given is None:
+                continue
+            a = np.ascontiguousarray(given, kind)
+            if a.shape != (n,):
+                raise ValueError(f"{name} has {n} values")
+            keep.append(a)
+            setattr(c, name, a.ctypes.data_as(C.POINTER(C.c_double) if kind is np.float64 else c_fp))
+        self.h = lib().mynah_b200_kv_create(C.byref(c))
+        if not self.h:
+            raise BackendError("kv_create: " + _err())
+        self.n_heads, self.n_kv_heads, self.head_dim, self.page_size, self.n_pages, self.fmt = n_heads, n_kv_heads, head_dim, page_size, n_pages, fmt
+        self._dtype = {F32: "torch.float32", F16: "torch.float16", BF16: "torch.bfloat16"}[fmt]
+        self._q_width, self._kv_width = n_heads * head_dim, n_kv_heads * head_dim
+        self._append, self._attend = lib().mynah_b200_kv_append, lib().mynah_b200_kv_attend
+
+    def close(self):
+        if getattr(self, "h", None):
+            lib().mynah_b200_kv_free(self.h)
+            self.h = None
+
+    __del__ = close
+
+    def pages(self):
+        """(keys, values): the pools [n_pages, n_kv_heads, page_size, head_dim] by __cuda_array_interface__; bf16 as int16 to be viewed."""
+        k, v = C.c_void_p(), C.c_void_p()
+        _check(lib().mynah_b200_kv_pages(self.h, C.byref(k), C.byref(v)), "kv_pages")
+        shape = (self.n_pages, self.n_kv_heads, self.page_size, self.head_dim)
+        return tuple(_Pool(self, p.value, shape, "<i2" if self.fmt == BF16 else "<f2") for p in (k, v))
+
+    def batch(self, kv_len, page_table, row_off=None, n_rows=None):
+        """kv_len [n_seq], page_table [n_seq, max_pages], row_off [n_seq + 1] or None (one row per sequence): int32 on the GPU."""
+        return KvBatch(kv_len, page_table, row_off, n_rows)
+
+    def _rows(self, t, width, batch, what):
+        """Address and row stride of a row tensor, as the library takes them."""
+        if isinstance(self._dtype, str) and str(t.dtype) == self._dtype:
+            self._dtype = t.dtype                        # from now on without the text
+        shape, stride = t.shape, t.stride()
+        if t.dtype != self._dtype or len(shape) != 2 or shape[1] != width or shape[0] < batch.n_rows or (stride[1] != 1 and width > 1) or t.device != batch.device:
+            raise ValueError(f"{what} is a {self._dtype} tensor [at least {batch.n_rows} rows, {width}] on the batch's device, each row's values side by side")
+        return t.data_ptr(), stride[0] if shape[0] > 1 else width
+
+    def append(self, batch, q, k, v, q_out, stream=None):
+        """Norm and rotation of the rows; q to q_out, k and v to their slots. stream: an integer handle as torch gives it (0: the
+        legacy default stream), or None for the handle's own. Asynchronous."""
+        a, b, c = self._rows(q, self._q_width, batch, "q"), self._rows(k, self._kv_width, batch, "k"), self._rows(v, self._kv_width, batch, "v")
+        o = self._rows(q_out, self._q_width, batch, "q_out")
+        if self._append(self.h, batch.at, *a, *b, *c, *o, 1 if stream == 0 else stream) != 0:
+            raise BackendError("kv_append: " + _err())
+
+    def attend(self, batch, q, out, stream=None):
+        """Attention of the batch's rows over the visible keys of their sequences, into out. Asynchronous, as append."""
+        a, o = self._rows(q, self._q_width, batch, "q"), self._rows(out, self._q_width, batch, "out")
+        if self._attend(self.h, batch.at, *a, *o, 1 if stream == 0 else stream) != 0:
+            raise BackendError("kv_attend: " + _err())
+
+    def sync(self, stream=None):
+        """Waits, and raises for what the calls since the last sync have found."""
+        _check(lib().mynah_b200_kv_sync(self.h, 1 if stream == 0 else stream), "kv_sync")
 
 
 class QMat:

@@ -60,7 +60,8 @@ static inline size_t align_up(size_t v, size_t a) { return (v + a - 1) / a * a; 
 // Device status word codes written by kernels whose bounded waits ran out.
 // ST_RANGE: a value that had to become an fp16 (hi, lo) operand pair was not finite or reached 65504 in
 // magnitude (the planes cannot hold it), so the result is not to be trusted.
-enum { ST_OK = 0, ST_TIMEOUT_PRODUCER = 1, ST_TIMEOUT_MMA = 2, ST_TIMEOUT_EPILOGUE = 3, ST_RANGE = 4 };
+// ST_PAGE: a table of a paged cache names a page, a length or a row that does not exist.
+enum { ST_OK = 0, ST_TIMEOUT_PRODUCER = 1, ST_TIMEOUT_MMA = 2, ST_TIMEOUT_EPILOGUE = 3, ST_RANGE = 4, ST_PAGE = 5 };
 
 // A matrix stored as two fp16 planes: value = hi + lo * 2^-11 (22 significant bits).
 // The residual is kept pre-scaled by 2^11 so that it has the magnitude of hi and never

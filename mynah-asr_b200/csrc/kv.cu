@@ -1,0 +1,225 @@
+// The paged key/value cache at the C boundary (include/mynah_b200.h): checks of arguments, the handle and its memory.
+#include <math.h>
+#include <string.h>
+
+#include <new>
+
+#include "../../include/mynah_b200.h"
+#include "kv.h"
+
+using namespace mb;
+
+// Device memory of a handle: the two pools, and a block [status, 256 B | turns of the rotation | norm weights].
+struct mynah_b200_kv {
+    mynah_b200_kv_config cfg;
+    int fmt = KV_BF16, device = 0;
+    cudaStream_t stream = nullptr;
+    uint16_t *k = nullptr, *v = nullptr;
+    uint8_t *block = nullptr;
+    double *turns = nullptr;
+    float *q_norm = nullptr, *k_norm = nullptr;
+    int *status() const { return reinterpret_cast<int *>(block); }
+    ~mynah_b200_kv() {
+        cudaFree(k); cudaFree(v); cudaFree(block);              // (waits for the handle's work)
+        if (stream) cudaStreamDestroy(stream);
+    }
+};
+
+namespace {
+// The handle's device is the current one while a call runs
+struct OnDevice {
+    int before = -1;
+    explicit OnDevice(int dev) {
+        if (cudaGetDevice(&before) != cudaSuccess) { cudaGetLastError(); before = -1; }
+        if (before != dev) cudaSetDevice(dev); else before = -1;
+    }
+    ~OnDevice() { if (before >= 0) cudaSetDevice(before); }
+};
+
+int row_bytes(int fmt) { return fmt == KV_F32 ? 4 : 2; }
+
+bool power_of_two(int v) { return v > 0 && (v & (v - 1)) == 0; }
+
+const char *refuse_config(const mynah_b200_kv_config &c, int *fmt) {
+    if (c.fmt == MYNAH_B200_F32) *fmt = KV_F32;
+    else if (c.fmt == MYNAH_B200_F16) *fmt = KV_F16;
+    else if (c.fmt == MYNAH_B200_BF16) *fmt = KV_BF16;
+    else return "rows are F32, F16 or BF16";
+    if (c.n_kv_heads < 1 || c.n_heads < 1 || c.n_heads % c.n_kv_heads || c.n_heads / c.n_kv_heads > 64 || c.n_heads > 1024)
+        return "n_heads is 1 to 64 times n_kv_heads, at most 1024";
+    if (c.head_dim < 16 || c.head_dim > 128 || c.head_dim % 16) return "head_dim is a multiple of 16 up to 128";
+    if (!power_of_two(c.page_size) || c.page_size < 8 || c.page_size > 256) return "page_size is a power of two from 8 to 256";
+    if (c.n_pages < 1 || (int64_t)c.n_pages * c.page_size * c.n_kv_heads > 0x7fffffffll) return "n_pages x page_size x n_kv_heads is from 1 page to 2^31 - 1 rows";
+    if (c.rotary_dim < 0 || c.rotary_dim > c.head_dim || c.rotary_dim % 8) return "rotary_dim is a multiple of 8 up to head_dim";
+    if (c.rotary_dim && !c.inv_freq && !(c.rope_theta > 0 && isfinite(c.rope_theta))) return "rope_theta is positive";
+    if (c.window < 0 || c.n_sinks < 0 || (c.n_sinks && !c.window)) return "window and n_sinks are not negative, and sinks need a window";
+    if (!(c.scale >= 0) || !isfinite(c.scale)) return "scale is not negative";
+    if ((c.q_norm || c.k_norm) && !(c.norm_eps >= 0 && isfinite(c.norm_eps))) return "norm_eps is not negative";
+    return nullptr;
+}
+
+// Memory that a kernel on `dev` can reach. An address of the host or of another GPU would be a fault there.
+bool reachable(const void *p, int dev) {
+    cudaPointerAttributes at;
+    if (cudaPointerGetAttributes(&at, p) != cudaSuccess) { cudaGetLastError(); return false; }
+    return at.type == cudaMemoryTypeManaged || (at.type == cudaMemoryTypeDevice && at.device == dev) ||
+           (at.type == cudaMemoryTypeHost && at.devicePointer == p);
+}
+
+// Rows of `width` values with stride ld, of which the last one ends where the buffer does
+const char *refuse_rows(const mynah_b200_kv *h, const void *p, long long ld, int width) {
+    if (!p) return "a null pointer";
+    if (ld < width) return "a row stride below the row's width";
+    if (ld > (1ll << 40)) return "a row stride out of range";
+    if (((uintptr_t)p & 15) || (ld * row_bytes(h->fmt)) % 16) return "rows start on 16-byte boundaries";
+    if (!reachable(p, h->device)) return "a pointer that is not of the handle's device";
+    return nullptr;
+}
+
+// 1: nothing to do, 0: go on, -1: refused
+int take_batch(const char *what, const mynah_b200_kv *h, const mynah_b200_kv_batch *b, KvArgs *a) {
+    const mynah_b200_kv_config &c = h->cfg;
+    const char *no = nullptr;
+    if (b->n_seq < 0 || b->n_rows < 0) no = "a negative count";
+    else if (b->n_seq == 0 || b->n_rows == 0) return 1;
+    else if (!b->kv_len || !b->page_table) no = "a null table";
+    else if (b->max_pages < 1 || (int64_t)b->max_pages * c.page_size > 0x7fffffffll) no = "max_pages x page_size is from 1 page to 2^31 - 1 positions";
+    else if (!b->row_off && b->n_rows < b->n_seq) no = "fewer rows than sequences";
+    else if (((uintptr_t)b->kv_len | (uintptr_t)b->page_table | (uintptr_t)b->row_off) & 3) no = "a misaligned table";
+    else if (!reachable(b->kv_len, h->device) || !reachable(b->page_table, h->device) || (b->row_off && !reachable(b->row_off, h->device)))
+        no = "a table that is not of the handle's device";
+    if (no) { set_error("%s: %s", what, no); return -1; }
+    a->H = c.n_heads; a->Hkv = c.n_kv_heads; a->G = c.n_heads / c.n_kv_heads; a->D = c.head_dim;
+    a->page_shift = __builtin_ctz((unsigned)c.page_size); a->n_pages = c.n_pages;
+    a->window = c.window; a->sinks = c.n_sinks;
+    a->scale = c.scale > 0 ? c.scale : 1.f / sqrtf((float)c.head_dim);
+    a->k = h->k; a->v = h->v; a->status = h->status();
+    a->n_seq = b->n_seq; a->n_rows = b->n_rows; a->max_pages = b->max_pages;
+    a->row_off = b->row_off; a->kv_len = b->kv_len; a->table = b->page_table;
+    return 0;
+}
+}  // namespace
+
+extern "C" {
+
+void mynah_b200_kv_config_default(mynah_b200_kv_config *c) {
+    if (!c) return;
+    memset(c, 0, sizeof(*c));
+    c->page_size = 16;
+    c->fmt = MYNAH_B200_F32;
+    c->rope_theta = 10000.0;
+    c->norm_eps = 1e-6f;
+}
+
+mynah_b200_kv *mynah_b200_kv_create(const mynah_b200_kv_config *cfg) {
+    if (!mynah_b200_available()) { set_error("no sm_100 CUDA device available"); return nullptr; }
+    if (!cfg) { set_error("kv_create: null config"); return nullptr; }
+    int fmt = 0;
+    if (const char *no = refuse_config(*cfg, &fmt)) { set_error("kv_create: %s", no); return nullptr; }
+    const int rot = cfg->rotary_dim, D = cfg->head_dim;
+    double turns[64];
+    for (int i = 0; i < rot / 2; i++) {
+        const double f = cfg->inv_freq ? cfg->inv_freq[i] : pow(cfg->rope_theta, -2.0 * i / rot);
+        if (!isfinite(f)) { set_error("kv_create: a rotation frequency is not finite"); return nullptr; }
+        turns[i] = f / 6.283185307179586476925;
+    }
+    for (int i = 0; i < 2 * D; i++) {
+        const float *w = i < D ? cfg->q_norm : cfg->k_norm;
+        if (w && !isfinite(w[i % D])) { set_error("kv_create: a norm weight is not finite"); return nullptr; }
+    }
+    RelaxedCapture relaxed;
+    mynah_b200_kv *h = new (std::nothrow) mynah_b200_kv();
+    if (!h) { set_error("kv_create: host allocation failed"); return nullptr; }
+    h->cfg = *cfg; h->fmt = fmt;
+    h->cfg.inv_freq = nullptr; h->cfg.q_norm = h->cfg.k_norm = nullptr;              // borrowed for this call only
+    const size_t pool = (size_t)cfg->n_pages * cfg->page_size * cfg->n_kv_heads * D * sizeof(uint16_t);
+    const size_t block = 256 + sizeof(turns) + 2 * 128 * sizeof(float);
+    bool ok = cudaGetDevice(&h->device) == cudaSuccess && cudaStreamCreateWithFlags(&h->stream, cudaStreamNonBlocking) == cudaSuccess &&
+              cudaMalloc((void **)&h->block, block) == cudaSuccess && cudaMalloc((void **)&h->k, pool) == cudaSuccess &&
+              cudaMalloc((void **)&h->v, pool) == cudaSuccess;
+    if (ok) {
+        h->turns = reinterpret_cast<double *>(h->block + 256);
+        float *norms = reinterpret_cast<float *>(h->block + 256 + sizeof(turns));
+        if (cfg->q_norm) h->q_norm = norms;
+        if (cfg->k_norm) h->k_norm = norms + 128;
+        // every slot is finite from the start: what a mask hides is multiplied by a probability of 0
+        ok = cudaMemsetAsync(h->block, 0, block, h->stream) == cudaSuccess && cudaMemsetAsync(h->k, 0, pool, h->stream) == cudaSuccess &&
+             cudaMemsetAsync(h->v, 0, pool, h->stream) == cudaSuccess && cudaStreamSynchronize(h->stream) == cudaSuccess &&
+             (!rot || cudaMemcpy(h->turns, turns, (size_t)(rot / 2) * sizeof(double), cudaMemcpyHostToDevice) == cudaSuccess) &&
+             (!cfg->q_norm || cudaMemcpy(h->q_norm, cfg->q_norm, (size_t)D * sizeof(float), cudaMemcpyHostToDevice) == cudaSuccess) &&
+             (!cfg->k_norm || cudaMemcpy(h->k_norm, cfg->k_norm, (size_t)D * sizeof(float), cudaMemcpyHostToDevice) == cudaSuccess);
+    }
+    if (!ok) {
+        const cudaError_t e = cudaGetLastError();
+        set_error("kv_create: device memory for 2 x %zu bytes: %s", pool, cudaGetErrorString(e));
+        delete h;
+        return nullptr;
+    }
+    return h;
+}
+
+void mynah_b200_kv_free(mynah_b200_kv *h) {
+    if (!h) return;
+    OnDevice on(h->device);
+    RelaxedCapture relaxed;
+    delete h;
+}
+
+int mynah_b200_kv_pages(const mynah_b200_kv *h, void **k, void **v) {
+    if (!h || !k || !v) { set_error("kv_pages: bad argument"); return -1; }
+    *k = h->k; *v = h->v;
+    return 0;
+}
+
+int mynah_b200_kv_append(mynah_b200_kv *h, const mynah_b200_kv_batch *b, const void *q, long long ldq, const void *k, long long ldk,
+                         const void *v, long long ldv, void *q_out, long long ldqo, void *stream) {
+    if (!h || !b) { set_error("kv_append: bad argument"); return -1; }
+    OnDevice on(h->device);
+    KvAppendArgs p = {};
+    const int go = take_batch("kv_append", h, b, &p.a);
+    if (go) return go < 0 ? -1 : 0;
+    const int D = p.a.D;
+    const char *no = refuse_rows(h, q, ldq, p.a.H * D);
+    if (!no) no = refuse_rows(h, k, ldk, p.a.Hkv * D);
+    if (!no) no = refuse_rows(h, v, ldv, p.a.Hkv * D);
+    if (!no) no = refuse_rows(h, q_out, ldqo, p.a.H * D);
+    if (no) { set_error("kv_append: %s", no); return -1; }
+    p.a.q = q; p.a.ldq = ldq; p.a.out = q_out; p.a.ldo = ldqo;
+    p.k_rows = k; p.ldk = ldk; p.v_rows = v; p.ldv = ldv;
+    p.q_norm = h->q_norm; p.k_norm = h->k_norm; p.eps = h->cfg.norm_eps;
+    p.turns = h->turns; p.rot = h->cfg.rotary_dim; p.interleaved = h->cfg.rotary_interleaved != 0;
+    return kv_append(p, h->fmt, stream ? (cudaStream_t)stream : h->stream);
+}
+
+int mynah_b200_kv_attend(mynah_b200_kv *h, const mynah_b200_kv_batch *b, const void *q, long long ldq, void *out, long long ldo,
+                         void *stream) {
+    if (!h || !b) { set_error("kv_attend: bad argument"); return -1; }
+    OnDevice on(h->device);
+    KvArgs a = {};
+    const int go = take_batch("kv_attend", h, b, &a);
+    if (go) return go < 0 ? -1 : 0;
+    const char *no = refuse_rows(h, q, ldq, a.H * a.D);
+    if (!no) no = refuse_rows(h, out, ldo, a.H * a.D);
+    if (no) { set_error("kv_attend: %s", no); return -1; }
+    a.q = q; a.ldq = ldq; a.out = out; a.ldo = ldo;
+    return kv_attend_plain(a, h->fmt, stream ? (cudaStream_t)stream : h->stream);
+}
+
+int mynah_b200_kv_sync(mynah_b200_kv *h, void *stream) {
+    if (!h) { set_error("kv_sync: null handle"); return -1; }
+    OnDevice on(h->device);
+    const cudaStream_t st = stream ? (cudaStream_t)stream : h->stream;
+    MB_CUDA(cudaStreamSynchronize(st));
+    int code = 0;
+    MB_CUDA(cudaMemcpyAsync(&code, h->status(), sizeof(int), cudaMemcpyDeviceToHost, h->stream));
+    MB_CUDA(cudaStreamSynchronize(h->stream));
+    if (code == ST_OK) return 0;
+    MB_CUDA(cudaMemsetAsync(h->status(), 0, sizeof(int), h->stream));
+    MB_CUDA(cudaStreamSynchronize(h->stream));
+    if (code == ST_RANGE) set_error("kv: a value did not fit its 16 bits (f16: |v| >= 65504) or was not finite");
+    else if (code == ST_PAGE) set_error("kv: a table names a page, a length or a row that does not exist");
+    else set_error("kv: a bounded wait inside an attention kernel ran out (code %d)", code);
+    return -1;
+}
+
+}  // extern "C"

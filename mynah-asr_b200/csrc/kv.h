@@ -1,0 +1,78 @@
+// Paged key/value cache of one decoder layer: what the kernels of kv_append.cu, kv_step.cu and kv_chunk.cu get.
+#pragma once
+#include "kernels.h"
+#include "kv_index.h"
+
+namespace mb {
+
+enum { KV_F32 = 0, KV_F16 = 1, KV_BF16 = 2 };       // rows; the cache holds f16 for the first two, bf16 for the third
+
+// Pools are [page][kv head][slot][D], 16 bits a value: the keys of one head in one page are one run of memory.
+struct KvArgs {
+    int H, Hkv, G, D;                                // G = H / Hkv query heads share a kv head
+    int page_shift, n_pages;
+    int window, sinks;
+    float scale;
+    uint16_t *k, *v;                                 // pools
+    int *status;
+    // the call
+    int n_seq, n_rows, max_pages;
+    const int *row_off, *kv_len, *table;
+    const void *q;
+    void *out;
+    int64_t ldq, ldo;                                // row strides in values
+};
+struct KvAppendArgs {
+    KvArgs a;
+    const void *k_rows, *v_rows;
+    int64_t ldk, ldv;
+    const float *q_norm, *k_norm;                    // [D] or null
+    float eps;
+    const double *turns;                             // [rot / 2]: turns of a pair per position
+    int rot, interleaved;
+};
+
+#ifdef __CUDACC__
+__device__ __forceinline__ int64_t kv_capacity(const KvArgs &a) { return (int64_t)a.max_pages << a.page_shift; }
+// Page of a position whose page index is in range; an entry that names no page is reported and read as page 0
+__device__ __forceinline__ int kv_page(const KvArgs &a, int seq, int page_index) {
+    const int p = a.table[(size_t)seq * a.max_pages + page_index];
+    if ((unsigned)p < (unsigned)a.n_pages) return p;
+    atomicExch(a.status, ST_PAGE);
+    return 0;
+}
+// Index of a cache row (one head at one slot)
+__device__ __forceinline__ size_t kv_row(const KvArgs &a, int page, int head, int slot) {
+    return ((((size_t)page * a.Hkv + head) << a.page_shift) + slot);
+}
+// The sequence that row r belongs to, found by a whole warp: the last s with row_off[s] <= r; -1 where there is none, or the row lies
+// behind the last sequence. Each round looks at 32 places of what is left.
+__device__ __forceinline__ int kv_find_seq(const KvArgs &a, int r, int lane) {
+    if (!a.row_off) return r < a.n_seq ? r : -1;
+    int lo = 0, hi = a.n_seq + 1;                    // the answer lies in [lo, hi)
+    bool first = true;
+    while (first || hi - lo > 1) {
+        const int step = (hi - lo + 31) / 32, at = lo + lane * step;
+        const unsigned below = __ballot_sync(0xffffffffu, at < hi && a.row_off[at < hi ? at : lo] <= r);
+        if (below == 0) return -1;
+        lo += (31 - __clz(below)) * step;
+        if (hi > lo + step) hi = lo + step;
+        first = false;
+    }
+    return lo < a.n_seq ? lo : -1;
+}
+// Reports sequences whose tables contradict the call (rows are found from the offsets, so a row may miss that they decrease)
+__device__ __forceinline__ void kv_look_over(const KvArgs &a, int lane) {
+    bool bad = false;
+    for (int s = lane; s < a.n_seq; s += 32) {
+        KvSeq q;
+        bad |= !kv_seq(a.row_off, a.kv_len, s, a.n_rows, kv_capacity(a), &q);
+    }
+    if (bad) atomicExch(a.status, ST_PAGE);
+}
+#endif
+
+int kv_append(const KvAppendArgs &a, int fmt, cudaStream_t st);
+int kv_attend_plain(const KvArgs &a, int fmt, cudaStream_t st);
+
+}  // namespace mb

@@ -1,0 +1,228 @@
+"""The paged key/value cache without a GPU: the index arithmetic of its kernels compiled for the host, and the library's host side on
+a CUDA runtime of host memory (fake_cudart.cpp): what it refuses, and what its launches get."""
+import ctypes as C
+import os
+import subprocess
+import sys
+
+import numpy as np
+import pytest
+
+from test_host_paths import LAUNCH, _fake, fake_runtime  # noqa: F401 (a fixture)
+
+HERE = os.path.dirname(os.path.abspath(__file__))
+SCENARIOS = {}
+
+INDEX = r"""
+#include "kv_index.h"
+using namespace mb;
+extern "C" {
+int seq(const int *off, const int *len, int s, int rows, long long cap, int *out) {
+    KvSeq q; const bool ok = kv_seq(off, len, s, rows, cap, &q); out[0] = q.begin; out[1] = q.n; out[2] = q.len; return ok;
+}
+int sees(int pos, int j, int window, int sinks) { return kv_sees(pos, j, window, sinks); }
+int tiles(int p0, int p1, int window, int sinks, int tile, int *out, int cap) {
+    const KvTiles t = kv_tiles(p0, p1, window, sinks, tile);
+    for (int i = 0; i < t.count && i < cap; i++) out[i] = t.at(i);
+    return t.count;
+}
+}
+"""
+
+
+@pytest.fixture(scope="module")
+def index(tmp_path_factory):
+    out = tmp_path_factory.mktemp("kv_index")
+    (out / "index.cpp").write_text(INDEX)
+    subprocess.run(["g++", "-std=c++17", "-O1", "-fPIC", "-shared", "-fsanitize=undefined", "-fno-sanitize-recover", "-I",
+                    os.path.join(HERE, "..", "mynah-asr_b200", "csrc"), str(out / "index.cpp"), "-o", str(out / "index.so")], check=True)
+    return C.CDLL(str(out / "index.so"))
+
+
+def test_sequences_of_tables(index):
+    """Whatever the tables say, what comes out lies inside of the call's buffers."""
+    top = 2 ** 31 - 1
+    numbers = [0, 1, -1, 5, 9, 10, 11, top, -top - 1, top - 1]
+    out, cap = (C.c_int * 3)(), 96
+    for b in numbers:
+        for e in numbers:
+            for n in numbers:
+                off, length = (C.c_int * 2)(b, e), (C.c_int * 1)(n)
+                ok = index.seq(off, length, 0, 10, C.c_longlong(cap), out)
+                assert bool(ok) == (0 <= b <= e <= 10 and 0 <= n <= cap)
+                if ok:
+                    assert list(out) == [b, e - b, n]
+                else:
+                    assert out[1] == out[2] == 0
+                ok = index.seq(None, length, 0, 10, C.c_longlong(cap), out)
+                assert bool(ok) == (0 <= n <= cap) and (not ok or list(out) == [0, 1, n])
+
+
+@pytest.mark.parametrize("tile", [32, 128])
+def test_tiles_cover_what_is_seen(index, tile):
+    """The tiles of rows at [p0, p1]: in order, none twice, every visible key in one of them, and none of a window's without one."""
+    out = (C.c_int * 4096)()
+    for window in (0, 1, 5, tile - 1, tile, tile + 1, 3 * tile + 7, 2 ** 31 - 1):
+        for sinks in ((0, 1, tile, tile + 1, 5 * tile, 2 ** 31 - 1) if window else (0,)):
+            for p0 in (-7, -1, 0, 1, tile - 1, tile, 4 * tile, 9 * tile + 3, 20 * tile):
+                for more in (0, 1, tile - 1, tile, 2 * tile + 5):
+                    p1 = p0 + more
+                    n = index.tiles(p0, p1, window, sinks, tile, out, 4096)
+                    got = list(out[:n])
+                    rows = [p for p in {p0, p0 + more // 2, p1} if p >= 0]
+                    need = {j // tile for p in rows for j in range(p + 1) if index.sees(p, j, window, sinks)}
+                    assert got == sorted(set(got)) and need <= set(got), (window, sinks, p0, p1, got)
+                    assert all(0 <= t <= max(p1, 0) // tile for t in got)
+                    if window and more == 0 and p0 >= 0:
+                        assert set(got) - need <= {t for t in got if t < min(sinks, p0 + 1) / tile} | need
+    top = 2 ** 31 - 1
+    assert index.tiles(top - 5, top - 1, 64, 4, tile, out, 4096) in (2, 3, 4)
+    assert index.tiles(top - 5, top - 1, 64, top, tile, out, 4096) == (top - 1) // tile + 1
+
+
+# ------------------------------------------------------------------------------------------- in the child process
+def scenario(f):
+    SCENARIOS[f.__name__] = f
+    return f
+
+
+@pytest.mark.parametrize("name", ["kv_refuses", "kv_gives_back", "kv_launches", "kv_failed_calls"])
+def test_kv_host(fake_runtime, name):  # noqa: F811
+    env = dict(os.environ, LD_LIBRARY_PATH=fake_runtime + ":" + os.environ.get("LD_LIBRARY_PATH", ""), OMP_NUM_THREADS="1")
+    r = subprocess.run([sys.executable, os.path.abspath(__file__), name], env=env, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stdout + r.stderr
+
+
+def _config(pkg, **more):
+    c = pkg.KvConfig()
+    pkg.lib().mynah_b200_kv_config_default(C.byref(c))
+    for name, value in dict(dict(n_heads=4, n_kv_heads=2, head_dim=64, n_pages=8), **more).items():
+        setattr(c, name, value)
+    return c
+
+
+def _dev(n):
+    """n bytes of the fake device's memory."""
+    L, p = C.CDLL("libcudart.so.12"), C.c_void_p()
+    assert L.cudaMalloc(C.byref(p), C.c_size_t(n)) == 0
+    return p.value
+
+
+def _batch(pkg, n_seq=2, n_rows=2, row_off=None, kv_len=0, page_table=0, max_pages=4):
+    return pkg.KvBatchStruct(n_seq, n_rows, row_off, kv_len, page_table, max_pages)
+
+
+@scenario
+def kv_refuses(pkg, fake):
+    """Every refusal comes with its reason, before anything is launched or allocated."""
+    L = pkg.lib()
+    nan, inf = float("nan"), float("inf")
+    before = fake.fake_device_bytes()
+    for more in (dict(fmt=pkg.MYNAH_Q8), dict(fmt=77), dict(n_heads=0), dict(n_kv_heads=0), dict(n_heads=5), dict(n_heads=-4), dict(n_heads=130),
+                 dict(head_dim=8), dict(head_dim=72), dict(head_dim=144), dict(head_dim=0), dict(page_size=12), dict(page_size=4), dict(page_size=512),
+                 dict(page_size=0), dict(n_pages=0), dict(n_pages=2 ** 27), dict(rotary_dim=4), dict(rotary_dim=72), dict(rotary_dim=-8),
+                 dict(rotary_dim=8, rope_theta=0.0), dict(rotary_dim=8, rope_theta=nan), dict(window=-1), dict(n_sinks=2), dict(window=3, n_sinks=-1),
+                 dict(scale=-1.0), dict(scale=nan), dict(scale=inf), dict(norm_eps=nan, q_norm=(C.c_float * 64)()), dict(norm_eps=-1.0, k_norm=(C.c_float * 64)()),
+                 dict(q_norm=(C.c_float * 64)(*([1.0] * 63 + [nan]))), dict(rotary_dim=8, inv_freq=(C.c_double * 4)(1, 2, inf, 3))):
+        assert L.mynah_b200_kv_create(C.byref(_config(pkg, **more))) is None, more
+        assert b"kv_create" in L.mynah_b200_last_error(), more
+    assert L.mynah_b200_kv_create(None) is None and fake.fake_device_bytes() == before
+    h = L.mynah_b200_kv_create(C.byref(_config(pkg, rotary_dim=64)))
+    assert h
+    seen = []
+    cb = LAUNCH(lambda name, args, recorded: seen.append(name))
+    fake.fake_on_launch(cb)
+    lens, table, off, rows = _dev(64), _dev(256), _dev(64), _dev(1 << 16)
+    good = dict(kv_len=lens, page_table=table)
+    call = lambda b, q=rows, ldq=256, out=rows, ldo=256: L.mynah_b200_kv_attend(h, C.addressof(b), q, ldq, out, ldo, None)  # noqa: E731
+    host = np.zeros(4096, np.float32)
+    for b in (dict(good, n_seq=-1), dict(good, n_rows=-1), dict(good, kv_len=None), dict(good, page_table=None), dict(good, max_pages=0),
+              dict(good, max_pages=2 ** 28), dict(good, n_seq=3), dict(good, kv_len=lens + 2), dict(good, row_off=off + 1),
+              dict(good, kv_len=host.ctypes.data), dict(good, page_table=host.ctypes.data), dict(good, row_off=host.ctypes.data)):
+        assert call(_batch(pkg, **b)) == -1, b
+        assert b"kv_attend" in L.mynah_b200_last_error()
+    b = _batch(pkg, **good)
+    for more in (dict(q=None), dict(q=rows + 4), dict(q=host.ctypes.data), dict(ldq=255), dict(ldq=-256), dict(ldq=257), dict(ldq=2 ** 50), dict(out=None),
+                 dict(out=rows + 8), dict(out=host.ctypes.data), dict(ldo=128), dict(ldo=258)):
+        assert call(b, **more) == -1, more
+    at = C.addressof(b)
+    for bad in range(4):
+        for value, ld in ((None, 256), (rows + 4, 256), (rows, 100), (host.ctypes.data, 256)):
+            args = [x for i in range(4) for x in ((value, ld) if i == bad else (rows, 256))]
+            assert L.mynah_b200_kv_append(h, at, *args, None) == -1
+            assert b"kv_append" in L.mynah_b200_last_error()
+    assert L.mynah_b200_kv_append(None, at, *([rows, 256] * 4), None) == L.mynah_b200_kv_attend(h, None, rows, 256, rows, 256, None) == -1
+    assert L.mynah_b200_kv_sync(None, None) == -1 and L.mynah_b200_kv_pages(h, None, None) == -1
+    for empty in (dict(good, n_seq=0), dict(good, n_rows=0, n_seq=0), dict(good, n_rows=0, row_off=off)):
+        assert call(_batch(pkg, **empty)) == 0
+    assert not seen
+    assert call(b) == 0 and len(seen) == 1
+    assert L.mynah_b200_kv_append(h, at, *([rows, 256] * 4), None) == 0 and len(seen) == 2
+    assert L.mynah_b200_kv_sync(h, None) == 0
+    L.mynah_b200_kv_free(h)
+    L.mynah_b200_kv_free(None)
+
+
+@scenario
+def kv_gives_back(pkg, fake):
+    """Whatever fails while a handle is made, nothing stays allocated; a handle that is freed gives all of it back."""
+    L = pkg.lib()
+    before = fake.fake_device_bytes()
+    for name, most in ((b"cudaMalloc", 3), (b"cudaStreamCreate", 1), (b"cudaMemsetAsync", 3)):
+        for nth in range(1, most + 1):
+            fake.fake_fail(name, nth)
+            assert L.mynah_b200_kv_create(C.byref(_config(pkg))) is None
+            assert fake.fake_failed() and b"kv_create" in L.mynah_b200_last_error()
+            assert fake.fake_device_bytes() == before, name
+    h = L.mynah_b200_kv_create(C.byref(_config(pkg)))
+    assert fake.fake_device_bytes() - before >= 2 * 8 * 16 * 2 * 64 * 2
+    L.mynah_b200_kv_free(h)
+    assert fake.fake_device_bytes() == before
+
+
+@scenario
+def kv_launches(pkg, fake):
+    """A recorded call and a plain one are one launch each, allocate nothing and leave another thread's recording alone."""
+    L = pkg.lib()
+    w = (C.c_float * 64)(*range(64))
+    fake.fake_foreign_capture(1)
+    h = L.mynah_b200_kv_create(C.byref(_config(pkg, q_norm=w, rotary_dim=16)))
+    assert h and fake.fake_broken_captures() == 0
+    fake.fake_foreign_capture(0)
+    lens, table, off, rows = _dev(64), _dev(256), _dev(64), _dev(1 << 16)
+    seen = []
+    cb = LAUNCH(lambda name, args, recorded: seen.append(name))
+    fake.fake_on_launch(cb)
+    held, mallocs, count = fake.fake_device_bytes(), fake.fake_calls(b"cudaMalloc"), pkg.launch_count()
+    for row_off in (None, off):
+        b = _batch(pkg, kv_len=lens, page_table=table, row_off=row_off)
+        assert L.mynah_b200_kv_append(h, C.addressof(b), *([rows, 256] * 4), None) == 0
+        assert L.mynah_b200_kv_attend(h, C.addressof(b), rows, 256, rows, 256, None) == 0
+    assert len(seen) == 4 and pkg.launch_count() == count + 4
+    assert fake.fake_device_bytes() == held and fake.fake_calls(b"cudaMalloc") == mallocs
+    assert fake.fake_pending() == 1                      # asynchronous
+    assert L.mynah_b200_kv_sync(h, None) == 0 and fake.fake_pending() == 0
+    L.mynah_b200_kv_free(h)
+
+
+@scenario
+def kv_failed_calls(pkg, fake):
+    """A launch or a copy that fails is that call's error and not the next one's."""
+    L = pkg.lib()
+    h = L.mynah_b200_kv_create(C.byref(_config(pkg)))
+    lens, table, rows = _dev(64), _dev(256), _dev(1 << 16)
+    b = _batch(pkg, kv_len=lens, page_table=table)
+    for call in (lambda: L.mynah_b200_kv_append(h, C.addressof(b), *([rows, 256] * 4), None),
+                 lambda: L.mynah_b200_kv_attend(h, C.addressof(b), rows, 256, rows, 256, None)):
+        fake.fake_fail(b"cudaLaunchKernel", 1)
+        assert call() == -1 and fake.fake_failed()
+        assert call() == 0
+    fake.fake_fail(b"cudaMemcpyAsync", 1)
+    assert L.mynah_b200_kv_sync(h, None) == -1 and L.mynah_b200_kv_sync(h, None) == 0
+    L.mynah_b200_kv_free(h)
+
+
+if __name__ == "__main__":
+    sys.path.insert(0, HERE)
+    import conftest
+    SCENARIOS[sys.argv[1]](conftest.load_package(), _fake())
