@@ -18,6 +18,7 @@ struct mynah_b200_kv {
     uint8_t *block = nullptr;
     double *turns = nullptr;
     float *q_norm = nullptr, *k_norm = nullptr;
+    CUtensorMap step_k, step_v;
     int *status() const { return reinterpret_cast<int *>(block); }
     ~mynah_b200_kv() {
         cudaFree(k); cudaFree(v); cudaFree(block);              // (waits for the handle's work)
@@ -64,6 +65,26 @@ bool reachable(const void *p, int dev) {
     if (cudaPointerGetAttributes(&at, p) != cudaSuccess) { cudaGetLastError(); return false; }
     return at.type == cudaMemoryTypeManaged || (at.type == cudaMemoryTypeDevice && at.device == dev) ||
            (at.type == cudaMemoryTypeHost && at.devicePointer == p);
+}
+
+typedef CUresult (*EncodeFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
+                             const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion,
+                             CUtensorMapFloatOOBfill);
+
+// A pool as [rows][D]: boxes of 64 columns (zeros beyond D) and box_rows slots of one page and head, 128-byte swizzle
+bool pool_map(CUtensorMap *m, const uint16_t *pool, const mynah_b200_kv_config &c, int box_rows) {
+    void *p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess) {
+        cudaGetLastError();
+        return false;
+    }
+    cuuint64_t dims[2] = {(cuuint64_t)c.head_dim, (cuuint64_t)c.n_pages * c.page_size * c.n_kv_heads};
+    cuuint64_t strides[1] = {(cuuint64_t)c.head_dim * 2};
+    cuuint32_t box[2] = {64, (cuuint32_t)box_rows}, estr[2] = {1, 1};
+    return reinterpret_cast<EncodeFn>(p)(m, c.fmt == MYNAH_B200_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2,
+                                         const_cast<uint16_t *>(pool), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 // Rows of `width` values with stride ld, of which the last one ends where the buffer does
@@ -155,6 +176,12 @@ mynah_b200_kv *mynah_b200_kv_create(const mynah_b200_kv_config *cfg) {
         delete h;
         return nullptr;
     }
+    const int box = kv_step_box(D, cfg->page_size);
+    if (!pool_map(&h->step_k, h->k, *cfg, box) || !pool_map(&h->step_v, h->v, *cfg, box)) {
+        set_error("kv_create: no tensor map of the pools");
+        delete h;
+        return nullptr;
+    }
     return h;
 }
 
@@ -202,7 +229,8 @@ int mynah_b200_kv_attend(mynah_b200_kv *h, const mynah_b200_kv_batch *b, const v
     if (!no) no = refuse_rows(h, out, ldo, a.H * a.D);
     if (no) { set_error("kv_attend: %s", no); return -1; }
     a.q = q; a.ldq = ldq; a.out = out; a.ldo = ldo;
-    return kv_attend_plain(a, h->fmt, stream ? (cudaStream_t)stream : h->stream);
+    const cudaStream_t st = stream ? (cudaStream_t)stream : h->stream;
+    return a.row_off ? kv_attend_plain(a, h->fmt, st) : kv_step(h->step_k, h->step_v, a, h->fmt, st);
 }
 
 int mynah_b200_kv_sync(mynah_b200_kv *h, void *stream) {
