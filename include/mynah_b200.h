@@ -335,7 +335,7 @@ typedef struct {
     const float *q_norm, *k_norm;        /* [head_dim] weights of a root-mean-square norm of every q / k head; NULL: none */
     float norm_eps;
     int window, n_sinks;                 /* window > 0: a row at position p sees the keys j with p - window < j <= p, and j < n_sinks */
-    float scale;                         /* of the scores; 0: 1 / sqrt(head_dim) */
+    float scale;                         /* of the scores, from 1e-20 to 1e20; 0: 1 / sqrt(head_dim) */
 } mynah_b200_kv_config;
 void mynah_b200_kv_config_default(mynah_b200_kv_config *cfg);     /* zeros, pages of 16, theta 10000, eps 1e-6 */
 

@@ -18,7 +18,8 @@ struct mynah_b200_kv {
     uint8_t *block = nullptr;
     double *turns = nullptr;
     float *q_norm = nullptr, *k_norm = nullptr;
-    CUtensorMap step_k, step_v;
+    CUtensorMap map_k, map_v;
+    int box = 0;
     int *status() const { return reinterpret_cast<int *>(block); }
     ~mynah_b200_kv() {
         cudaFree(k); cudaFree(v); cudaFree(block);              // (waits for the handle's work)
@@ -54,7 +55,7 @@ const char *refuse_config(const mynah_b200_kv_config &c, int *fmt) {
     if (c.rotary_dim < 0 || c.rotary_dim > c.head_dim || c.rotary_dim % 8) return "rotary_dim is a multiple of 8 up to head_dim";
     if (c.rotary_dim && !c.inv_freq && !(c.rope_theta > 0 && isfinite(c.rope_theta))) return "rope_theta is positive";
     if (c.window < 0 || c.n_sinks < 0 || (c.n_sinks && !c.window)) return "window and n_sinks are not negative, and sinks need a window";
-    if (!(c.scale >= 0) || !isfinite(c.scale)) return "scale is not negative";
+    if (!(c.scale == 0 || (c.scale >= 1e-20f && c.scale <= 1e20f))) return "scale is 0 or from 1e-20 to 1e20";
     if ((c.q_norm || c.k_norm) && !(c.norm_eps >= 0 && isfinite(c.norm_eps))) return "norm_eps is not negative";
     return nullptr;
 }
@@ -176,8 +177,8 @@ mynah_b200_kv *mynah_b200_kv_create(const mynah_b200_kv_config *cfg) {
         delete h;
         return nullptr;
     }
-    const int box = kv_step_box(D, cfg->page_size);
-    if (!pool_map(&h->step_k, h->k, *cfg, box) || !pool_map(&h->step_v, h->v, *cfg, box)) {
+    h->box = kv_box(D, cfg->page_size);
+    if (!pool_map(&h->map_k, h->k, *cfg, h->box) || !pool_map(&h->map_v, h->v, *cfg, h->box)) {
         set_error("kv_create: no tensor map of the pools");
         delete h;
         return nullptr;
@@ -230,7 +231,7 @@ int mynah_b200_kv_attend(mynah_b200_kv *h, const mynah_b200_kv_batch *b, const v
     if (no) { set_error("kv_attend: %s", no); return -1; }
     a.q = q; a.ldq = ldq; a.out = out; a.ldo = ldo;
     const cudaStream_t st = stream ? (cudaStream_t)stream : h->stream;
-    return a.row_off ? kv_attend_plain(a, h->fmt, st) : kv_step(h->step_k, h->step_v, a, h->fmt, st);
+    return a.row_off ? kv_chunk(h->map_k, h->map_v, a, h->box, h->fmt, st) : kv_step(h->map_k, h->map_v, a, h->fmt, st);
 }
 
 int mynah_b200_kv_sync(mynah_b200_kv *h, void *stream) {

@@ -73,9 +73,9 @@ __device__ __forceinline__ void kv_look_over(const KvArgs &a, int lane) {
 #endif
 
 int kv_append(const KvAppendArgs &a, int fmt, cudaStream_t st);
-int kv_attend_plain(const KvArgs &a, int fmt, cudaStream_t st);
-// maps of the two pools as [rows][D] with boxes of 64 columns and kv_step_box slots
-int kv_step_box(int D, int page_size);
+// Attention of one row per sequence, and of many. Maps of the two pools as [rows][D] with boxes of 64 columns and kv_box slots.
+int kv_box(int D, int page_size);
 int kv_step(const CUtensorMap &k, const CUtensorMap &v, const KvArgs &a, int fmt, cudaStream_t st);
+int kv_chunk(const CUtensorMap &k, const CUtensorMap &v, const KvArgs &a, int box_rows, int fmt, cudaStream_t st);
 
 }  // namespace mb

@@ -496,7 +496,7 @@ static int step_heads(const CUtensorMap &k, const CUtensorMap &v, const KvArgs &
     return a.G <= 8 ? step_launch<DP, FMT, 1>(k, v, a, st) : step_launch<DP, FMT, 2>(k, v, a, st);
 }
 
-int kv_step_box(int D, int page_size) {
+int kv_box(int D, int page_size) {
     const int tile = D <= 64 ? StepShape<64>::TILE : StepShape<128>::TILE;
     return page_size < tile ? page_size : tile;
 }
