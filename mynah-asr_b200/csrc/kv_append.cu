@@ -3,55 +3,43 @@
 //   (a, b) -> (a cos t - b sin t, a sin t + b cos t), t = p f_i   (the first `rot` values of q and k heads, p the row's position)
 // then q heads go to q_out, k and v heads to their slot of the cache, each rounded once.
 //
-// HBM-bound: every value is read once and written once. A head is spread over D / 8 lanes (rounded up to a power of two), eight
-// values each, so that 16-bit rows move by 16-byte accesses; a warp takes a run of a row's heads, all of which turn by the same
-// angles: a lane keeps the cosines and sines of its eight values in registers. Sums of squares, norms and rotation are in f32; the
-// angle is formed as turns in f64 and reduced there (a position of 10^6 times a frequency near 1 has no correct digit behind the point
-// in f32), its sine and cosine then in f32.
+// HBM-bound: every value is read once and written once. A head is spread over D / 8 lanes (rounded up to a power of two), eight values
+// each as two quads: where halves turn against one another, lane l of the first rot / 8 holds the values 4 l of both halves, so that a
+// pair meets in one lane and nothing but the sum of squares crosses lanes; elsewhere the quads are neighbours. A warp takes a run of a
+// row's heads, all of which turn by the same angles: a lane keeps the cosines and sines of its four pairs and its norm weights in
+// registers, and has KA_AHEAD head groups in flight. Sums of squares, norms and rotation are in f32; the angle is formed as turns in
+// f64 and reduced there (a position of 10^6 times a frequency near 1 has no correct digit behind the point in f32), its sine and
+// cosine then in f32.
 #include "kv.h"
 #include <cuda_bf16.h>
 
 namespace mb {
 
-template <int FMT> struct KvRow;                     // eight values of a row, and of a 16-bit cache row
-template <> struct KvRow<KV_F32> {
-    static __device__ __forceinline__ void load(const void *p, int64_t i, float *v) {
-        const float4 *s = reinterpret_cast<const float4 *>(static_cast<const float *>(p) + i);
-        const float4 a = s[0], b = s[1];
-        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-    }
-    static __device__ __forceinline__ void store(void *p, int64_t i, const float *v) {
-        float4 *d = reinterpret_cast<float4 *>(static_cast<float *>(p) + i);
-        d[0] = make_float4(v[0], v[1], v[2], v[3]); d[1] = make_float4(v[4], v[5], v[6], v[7]);
-    }
-};
-__device__ __forceinline__ uint4 kv_pack8(const float *v, bool bf) {
-    uint32_t r[4];
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        if (bf) { const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]); r[i] = *reinterpret_cast<const uint32_t *>(&h); }
-        else { const __half2 h = __floats2half2_rn(v[2 * i], v[2 * i + 1]); r[i] = *reinterpret_cast<const uint32_t *>(&h); }
-    }
-    return make_uint4(r[0], r[1], r[2], r[3]);
+__device__ __forceinline__ uint32_t ka_pack(float x, float y, bool bf) {
+    if (bf) { const __nv_bfloat162 h = __floats2bfloat162_rn(x, y); return *reinterpret_cast<const uint32_t *>(&h); }
+    const __half2 h = __floats2half2_rn(x, y);
+    return *reinterpret_cast<const uint32_t *>(&h);
 }
-template <bool BF> struct KvRow16 {
-    static __device__ __forceinline__ void load(const void *p, int64_t i, float *v) {
-        const uint4 u = *reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(p) + i);
-        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-            float2 f;
-            if (BF) f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162 *>(&w[e]));
-            else f = __half22float2(*reinterpret_cast<const __half2 *>(&w[e]));
-            v[2 * e] = f.x; v[2 * e + 1] = f.y;
-        }
+__device__ __forceinline__ float2 ka_unpack(uint32_t u, bool bf) {
+    if (bf) return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162 *>(&u));
+    return __half22float2(*reinterpret_cast<const __half2 *>(&u));
+}
+// Four values of a row, as they lie in memory
+template <int FMT> struct KaQuad { typedef uint2 type; };
+template <> struct KaQuad<KV_F32> { typedef float4 type; };
+template <int FMT>
+__device__ __forceinline__ void ka_open(const typename KaQuad<FMT>::type &r, float *v) {
+    if constexpr (FMT == KV_F32) { v[0] = r.x; v[1] = r.y; v[2] = r.z; v[3] = r.w; }
+    else {
+        const float2 a = ka_unpack(r.x, FMT == KV_BF16), b = ka_unpack(r.y, FMT == KV_BF16);
+        v[0] = a.x; v[1] = a.y; v[2] = b.x; v[3] = b.y;
     }
-    static __device__ __forceinline__ void store(void *p, int64_t i, const float *v) {
-        *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(p) + i) = kv_pack8(v, BF);
-    }
-};
-template <> struct KvRow<KV_F16> : KvRow16<false> {};
-template <> struct KvRow<KV_BF16> : KvRow16<true> {};
+}
+template <int FMT>
+__device__ __forceinline__ typename KaQuad<FMT>::type ka_close(const float *v) {
+    if constexpr (FMT == KV_F32) return make_float4(v[0], v[1], v[2], v[3]);
+    else return make_uint2(ka_pack(v[0], v[1], FMT == KV_BF16), ka_pack(v[2], v[3], FMT == KV_BF16));
+}
 
 static constexpr int KA_WARPS = 8, KA_AHEAD = 4;     // head groups that a warp has in flight
 // The largest magnitude that a cache value may have: beyond it a bf16 would round to infinity; f16 as the operand planes
@@ -60,7 +48,8 @@ static constexpr float KA_BF16_MAX = 3.3895313e38f;
 template <int FMT, int LPH>
 __global__ void __launch_bounds__(KA_WARPS * 32)
 kv_append_kernel(const KvAppendArgs p, int parts, int per_part) {
-    constexpr int HPI = 32 / LPH;                    // heads side by side in a warp
+    typedef typename KaQuad<FMT>::type Quad;
+    constexpr int HPI = 32 / LPH, SIZE = FMT == KV_F32 ? 4 : 2;        // heads side by side in a warp; bytes of a row's value
     const KvArgs &a = p.a;
     const int lane = threadIdx.x & 31;
     chain_trigger();
@@ -69,6 +58,34 @@ kv_append_kernel(const KvAppendArgs p, int parts, int per_part) {
     const int row = (int)(unit / parts), part = (int)(unit % parts);
     if (unit == 0 && a.row_off) kv_look_over(a, lane);
     if (row >= a.n_rows) return;
+    const int sub = lane / LPH, l = lane % LPH;
+    const bool on = l * 8 < a.D, pairs = !p.interleaved && l * 8 < p.rot;
+    const int qa = pairs ? 4 * l : 8 * l, qb = pairs ? p.rot / 2 + 4 * l : 8 * l + 4;         // first values of the lane's quads
+    const int heads = a.H + 2 * a.Hkv, g0 = part * per_part, g_end = min(g0 + per_part, (heads + HPI - 1) / HPI);
+    const char *q = static_cast<const char *>(a.q) + row * a.ldq * SIZE, *k = static_cast<const char *>(p.k_rows) + row * p.ldk * SIZE,
+               *v = static_cast<const char *>(p.v_rows) + row * p.ldv * SIZE;
+    Quad in[KA_AHEAD][2];
+    auto fetch = [&](int g) {
+#pragma unroll
+        for (int u = 0; u < KA_AHEAD; u++) {
+            const int h = (g + u) * HPI + sub;
+            if (on && g + u < g_end && h < heads) {
+                const char *s = h < a.H ? q + (size_t)h * a.D * SIZE : h < a.H + a.Hkv ? k + (size_t)(h - a.H) * a.D * SIZE : v + (size_t)(h - a.H - a.Hkv) * a.D * SIZE;
+                in[u][0] = *reinterpret_cast<const Quad *>(s + qa * SIZE);
+                in[u][1] = *reinterpret_cast<const Quad *>(s + qb * SIZE);
+            } else {
+                in[u][0] = in[u][1] = Quad();
+            }
+        }
+    };
+    fetch(g0);                                       // (rows that turn out to have no place are within the buffers, too)
+    float wq[8], wk[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        const int e = (i < 4 ? qa : qb - 4) + i;
+        wq[i] = p.q_norm && on ? p.q_norm[e] : 1.f;
+        wk[i] = p.k_norm && on ? p.k_norm[e] : 1.f;
+    }
     const int seq = kv_find_seq(a, row, lane);
     if (seq < 0) return;                             // behind the last sequence: everything stays as it was
     KvSeq s;
@@ -79,86 +96,72 @@ kv_append_kernel(const KvAppendArgs p, int parts, int per_part) {
     const int pos = s.len - s.n + (row - s.begin);
     if (pos < 0) return;                             // in front of the first position
     const int page = a.table[(size_t)seq * a.max_pages + (pos >> a.page_shift)], slot = pos & ((1 << a.page_shift) - 1);
+    float cs[4], sn[4];                              // of the lane's pairs: values (i, i + 4), or (2 i, 2 i + 1) where interleaved
+    if (p.rot) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            cs[i] = 1.f; sn[i] = 0.f;
+            if (l * 8 < p.rot) {
+                double t = (double)pos * p.turns[4 * l + i];
+                t -= rint(t);
+                sincospif(2.f * (float)t, &sn[i], &cs[i]);
+            }
+        }
+    }
     if ((unsigned)page >= (unsigned)a.n_pages) {
         if (lane == 0) atomicExch(a.status, ST_PAGE);
         return;
     }
-    const int sub = lane / LPH, e0 = (lane % LPH) * 8, half = p.rot / 2;
-    const bool on = e0 < a.D;
-    float cs[8], sn[8];                              // value i becomes v[i] cs[i] + partner sn[i]
-#pragma unroll
-    for (int i = 0; i < 8; i++) {
-        const int e = e0 + i;
-        cs[i] = 1.f; sn[i] = 0.f;
-        if (e < p.rot) {
-            const int f = p.interleaved ? e >> 1 : (e < half ? e : e - half);
-            double t = (double)pos * p.turns[f];
-            t -= rint(t);
-            float sv, cv;
-            sincospif(2.f * (float)t, &sv, &cv);
-            cs[i] = cv;
-            sn[i] = (p.interleaved ? (e & 1) : e >= half) ? sv : -sv;
-        }
-    }
-    const int heads = a.H + 2 * a.Hkv;
-    const float top = FMT == KV_BF16 ? KA_BF16_MAX : H16_MAX;
+    const size_t head_step = (size_t)a.D << a.page_shift, base = kv_row(a, page, 0, slot) * a.D;
+    char *out = static_cast<char *>(a.out) + row * a.ldo * SIZE;
+    const float top = FMT == KV_BF16 ? KA_BF16_MAX : H16_MAX, inv_d = 1.f / (float)a.D;
     bool bad = false;
-    const int g_end = min((part + 1) * per_part, (heads + HPI - 1) / HPI);
-    for (int g0 = part * per_part; g0 < g_end; g0 += KA_AHEAD) {
-        float v[KA_AHEAD][8];
+    for (int g = g0; g < g_end; g += KA_AHEAD) {
+        if (g > g0) fetch(g);
 #pragma unroll
         for (int u = 0; u < KA_AHEAD; u++) {
-            const int h = (g0 + u) * HPI + sub;
-#pragma unroll
-            for (int i = 0; i < 8; i++) v[u][i] = 0.f;
-            if (on && g0 + u < g_end && h < heads) {
-                if (h < a.H) KvRow<FMT>::load(a.q, row * a.ldq + h * a.D + e0, v[u]);
-                else if (h < a.H + a.Hkv) KvRow<FMT>::load(p.k_rows, row * p.ldk + (h - a.H) * a.D + e0, v[u]);
-                else KvRow<FMT>::load(p.v_rows, row * p.ldv + (h - a.H - a.Hkv) * a.D + e0, v[u]);
-            }
-        }
-#pragma unroll
-        for (int u = 0; u < KA_AHEAD; u++) {
-            const int h = (g0 + u) * HPI + sub;
-            if (g0 + u >= g_end) break;              // the same for the whole warp
-            float *x = v[u];
-            const float *w = h < a.H ? p.q_norm : p.k_norm;
+            const int h = (g + u) * HPI + sub;
+            if (g + u >= g_end) break;               // the same for the whole warp
+            float x[8];
+            ka_open<FMT>(in[u][0], x);
+            ka_open<FMT>(in[u][1], x + 4);
             const bool turns = h < a.H + a.Hkv;      // (v heads pass as they are)
-            float ss = 0.f;
+            if (p.q_norm || p.k_norm) {              // the same for the whole launch
+                float ss = 0.f;
 #pragma unroll
-            for (int i = 0; i < 8; i++) ss = fmaf(x[i], x[i], ss);
+                for (int i = 0; i < 8; i++) ss = fmaf(x[i], x[i], ss);
 #pragma unroll
-            for (int o = LPH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-            if (turns && w && on) {
-                const float r = 1.f / sqrtf(ss / (float)a.D + p.eps);
+                for (int o = LPH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+                const float r = rsqrtf(fmaf(ss, inv_d, p.eps));
+                if (h < a.H ? p.q_norm != nullptr : turns && p.k_norm != nullptr) {
 #pragma unroll
-                for (int i = 0; i < 8; i++) x[i] *= r * w[e0 + i];
+                    for (int i = 0; i < 8; i++) x[i] *= r * (h < a.H ? wq[i] : wk[i]);
+                }
             }
-            if (p.rot) {                             // the same for the whole launch
-                float y[8];
+            if (p.rot && turns) {
                 if (p.interleaved) {
 #pragma unroll
-                    for (int i = 0; i < 8; i++) y[i] = x[i ^ 1];
-                } else {
-                    // value e turns with e + half or e - half: eight values further on a lane boundary, or four (half % 8 is 0 or 4)
-                    const bool split = half & 4;
-#pragma unroll
-                    for (int i = 0; i < 8; i++) {
-                        const int e = e0 + i, other = e < half ? e + half : e < p.rot ? e - half : e;
-                        const float mine = split ? x[i ^ 4] : x[i];
-                        y[i] = __shfl_sync(0xffffffffu, mine, (sub * LPH) + ((other >> 3) & (LPH - 1)));
+                    for (int i = 0; i < 4; i++) {
+                        const float c = x[2 * i], d = x[2 * i + 1];
+                        x[2 * i] = fmaf(c, cs[i], -d * sn[i]);
+                        x[2 * i + 1] = fmaf(c, sn[i], d * cs[i]);
                     }
-                }
-                if (turns) {
+                } else {
 #pragma unroll
-                    for (int i = 0; i < 8; i++) x[i] = e0 + i < p.rot ? fmaf(x[i], cs[i], y[i] * sn[i]) : x[i];
+                    for (int i = 0; i < 4; i++) {
+                        const float c = x[i], d = x[i + 4];
+                        x[i] = fmaf(c, cs[i], -d * sn[i]);
+                        x[i + 4] = fmaf(c, sn[i], d * cs[i]);
+                    }
                 }
             }
             if (!on || h >= heads) continue;
             if (h < a.H) {
 #pragma unroll
                 for (int i = 0; i < 8; i++) bad |= !(fabsf(x[i]) < (FMT == KV_F32 ? INFINITY : top));
-                KvRow<FMT>::store(a.out, row * a.ldo + h * a.D + e0, x);
+                char *to = out + (size_t)h * a.D * SIZE;
+                *reinterpret_cast<Quad *>(to + qa * SIZE) = ka_close<FMT>(x);
+                *reinterpret_cast<Quad *>(to + qb * SIZE) = ka_close<FMT>(x + 4);
             } else {
                 // the cache holds finite values only: what a mask hides is multiplied by a probability of 0
 #pragma unroll
@@ -167,9 +170,9 @@ kv_append_kernel(const KvAppendArgs p, int parts, int per_part) {
                     bad |= !fits;
                     x[i] = fits ? x[i] : 0.f;
                 }
-                const bool key = h < a.H + a.Hkv;
-                const size_t at = kv_row(a, page, h - a.H - (key ? 0 : a.Hkv), slot) * a.D + e0;
-                *reinterpret_cast<uint4 *>((key ? a.k : a.v) + at) = kv_pack8(x, FMT == KV_BF16);
+                uint16_t *to = (turns ? a.k : a.v) + base + (size_t)(h - a.H - (turns ? 0 : a.Hkv)) * head_step;
+                *reinterpret_cast<uint2 *>(to + qa) = ka_close<FMT == KV_BF16 ? KV_BF16 : KV_F16>(x);
+                *reinterpret_cast<uint2 *>(to + qb) = ka_close<FMT == KV_BF16 ? KV_BF16 : KV_F16>(x + 4);
             }
         }
     }

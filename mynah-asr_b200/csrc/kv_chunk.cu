@@ -21,6 +21,7 @@ namespace mb {
 static constexpr int KC_ROWS = 128, KC_KEYS = 128, KC_HALF = 128 * 128;      // a 128-row x 64-column box of 16-bit values: 16 KB
 static constexpr int KC_SOFT = 8, KC_W_TMA = 8, KC_W_MMA = 9, KC_THREADS = 320;
 static constexpr int KC_HEAD = 1024;
+static constexpr int KC_PART = 6;                    // P V begins when the first 6 x 16 keys' probabilities are there
 static constexpr float KC_NONE = -1e30f;             // "maximum" of no keys
 
 template <int DP, int FMT> struct ChunkShape {
@@ -52,11 +53,37 @@ __device__ __forceinline__ void kc_st16(uint32_t taddr, const uint32_t *r) {
           "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
         : "memory");
 }
+__device__ __forceinline__ void kc_st8(uint32_t taddr, const uint32_t *r) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+        ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]) : "memory");
+}
 __device__ __forceinline__ void kc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ float kc_ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+// Two f32 operations in one instruction
+__device__ __forceinline__ float2 kc_fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("{\n\t.reg .b64 ra, rb, rc, rd;\n\tmov.b64 ra, {%2, %3};\n\tmov.b64 rb, {%4, %5};\n\tmov.b64 rc, {%6, %7};\n\t"
+        "fma.rn.f32x2 rd, ra, rb, rc;\n\tmov.b64 {%0, %1}, rd;\n\t}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+__device__ __forceinline__ float2 kc_add2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n\t.reg .b64 ra, rb, rd;\n\tmov.b64 ra, {%2, %3};\n\tmov.b64 rb, {%4, %5};\n\tadd.rn.f32x2 rd, ra, rb;\n\tmov.b64 {%0, %1}, rd;\n\t}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+// Waits for loads from tensor memory; the values that they bring are not to be touched before (nor their use moved up)
+__device__ __forceinline__ void kc_wait_ld32(float *x) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+f"(x[0]), "+f"(x[1]), "+f"(x[2]), "+f"(x[3]), "+f"(x[4]), "+f"(x[5]), "+f"(x[6]), "+f"(x[7]), "+f"(x[8]), "+f"(x[9]), "+f"(x[10]),
+                   "+f"(x[11]), "+f"(x[12]), "+f"(x[13]), "+f"(x[14]), "+f"(x[15]), "+f"(x[16]), "+f"(x[17]), "+f"(x[18]), "+f"(x[19]), "+f"(x[20]),
+                   "+f"(x[21]), "+f"(x[22]), "+f"(x[23]), "+f"(x[24]), "+f"(x[25]), "+f"(x[26]), "+f"(x[27]), "+f"(x[28]), "+f"(x[29]), "+f"(x[30]), "+f"(x[31])
+                 :: "memory");
 }
 template <bool BF>
 __device__ __forceinline__ uint32_t kc_pack(float x, float y) {
@@ -124,7 +151,7 @@ kv_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
     uint8_t *head = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(kc_raw) + 1023) & ~uintptr_t(1023));
     uint8_t *qst = head + KC_HEAD, *ring = qst + Sh::Q;
     uint64_t *full = reinterpret_cast<uint64_t *>(head), *empty = full + STAGES, *q_full = empty + STAGES, *s_full = q_full + 1,
-             *p_full = s_full + 2, *o_full = p_full + 2, *drain = o_full + 2;
+             *p_part = s_full + 2, *p_full = p_part + 2, *o_full = p_full + 2, *drain = o_full + 2;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(drain + 1);
     volatile int *place = reinterpret_cast<volatile int *>(tmem_slot + 1);
     const int warp = warp_index(), lane = threadIdx.x & 31;
@@ -141,7 +168,7 @@ kv_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
         tma_prefetch_desc(&tmK); tma_prefetch_desc(&tmV);
         for (int s = 0; s < STAGES; s++) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
         mbar_init(q_full, KC_SOFT);
-        for (int t = 0; t < 2; t++) { mbar_init(&s_full[t], 1); mbar_init(&p_full[t], KC_SOFT / 2); mbar_init(&o_full[t], 1); }
+        for (int t = 0; t < 2; t++) { mbar_init(&s_full[t], 1); mbar_init(&p_part[t], KC_SOFT / 2); mbar_init(&p_full[t], KC_SOFT / 2); mbar_init(&o_full[t], 1); }
         mbar_init(drain, 1);
         mbar_fence_init();
     }
@@ -215,47 +242,53 @@ kv_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
                 }
             }
         };
-        auto issue_o = [&](int t, int s, bool first) {
+        auto issue_o = [&](int t, int s, bool first, int k0, int k1) {
             const uint64_t vd = vdesc + (uint64_t)((s * Sh::OPERAND) >> 4);
+#pragma unroll
             for (int plane = 0; plane < Sh::PLANES; plane++) {
 #pragma unroll
-                for (int kk = 0; kk < KC_KEYS / 16; kk++)
+                for (int kk = k0; kk < k1; kk++)
                     kc_mma_ts(tmem + Sh::COL_O + t * DP, tmem + Sh::COL_S + t * 128 + plane * 64 + 8 * kk, vd + (uint64_t)((kk * 2048) >> 4), idesc_o,
                               !first || (kk | plane) != 0);
             }
         };
         int s = 0, ph = 0;                                     // ring place of the next item
-        auto step = [&]() { if (++s == STAGES) { s = 0; ph ^= 1; } };
-        if (ok && n > 0) ok = mbar_wait_warp(&full[0], 0);
-        if (ok && n > 0) {
+        auto take = [&](int *at) {                             // waits for the next item
+            *at = s;
+            const bool got = mbar_wait_warp(&full[s], (uint32_t)ph);
+            if (++s == STAGES) { s = 0; ph ^= 1; }
+            return got;
+        };
+        int sk = 0, sv = 0;
+        if (ok && n > 0 && (ok = take(&sk))) {
             tc_fence_after();
             if (elect_one()) {
-                issue_s(0, 0); tc_commit(&s_full[0]);
-                issue_s(1, 0); tc_commit(&s_full[1]);
-                tc_commit(&empty[0]);
+                issue_s(0, sk); tc_commit(&s_full[0]);
+                issue_s(1, sk); tc_commit(&s_full[1]);
+                tc_commit(&empty[sk]);
             }
             __syncwarp();
-            step();
+            ok = take(&sv);
         }
+        // An issued product keeps the pipe busy for 60 clocks, a wait that has come true costs as much: the waits stand where
+        // products are still under way.
         for (int i = 0; i < n && ok; i++) {
-            const int sv = s;
-            if (!mbar_wait_warp(&full[sv], (uint32_t)ph)) { ok = false; break; }
-            step();
-            const int sk = s;
             const bool more = i + 1 < n;
-            if (more) {
-                if (!mbar_wait_warp(&full[sk], (uint32_t)ph)) { ok = false; break; }
-                step();
-            }
+            const int v = sv;
 #pragma unroll
             for (int t = 0; t < 2; t++) {
+                if (!mbar_wait_warp(&p_part[t], (uint32_t)(i & 1))) { ok = false; break; }
+                tc_fence_after();
+                if (elect_one()) issue_o(t, v, i == 0, 0, KC_PART);
+                __syncwarp();
+                if (more && !take(t == 0 ? &sk : &sv)) { ok = false; break; }      // K(i + 1), V(i + 1)
                 if (!mbar_wait_warp(&p_full[t], (uint32_t)(i & 1))) { ok = false; break; }
                 tc_fence_after();
                 if (elect_one()) {
-                    issue_o(t, sv, i == 0);
+                    issue_o(t, v, i == 0, KC_PART, KC_KEYS / 16);
                     if (more) { issue_s(t, sk); tc_commit(&s_full[t]); }
                     else tc_commit(&o_full[t]);
-                    if (t == 1) { tc_commit(&empty[sv]); if (more) tc_commit(&empty[sk]); }
+                    if (t == 1) { tc_commit(&empty[v]); if (more) tc_commit(&empty[sk]); }
                 }
                 __syncwarp();
             }
@@ -306,60 +339,91 @@ kv_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
             if (lane == 0) mbar_arrive(q_full);
         }
         const float sc = a.scale * 1.4426950408889634f;
-        float m = KC_NONE, l = 0.f;
+        float m = KC_NONE;
+        float2 l2[2] = {{0.f, 0.f}, {0.f, 0.f}};
         bool ok = true;
         for (int i = 0; i < n && ok; i++) {
             if (!mbar_wait_warp(&s_full[t], (uint32_t)(i & 1))) { ok = false; break; }
             tc_fence_after();
             float x[KC_KEYS];
+            const uint32_t s_at = trow + Sh::COL_S + t * 128;
+            tc_ld32(s_at, x);
+            tc_ld32(s_at + 32, x + 32);
+            kc_wait_ld32(x); kc_wait_ld32(x + 32);
+            tc_ld32(s_at + 64, x + 64);
+            tc_ld32(s_at + 96, x + 96);
+            float m4[4] = {x[0], x[1], x[2], x[3]};
 #pragma unroll
-            for (int c = 0; c < 4; c++) tc_ld32(trow + Sh::COL_S + t * 128 + 32 * c, x + 32 * c);
-            tc_wait_ld();
+            for (int c = 4; c < 60; c += 8)
+#pragma unroll
+                for (int e = 0; e < 4; e++) m4[e] = fmaxf(m4[e], fmaxf(x[c + e], x[c + 4 + e]));
+#pragma unroll
+            for (int e = 0; e < 4; e++) m4[e] = fmaxf(m4[e], x[60 + e]);
+            kc_wait_ld32(x + 64); kc_wait_ld32(x + 96);
+#pragma unroll
+            for (int c = 64; c < 128; c += 8)
+#pragma unroll
+                for (int e = 0; e < 4; e++) m4[e] = fmaxf(m4[e], fmaxf(x[c + e], x[c + 4 + e]));
             const int j0 = tiles.at(i) * KC_KEYS, d = pos - j0;
             const bool whole = d >= KC_KEYS - 1 && (a.window <= 0 || d < a.window || j0 + KC_KEYS - 1 < a.sinks);
             if (!__all_sync(0xffffffffu, whole)) {
                 const int low = a.window > 0 ? d - a.window : -1, keep = a.sinks - j0;       // hidden: above d; up to low, from keep on
+                m4[0] = m4[1] = m4[2] = m4[3] = -INFINITY;
 #pragma unroll
-                for (int c = 0; c < KC_KEYS; c++)
+                for (int c = 0; c < KC_KEYS; c++) {
                     if (c > d || (c <= low && c >= keep)) x[c] = -INFINITY;
+                    m4[c & 3] = fmaxf(m4[c & 3], x[c]);
+                }
             }
-            float mt = fmaxf(x[0], x[1]);
-#pragma unroll
-            for (int c = 2; c < KC_KEYS; c += 2) mt = fmaxf(mt, fmaxf(x[c], x[c + 1]));
-            mt *= sc;
+            const float mt = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * sc;
             const bool grow = mt > m + 8.f;
             if (__any_sync(0xffffffffu, grow)) {
                 const float alpha = grow ? kc_ex2(m - mt) : 1.f;
                 if (grow) m = mt;
-                l *= alpha;
+                l2[0].x *= alpha; l2[0].y *= alpha; l2[1].x *= alpha; l2[1].y *= alpha;
                 if (i > 0) {
 #pragma unroll 1
-                    for (int c = 0; c < DP / 32; c++) {
-                        float o[32];
-                        tc_ld32(trow + Sh::COL_O + t * DP + 32 * c, o);
+                    for (int c = 0; c < DP / 16; c++) {
+                        float o[16];
+                        tc_ld16(trow + Sh::COL_O + t * DP + 16 * c, o);
                         tc_wait_ld();
 #pragma unroll
-                        for (int e = 0; e < 32; e++) o[e] *= alpha;
-                        kc_st16(trow + Sh::COL_O + t * DP + 32 * c, reinterpret_cast<const uint32_t *>(o));
-                        kc_st16(trow + Sh::COL_O + t * DP + 32 * c + 16, reinterpret_cast<const uint32_t *>(o) + 16);
+                        for (int e = 0; e < 16; e++) o[e] *= alpha;
+                        kc_st16(trow + Sh::COL_O + t * DP + 16 * c, reinterpret_cast<const uint32_t *>(o));
                     }
                 }
             }
-            float l0 = 0.f, l1 = 0.f;
+            const float2 sc2 = make_float2(sc, sc), neg = make_float2(-m, -m);
+            // groups of 16 keys: a group's exponentials are under way while the one before is summed, packed and stored
 #pragma unroll
-            for (int c = 0; c < 4; c++) {
-                uint32_t hi[16], lo[F32 ? 16 : 1];
+            for (int c = 0; c <= 8; c++) {
+                if (c < 8) {
 #pragma unroll
-                for (int e = 0; e < 16; e++) {
-                    const float p0 = kc_ex2(fmaf(x[c * 32 + 2 * e], sc, -m)), p1 = kc_ex2(fmaf(x[c * 32 + 2 * e + 1], sc, -m));
-                    l0 += p0; l1 += p1;
-                    if (F32) kc_split(p0, p1, hi[e], lo[F32 ? e : 0]);
-                    else hi[e] = kc_pack<BF>(p0, p1);
+                    for (int e = 0; e < 8; e++) {
+                        float *v = x + c * 16 + 2 * e;
+                        const float2 y = kc_fma2(make_float2(v[0], v[1]), sc2, neg);
+                        v[0] = kc_ex2(y.x); v[1] = kc_ex2(y.y);
+                    }
                 }
-                kc_st16(trow + Sh::COL_S + t * 128 + 16 * c, hi);
-                if (F32) kc_st16(trow + Sh::COL_S + t * 128 + 64 + 16 * c, lo);
+                if (c > 0) {
+                    uint32_t hi[8], lo[F32 ? 8 : 1];
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        const float *v = x + (c - 1) * 16 + 2 * e;
+                        l2[e & 1] = kc_add2(l2[e & 1], make_float2(v[0], v[1]));
+                        if (F32) kc_split(v[0], v[1], hi[e], lo[F32 ? e : 0]);
+                        else hi[e] = kc_pack<BF>(v[0], v[1]);
+                    }
+                    kc_st8(trow + Sh::COL_S + t * 128 + 8 * (c - 1), hi);
+                    if (F32) kc_st8(trow + Sh::COL_S + t * 128 + 64 + 8 * (c - 1), lo);
+                    if (c == KC_PART) {
+                        kc_wait_st();
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&p_part[t]);
+                    }
+                }
             }
-            l += l0 + l1;
             kc_wait_st();
             tc_fence_before();
             __syncwarp();
@@ -368,7 +432,7 @@ kv_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
         if (n > 0 && ok) ok = mbar_wait_warp(&o_full[t], 0);
         if (!ok && lane == 0) atomicExch(a.status, ST_TIMEOUT_EPILOGUE);
         tc_fence_after();
-        const float inv = l != 0.f ? 1.f / l : 0.f;
+        const float l = (l2[0].x + l2[0].y) + (l2[1].x + l2[1].y), inv = l != 0.f ? 1.f / l : 0.f;
         const int64_t to = (int64_t)(sq.begin + tok) * a.ldo + (int64_t)h * a.D;
 #pragma unroll 1
         for (int c = 0; c < DP / 32; c++) {
