@@ -7,7 +7,7 @@
 // each as two quads: where halves turn against one another, lane l of the first rot / 8 holds the values 4 l of both halves, so that a
 // pair meets in one lane and nothing but the sum of squares crosses lanes; elsewhere the quads are neighbours. A warp takes a run of a
 // row's heads, all of which turn by the same angles: a lane keeps the cosines and sines of its four pairs and its norm weights in
-// registers, and has KA_AHEAD head groups in flight. Sums of squares, norms and rotation are in f32; the angle is formed as turns in
+// registers, and has 2 KB of reads in flight. Sums of squares, norms and rotation are in f32; the angle is formed as turns in
 // f64 and reduced there (a position of 10^6 times a frequency near 1 has no correct digit behind the point in f32), its sine and
 // cosine then in f32.
 #include "kv.h"
@@ -41,50 +41,164 @@ __device__ __forceinline__ typename KaQuad<FMT>::type ka_close(const float *v) {
     else return make_uint2(ka_pack(v[0], v[1], FMT == KV_BF16), ka_pack(v[2], v[3], FMT == KV_BF16));
 }
 
-static constexpr int KA_WARPS = 8, KA_AHEAD = 4;     // head groups that a warp has in flight
+static constexpr int KA_WARPS = 8;
 // The largest magnitude that a cache value may have: beyond it a bf16 would round to infinity; f16 as the operand planes
 static constexpr float KA_BF16_MAX = 3.3895313e38f;
 
-template <int FMT, int LPH>
-__global__ void __launch_bounds__(KA_WARPS * 32)
-kv_append_kernel(const KvAppendArgs p, int parts, int per_part) {
+// Two f32 operations in one instruction
+__device__ __forceinline__ float2 ka_fma(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("{\n\t.reg .b64 ra, rb, rc, rd;\n\tmov.b64 ra, {%2, %3};\n\tmov.b64 rb, {%4, %5};\n\tmov.b64 rc, {%6, %7};\n\t"
+        "fma.rn.f32x2 rd, ra, rb, rc;\n\tmov.b64 {%0, %1}, rd;\n\t}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+__device__ __forceinline__ float2 ka_mul(float2 a, float2 b) {
+    float2 d;
+    asm("{\n\t.reg .b64 ra, rb, rd;\n\tmov.b64 ra, {%2, %3};\n\tmov.b64 rb, {%4, %5};\n\tmul.rn.f32x2 rd, ra, rb;\n\tmov.b64 {%0, %1}, rd;\n\t}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+
+enum { KA_Q, KA_K, KA_V };
+// What a lane knows of its row: where its quads begin, cosines and sines of its pairs, the row's slot
+struct KaLane {
+    int sub, qa, qb;
+    bool on, turns;
+    float2 cs[2], sn[2], nsn[2];                     // pairs (0, 1) and (2, 3)
+};
+template <int FMT> struct KaAhead { static constexpr int N = FMT == KV_F32 ? 2 : 4; };   // head groups in flight: 2 KB of a warp's reads
+
+// The heads [h0 + sub, end) of one kind in steps of a warp's heads, from rows at `from` to `to` (elements of a head apart: step)
+template <int FMT, int LPH, int KIND>
+__device__ __forceinline__ bool ka_heads(const KvAppendArgs &p, const KaLane &w, const char *from, int g, int g_end, int heads, void *to, size_t step,
+                                         typename KaQuad<FMT>::type (&in)[KaAhead<FMT>::N][2], bool fetched) {
     typedef typename KaQuad<FMT>::type Quad;
-    constexpr int HPI = 32 / LPH, SIZE = FMT == KV_F32 ? 4 : 2;        // heads side by side in a warp; bytes of a row's value
+    constexpr int HPI = 32 / LPH, SIZE = FMT == KV_F32 ? 4 : 2, N = KaAhead<FMT>::N;
+    constexpr int OUT = KIND == KA_Q ? FMT : FMT == KV_BF16 ? KV_BF16 : KV_F16;
+    typedef typename KaQuad<OUT>::type Out;
+    const float *norm = KIND == KA_Q ? p.q_norm : KIND == KA_K ? p.k_norm : nullptr;
+    const float top = KIND == KA_Q && FMT == KV_F32 ? INFINITY : FMT == KV_BF16 ? KA_BF16_MAX : H16_MAX;
+    float2 wt[4];
+    if (KIND != KA_V && norm && w.on) {
+        *reinterpret_cast<float4 *>(wt) = *reinterpret_cast<const float4 *>(norm + w.qa);
+        *reinterpret_cast<float4 *>(wt + 2) = *reinterpret_cast<const float4 *>(norm + w.qb);
+    }
+    const float inv_d = 1.f / (float)p.a.D;
+    bool bad = false;
+    for (; g < g_end; g += N) {
+        if (!fetched) {
+#pragma unroll
+            for (int u = 0; u < N; u++) {
+                const int h = (g + u) * HPI + w.sub;
+                in[u][0] = in[u][1] = Quad();
+                if (w.on && h < heads && g + u < g_end) {
+                    const char *s = from + (size_t)h * (p.a.D * SIZE);
+                    in[u][0] = *reinterpret_cast<const Quad *>(s + w.qa * SIZE);
+                    in[u][1] = *reinterpret_cast<const Quad *>(s + w.qb * SIZE);
+                }
+            }
+        }
+        fetched = false;
+#pragma unroll
+        for (int u = 0; u < N; u++) {
+            const int h = (g + u) * HPI + w.sub;
+            if (g + u >= g_end) break;               // the same for the whole warp
+            float2 x[4];
+            ka_open<FMT>(in[u][0], reinterpret_cast<float *>(x));
+            ka_open<FMT>(in[u][1], reinterpret_cast<float *>(x + 2));
+            if (KIND != KA_V && norm) {              // the same for the whole launch
+                float2 s2 = ka_mul(x[0], x[0]);
+#pragma unroll
+                for (int i = 1; i < 4; i++) s2 = ka_fma(x[i], x[i], s2);
+                float ss = s2.x + s2.y;
+#pragma unroll
+                for (int o = LPH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+                const float r = rsqrtf(fmaf(ss, inv_d, p.eps));
+#pragma unroll
+                for (int i = 0; i < 4; i++) x[i] = ka_mul(ka_mul(x[i], wt[i]), make_float2(r, r));
+            }
+            if (KIND != KA_V && w.turns) {
+                if (p.interleaved) {
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const float c = i & 1 ? w.cs[i >> 1].y : w.cs[i >> 1].x, n = i & 1 ? w.sn[i >> 1].y : w.sn[i >> 1].x, b = x[i].x;
+                        x[i].x = fmaf(b, c, -x[i].y * n);
+                        x[i].y = fmaf(b, n, x[i].y * c);
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 2; i++) {
+                        const float2 b = x[i];
+                        x[i] = ka_fma(b, w.cs[i], ka_mul(x[i + 2], w.nsn[i]));
+                        x[i + 2] = ka_fma(b, w.sn[i], ka_mul(x[i + 2], w.cs[i]));
+                    }
+                }
+            }
+            if (w.on && h < heads) {
+                bool over = false;
+#pragma unroll
+                for (int i = 0; i < 4; i++) over |= !(fabsf(x[i].x) < top) | !(fabsf(x[i].y) < top);
+                if (over) {
+                    bad = true;
+                    if (KIND != KA_Q) {
+                        // the cache holds finite values only: what a mask hides is multiplied by a probability of 0
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            x[i].x = fabsf(x[i].x) < top ? x[i].x : 0.f;
+                            x[i].y = fabsf(x[i].y) < top ? x[i].y : 0.f;
+                        }
+                    }
+                }
+                char *d = static_cast<char *>(to) + (size_t)h * step * (KIND == KA_Q ? SIZE : 2);
+                *reinterpret_cast<Out *>(d + w.qa * (KIND == KA_Q ? SIZE : 2)) = ka_close<OUT>(reinterpret_cast<const float *>(x));
+                *reinterpret_cast<Out *>(d + w.qb * (KIND == KA_Q ? SIZE : 2)) = ka_close<OUT>(reinterpret_cast<const float *>(x + 2));
+            }
+        }
+    }
+    return bad;
+}
+
+// Warp = row x of 8 per block, and the block's part of the row's head groups: q's, then k's, then v's
+template <int FMT, int LPH>
+__global__ void __launch_bounds__(KA_WARPS * 32, FMT == KV_F32 ? 3 : 4)
+kv_append_kernel(const KvAppendArgs p, int per_part) {
+    typedef typename KaQuad<FMT>::type Quad;
+    constexpr int HPI = 32 / LPH, SIZE = FMT == KV_F32 ? 4 : 2, N = KaAhead<FMT>::N;
     const KvArgs &a = p.a;
     const int lane = threadIdx.x & 31;
     chain_trigger();
     chain_wait();
-    const int64_t unit = (int64_t)blockIdx.x * KA_WARPS + (threadIdx.x >> 5);
-    const int row = (int)(unit / parts), part = (int)(unit % parts);
-    if (unit == 0 && a.row_off) kv_look_over(a, lane);
+    const int row = (int)blockIdx.x * KA_WARPS + (int)(threadIdx.x >> 5);
+    if (row == 0 && blockIdx.y == 0 && a.row_off) kv_look_over(a, lane);
     if (row >= a.n_rows) return;
-    const int sub = lane / LPH, l = lane % LPH;
-    const bool on = l * 8 < a.D, pairs = !p.interleaved && l * 8 < p.rot;
-    const int qa = pairs ? 4 * l : 8 * l, qb = pairs ? p.rot / 2 + 4 * l : 8 * l + 4;         // first values of the lane's quads
-    const int heads = a.H + 2 * a.Hkv, g0 = part * per_part, g_end = min(g0 + per_part, (heads + HPI - 1) / HPI);
+    KaLane w;
+    const int l = lane % LPH;
+    w.sub = lane / LPH;
+    w.on = l * 8 < a.D;
+    w.turns = l * 8 < p.rot;
+    w.qa = w.turns && !p.interleaved ? 4 * l : 8 * l;
+    w.qb = w.turns && !p.interleaved ? p.rot / 2 + 4 * l : 8 * l + 4;
+    const int gq = (a.H + HPI - 1) / HPI, gk = (a.Hkv + HPI - 1) / HPI;
+    const int g0 = (int)blockIdx.y * per_part, g1 = g0 + per_part;
     const char *q = static_cast<const char *>(a.q) + row * a.ldq * SIZE, *k = static_cast<const char *>(p.k_rows) + row * p.ldk * SIZE,
                *v = static_cast<const char *>(p.v_rows) + row * p.ldv * SIZE;
-    Quad in[KA_AHEAD][2];
-    auto fetch = [&](int g) {
+    // the first reads are under way while the tables are looked up (rows that turn out to have no place are within the buffers, too)
+    Quad in[N][2];
+    {
+        const int kind = g0 < gq ? KA_Q : g0 < gq + gk ? KA_K : KA_V, g = kind == KA_Q ? g0 : kind == KA_K ? g0 - gq : g0 - gq - gk;
+        const int heads = kind == KA_Q ? a.H : a.Hkv, end = min(g1 - g0 + g, kind == KA_Q ? gq : gk);
+        const char *from = kind == KA_Q ? q : kind == KA_K ? k : v;
 #pragma unroll
-        for (int u = 0; u < KA_AHEAD; u++) {
-            const int h = (g + u) * HPI + sub;
-            if (on && g + u < g_end && h < heads) {
-                const char *s = h < a.H ? q + (size_t)h * a.D * SIZE : h < a.H + a.Hkv ? k + (size_t)(h - a.H) * a.D * SIZE : v + (size_t)(h - a.H - a.Hkv) * a.D * SIZE;
-                in[u][0] = *reinterpret_cast<const Quad *>(s + qa * SIZE);
-                in[u][1] = *reinterpret_cast<const Quad *>(s + qb * SIZE);
-            } else {
-                in[u][0] = in[u][1] = Quad();
+        for (int u = 0; u < N; u++) {
+            const int h = (g + u) * HPI + w.sub;
+            in[u][0] = in[u][1] = Quad();
+            if (w.on && h < heads && g + u < end) {
+                const char *s = from + (size_t)h * (a.D * SIZE);
+                in[u][0] = *reinterpret_cast<const Quad *>(s + w.qa * SIZE);
+                in[u][1] = *reinterpret_cast<const Quad *>(s + w.qb * SIZE);
             }
         }
-    };
-    fetch(g0);                                       // (rows that turn out to have no place are within the buffers, too)
-    float wq[8], wk[8];
-#pragma unroll
-    for (int i = 0; i < 8; i++) {
-        const int e = (i < 4 ? qa : qb - 4) + i;
-        wq[i] = p.q_norm && on ? p.q_norm[e] : 1.f;
-        wk[i] = p.k_norm && on ? p.k_norm[e] : 1.f;
     }
     const int seq = kv_find_seq(a, row, lane);
     if (seq < 0) return;                             // behind the last sequence: everything stays as it was
@@ -96,104 +210,52 @@ kv_append_kernel(const KvAppendArgs p, int parts, int per_part) {
     const int pos = s.len - s.n + (row - s.begin);
     if (pos < 0) return;                             // in front of the first position
     const int page = a.table[(size_t)seq * a.max_pages + (pos >> a.page_shift)], slot = pos & ((1 << a.page_shift) - 1);
-    float cs[4], sn[4];                              // of the lane's pairs: values (i, i + 4), or (2 i, 2 i + 1) where interleaved
-    if (p.rot) {
+    if (w.turns) {
+        float c4[4], s4[4];                          // of the lane's pairs: values (i, i + 4), or (2 i, 2 i + 1) where interleaved
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            cs[i] = 1.f; sn[i] = 0.f;
-            if (l * 8 < p.rot) {
-                double t = (double)pos * p.turns[4 * l + i];
-                t -= rint(t);
-                sincospif(2.f * (float)t, &sn[i], &cs[i]);
-            }
+            double t = (double)pos * p.turns[4 * l + i];
+            t -= rint(t);
+            sincospif(2.f * (float)t, &s4[i], &c4[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            w.cs[i] = make_float2(c4[2 * i], c4[2 * i + 1]);
+            w.sn[i] = make_float2(s4[2 * i], s4[2 * i + 1]);
+            w.nsn[i] = make_float2(-s4[2 * i], -s4[2 * i + 1]);
         }
     }
     if ((unsigned)page >= (unsigned)a.n_pages) {
         if (lane == 0) atomicExch(a.status, ST_PAGE);
         return;
     }
-    const size_t head_step = (size_t)a.D << a.page_shift, base = kv_row(a, page, 0, slot) * a.D;
-    char *out = static_cast<char *>(a.out) + row * a.ldo * SIZE;
-    const float top = FMT == KV_BF16 ? KA_BF16_MAX : H16_MAX, inv_d = 1.f / (float)a.D;
-    bool bad = false;
-    for (int g = g0; g < g_end; g += KA_AHEAD) {
-        if (g > g0) fetch(g);
-#pragma unroll
-        for (int u = 0; u < KA_AHEAD; u++) {
-            const int h = (g + u) * HPI + sub;
-            if (g + u >= g_end) break;               // the same for the whole warp
-            float x[8];
-            ka_open<FMT>(in[u][0], x);
-            ka_open<FMT>(in[u][1], x + 4);
-            const bool turns = h < a.H + a.Hkv;      // (v heads pass as they are)
-            if (p.q_norm || p.k_norm) {              // the same for the whole launch
-                float ss = 0.f;
-#pragma unroll
-                for (int i = 0; i < 8; i++) ss = fmaf(x[i], x[i], ss);
-#pragma unroll
-                for (int o = LPH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-                const float r = rsqrtf(fmaf(ss, inv_d, p.eps));
-                if (h < a.H ? p.q_norm != nullptr : turns && p.k_norm != nullptr) {
-#pragma unroll
-                    for (int i = 0; i < 8; i++) x[i] *= r * (h < a.H ? wq[i] : wk[i]);
-                }
-            }
-            if (p.rot && turns) {
-                if (p.interleaved) {
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const float c = x[2 * i], d = x[2 * i + 1];
-                        x[2 * i] = fmaf(c, cs[i], -d * sn[i]);
-                        x[2 * i + 1] = fmaf(c, sn[i], d * cs[i]);
-                    }
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const float c = x[i], d = x[i + 4];
-                        x[i] = fmaf(c, cs[i], -d * sn[i]);
-                        x[i + 4] = fmaf(c, sn[i], d * cs[i]);
-                    }
-                }
-            }
-            if (!on || h >= heads) continue;
-            if (h < a.H) {
-#pragma unroll
-                for (int i = 0; i < 8; i++) bad |= !(fabsf(x[i]) < (FMT == KV_F32 ? INFINITY : top));
-                char *to = out + (size_t)h * a.D * SIZE;
-                *reinterpret_cast<Quad *>(to + qa * SIZE) = ka_close<FMT>(x);
-                *reinterpret_cast<Quad *>(to + qb * SIZE) = ka_close<FMT>(x + 4);
-            } else {
-                // the cache holds finite values only: what a mask hides is multiplied by a probability of 0
-#pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    const bool fits = fabsf(x[i]) < top;
-                    bad |= !fits;
-                    x[i] = fits ? x[i] : 0.f;
-                }
-                uint16_t *to = (turns ? a.k : a.v) + base + (size_t)(h - a.H - (turns ? 0 : a.Hkv)) * head_step;
-                *reinterpret_cast<uint2 *>(to + qa) = ka_close<FMT == KV_BF16 ? KV_BF16 : KV_F16>(x);
-                *reinterpret_cast<uint2 *>(to + qb) = ka_close<FMT == KV_BF16 ? KV_BF16 : KV_F16>(x + 4);
-            }
-        }
+    const size_t step = (size_t)a.D << a.page_shift, base = kv_row(a, page, 0, slot) * a.D;
+    bool bad = false, fetched = true;
+    if (g0 < gq) {
+        bad |= ka_heads<FMT, LPH, KA_Q>(p, w, q, g0, min(g1, gq), a.H, static_cast<char *>(a.out) + row * a.ldo * SIZE, (size_t)a.D, in, fetched);
+        fetched = false;
     }
+    if (g0 < gq + gk && g1 > gq) {
+        bad |= ka_heads<FMT, LPH, KA_K>(p, w, k, max(g0 - gq, 0), min(g1 - gq, gk), a.Hkv, a.k + base, step, in, fetched);
+        fetched = false;
+    }
+    if (g1 > gq + gk) bad |= ka_heads<FMT, LPH, KA_V>(p, w, v, max(g0 - gq - gk, 0), min(g1 - gq - gk, gk), a.Hkv, a.v + base, step, in, fetched);
     if (bad) atomicExch(a.status, ST_RANGE);
 }
 
 template <int FMT>
 static int append_fmt(const KvAppendArgs &p, cudaStream_t st) {
     const KvArgs &a = p.a;
-    const int lph = a.D <= 16 ? 2 : a.D <= 32 ? 4 : a.D <= 64 ? 8 : 16;
-    const int groups = cdiv(a.H + 2 * a.Hkv, 32 / lph);
+    const int lph = a.D <= 16 ? 2 : a.D <= 32 ? 4 : a.D <= 64 ? 8 : 16, hpi = 32 / lph;
+    const int groups = cdiv(a.H, hpi) + 2 * cdiv(a.Hkv, hpi);
     // A warp takes a whole row where there are rows enough to fill the SMs (32 warps each), a part of one otherwise
     const int64_t want = 32ll * device_sm_count();
     int parts = (int)((want + a.n_rows - 1) / a.n_rows);
     if (parts > groups) parts = groups;
     const int per_part = cdiv(groups, parts);
     parts = cdiv(groups, per_part);
-    const int64_t blocks = ((int64_t)a.n_rows * parts + KA_WARPS - 1) / KA_WARPS;
-    if (blocks > 0x7fffffff) { set_error("kv_append: too many rows in one call"); return -1; }
     auto kernel = lph == 2 ? kv_append_kernel<FMT, 2> : lph == 4 ? kv_append_kernel<FMT, 4> : lph == 8 ? kv_append_kernel<FMT, 8> : kv_append_kernel<FMT, 16>;
-    MB_CUDA(launch_kernel(kernel, dim3((unsigned)blocks), dim3(KA_WARPS * 32), 0, st, true, 1, p, parts, per_part));
+    MB_CUDA(launch_kernel(kernel, dim3((unsigned)((a.n_rows - 1) / KA_WARPS + 1), (unsigned)parts), dim3(KA_WARPS * 32), 0, st, true, 1, p, per_part));
     note_launch();
     return 0;
 }
