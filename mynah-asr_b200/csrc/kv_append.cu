@@ -11,15 +11,9 @@
 // f64 and reduced there (a position of 10^6 times a frequency near 1 has no correct digit behind the point in f32), its sine and
 // cosine then in f32.
 #include "kv.h"
-#include <cuda_bf16.h>
 
 namespace mb {
 
-__device__ __forceinline__ uint32_t ka_pack(float x, float y, bool bf) {
-    if (bf) { const __nv_bfloat162 h = __floats2bfloat162_rn(x, y); return *reinterpret_cast<const uint32_t *>(&h); }
-    const __half2 h = __floats2half2_rn(x, y);
-    return *reinterpret_cast<const uint32_t *>(&h);
-}
 __device__ __forceinline__ float2 ka_unpack(uint32_t u, bool bf) {
     if (bf) return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162 *>(&u));
     return __half22float2(*reinterpret_cast<const __half2 *>(&u));
@@ -38,27 +32,12 @@ __device__ __forceinline__ void ka_open(const typename KaQuad<FMT>::type &r, flo
 template <int FMT>
 __device__ __forceinline__ typename KaQuad<FMT>::type ka_close(const float *v) {
     if constexpr (FMT == KV_F32) return make_float4(v[0], v[1], v[2], v[3]);
-    else return make_uint2(ka_pack(v[0], v[1], FMT == KV_BF16), ka_pack(v[2], v[3], FMT == KV_BF16));
+    else return make_uint2(kv_pack<FMT == KV_BF16>(v[0], v[1]), kv_pack<FMT == KV_BF16>(v[2], v[3]));
 }
 
 static constexpr int KA_WARPS = 8;
 // The largest magnitude that a cache value may have: beyond it a bf16 would round to infinity; f16 as the operand planes
 static constexpr float KA_BF16_MAX = 3.3895313e38f;
-
-// Two f32 operations in one instruction
-__device__ __forceinline__ float2 ka_fma(float2 a, float2 b, float2 c) {
-    float2 d;
-    asm("{\n\t.reg .b64 ra, rb, rc, rd;\n\tmov.b64 ra, {%2, %3};\n\tmov.b64 rb, {%4, %5};\n\tmov.b64 rc, {%6, %7};\n\t"
-        "fma.rn.f32x2 rd, ra, rb, rc;\n\tmov.b64 {%0, %1}, rd;\n\t}"
-        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
-    return d;
-}
-__device__ __forceinline__ float2 ka_mul(float2 a, float2 b) {
-    float2 d;
-    asm("{\n\t.reg .b64 ra, rb, rd;\n\tmov.b64 ra, {%2, %3};\n\tmov.b64 rb, {%4, %5};\n\tmul.rn.f32x2 rd, ra, rb;\n\tmov.b64 {%0, %1}, rd;\n\t}"
-        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-    return d;
-}
 
 enum { KA_Q, KA_K, KA_V };
 // What a lane knows of its row: where its quads begin, cosines and sines of its pairs, the row's slot
@@ -108,15 +87,15 @@ __device__ __forceinline__ bool ka_heads(const KvAppendArgs &p, const KaLane &w,
             ka_open<FMT>(in[u][0], reinterpret_cast<float *>(x));
             ka_open<FMT>(in[u][1], reinterpret_cast<float *>(x + 2));
             if (KIND != KA_V && norm) {              // the same for the whole launch
-                float2 s2 = ka_mul(x[0], x[0]);
+                float2 s2 = kv_mul2(x[0], x[0]);
 #pragma unroll
-                for (int i = 1; i < 4; i++) s2 = ka_fma(x[i], x[i], s2);
+                for (int i = 1; i < 4; i++) s2 = kv_fma2(x[i], x[i], s2);
                 float ss = s2.x + s2.y;
 #pragma unroll
                 for (int o = LPH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
                 const float r = rsqrtf(fmaf(ss, inv_d, p.eps));
 #pragma unroll
-                for (int i = 0; i < 4; i++) x[i] = ka_mul(ka_mul(x[i], wt[i]), make_float2(r, r));
+                for (int i = 0; i < 4; i++) x[i] = kv_mul2(kv_mul2(x[i], wt[i]), make_float2(r, r));
             }
             if (KIND != KA_V && w.turns) {
                 if (p.interleaved) {
@@ -130,8 +109,8 @@ __device__ __forceinline__ bool ka_heads(const KvAppendArgs &p, const KaLane &w,
 #pragma unroll
                     for (int i = 0; i < 2; i++) {
                         const float2 b = x[i];
-                        x[i] = ka_fma(b, w.cs[i], ka_mul(x[i + 2], w.nsn[i]));
-                        x[i + 2] = ka_fma(b, w.sn[i], ka_mul(x[i + 2], w.cs[i]));
+                        x[i] = kv_fma2(b, w.cs[i], kv_mul2(x[i + 2], w.nsn[i]));
+                        x[i + 2] = kv_fma2(b, w.sn[i], kv_mul2(x[i + 2], w.cs[i]));
                     }
                 }
             }

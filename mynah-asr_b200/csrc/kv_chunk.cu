@@ -4,39 +4,49 @@
 // Bound by the tensor cores and, as much, by the exponentials (4 D operations and one exponential per pair of row and key). A CTA
 // owns one kv head and two tiles of 128 rows: the G query heads of 128 / G positions each (row r is head r % G of position r / G), so
 // that short pieces fill a tile and all heads share the keys' tiles. Keys and values come in tiles of 128 by TMA, from their pages
-// straight into the swizzled operand layout.
-//   tensor memory  S0, S1: scores of the two tiles (128 columns each; the probabilities overwrite them as 16-bit operands),
-//                  O0, O1: results (D columns each)
+// straight into the swizzled operand layout; of a tile at the edge of what is visible only the groups of 16 keys that some row sees
+// are computed.
+//   tensor memory  S0, S1: scores of the two tiles (128 columns each), O0, O1: results; the probabilities, as 16-bit operands, overwrite
+//                  the scores, or have columns of their own where D <= 64 leaves room (then S(i + 1) is computed under the exponentials
+//                  of tile i)
 //   warps          0-3 and 4-7: softmax of tile 0 and 1, a thread per row; 8: TMA; 9: MMA
 //   order of MMAs  P0 V(i), S0(i + 1), P1 V(i), S1(i + 1): one tile's exponentials run under the other's products. MMAs run in the
 //                  order of their issue, so S(i + 1) does not overwrite the P(i) that P V(i) reads, and whoever sees S(i + 1) finished
-//                  finds O at rest.
+//                  finds O at rest. With columns of their own for P: S0(i + 1), S1(i + 1), P0 V(i), P1 V(i).
 // The softmax keeps a running maximum per row; O is rescaled only when it has grown by more than 2^8 (what is stale cancels in the
 // final division). F32 rows: queries and probabilities as (hi, lo) f16 pairs, two products each.
+// A call with few blocks is launched as clusters: the CTAs of a cluster take a block's tiles in turn, two at least each, and join their
+// results through distributed shared memory.
 #include "kv.h"
-#include <cuda_bf16.h>
+#include <stdlib.h>
 
 namespace mb {
 
 static constexpr int KC_ROWS = 128, KC_KEYS = 128, KC_HALF = 128 * 128;      // a 128-row x 64-column box of 16-bit values: 16 KB
-static constexpr int KC_SOFT = 8, KC_W_TMA = 8, KC_W_MMA = 9, KC_THREADS = 320;
 static constexpr int KC_HEAD = 1024;
 static constexpr int KC_PART = 6;                    // P V begins when the first 6 x 16 keys' probabilities are there
 static constexpr float KC_NONE = -1e30f;             // "maximum" of no keys
 
 template <int DP, int FMT> struct ChunkShape {
     static constexpr int HALVES = DP / 64, PLANES = FMT == KV_F32 ? 2 : 1;
+    static constexpr int TILES = DP == 64 ? 1 : 2, PER_SM = DP == 64 ? 2 : 1;          // tiles of rows of a CTA, CTAs of an SM
+    static constexpr int SOFT = 4 * TILES, W_TMA = SOFT, W_MMA = SOFT + 1;             // warps
+    static constexpr int THREADS = TILES == 2 ? 384 : 192;     // (warps 10 and 11 of twelve lend their registers)
     static constexpr int OPERAND = HALVES * KC_HALF;           // a tile of queries (one plane), of keys, or of values
-    static constexpr int Q = 2 * PLANES * OPERAND;
-    static constexpr int STAGES = DP == 64 ? 6 : PLANES == 1 ? 5 : 3;
+    static constexpr int Q = TILES * PLANES * OPERAND;
+    static constexpr int STAGES = DP == 64 ? 6 - PLANES : PLANES == 1 ? 5 : 3;
     static constexpr int SMEM = KC_HEAD + Q + STAGES * OPERAND + 1024;
-    static_assert(SMEM <= 232448, "shared memory");
-    static constexpr int COL_S = 0, COL_O = 256;
+    static_assert(PER_SM * (SMEM + 1024) <= 233472, "shared memory");
+    static constexpr bool OWN_P = DP == 64 && PLANES == 1;     // columns of their own for the probabilities
+    static constexpr int COL_S = 0, COL_P = OWN_P ? 128 * TILES : 0, STEP_P = OWN_P ? 64 : 128, COL_O = 128 * TILES + (OWN_P ? 64 * TILES : 0);
+    static constexpr int TMEM = 512 / PER_SM;
+    static_assert(COL_O + TILES * DP <= TMEM, "tensor memory");
+    static constexpr int LDO = DP + 4;                         // a part of a row's result in shared memory
+    static_assert(TILES * 128 * (LDO * 4 + 8 + 64) <= Q + STAGES * OPERAND, "parts");
 };
 
 struct KcPlace { int seq, block; };
 
-__device__ __forceinline__ void kc_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) { tc_mma_f16(d, a, b, idesc, acc); }
 __device__ __forceinline__ void kc_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
@@ -58,25 +68,6 @@ __device__ __forceinline__ void kc_st8(uint32_t taddr, const uint32_t *r) {
         ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]) : "memory");
 }
 __device__ __forceinline__ void kc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ float kc_ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-// Two f32 operations in one instruction
-__device__ __forceinline__ float2 kc_fma2(float2 a, float2 b, float2 c) {
-    float2 d;
-    asm("{\n\t.reg .b64 ra, rb, rc, rd;\n\tmov.b64 ra, {%2, %3};\n\tmov.b64 rb, {%4, %5};\n\tmov.b64 rc, {%6, %7};\n\t"
-        "fma.rn.f32x2 rd, ra, rb, rc;\n\tmov.b64 {%0, %1}, rd;\n\t}"
-        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
-    return d;
-}
-__device__ __forceinline__ float2 kc_add2(float2 a, float2 b) {
-    float2 d;
-    asm("{\n\t.reg .b64 ra, rb, rd;\n\tmov.b64 ra, {%2, %3};\n\tmov.b64 rb, {%4, %5};\n\tadd.rn.f32x2 rd, ra, rb;\n\tmov.b64 {%0, %1}, rd;\n\t}"
-        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-    return d;
-}
 // Waits for loads from tensor memory; the values that they bring are not to be touched before (nor their use moved up)
 __device__ __forceinline__ void kc_wait_ld32(float *x) {
     asm volatile("tcgen05.wait::ld.sync.aligned;"
@@ -85,20 +76,11 @@ __device__ __forceinline__ void kc_wait_ld32(float *x) {
                    "+f"(x[21]), "+f"(x[22]), "+f"(x[23]), "+f"(x[24]), "+f"(x[25]), "+f"(x[26]), "+f"(x[27]), "+f"(x[28]), "+f"(x[29]), "+f"(x[30]), "+f"(x[31])
                  :: "memory");
 }
-template <bool BF>
-__device__ __forceinline__ uint32_t kc_pack(float x, float y) {
-    if (BF) { const __nv_bfloat162 h = __floats2bfloat162_rn(x, y); return *reinterpret_cast<const uint32_t *>(&h); }
-    const __half2 h = __floats2half2_rn(x, y);
-    return *reinterpret_cast<const uint32_t *>(&h);
-}
-// x, y as f16 pairs: hi and what it leaves, unscaled: both products go into one accumulator
-__device__ __forceinline__ void kc_split(float x, float y, uint32_t &hi, uint32_t &lo) {
-    const __half2 h = __floats2half2_rn(x, y);
-    const float2 f = __half22float2(h);
-    const __half2 l = __floats2half2_rn(x - f.x, y - f.y);
-    hi = *reinterpret_cast<const uint32_t *>(&h);
-    lo = *reinterpret_cast<const uint32_t *>(&l);
-}
+// The registers of the launch, KC_REGS a thread, are dealt out anew: 2 x 128 threads with 208 and 128 with 88 are 384 with 168.
+static constexpr int KC_REGS = 168, KC_REGS_MORE = 208, KC_REGS_LESS = 88;
+static_assert(256 * KC_REGS_MORE + 128 * KC_REGS_LESS <= 384 * KC_REGS, "a share beyond the launch's registers waits for good");
+__device__ __forceinline__ void kc_regs_more() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(KC_REGS_MORE)); }
+__device__ __forceinline__ void kc_regs_less() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(KC_REGS_LESS)); }
 // Instruction descriptor: f32 accumulators, A and B both f16 (or both bf16: formats 1 << 7 and 1 << 10), M x N
 __host__ __device__ constexpr uint32_t kc_idesc(bool bf, int N) { return umma_idesc_f16(KC_ROWS, N) | (bf ? (1u << 7) | (1u << 10) : 0u); }
 // B operand [keys][D] with D contiguous: eight-key groups 1024 bytes apart, 64-wide blocks of D one half apart
@@ -142,16 +124,16 @@ __device__ __forceinline__ bool kc_place(const KvArgs &a, int x, int per_block, 
 }
 
 template <int DP, int FMT>
-__global__ void __launch_bounds__(KC_THREADS, 1)
-kv_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const KvArgs a, int box_rows) {
+__global__ void __launch_bounds__(ChunkShape<DP, FMT>::THREADS, ChunkShape<DP, FMT>::PER_SM)
+kv_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const KvArgs a, int box_rows, int log_size) {
     using Sh = ChunkShape<DP, FMT>;
-    constexpr bool BF = FMT == KV_BF16, F32 = FMT == KV_F32;
-    constexpr int STAGES = Sh::STAGES;
+    constexpr bool BF = FMT == KV_BF16, F32 = FMT == KV_F32, OWN_P = Sh::OWN_P;
+    constexpr int STAGES = Sh::STAGES, TILES = Sh::TILES;
     extern __shared__ uint8_t kc_raw[];
     uint8_t *head = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(kc_raw) + 1023) & ~uintptr_t(1023));
     uint8_t *qst = head + KC_HEAD, *ring = qst + Sh::Q;
     uint64_t *full = reinterpret_cast<uint64_t *>(head), *empty = full + STAGES, *q_full = empty + STAGES, *s_full = q_full + 1,
-             *p_part = s_full + 2, *p_full = p_part + 2, *o_full = p_full + 2, *drain = o_full + 2;
+             *s_free = s_full + 2, *p_part = s_free + 2, *p_full = p_part + 2, *o_full = p_full + 2, *drain = o_full + 2;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(drain + 1);
     volatile int *place = reinterpret_cast<volatile int *>(tmem_slot + 1);
     const int warp = warp_index(), lane = threadIdx.x & 31;
@@ -159,52 +141,82 @@ kv_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
     chain_trigger();
     chain_wait();
     const int tq = KC_ROWS / a.G;                              // positions of a tile
+    const uint32_t inv_g = (65536u + a.G - 1) / a.G;           // x / G = x inv_g / 2^16 for x < 1024, G <= 64
+    auto by_g = [&](int x) { return (int)(((uint32_t)x * inv_g) >> 16); };
+    const int size = 1 << log_size, rank = (int)blockIdx.x & (size - 1);
     if (warp == 0) {
         KcPlace at = {-1, 0};
-        if (!kc_place(a, (int)blockIdx.x, 2 * tq, lane, &at)) at.seq = -1;
+        if (!kc_place(a, (int)(blockIdx.x >> log_size), TILES * tq, lane, &at)) at.seq = -1;
         if (lane == 0) { place[0] = at.seq; place[1] = at.block; }
     }
     if (threadIdx.x == 32) {
         tma_prefetch_desc(&tmK); tma_prefetch_desc(&tmV);
         for (int s = 0; s < STAGES; s++) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
-        mbar_init(q_full, KC_SOFT);
-        for (int t = 0; t < 2; t++) { mbar_init(&s_full[t], 1); mbar_init(&p_part[t], KC_SOFT / 2); mbar_init(&p_full[t], KC_SOFT / 2); mbar_init(&o_full[t], 1); }
+        mbar_init(q_full, Sh::SOFT);
+        for (int t = 0; t < TILES; t++) {
+            mbar_init(&s_full[t], 1); mbar_init(&o_full[t], 1);
+            mbar_init(&s_free[t], 4); mbar_init(&p_part[t], 4); mbar_init(&p_full[t], 4);
+        }
         mbar_init(drain, 1);
         mbar_fence_init();
     }
-    __syncthreads();
-    const int seq = place[0], block = place[1];
-    if (seq < 0) return;                                       // the whole CTA
-    if (warp == KC_W_MMA) { tc_alloc(tmem_slot, 512); tc_relinquish(); }
+    if (warp == Sh::W_MMA) { tc_alloc(tmem_slot, Sh::TMEM); tc_relinquish(); }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
+    // (one lane's values for all, so that the compiler keeps them and what follows from them in uniform registers)
+    auto same = [](int v) { return __shfl_sync(0xffffffffu, v, 0); };
+    const int seq = same(place[0]), block = same(place[1]);
 
-    KvSeq sq;
-    kv_seq(a.row_off, a.kv_len, seq, a.n_rows, kv_capacity(a), &sq);
-    const int kvh = blockIdx.y, t0 = block * 2 * tq;           // first position's place among the sequence's rows
+    KvSeq sq = {0, 0, 0};
+    if (seq >= 0) kv_seq(a.row_off, a.kv_len, seq, a.n_rows, kv_capacity(a), &sq);
+    sq.begin = same(sq.begin); sq.n = same(sq.n); sq.len = same(sq.len);
+    const int kvh = blockIdx.y, t0 = block * TILES * tq;          // first position's place among the sequence's rows
     const int base_pos = sq.len - sq.n;
-    const int last = min(t0 + 2 * tq, sq.n) - 1;
-    const KvTiles tiles = kv_tiles(base_pos + t0 > 0 ? base_pos + t0 : 0, base_pos + last, a.window, a.sinks, KC_KEYS);
-    const int n = tiles.count;
+    const int last = min(t0 + TILES * tq, sq.n) - 1;
+    const int top = base_pos + last, low = base_pos + t0 - a.window + 1;     // last key that any row sees; first that a window shows
+    KvTiles tiles = {0, 0, 0};
+    if (seq >= 0) tiles = kv_tiles(base_pos + t0 > 0 ? base_pos + t0 : 0, top, a.window, a.sinks, KC_KEYS);
+    // CTAs that share the block: two tiles each at least, by the block's own tiles
+    const int shares = min(size, tiles.count < 4 ? 1 : 1 << (30 - __clz(tiles.count)));
+    const int n = rank < shares ? (tiles.count - rank + shares - 1) / shares : 0;
+    const int nt = TILES == 2 && t0 + tq <= last ? 2 : 1;                    // tiles that have rows
+    auto tile_at = [&](int i) { return tiles.at(rank + i * shares) * KC_KEYS; };       // first key of this CTA's i-th tile
+    // its groups of 16 keys [lo, hi) that some row sees
+    auto groups = [&](int j0, int *lo, int *hi) {
+        *lo = 0;
+        *hi = min(8, ((top - j0) >> 4) + 1);
+        if (a.window > 0) {
+            if (j0 + KC_KEYS <= low) *hi = min(*hi, (a.sinks - j0 + 15) >> 4);         // a tile of the first tokens
+            else if (low > j0 && a.sinks <= j0) *lo = (low - j0) >> 4;
+        }
+    };
 
-    if (warp == KC_W_TMA) {
+    // row of a softmax thread, in tile t
+    const int t = TILES == 2 ? (warp >> 2) & 1 : 0, r = (warp & 3) * 32 + lane;
+    const int tok = t0 + t * tq + by_g(r);
+    const bool soft = warp < Sh::SOFT;
+    const uint32_t trow = tmem + ((uint32_t)((warp & 3) * 32) << 16), s_at = trow + Sh::COL_S + t * 128, p_at = trow + Sh::COL_P + t * Sh::STEP_P,
+                   o_at = trow + Sh::COL_O + t * DP;
+    float m = KC_NONE, l = 0.f;                                // of the row: running maximum and sum
+    if (!soft) {
+    if (TILES == 2) kc_regs_less();                            // (one instruction for the four warps)
+    if (warp == Sh::W_TMA) {
         // ---- lane = one box of a tile: 64 of the D columns, the slots of one page. Item 2 i of the ring is K(i), 2 i + 1 V(i).
         const int shift = a.page_shift, boxes = KC_KEYS / box_rows * Sh::HALVES;
         const int b_half = lane % Sh::HALVES, b_sub = lane / Sh::HALVES;
         const uint32_t b_at = b_half * KC_HALF + b_sub * box_rows * 128;
-        const int top = base_pos + last, low = base_pos + t0;  // what the CTA's rows see between them
-        auto seen = [&](int j) { return j <= top && (a.window <= 0 || j + box_rows - 1 > low - a.window || j < a.sinks); };
+        auto seen = [&](int j) { return j <= top && (a.window <= 0 || j + box_rows - 1 >= low || j < a.sinks); };
         auto entry_of = [&](int i) -> int {
-            const int j = tiles.at(i) * KC_KEYS + b_sub * box_rows;
+            const int j = tile_at(i) + b_sub * box_rows;
             return lane < boxes && i < n && seen(j) ? a.table[(size_t)seq * a.max_pages + (j >> shift)] : -1;
         };
         int entry = entry_of(0), s = 0, ph = 0, r = 0;
         bool ok = true;
         for (int i = 0; i < n && ok; i++) {
             const int next = entry_of(i + 1);
-            const int j = tiles.at(i) * KC_KEYS + b_sub * box_rows;
+            const int j = tile_at(i) + b_sub * box_rows;
             if (lane < boxes && (unsigned)entry >= (unsigned)a.n_pages) {
                 if (seen(j)) atomicExch(a.status, ST_PAGE);
                 entry = 0;                                     // any finite rows do
@@ -226,30 +238,43 @@ kv_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
             if (s == 0) { s = STAGES; ph ^= 1; }
             if (!mbar_wait_warp(&full[--s], (uint32_t)ph)) break;
         }
-    } else if (warp == KC_W_MMA) {
-        const uint32_t idesc_s = kc_idesc(BF, KC_KEYS), idesc_o = kc_idesc(BF, a.D) | (1u << 16);       // V: MN-major
+    } else if (warp == Sh::W_MMA) {
+        const uint32_t idesc_o = kc_idesc(BF, a.D) | (1u << 16);       // V: MN-major
         const uint64_t qdesc = umma_desc_sw128(smem_u32(qst)), kdesc = umma_desc_sw128(smem_u32(ring)), vdesc = kc_desc_mn(smem_u32(ring));
         const int steps = a.D / 16;
-        bool ok = n > 0 ? mbar_wait_warp(q_full, 0) : true;
-        auto issue_s = [&](int t, int s) {                     // by one lane
+        auto issue_s = [&](int t, int s, int hi) {             // by one lane: the scores of the first 16 hi keys
             const uint64_t kd = kdesc + (uint64_t)((s * Sh::OPERAND) >> 4);
+            const uint32_t idesc = kc_idesc(BF, 16 * hi);
+#pragma unroll
             for (int plane = 0; plane < Sh::PLANES; plane++) {
                 const uint64_t qd = qdesc + (uint64_t)(((t * Sh::PLANES + plane) * Sh::OPERAND) >> 4);
 #pragma unroll
                 for (int kk = 0; kk < DP / 16; kk++) {
                     const uint64_t ko = (uint64_t)(((kk >> 2) * KC_HALF + (kk & 3) * 32) >> 4);
-                    if (kk < steps) kc_mma(tmem + Sh::COL_S + t * 128, qd + ko, kd + ko, idesc_s, (kk | plane) != 0);
+                    if (kk < steps) tc_mma_f16(tmem + Sh::COL_S + t * 128, qd + ko, kd + ko, idesc, (kk | plane) != 0);
                 }
             }
         };
-        auto issue_o = [&](int t, int s, bool first, int k0, int k1) {
+        // group kk of P V; group `start` of the first tile begins the sum
+        auto issue_o1 = [&](int t, uint64_t vd, int kk, int start) {
+#pragma unroll
+            for (int plane = 0; plane < Sh::PLANES; plane++)
+                kc_mma_ts(tmem + Sh::COL_O + t * DP, tmem + Sh::COL_P + t * Sh::STEP_P + plane * 64 + 8 * kk, vd + (uint64_t)((kk * 2048) >> 4), idesc_o,
+                          kk != start || plane != 0);
+        };
+        // part 0: the groups in front of KC_PART, part 1: the others
+        auto issue_o = [&](int t, int s, int part, int lo, int hi, int start) {
             const uint64_t vd = vdesc + (uint64_t)((s * Sh::OPERAND) >> 4);
+            if (lo == 0 && hi == 8) {
+                if (part == 0) {
 #pragma unroll
-            for (int plane = 0; plane < Sh::PLANES; plane++) {
+                    for (int kk = 0; kk < KC_PART; kk++) issue_o1(t, vd, kk, start);
+                } else {
 #pragma unroll
-                for (int kk = k0; kk < k1; kk++)
-                    kc_mma_ts(tmem + Sh::COL_O + t * DP, tmem + Sh::COL_S + t * 128 + plane * 64 + 8 * kk, vd + (uint64_t)((kk * 2048) >> 4), idesc_o,
-                              !first || (kk | plane) != 0);
+                    for (int kk = KC_PART; kk < 8; kk++) issue_o1(t, vd, kk, start);
+                }
+            } else {
+                for (int kk = max(lo, part * KC_PART); kk < (part ? hi : min(hi, KC_PART)); kk++) issue_o1(t, vd, kk, start);
             }
         };
         int s = 0, ph = 0;                                     // ring place of the next item
@@ -259,12 +284,13 @@ kv_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
             if (++s == STAGES) { s = 0; ph ^= 1; }
             return got;
         };
-        int sk = 0, sv = 0;
+        bool ok = n > 0 ? mbar_wait_warp(q_full, 0) : true;
+        int sk = 0, sv = 0, lo = 0, hi = 8;
+        if (n > 0) groups(tile_at(0), &lo, &hi);
         if (ok && n > 0 && (ok = take(&sk))) {
             tc_fence_after();
             if (elect_one()) {
-                issue_s(0, sk); tc_commit(&s_full[0]);
-                issue_s(1, sk); tc_commit(&s_full[1]);
+                for (int t = 0; t < nt; t++) { issue_s(t, sk, hi); tc_commit(&s_full[t]); }
                 tc_commit(&empty[sk]);
             }
             __syncwarp();
@@ -274,24 +300,39 @@ kv_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
         // products are still under way.
         for (int i = 0; i < n && ok; i++) {
             const bool more = i + 1 < n;
-            const int v = sv;
-#pragma unroll
-            for (int t = 0; t < 2; t++) {
+            const int v = sv, start = i == 0 ? lo : -1;
+            int lo2 = 0, hi2 = 8;
+            if (more) groups(tile_at(i + 1), &lo2, &hi2);
+            if (OWN_P && more) {
+                ok = take(&sk);
+                for (int t = 0; t < nt && ok; t++) {
+                    if (!mbar_wait_warp(&s_free[t], (uint32_t)(i & 1))) { ok = false; break; }
+                    tc_fence_after();
+                    if (elect_one()) {
+                        issue_s(t, sk, hi2); tc_commit(&s_full[t]);
+                        if (t == nt - 1) tc_commit(&empty[sk]);
+                    }
+                    __syncwarp();
+                }
+            }
+            for (int t = 0; t < nt && ok; t++) {
                 if (!mbar_wait_warp(&p_part[t], (uint32_t)(i & 1))) { ok = false; break; }
                 tc_fence_after();
-                if (elect_one()) issue_o(t, v, i == 0, 0, KC_PART);
+                if (elect_one()) issue_o(t, v, 0, lo, hi, start);
                 __syncwarp();
-                if (more && !take(t == 0 ? &sk : &sv)) { ok = false; break; }      // K(i + 1), V(i + 1)
+                if (more && !OWN_P && t == 0 && !take(&sk)) { ok = false; break; }     // K(i + 1)
+                if (more && t == nt - 1 && !take(&sv)) { ok = false; break; }          // V(i + 1)
                 if (!mbar_wait_warp(&p_full[t], (uint32_t)(i & 1))) { ok = false; break; }
                 tc_fence_after();
                 if (elect_one()) {
-                    issue_o(t, v, i == 0, KC_PART, KC_KEYS / 16);
-                    if (more) { issue_s(t, sk); tc_commit(&s_full[t]); }
-                    else tc_commit(&o_full[t]);
-                    if (t == 1) { tc_commit(&empty[v]); if (more) tc_commit(&empty[sk]); }
+                    issue_o(t, v, 1, lo, hi, start);
+                    if (OWN_P || !more) tc_commit(&o_full[t]);
+                    if (more && !OWN_P) { issue_s(t, sk, hi2); tc_commit(&s_full[t]); }
+                    if (t == nt - 1) { tc_commit(&empty[v]); if (more && !OWN_P) tc_commit(&empty[sk]); }
                 }
                 __syncwarp();
             }
+            lo = lo2; hi = hi2;
         }
         if (!ok) {                                             // nothing may run on when tensor memory is given back
             if (lane == 0) atomicExch(a.status, ST_TIMEOUT_MMA);
@@ -299,54 +340,65 @@ kv_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
             __syncwarp();
             mbar_wait_warp(drain, 0);
         }
+    }
     } else {
-        // ---- softmax: thread = row of tile t
-        const int t = warp >> 2, r = (warp & 3) * 32 + lane;
-        const int tok = t0 + t * tq + r / a.G, h = kvh * a.G + r % a.G;
-        const bool valid = r < tq * a.G && tok < sq.n;
-        // rows that do not exist take the last one's position, so that they need no mask of their own
-        const int pos = base_pos + min(r < tq * a.G ? tok : t0 + t * tq, sq.n - 1);
-        const uint32_t trow = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-        if (n > 0) {
-            uint8_t *qt = qst + t * Sh::PLANES * Sh::OPERAND + r * 128;
-            const int64_t at = (int64_t)(sq.begin + tok) * a.ldq + (int64_t)h * a.D;
-            bool bad = false;
-#pragma unroll 4
-            for (int c = 0; c < DP / 8; c++) {
-                const uint32_t to = (c >> 3) * KC_HALF + (((c & 7) ^ (r & 7)) << 4);
-                const bool on = valid && c * 8 < a.D;
-                if (F32) {
-                    float4 x = make_float4(0.f, 0.f, 0.f, 0.f), y = x;
-                    if (on) {
-                        const float4 *p = reinterpret_cast<const float4 *>(static_cast<const float *>(a.q) + at + c * 8);
-                        x = p[0]; y = p[1];
+    // ---- softmax: thread = row
+    if (TILES == 2) kc_regs_more();
+    if (n > 0) {
+        // the warp's 32 rows, neighbouring lanes on neighbouring pieces of eight values; all reads under way at once
+        constexpr int PIECES = DP / 8, ROWS = 32 / PIECES, ROUNDS = 32 / ROWS, BATCH = F32 && ROUNDS > 8 ? 8 : ROUNDS;
+        uint8_t *qt = qst + t * Sh::PLANES * Sh::OPERAND;
+        const int c = lane % PIECES;
+        bool bad = false;
+        if (t < nt) {
+#pragma unroll
+            for (int b = 0; b < ROUNDS; b += BATCH) {
+                uint4 in[BATCH][F32 ? 2 : 1];
+#pragma unroll
+                for (int i = 0; i < BATCH; i++) {
+                    const int row = (warp & 3) * 32 + (b + i) * ROWS + lane / PIECES, pl = by_g(row), at = t0 + t * tq + pl;
+                    in[i][0] = make_uint4(0, 0, 0, 0);
+                    if (F32) in[i][F32 ? 1 : 0] = make_uint4(0, 0, 0, 0);
+                    if (row < tq * a.G && at < sq.n && c * 8 < a.D) {
+                        const int64_t from = (int64_t)(sq.begin + at) * a.ldq + (int64_t)(kvh * a.G + row - pl * a.G) * a.D + c * 8;
+                        const uint4 *p = reinterpret_cast<const uint4 *>(static_cast<const uint8_t *>(a.q) + from * (F32 ? 4 : 2));
+                        in[i][0] = p[0];
+                        if (F32) in[i][F32 ? 1 : 0] = p[1];
                     }
-                    bad |= !(fabsf(x.x) < H16_MAX) | !(fabsf(x.y) < H16_MAX) | !(fabsf(x.z) < H16_MAX) | !(fabsf(x.w) < H16_MAX) |
-                           !(fabsf(y.x) < H16_MAX) | !(fabsf(y.y) < H16_MAX) | !(fabsf(y.z) < H16_MAX) | !(fabsf(y.w) < H16_MAX);
-                    uint4 hi, lo;
-                    kc_split(x.x, x.y, hi.x, lo.x); kc_split(x.z, x.w, hi.y, lo.y); kc_split(y.x, y.y, hi.z, lo.z); kc_split(y.z, y.w, hi.w, lo.w);
-                    *reinterpret_cast<uint4 *>(qt + to) = hi;
-                    *reinterpret_cast<uint4 *>(qt + Sh::OPERAND + to) = lo;
-                } else {
-                    uint4 x = make_uint4(0, 0, 0, 0);
-                    if (on) x = *reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(a.q) + at + c * 8);
-                    *reinterpret_cast<uint4 *>(qt + to) = x;
+                }
+#pragma unroll
+                for (int i = 0; i < BATCH; i++) {
+                    const int row = (warp & 3) * 32 + (b + i) * ROWS + lane / PIECES;
+                    uint8_t *to = qt + (c >> 3) * KC_HALF + row * 128 + (((c & 7) ^ (row & 7)) << 4);
+                    if (F32) {
+                        const float *f = reinterpret_cast<const float *>(in[i]);
+                        uint4 hi, lo;
+#pragma unroll
+                        for (int e = 0; e < 8; e++) bad |= !(fabsf(f[e]) < H16_MAX);
+                        kv_split(f[0], f[1], hi.x, lo.x); kv_split(f[2], f[3], hi.y, lo.y); kv_split(f[4], f[5], hi.z, lo.z); kv_split(f[6], f[7], hi.w, lo.w);
+                        *reinterpret_cast<uint4 *>(to) = hi;
+                        *reinterpret_cast<uint4 *>(to + Sh::OPERAND) = lo;
+                    } else {
+                        *reinterpret_cast<uint4 *>(to) = in[i][0];
+                    }
                 }
             }
             if (bad) atomicExch(a.status, ST_RANGE);
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");       // generic-proxy stores -> visible to the tensor core
-            __syncwarp();
-            if (lane == 0) mbar_arrive(q_full);
         }
-        const float sc = a.scale * 1.4426950408889634f;
-        float m = KC_NONE;
-        float2 l2[2] = {{0.f, 0.f}, {0.f, 0.f}};
+        __syncwarp();
+        if (lane == 0) mbar_arrive(q_full);
+    }
+    if (t < nt) {
         bool ok = true;
+        // rows that do not exist take the last one's position, so that they need no mask of their own
+        const int pos = base_pos + min(r < tq * a.G ? tok : t0 + t * tq, sq.n - 1);
+        const float sc = a.scale * 1.4426950408889634f;
+        float2 l2[2] = {{0.f, 0.f}, {0.f, 0.f}};
         for (int i = 0; i < n && ok; i++) {
             if (!mbar_wait_warp(&s_full[t], (uint32_t)(i & 1))) { ok = false; break; }
             tc_fence_after();
             float x[KC_KEYS];
-            const uint32_t s_at = trow + Sh::COL_S + t * 128;
             tc_ld32(s_at, x);
             tc_ld32(s_at + 32, x + 32);
             kc_wait_ld32(x); kc_wait_ld32(x + 32);
@@ -360,106 +412,217 @@ kv_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
 #pragma unroll
             for (int e = 0; e < 4; e++) m4[e] = fmaxf(m4[e], x[60 + e]);
             kc_wait_ld32(x + 64); kc_wait_ld32(x + 96);
+            if (OWN_P) {                                       // the scores are in registers
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&s_free[t]);
+            }
 #pragma unroll
             for (int c = 64; c < 128; c += 8)
 #pragma unroll
                 for (int e = 0; e < 4; e++) m4[e] = fmaxf(m4[e], fmaxf(x[c + e], x[c + 4 + e]));
-            const int j0 = tiles.at(i) * KC_KEYS, d = pos - j0;
+            const int j0 = tile_at(i), d = pos - j0;
             const bool whole = d >= KC_KEYS - 1 && (a.window <= 0 || d < a.window || j0 + KC_KEYS - 1 < a.sinks);
-            if (!__all_sync(0xffffffffu, whole)) {
-                const int low = a.window > 0 ? d - a.window : -1, keep = a.sinks - j0;       // hidden: above d; up to low, from keep on
+            const bool all = __all_sync(0xffffffffu, whole);
+            if (!all) {                                        // (columns that have no scores are hidden, too)
+                // a bit per column: visible up to d, above `under`, or below `keep`
+                const int under = a.window > 0 ? d - a.window : -1, keep = a.sinks - j0;
+                auto upto = [](int c) -> uint32_t { return c < 0 ? 0u : c >= 31 ? 0xffffffffu : (2u << c) - 1u; };      // bits 0 to c
                 m4[0] = m4[1] = m4[2] = m4[3] = -INFINITY;
 #pragma unroll
-                for (int c = 0; c < KC_KEYS; c++) {
-                    if (c > d || (c <= low && c >= keep)) x[c] = -INFINITY;
-                    m4[c & 3] = fmaxf(m4[c & 3], x[c]);
+                for (int w = 0; w < 4; w++) {
+                    const uint32_t see = upto(d - 32 * w) & (~upto(under - 32 * w) | upto(keep - 1 - 32 * w));
+#pragma unroll
+                    for (int c = 0; c < 32; c++) {
+                        if (!(see >> c & 1)) x[32 * w + c] = -INFINITY;
+                        m4[c & 3] = fmaxf(m4[c & 3], x[32 * w + c]);
+                    }
                 }
             }
             const float mt = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * sc;
+            if (OWN_P && i > 0) {                              // P(i - 1) has been read, and O is at rest
+                if (!mbar_wait_warp(&o_full[t], (uint32_t)((i - 1) & 1))) { ok = false; break; }
+                tc_fence_after();
+            }
             const bool grow = mt > m + 8.f;
             if (__any_sync(0xffffffffu, grow)) {
-                const float alpha = grow ? kc_ex2(m - mt) : 1.f;
+                const float alpha = grow ? kv_ex2(m - mt) : 1.f;
                 if (grow) m = mt;
                 l2[0].x *= alpha; l2[0].y *= alpha; l2[1].x *= alpha; l2[1].y *= alpha;
                 if (i > 0) {
 #pragma unroll 1
                     for (int c = 0; c < DP / 16; c++) {
                         float o[16];
-                        tc_ld16(trow + Sh::COL_O + t * DP + 16 * c, o);
+                        tc_ld16(o_at + 16 * c, o);
                         tc_wait_ld();
 #pragma unroll
                         for (int e = 0; e < 16; e++) o[e] *= alpha;
-                        kc_st16(trow + Sh::COL_O + t * DP + 16 * c, reinterpret_cast<const uint32_t *>(o));
+                        kc_st16(o_at + 16 * c, reinterpret_cast<const uint32_t *>(o));
                     }
                 }
             }
             const float2 sc2 = make_float2(sc, sc), neg = make_float2(-m, -m);
-            // groups of 16 keys: a group's exponentials are under way while the one before is summed, packed and stored
+            auto open = [&](int c) {                           // a group's exponentials, in place
 #pragma unroll
-            for (int c = 0; c <= 8; c++) {
-                if (c < 8) {
-#pragma unroll
-                    for (int e = 0; e < 8; e++) {
-                        float *v = x + c * 16 + 2 * e;
-                        const float2 y = kc_fma2(make_float2(v[0], v[1]), sc2, neg);
-                        v[0] = kc_ex2(y.x); v[1] = kc_ex2(y.y);
-                    }
+                for (int e = 0; e < 8; e++) {
+                    float *v = x + c * 16 + 2 * e;
+                    const float2 y = kv_fma2(make_float2(v[0], v[1]), sc2, neg);
+                    v[0] = kv_ex2(y.x); v[1] = kv_ex2(y.y);
                 }
-                if (c > 0) {
-                    uint32_t hi[8], lo[F32 ? 8 : 1];
+            };
+            auto close = [&](int c) {                          // summed, packed and stored
+                uint32_t hi[8], lo[F32 ? 8 : 1];
 #pragma unroll
-                    for (int e = 0; e < 8; e++) {
-                        const float *v = x + (c - 1) * 16 + 2 * e;
-                        l2[e & 1] = kc_add2(l2[e & 1], make_float2(v[0], v[1]));
-                        if (F32) kc_split(v[0], v[1], hi[e], lo[F32 ? e : 0]);
-                        else hi[e] = kc_pack<BF>(v[0], v[1]);
-                    }
-                    kc_st8(trow + Sh::COL_S + t * 128 + 8 * (c - 1), hi);
-                    if (F32) kc_st8(trow + Sh::COL_S + t * 128 + 64 + 8 * (c - 1), lo);
-                    if (c == KC_PART) {
-                        kc_wait_st();
-                        tc_fence_before();
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(&p_part[t]);
-                    }
+                for (int e = 0; e < 8; e++) {
+                    const float *v = x + c * 16 + 2 * e;
+                    l2[e & 1] = kv_add2(l2[e & 1], make_float2(v[0], v[1]));
+                    if (F32) kv_split(v[0], v[1], hi[e], lo[F32 ? e : 0]);
+                    else hi[e] = kv_pack<BF>(v[0], v[1]);
+                }
+                kc_st8(p_at + 8 * c, hi);
+                if (F32) kc_st8(p_at + 64 + 8 * c, lo);
+            };
+            auto ready = [&](uint64_t *bar) {
+                kc_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar);
+            };
+            if (all) {
+                // a group's exponentials are under way while the one before is summed, packed and stored
+#pragma unroll
+                for (int c = 0; c <= 8; c++) {
+                    if (c < 8) open(c);
+                    if (c > 0) close(c - 1);
+                    if (c == KC_PART) ready(&p_part[t]);
+                }
+            } else {
+                int lo, hi;
+                groups(j0, &lo, &hi);
+#pragma unroll
+                for (int c = 0; c <= 8; c++) {
+                    if (c >= lo && c < hi) open(c);
+                    if (c > lo && c <= hi) close(c - 1);
+                    if (c == KC_PART) ready(&p_part[t]);
                 }
             }
-            kc_wait_st();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&p_full[t]);
+            ready(&p_full[t]);
         }
-        if (n > 0 && ok) ok = mbar_wait_warp(&o_full[t], 0);
+        if (n > 0 && ok) ok = mbar_wait_warp(&o_full[t], (uint32_t)(OWN_P ? (n - 1) & 1 : 0));
         if (!ok && lane == 0) atomicExch(a.status, ST_TIMEOUT_EPILOGUE);
         tc_fence_after();
-        const float l = (l2[0].x + l2[0].y) + (l2[1].x + l2[1].y), inv = l != 0.f ? 1.f / l : 0.f;
-        const int64_t to = (int64_t)(sq.begin + tok) * a.ldo + (int64_t)h * a.D;
+        l = (l2[0].x + l2[0].y) + (l2[1].x + l2[1].y);
+    }
+    }
+    if (shares == 1) {
+        // through shared memory, where the tile's queries were (its products are done): a warp's 32 rows in pieces of 16 bytes, turned by
+        // the row so that both sides touch all banks, and out in whole rows
+        if (soft && rank == 0 && t < nt) {
+            constexpr int PIECE = F32 ? 4 : 8, PIECES = DP / PIECE;            // values of 16 bytes; pieces of a row
+            uint8_t *stage = qst + t * Sh::PLANES * Sh::OPERAND + (warp & 3) * (32 * PIECES * 16);
+            const float inv = l != 0.f ? 1.f / l : 0.f;
 #pragma unroll 1
-        for (int c = 0; c < DP / 32; c++) {
-            float o[32];
-            if (n > 0) {
-                tc_ld32(trow + Sh::COL_O + t * DP + 32 * c, o);
-                tc_wait_ld();
+            for (int c = 0; c < DP / 32; c++) {
+                float o[32];
+                if (n > 0) {
+                    tc_ld32(o_at + 32 * c, o);
+                    tc_wait_ld();
+                }
+#pragma unroll
+                for (int e = 0; e < 32; e++) o[e] = inv != 0.f ? o[e] * inv : 0.f;
+#pragma unroll
+                for (int e = 0; e < 32; e += PIECE) {
+                    const int k = c * (32 / PIECE) + e / PIECE;
+                    uint4 v;
+                    if (F32) v = make_uint4(__float_as_uint(o[e]), __float_as_uint(o[e + 1]), __float_as_uint(o[e + 2]), __float_as_uint(o[e + 3]));
+                    else v = make_uint4(kv_pack<BF>(o[e], o[e + 1]), kv_pack<BF>(o[e + 2], o[e + 3]), kv_pack<BF>(o[e + (F32 ? 0 : 4)], o[e + (F32 ? 0 : 5)]), kv_pack<BF>(o[e + (F32 ? 0 : 6)], o[e + (F32 ? 0 : 7)]));
+                    *reinterpret_cast<uint4 *>(stage + (lane * PIECES + (k ^ (lane & 7))) * 16) = v;
+                }
             }
-#pragma unroll
-            for (int e = 0; e < 32; e++) o[e] = inv != 0.f ? o[e] * inv : 0.f;
-#pragma unroll
-            for (int e = 0; e < 32; e += 8) {
-                if (!valid || c * 32 + e >= a.D) continue;
-                if (F32) {
-                    float *p = static_cast<float *>(a.out) + to + c * 32 + e;
-                    *reinterpret_cast<float4 *>(p) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
-                    *reinterpret_cast<float4 *>(p + 4) = make_float4(o[e + 4], o[e + 5], o[e + 6], o[e + 7]);
-                } else {
-                    *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(a.out) + to + c * 32 + e) =
-                        make_uint4(kc_pack<BF>(o[e], o[e + 1]), kc_pack<BF>(o[e + 2], o[e + 3]), kc_pack<BF>(o[e + 4], o[e + 5]), kc_pack<BF>(o[e + 6], o[e + 7]));
+            __syncwarp();
+            const int k = lane % PIECES;
+#pragma unroll 4
+            for (int i = 0; i < PIECES; i++) {                 // 32 / PIECES rows each
+                const int row = i * (32 / PIECES) + lane / PIECES, rt = (warp & 3) * 32 + row, pl = by_g(rt), at = t0 + t * tq + pl;
+                if (rt < tq * a.G && at < sq.n && k * PIECE < a.D) {
+                    const uint4 v = *reinterpret_cast<const uint4 *>(stage + (row * PIECES + (k ^ (row & 7))) * 16);
+                    const int64_t to = (int64_t)(sq.begin + at) * a.ldo + (int64_t)(kvh * a.G + rt - pl * a.G) * a.D + k * PIECE;
+                    *reinterpret_cast<uint4 *>(static_cast<uint8_t *>(a.out) + to * (F32 ? 4 : 2)) = v;
                 }
             }
         }
+    } else {
+        // parts of the rows' results and (maximum, sum) of each, where queries and tiles were; then the weights of the parts, and their sum
+        // by all CTAs of the cluster, each for its rows
+        float *part = reinterpret_cast<float *>(qst), *weight = part + TILES * 128 * (Sh::LDO + 2);
+        float2 *ml = reinterpret_cast<float2 *>(part + TILES * 128 * Sh::LDO);
+        __syncthreads();                                       // (both tiles' products have been waited for)
+        if (soft && t < nt && n > 0) {
+            float *row = part + (t * 128 + r) * Sh::LDO;
+#pragma unroll 1
+            for (int c = 0; c < DP / 32; c++) {
+                float o[32];
+                tc_ld32(o_at + 32 * c, o);
+                tc_wait_ld();
+#pragma unroll
+                for (int e = 0; e < 32; e += 4) *reinterpret_cast<float4 *>(row + c * 32 + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+            }
+            ml[t * 128 + r] = make_float2(m, l);
+        }
+        kv_cluster_sync();
+        const uint32_t part0 = smem_u32(part), ml0 = smem_u32(ml);
+        const int per_tile = tq * a.G, rows = min((last - t0 + 1) * a.G, nt * per_tile), share = (rows + size - 1) >> log_size;
+        const int v0 = rank * share, mine = max(0, min(share, rows - v0)), quads = a.D / 4;
+        auto place_of = [&](int v) { return v < per_tile ? v : 128 + v - per_tile; };
+        for (int v = threadIdx.x; v < mine; v += Sh::THREADS) {
+            const int at = place_of(v0 + v);
+            float2 e[16];
+            float top_m = KC_NONE, total = 0.f;
+#pragma unroll
+            for (int p = 0; p < 16; p++) {
+                e[p] = make_float2(KC_NONE, 0.f);
+                if (p < shares) e[p] = kv_peer2(kv_peer(ml0 + at * 8, p));
+            }
+#pragma unroll
+            for (int p = 0; p < 16; p++) top_m = fmaxf(top_m, e[p].x);
+#pragma unroll
+            for (int p = 0; p < 16; p++) {
+                e[p].x = kv_ex2(e[p].x - top_m);
+                total = fmaf(e[p].x, e[p].y, total);
+            }
+            const float inv = total != 0.f ? 1.f / total : 0.f;
+#pragma unroll
+            for (int p = 0; p < 16; p++)
+                if (p < shares) weight[v * 16 + p] = e[p].x * inv;
+        }
+        __syncthreads();
+        for (int u = threadIdx.x; u < mine * quads; u += Sh::THREADS) {
+            const int v = u / quads, c = (u - v * quads) * 4, at = place_of(v0 + v);
+            float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int p0 = 0; p0 < shares; p0 += 4) {
+                float4 o[4];
+#pragma unroll
+                for (int p = 0; p < 4; p++) {
+                    o[p] = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (p0 + p < shares) o[p] = kv_peer4(kv_peer(part0 + (at * Sh::LDO + c) * 4, p0 + p));
+                }
+#pragma unroll
+                for (int p = 0; p < 4; p++)
+                    if (p0 + p < shares) {
+                        const float w = weight[v * 16 + p0 + p];
+                        sum.x = fmaf(w, o[p].x, sum.x); sum.y = fmaf(w, o[p].y, sum.y); sum.z = fmaf(w, o[p].z, sum.z); sum.w = fmaf(w, o[p].w, sum.w);
+                    }
+            }
+            const int pl = by_g(v0 + v);
+            const int64_t to = (int64_t)(sq.begin + t0 + pl) * a.ldo + (int64_t)(kvh * a.G + v0 + v - pl * a.G) * a.D + c;
+            if (F32) *reinterpret_cast<float4 *>(static_cast<float *>(a.out) + to) = sum;
+            else *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(a.out) + to) = make_uint2(kv_pack<BF>(sum.x, sum.y), kv_pack<BF>(sum.z, sum.w));
+        }
+        kv_cluster_sync();                                     // nobody leaves while its part is being read
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == KC_W_MMA) tc_dealloc(tmem, 512);
+    if (warp == Sh::W_MMA) tc_dealloc(tmem, Sh::TMEM);
 }
 
 template <int DP, int FMT>
@@ -469,13 +632,23 @@ static int chunk_launch(const CUtensorMap &k, const CUtensorMap &v, const KvArgs
     static PerDevice configured = {};
     int dev = 0;
     if (configured.below((size_t)Sh::SMEM, &dev)) {
+        cudaFuncAttributes at;
+        MB_CUDA(cudaFuncGetAttributes(&at, kernel));
+        if (Sh::TILES == 2 && at.numRegs != KC_REGS) { set_error("kv_attend: the kernel was built with %d registers, not %d", at.numRegs, KC_REGS); return -1; }
         MB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::SMEM));
+        MB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
         configured.record(dev, (size_t)Sh::SMEM);
     }
-    const int per_block = 2 * (KC_ROWS / a.G);
-    const int64_t blocks = (int64_t)a.n_rows / per_block + (a.n_seq < a.n_rows ? a.n_seq : a.n_rows);      // the last block of each may be short
-    if (blocks > 0x7fffffff) { set_error("kv_attend: too many rows in one call"); return -1; }
-    MB_CUDA(launch_kernel(kernel, dim3((unsigned)blocks, (unsigned)a.Hkv), dim3(KC_THREADS), (size_t)Sh::SMEM, st, true, 1, k, v, a, box_rows));
+    const int per_block = Sh::TILES * (KC_ROWS / a.G);
+    const int64_t full = ((int64_t)a.n_rows + per_block - 1) / per_block, seqs = a.n_seq < a.n_rows ? a.n_seq : a.n_rows;
+    const int64_t blocks = a.n_rows / per_block + seqs;        // the last block of each sequence may be short
+    // Clusters where the blocks that are likely (whole ones, or one per sequence) leave SMs without work, as large as those fill
+    const int64_t likely = (full > seqs ? full : seqs) * a.Hkv;
+    int log_size = 0;
+    if (const char *e = getenv("KV_S")) log_size = atoi(e);
+    else while (log_size < 4 && likely << (log_size + 1) <= Sh::PER_SM * device_sm_count() && (int64_t)KC_KEYS * 2 << log_size < ((int64_t)a.max_pages << a.page_shift)) log_size++;
+    if (blocks << log_size > 0x7fffffff) { set_error("kv_attend: too many rows in one call"); return -1; }
+    MB_CUDA(launch_kernel(kernel, dim3((unsigned)(blocks << log_size), (unsigned)a.Hkv), dim3(Sh::THREADS), (size_t)Sh::SMEM, st, true, 1 << log_size, k, v, a, box_rows, log_size));
     note_launch();
     return 0;
 }

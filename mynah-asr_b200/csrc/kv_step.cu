@@ -16,7 +16,6 @@
 // 128 us for the first (each TMA instruction of a diverged lane waits for its operands, in front of the products), query heads as the
 // 16 rows of the products 192 us.
 #include "kv.h"
-#include <cuda_bf16.h>
 
 namespace mb {
 
@@ -53,44 +52,6 @@ __device__ __forceinline__ void ks_mma(float *c, const uint32_t *a, uint32_t b0,
         asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-template <bool BF>
-__device__ __forceinline__ uint32_t ks_pack(float x, float y) {
-    if (BF) { const __nv_bfloat162 h = __floats2bfloat162_rn(x, y); return *reinterpret_cast<const uint32_t *>(&h); }
-    const __half2 h = __floats2half2_rn(x, y);
-    return *reinterpret_cast<const uint32_t *>(&h);
-}
-// x, y as f16 pairs: hi and what it leaves. The rest stays unscaled (it may be subnormal): both products go into one accumulator.
-__device__ __forceinline__ void ks_split(float x, float y, uint32_t &hi, uint32_t &lo) {
-    const __half2 h = __floats2half2_rn(x, y);
-    const float2 f = __half22float2(h);
-    const __half2 l = __floats2half2_rn(x - f.x, y - f.y);
-    hi = *reinterpret_cast<const uint32_t *>(&h);
-    lo = *reinterpret_cast<const uint32_t *>(&l);
-}
-__device__ __forceinline__ float ks_ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-__device__ __forceinline__ uint32_t ks_peer(uint32_t addr, int rank) {
-    uint32_t r;
-    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
-    return r;
-}
-__device__ __forceinline__ float4 ks_peer4(uint32_t addr) {
-    float4 v;
-    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
-    return v;
-}
-__device__ __forceinline__ float2 ks_peer2(uint32_t addr) {
-    float2 v;
-    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
-    return v;
-}
-__device__ __forceinline__ void ks_cluster_sync() {
-    asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
-}
-
 // Who does what. A sequence's tiles are cut for 2^k CTAs by its own length: for as many as 2^log_even (what fills the GPU once with the
 // call's units) down to a tile each, for more, up to a cluster, as long as each has over half of KS_CHUNK tiles. The units (sequence,
 // kv head, head tile) of one k stand side by side in clusters, those of the largest k first, so that what takes longest begins first;
@@ -241,7 +202,7 @@ kv_step_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
                         float2 f = make_float2(0.f, 0.f);
                         if (on) f = *reinterpret_cast<const float2 *>(static_cast<const float *>(a.q) + at);
                         bad |= !(fabsf(f.x) < H16_MAX) | !(fabsf(f.y) < H16_MAX);
-                        ks_split(f.x, f.y, qh[nt][kk][e], ql[F32 ? nt : 0][F32 ? kk : 0][e]);
+                        kv_split(f.x, f.y, qh[nt][kk][e], ql[F32 ? nt : 0][F32 ? kk : 0][e]);
                     } else if (on) {
                         qh[nt][kk][e] = *reinterpret_cast<const uint32_t *>(static_cast<const uint16_t *>(a.q) + at);
                     }
@@ -325,7 +286,7 @@ kv_step_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
                     }
                     const float n0 = fmaxf(m[nt][0], t[0] * sc), n1 = fmaxf(m[nt][1], t[1] * sc);
                     if (__any_sync(0xffffffffu, n0 > m[nt][0] || n1 > m[nt][1])) {
-                        const float a0 = ks_ex2(m[nt][0] - n0), a1 = ks_ex2(m[nt][1] - n1);
+                        const float a0 = kv_ex2(m[nt][0] - n0), a1 = kv_ex2(m[nt][1] - n1);
                         l[nt][0] *= a0; l[nt][1] *= a1;
 #pragma unroll
                         for (int d = 0; d < DP / 16; d++) { o[nt][d][0] *= a0; o[nt][d][1] *= a1; o[nt][d][2] *= a0; o[nt][d][3] *= a1; }
@@ -336,17 +297,17 @@ kv_step_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
                     for (int mt = 0; mt < MT; mt++) {
                         float p[4];
 #pragma unroll
-                        for (int e = 0; e < 4; e++) p[e] = ks_ex2(fmaf(x[nt][mt][e], sc, -m[nt][e & 1]));
+                        for (int e = 0; e < 4; e++) p[e] = kv_ex2(fmaf(x[nt][mt][e], sc, -m[nt][e & 1]));
                         l[nt][0] += p[0] + p[2]; l[nt][1] += p[1] + p[3];
 #pragma unroll
                         for (int e = 0; e < 2; e++) {
                             if (F32) {
                                 uint32_t hi, lo;
-                                ks_split(p[2 * e], p[2 * e + 1], hi, lo);
+                                kv_split(p[2 * e], p[2 * e + 1], hi, lo);
                                 pb[nt][mt][e] = ks_turn(hi);
                                 pl[F32 ? nt : 0][F32 ? mt : 0][e] = ks_turn(lo);
                             } else {
-                                pb[nt][mt][e] = ks_turn(ks_pack<BF>(p[2 * e], p[2 * e + 1]));
+                                pb[nt][mt][e] = ks_turn(kv_pack<BF>(p[2 * e], p[2 * e + 1]));
                             }
                         }
                     }
@@ -401,7 +362,7 @@ kv_step_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
         const float inv = total != 0.f ? 1.f / total : 0.f;
         const int64_t at = (int64_t)seq * a.ldo + (int64_t)(kvh * a.G + g0 + r) * a.D + c;
         if (F32) *reinterpret_cast<float4 *>(static_cast<float *>(a.out) + at) = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
-        else *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(a.out) + at) = make_uint2(ks_pack<BF>(v.x * inv, v.y * inv), ks_pack<BF>(v.z * inv, v.w * inv));
+        else *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(a.out) + at) = make_uint2(kv_pack<BF>(v.x * inv, v.y * inv), kv_pack<BF>(v.z * inv, v.w * inv));
     };
     for (int q = threadIdx.x; q < rows * quads; q += KS_THREADS) {
         const int r = q / quads, c = (q % quads) * 4;
@@ -416,7 +377,7 @@ kv_step_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
 #pragma unroll
         for (int w = 0; w < KS_WARPS; w++) {
             const float4 v = *reinterpret_cast<const float4 *>(parts + w * PART + r * Sh::LDO + c);
-            const float f = ks_ex2(e[w].x - top);
+            const float f = kv_ex2(e[w].x - top);
             total = fmaf(f, e[w].y, total);
             sum.x = fmaf(f, v.x, sum.x); sum.y = fmaf(f, v.y, sum.y); sum.z = fmaf(f, v.z, sum.z); sum.w = fmaf(f, v.w, sum.w);
         }
@@ -429,7 +390,7 @@ kv_step_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
     }
     // then those of the CTAs that share the unit, in their order, each CTA for its slice of the values
     if (log_parts > 0) {
-        ks_cluster_sync();
+        kv_cluster_sync();
         const uint32_t at0 = smem_u32(mine);
         const int base = rank - part_no;
         for (int q = part_no * KS_THREADS + (int)threadIdx.x; q < rows * quads; q += parts_n * KS_THREADS) {
@@ -439,7 +400,7 @@ kv_step_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
 #pragma unroll
             for (int p = 0; p < 16; p++) {
                 e[p] = make_float2(KS_NONE, 0.f);
-                if (p < parts_n) e[p] = ks_peer2(ks_peer(at0 + (HEADS * Sh::LDO + 2 * r) * 4, base + p));
+                if (p < parts_n) e[p] = kv_peer2(kv_peer(at0 + (HEADS * Sh::LDO + 2 * r) * 4, base + p));
             }
 #pragma unroll
             for (int p = 0; p < 16; p++) top = fmaxf(top, e[p].x);
@@ -447,14 +408,14 @@ kv_step_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
 #pragma unroll
             for (int p = 0; p < 16; p++)
                 if (p < parts_n) {
-                    const float4 v4 = ks_peer4(ks_peer(at0 + (r * Sh::LDO + c) * 4, base + p));
-                    const float f = ks_ex2(e[p].x - top);
+                    const float4 v4 = kv_peer4(kv_peer(at0 + (r * Sh::LDO + c) * 4, base + p));
+                    const float f = kv_ex2(e[p].x - top);
                     total = fmaf(f, e[p].y, total);
                     sum.x = fmaf(f, v4.x, sum.x); sum.y = fmaf(f, v4.y, sum.y); sum.z = fmaf(f, v4.z, sum.z); sum.w = fmaf(f, v4.w, sum.w);
                 }
             store(r, c, sum, total);
         }
-        ks_cluster_sync();                                     // nobody leaves while its part is being read
+        kv_cluster_sync();                                     // nobody leaves while its part is being read
     }
 }
 
