@@ -4,7 +4,7 @@
 // Bound by the tensor cores and, as much, by the exponentials (4 D operations and one exponential per pair of row and key). A CTA
 // owns one kv head and two tiles of 128 rows: the G query heads of 128 / G positions each (row r is head r % G of position r / G), so
 // that short pieces fill a tile and all heads share the keys' tiles. Keys and values come in tiles of 128 by TMA, from their pages
-// straight into the swizzled operand layout; of a tile at the edge of what is visible only the groups of 16 keys that some row sees
+// straight into the swizzled operand layout; of a tile at the edge of what is visible only the groups of 32 keys that some row sees
 // are computed.
 //   tensor memory  S0, S1: scores of the two tiles (128 columns each), O0, O1: results; the probabilities, as 16-bit operands, overwrite
 //                  the scores, or have columns of their own where D <= 64 leaves room (then S(i + 1) is computed under the exponentials
@@ -24,7 +24,7 @@ namespace mb {
 
 static constexpr int KC_ROWS = 128, KC_KEYS = 128, KC_HALF = 128 * 128;      // a 128-row x 64-column box of 16-bit values: 16 KB
 static constexpr int KC_HEAD = 1024;
-static constexpr int KC_PART = 6;                    // P V begins when the first 6 x 16 keys' probabilities are there
+static constexpr int KC_PART = 3;                    // P V begins when the first 3 x 32 keys' probabilities are there
 static constexpr float KC_NONE = -1e30f;             // "maximum" of no keys
 
 template <int DP, int FMT> struct ChunkShape {
@@ -38,6 +38,8 @@ template <int DP, int FMT> struct ChunkShape {
     static constexpr int SMEM = KC_HEAD + Q + STAGES * OPERAND + 1024;
     static_assert(PER_SM * (SMEM + 1024) <= 233472, "shared memory");
     static constexpr bool OWN_P = DP == 64 && PLANES == 1;     // columns of their own for the probabilities
+    // a path of its own for tiles that all rows see: more code, which pays where most tiles are such
+    static constexpr bool WHOLE = DP == 128 && PLANES == 1;
     static constexpr int COL_S = 0, COL_P = OWN_P ? 128 * TILES : 0, STEP_P = OWN_P ? 64 : 128, COL_O = 128 * TILES + (OWN_P ? 64 * TILES : 0);
     static constexpr int TMEM = 512 / PER_SM;
     static_assert(COL_O + TILES * DP <= TMEM, "tensor memory");
@@ -183,13 +185,13 @@ kv_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
     const int n = rank < shares ? (tiles.count - rank + shares - 1) / shares : 0;
     const int nt = TILES == 2 && t0 + tq <= last ? 2 : 1;                    // tiles that have rows
     auto tile_at = [&](int i) { return tiles.at(rank + i * shares) * KC_KEYS; };       // first key of this CTA's i-th tile
-    // its groups of 16 keys [lo, hi) that some row sees
+    // its groups of 32 keys [lo, hi) that some row sees
     auto groups = [&](int j0, int *lo, int *hi) {
         *lo = 0;
-        *hi = min(8, ((top - j0) >> 4) + 1);
+        *hi = min(4, ((top - j0) >> 5) + 1);
         if (a.window > 0) {
-            if (j0 + KC_KEYS <= low) *hi = min(*hi, (a.sinks - j0 + 15) >> 4);         // a tile of the first tokens
-            else if (low > j0 && a.sinks <= j0) *lo = (low - j0) >> 4;
+            if (j0 + KC_KEYS <= low) *hi = min(*hi, (a.sinks - j0 + 31) >> 5);         // a tile of the first tokens
+            else if (low > j0 && a.sinks <= j0) *lo = (low - j0) >> 5;
         }
     };
 
@@ -242,9 +244,9 @@ kv_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
         const uint32_t idesc_o = kc_idesc(BF, a.D) | (1u << 16);       // V: MN-major
         const uint64_t qdesc = umma_desc_sw128(smem_u32(qst)), kdesc = umma_desc_sw128(smem_u32(ring)), vdesc = kc_desc_mn(smem_u32(ring));
         const int steps = a.D / 16;
-        auto issue_s = [&](int t, int s, int hi) {             // by one lane: the scores of the first 16 hi keys
+        auto issue_s = [&](int t, int s, int hi) {             // by one lane: the scores of the first 32 hi keys
             const uint64_t kd = kdesc + (uint64_t)((s * Sh::OPERAND) >> 4);
-            const uint32_t idesc = kc_idesc(BF, 16 * hi);
+            const uint32_t idesc = kc_idesc(BF, 32 * hi);
 #pragma unroll
             for (int plane = 0; plane < Sh::PLANES; plane++) {
                 const uint64_t qd = qdesc + (uint64_t)(((t * Sh::PLANES + plane) * Sh::OPERAND) >> 4);
@@ -255,26 +257,17 @@ kv_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
                 }
             }
         };
-        // group kk of P V; group `start` of the first tile begins the sum
-        auto issue_o1 = [&](int t, uint64_t vd, int kk, int start) {
-#pragma unroll
-            for (int plane = 0; plane < Sh::PLANES; plane++)
-                kc_mma_ts(tmem + Sh::COL_O + t * DP, tmem + Sh::COL_P + t * Sh::STEP_P + plane * 64 + 8 * kk, vd + (uint64_t)((kk * 2048) >> 4), idesc_o,
-                          kk != start || plane != 0);
-        };
-        // part 0: the groups in front of KC_PART, part 1: the others
-        auto issue_o = [&](int t, int s, int part, int lo, int hi, int start) {
+        // groups [k0, k1) of P V; group `start` of the first tile begins the sum
+        auto issue_o = [&](int t, int s, int k0, int k1, int start) {
             const uint64_t vd = vdesc + (uint64_t)((s * Sh::OPERAND) >> 4);
-            if (lo == 0 && hi == 8) {
-                if (part == 0) {
+            for (int k = k0; k < k1; k++) {
 #pragma unroll
-                    for (int kk = 0; kk < KC_PART; kk++) issue_o1(t, vd, kk, start);
-                } else {
+                for (int b = 0; b < 2; b++) {
 #pragma unroll
-                    for (int kk = KC_PART; kk < 8; kk++) issue_o1(t, vd, kk, start);
+                    for (int plane = 0; plane < Sh::PLANES; plane++)
+                        kc_mma_ts(tmem + Sh::COL_O + t * DP, tmem + Sh::COL_P + t * Sh::STEP_P + plane * 64 + 16 * k + 8 * b,
+                                  vd + (uint64_t)((k * 4096 + b * 2048) >> 4), idesc_o, k != start || b != 0 || plane != 0);
                 }
-            } else {
-                for (int kk = max(lo, part * KC_PART); kk < (part ? hi : min(hi, KC_PART)); kk++) issue_o1(t, vd, kk, start);
             }
         };
         int s = 0, ph = 0;                                     // ring place of the next item
@@ -285,7 +278,7 @@ kv_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
             return got;
         };
         bool ok = n > 0 ? mbar_wait_warp(q_full, 0) : true;
-        int sk = 0, sv = 0, lo = 0, hi = 8;
+        int sk = 0, sv = 0, lo = 0, hi = 4;
         if (n > 0) groups(tile_at(0), &lo, &hi);
         if (ok && n > 0 && (ok = take(&sk))) {
             tc_fence_after();
@@ -301,7 +294,7 @@ kv_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
         for (int i = 0; i < n && ok; i++) {
             const bool more = i + 1 < n;
             const int v = sv, start = i == 0 ? lo : -1;
-            int lo2 = 0, hi2 = 8;
+            int lo2 = 0, hi2 = 4;
             if (more) groups(tile_at(i + 1), &lo2, &hi2);
             if (OWN_P && more) {
                 ok = take(&sk);
@@ -318,14 +311,14 @@ kv_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
             for (int t = 0; t < nt && ok; t++) {
                 if (!mbar_wait_warp(&p_part[t], (uint32_t)(i & 1))) { ok = false; break; }
                 tc_fence_after();
-                if (elect_one()) issue_o(t, v, 0, lo, hi, start);
+                if (elect_one()) issue_o(t, v, lo, min(hi, KC_PART), start);
                 __syncwarp();
                 if (more && !OWN_P && t == 0 && !take(&sk)) { ok = false; break; }     // K(i + 1)
                 if (more && t == nt - 1 && !take(&sv)) { ok = false; break; }          // V(i + 1)
                 if (!mbar_wait_warp(&p_full[t], (uint32_t)(i & 1))) { ok = false; break; }
                 tc_fence_after();
                 if (elect_one()) {
-                    issue_o(t, v, 1, lo, hi, start);
+                    issue_o(t, v, max(lo, KC_PART), hi, start);
                     if (OWN_P || !more) tc_commit(&o_full[t]);
                     if (more && !OWN_P) { issue_s(t, sk, hi2); tc_commit(&s_full[t]); }
                     if (t == nt - 1) { tc_commit(&empty[v]); if (more && !OWN_P) tc_commit(&empty[sk]); }
@@ -346,12 +339,12 @@ kv_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
     if (TILES == 2) kc_regs_more();
     if (n > 0) {
         // the warp's 32 rows, neighbouring lanes on neighbouring pieces of eight values; all reads under way at once
-        constexpr int PIECES = DP / 8, ROWS = 32 / PIECES, ROUNDS = 32 / ROWS, BATCH = F32 && ROUNDS > 8 ? 8 : ROUNDS;
+        constexpr int PIECES = DP / 8, ROWS = 32 / PIECES, ROUNDS = 32 / ROWS, BATCH = 8;
         uint8_t *qt = qst + t * Sh::PLANES * Sh::OPERAND;
         const int c = lane % PIECES;
         bool bad = false;
         if (t < nt) {
-#pragma unroll
+#pragma unroll 1
             for (int b = 0; b < ROUNDS; b += BATCH) {
                 uint4 in[BATCH][F32 ? 2 : 1];
 #pragma unroll
@@ -425,18 +418,23 @@ kv_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
             const bool whole = d >= KC_KEYS - 1 && (a.window <= 0 || d < a.window || j0 + KC_KEYS - 1 < a.sinks);
             const bool all = __all_sync(0xffffffffu, whole);
             if (!all) {                                        // (columns that have no scores are hidden, too)
-                // a bit per column: visible up to d, above `under`, or below `keep`
+                // 32 columns at a time, where some row of the warp does not see them all: a bit per column, visible up to d, above
+                // `under`, or below `keep`
                 const int under = a.window > 0 ? d - a.window : -1, keep = a.sinks - j0;
                 auto upto = [](int c) -> uint32_t { return c < 0 ? 0u : c >= 31 ? 0xffffffffu : (2u << c) - 1u; };      // bits 0 to c
                 m4[0] = m4[1] = m4[2] = m4[3] = -INFINITY;
 #pragma unroll
                 for (int w = 0; w < 4; w++) {
                     const uint32_t see = upto(d - 32 * w) & (~upto(under - 32 * w) | upto(keep - 1 - 32 * w));
+                    if (!__all_sync(0xffffffffu, see == 0xffffffffu)) {
 #pragma unroll
-                    for (int c = 0; c < 32; c++) {
-                        if (!(see >> c & 1)) x[32 * w + c] = -INFINITY;
-                        m4[c & 3] = fmaxf(m4[c & 3], x[32 * w + c]);
+                        for (int c = 0; c < 32; c++)
+                            if (!(see >> c & 1)) x[32 * w + c] = -INFINITY;
                     }
+#pragma unroll
+                    for (int c = 0; c < 32; c += 8)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) m4[e] = fmaxf(m4[e], fmaxf(x[32 * w + c + e], x[32 * w + c + 4 + e]));
                 }
             }
             const float mt = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * sc;
@@ -462,7 +460,7 @@ kv_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
                 }
             }
             const float2 sc2 = make_float2(sc, sc), neg = make_float2(-m, -m);
-            auto open = [&](int c) {                           // a group's exponentials, in place
+            auto open = [&](int c) {                           // the exponentials of 16 keys, in place
 #pragma unroll
                 for (int e = 0; e < 8; e++) {
                     float *v = x + c * 16 + 2 * e;
@@ -488,21 +486,21 @@ kv_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
                 __syncwarp();
                 if (lane == 0) mbar_arrive(bar);
             };
-            if (all) {
-                // a group's exponentials are under way while the one before is summed, packed and stored
+            // some keys' exponentials are under way while those before are summed, packed and stored
+            if (Sh::WHOLE && all) {
 #pragma unroll
                 for (int c = 0; c <= 8; c++) {
                     if (c < 8) open(c);
                     if (c > 0) close(c - 1);
-                    if (c == KC_PART) ready(&p_part[t]);
+                    if (c == 2 * KC_PART) ready(&p_part[t]);
                 }
             } else {
                 int lo, hi;
                 groups(j0, &lo, &hi);
 #pragma unroll
-                for (int c = 0; c <= 8; c++) {
-                    if (c >= lo && c < hi) open(c);
-                    if (c > lo && c <= hi) close(c - 1);
+                for (int c = 0; c <= 4; c++) {
+                    if (c < 4 && c >= lo && c < hi) { open(2 * c); open(2 * c + 1); }
+                    if (c > 0 && c > lo && c <= hi) { close(2 * c - 2); close(2 * c - 1); }
                     if (c == KC_PART) ready(&p_part[t]);
                 }
             }
