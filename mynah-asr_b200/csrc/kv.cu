@@ -68,31 +68,46 @@ bool reachable(const void *p, int dev) {
            (at.type == cudaMemoryTypeHost && at.devicePointer == p);
 }
 
+}  // namespace
+
+namespace mb {
 typedef CUresult (*EncodeFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
                              const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion,
                              CUtensorMapFloatOOBfill);
 
-// A pool as [rows][D]: boxes of 64 columns (zeros beyond D) and box_rows slots of one page and head, 128-byte swizzle
-bool pool_map(CUtensorMap *m, const uint16_t *pool, const mynah_b200_kv_config &c, int box_rows) {
-    void *p = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess) {
+static bool encode(CUtensorMap *m, bool bf, int rank, const void *base, const cuuint64_t *dims, const cuuint64_t *strides, const cuuint32_t *box) {
+    static const EncodeFn fn = [] {
+        void *p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess)
+            return reinterpret_cast<EncodeFn>(p);
         cudaGetLastError();
-        return false;
-    }
-    cuuint64_t dims[2] = {(cuuint64_t)c.head_dim, (cuuint64_t)c.n_pages * c.page_size * c.n_kv_heads};
-    cuuint64_t strides[1] = {(cuuint64_t)c.head_dim * 2};
-    cuuint32_t box[2] = {64, (cuuint32_t)box_rows}, estr[2] = {1, 1};
-    return reinterpret_cast<EncodeFn>(p)(m, c.fmt == MYNAH_B200_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2,
-                                         const_cast<uint16_t *>(pool), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+        return EncodeFn(nullptr);
+    }();
+    const cuuint32_t one[3] = {1, 1, 1};
+    return fn && fn(m, bf ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, (cuuint32_t)rank, const_cast<void *>(base), dims, strides, box, one,
+                    CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
+// A pool as [rows][D]: boxes of 64 columns (zeros beyond D) and box_rows slots of one page and head, 128-byte swizzle
+static bool pool_map(CUtensorMap *m, const uint16_t *pool, const mynah_b200_kv_config &c, int box_rows) {
+    const cuuint64_t dims[2] = {(cuuint64_t)c.head_dim, (cuuint64_t)c.n_pages * c.page_size * c.n_kv_heads}, strides[1] = {(cuuint64_t)c.head_dim * 2};
+    const cuuint32_t box[2] = {64, (cuuint32_t)box_rows};
+    return encode(m, c.fmt == MYNAH_B200_BF16, 2, pool, dims, strides, box);
+}
+bool kv_rows_map(CUtensorMap *m, const KvArgs &a, bool bf) {
+    const cuuint64_t dims[3] = {(cuuint64_t)a.D, (cuuint64_t)a.H, (cuuint64_t)a.n_rows}, strides[2] = {(cuuint64_t)a.D * 2, (cuuint64_t)a.ldq * 2};
+    const cuuint32_t box[3] = {64, (cuuint32_t)a.G, (cuuint32_t)(128 / a.G)};
+    return encode(m, bf, 3, a.q, dims, strides, box);
+}
+}  // namespace mb
+
+namespace {
 
 // Rows of `width` values with stride ld, of which the last one ends where the buffer does
 const char *refuse_rows(const mynah_b200_kv *h, const void *p, long long ld, int width) {
     if (!p) return "a null pointer";
     if (ld < width) return "a row stride below the row's width";
-    if (ld > (1ll << 40)) return "a row stride out of range";
+    if (ld > (1ll << 36)) return "a row stride out of range";
     if (((uintptr_t)p & 15) || (ld * row_bytes(h->fmt)) % 16) return "rows start on 16-byte boundaries";
     if (!reachable(p, h->device)) return "a pointer that is not of the handle's device";
     return nullptr;

@@ -139,6 +139,8 @@ int kv_append(const KvAppendArgs &a, int fmt, cudaStream_t st);
 // Attention of one row per sequence, and of many. Maps of the two pools as [rows][D] with boxes of 64 columns and kv_box slots.
 int kv_box(int D, int page_size);
 int kv_step(const CUtensorMap &k, const CUtensorMap &v, const KvArgs &a, int fmt, cudaStream_t st);
+// 16-bit query rows as [rows][H][D]: boxes of 64 columns, G heads and 128 / G rows
+bool kv_rows_map(CUtensorMap *m, const KvArgs &a, bool bf);
 int kv_chunk(const CUtensorMap &k, const CUtensorMap &v, const KvArgs &a, int box_rows, int fmt, cudaStream_t st);
 
 }  // namespace mb

@@ -47,7 +47,7 @@ template <int DP, int FMT> struct ChunkShape {
     static_assert(TILES * 128 * (LDO * 4 + 8 + 64) <= Q + STAGES * OPERAND, "parts");
 };
 
-struct KcPlace { int seq, block; };
+struct KcPlace { int seq, block; KvSeq q; };
 
 __device__ __forceinline__ void kc_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
     asm volatile(
@@ -55,6 +55,12 @@ __device__ __forceinline__ void kc_mma_ts(uint32_t d, uint32_t a, uint64_t b, ui
         "setp.ne.b32 p, %4, 0;\n\t"
         "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
         ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc)
+        : "memory");
+}
+__device__ __forceinline__ void kc_load_3d(void *dst, const CUtensorMap *m, int x, int y, int z, uint64_t *bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+        ::"r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(m)), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
         : "memory");
 }
 __device__ __forceinline__ void kc_st16(uint32_t taddr, const uint32_t *r) {
@@ -95,8 +101,9 @@ __device__ __forceinline__ uint64_t kc_desc_mn(uint32_t addr) {
 __device__ __forceinline__ bool kc_place(const KvArgs &a, int x, int per_block, int lane, KcPlace *at) {
     int total = 0;
     bool bad = false;
+    KvSeq q = {0, 0, 0};
     for (int s0 = 0; s0 < a.n_seq; s0 += 32) {
-        KvSeq q = {0, 0, 0};
+        q = {0, 0, 0};
         if (s0 + lane < a.n_seq) bad |= !kv_seq(a.row_off, a.kv_len, s0 + lane, a.n_rows, kv_capacity(a), &q);
         total += __reduce_add_sync(0xffffffffu, (q.n + per_block - 1) / per_block);
     }
@@ -104,8 +111,10 @@ __device__ __forceinline__ bool kc_place(const KvArgs &a, int x, int per_block, 
     int nth = total - 1 - x;
     if (nth < 0) return false;
     for (int s0 = 0; s0 < a.n_seq; s0 += 32) {
-        KvSeq q = {0, 0, 0};
-        if (s0 + lane < a.n_seq) kv_seq(a.row_off, a.kv_len, s0 + lane, a.n_rows, kv_capacity(a), &q);
+        if (a.n_seq > 32) {
+            q = {0, 0, 0};
+            if (s0 + lane < a.n_seq) kv_seq(a.row_off, a.kv_len, s0 + lane, a.n_rows, kv_capacity(a), &q);
+        }
         const int n = (q.n + per_block - 1) / per_block;
         int upto = n;
 #pragma unroll
@@ -118,6 +127,9 @@ __device__ __forceinline__ bool kc_place(const KvArgs &a, int x, int per_block, 
             const int who = __ffs(in) - 1;
             at->seq = s0 + who;
             at->block = nth - __shfl_sync(0xffffffffu, upto - n, who);
+            at->q.begin = __shfl_sync(0xffffffffu, q.begin, who);
+            at->q.n = __shfl_sync(0xffffffffu, q.n, who);
+            at->q.len = __shfl_sync(0xffffffffu, q.len, who);
             return true;
         }
         nth -= __shfl_sync(0xffffffffu, upto, 31);
@@ -127,7 +139,7 @@ __device__ __forceinline__ bool kc_place(const KvArgs &a, int x, int per_block, 
 
 template <int DP, int FMT>
 __global__ void __launch_bounds__(ChunkShape<DP, FMT>::THREADS, ChunkShape<DP, FMT>::PER_SM)
-kv_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const KvArgs a, int box_rows, int log_size) {
+kv_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const KvArgs a, int box_rows, int log_size) {
     using Sh = ChunkShape<DP, FMT>;
     constexpr bool BF = FMT == KV_BF16, F32 = FMT == KV_F32, OWN_P = Sh::OWN_P;
     constexpr int STAGES = Sh::STAGES, TILES = Sh::TILES;
@@ -147,14 +159,14 @@ kv_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
     auto by_g = [&](int x) { return (int)(((uint32_t)x * inv_g) >> 16); };
     const int size = 1 << log_size, rank = (int)blockIdx.x & (size - 1);
     if (warp == 0) {
-        KcPlace at = {-1, 0};
+        KcPlace at = {-1, 0, {0, 0, 0}};
         if (!kc_place(a, (int)(blockIdx.x >> log_size), TILES * tq, lane, &at)) at.seq = -1;
-        if (lane == 0) { place[0] = at.seq; place[1] = at.block; }
+        if (lane == 0) { place[0] = at.seq; place[1] = at.block; place[2] = at.q.begin; place[3] = at.q.n; place[4] = at.q.len; }
     }
     if (threadIdx.x == 32) {
         tma_prefetch_desc(&tmK); tma_prefetch_desc(&tmV);
         for (int s = 0; s < STAGES; s++) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
-        mbar_init(q_full, Sh::SOFT);
+        mbar_init(q_full, F32 ? Sh::SOFT : 1);
         for (int t = 0; t < TILES; t++) {
             mbar_init(&s_full[t], 1); mbar_init(&o_full[t], 1);
             mbar_init(&s_free[t], 4); mbar_init(&p_part[t], 4); mbar_init(&p_full[t], 4);
@@ -170,10 +182,7 @@ kv_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
     // (one lane's values for all, so that the compiler keeps them and what follows from them in uniform registers)
     auto same = [](int v) { return __shfl_sync(0xffffffffu, v, 0); };
     const int seq = same(place[0]), block = same(place[1]);
-
-    KvSeq sq = {0, 0, 0};
-    if (seq >= 0) kv_seq(a.row_off, a.kv_len, seq, a.n_rows, kv_capacity(a), &sq);
-    sq.begin = same(sq.begin); sq.n = same(sq.n); sq.len = same(sq.len);
+    const KvSeq sq = {same(place[2]), same(place[3]), same(place[4])};
     const int kvh = blockIdx.y, t0 = block * TILES * tq;          // first position's place among the sequence's rows
     const int base_pos = sq.len - sq.n;
     const int last = min(t0 + TILES * tq, sq.n) - 1;
@@ -216,6 +225,13 @@ kv_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
         };
         int entry = entry_of(0), s = 0, ph = 0, r = 0;
         bool ok = true;
+        if (!F32 && n > 0) {                                   // 16-bit queries: rows as they lie are the tile's rows
+            if (lane == 0) mbar_expect_tx(q_full, (uint32_t)(nt * Sh::HALVES * 128 * tq * a.G));
+            __syncwarp();
+            if (lane < nt * Sh::HALVES)
+                kc_load_3d(qst + (lane / Sh::HALVES) * Sh::OPERAND + (lane % Sh::HALVES) * KC_HALF, &tmQ, (lane % Sh::HALVES) * 64, kvh * a.G,
+                           sq.begin + t0 + lane / Sh::HALVES * tq, q_full);
+        }
         for (int i = 0; i < n && ok; i++) {
             const int next = entry_of(i + 1);
             const int j = tile_at(i) + b_sub * box_rows;
@@ -240,6 +256,7 @@ kv_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
             if (s == 0) { s = STAGES; ph ^= 1; }
             if (!mbar_wait_warp(&full[--s], (uint32_t)ph)) break;
         }
+        if (!F32 && n > 0) mbar_wait_warp(q_full, 0);
     } else if (warp == Sh::W_MMA) {
         const uint32_t idesc_o = kc_idesc(BF, a.D) | (1u << 16);       // V: MN-major
         const uint64_t qdesc = umma_desc_sw128(smem_u32(qst)), kdesc = umma_desc_sw128(smem_u32(ring)), vdesc = kc_desc_mn(smem_u32(ring));
@@ -337,8 +354,8 @@ kv_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
     } else {
     // ---- softmax: thread = row
     if (TILES == 2) kc_regs_more();
-    if (n > 0) {
-        // the warp's 32 rows, neighbouring lanes on neighbouring pieces of eight values; all reads under way at once
+    if (F32 && n > 0) {
+        // the warp's 32 rows, neighbouring lanes on neighbouring pieces of eight values
         constexpr int PIECES = DP / 8, ROWS = 32 / PIECES, ROUNDS = 32 / ROWS, BATCH = 8;
         uint8_t *qt = qst + t * Sh::PLANES * Sh::OPERAND;
         const int c = lane % PIECES;
@@ -346,34 +363,28 @@ kv_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
         if (t < nt) {
 #pragma unroll 1
             for (int b = 0; b < ROUNDS; b += BATCH) {
-                uint4 in[BATCH][F32 ? 2 : 1];
+                float4 in[BATCH][2];
 #pragma unroll
                 for (int i = 0; i < BATCH; i++) {
                     const int row = (warp & 3) * 32 + (b + i) * ROWS + lane / PIECES, pl = by_g(row), at = t0 + t * tq + pl;
-                    in[i][0] = make_uint4(0, 0, 0, 0);
-                    if (F32) in[i][F32 ? 1 : 0] = make_uint4(0, 0, 0, 0);
+                    in[i][0] = in[i][1] = make_float4(0.f, 0.f, 0.f, 0.f);
                     if (row < tq * a.G && at < sq.n && c * 8 < a.D) {
-                        const int64_t from = (int64_t)(sq.begin + at) * a.ldq + (int64_t)(kvh * a.G + row - pl * a.G) * a.D + c * 8;
-                        const uint4 *p = reinterpret_cast<const uint4 *>(static_cast<const uint8_t *>(a.q) + from * (F32 ? 4 : 2));
-                        in[i][0] = p[0];
-                        if (F32) in[i][F32 ? 1 : 0] = p[1];
+                        const float4 *p = reinterpret_cast<const float4 *>(static_cast<const float *>(a.q) + (int64_t)(sq.begin + at) * a.ldq +
+                                                                           (int64_t)(kvh * a.G + row - pl * a.G) * a.D + c * 8);
+                        in[i][0] = p[0]; in[i][1] = p[1];
                     }
                 }
 #pragma unroll
                 for (int i = 0; i < BATCH; i++) {
                     const int row = (warp & 3) * 32 + (b + i) * ROWS + lane / PIECES;
                     uint8_t *to = qt + (c >> 3) * KC_HALF + row * 128 + (((c & 7) ^ (row & 7)) << 4);
-                    if (F32) {
-                        const float *f = reinterpret_cast<const float *>(in[i]);
-                        uint4 hi, lo;
+                    const float *f = reinterpret_cast<const float *>(in[i]);
+                    uint4 hi, lo;
 #pragma unroll
-                        for (int e = 0; e < 8; e++) bad |= !(fabsf(f[e]) < H16_MAX);
-                        kv_split(f[0], f[1], hi.x, lo.x); kv_split(f[2], f[3], hi.y, lo.y); kv_split(f[4], f[5], hi.z, lo.z); kv_split(f[6], f[7], hi.w, lo.w);
-                        *reinterpret_cast<uint4 *>(to) = hi;
-                        *reinterpret_cast<uint4 *>(to + Sh::OPERAND) = lo;
-                    } else {
-                        *reinterpret_cast<uint4 *>(to) = in[i][0];
-                    }
+                    for (int e = 0; e < 8; e++) bad |= !(fabsf(f[e]) < H16_MAX);
+                    kv_split(f[0], f[1], hi.x, lo.x); kv_split(f[2], f[3], hi.y, lo.y); kv_split(f[4], f[5], hi.z, lo.z); kv_split(f[6], f[7], hi.w, lo.w);
+                    *reinterpret_cast<uint4 *>(to) = hi;
+                    *reinterpret_cast<uint4 *>(to + Sh::OPERAND) = lo;
                 }
             }
             if (bad) atomicExch(a.status, ST_RANGE);
@@ -646,7 +657,10 @@ static int chunk_launch(const CUtensorMap &k, const CUtensorMap &v, const KvArgs
     if (const char *e = getenv("KV_S")) log_size = atoi(e);
     else while (log_size < 4 && likely << (log_size + 1) <= Sh::PER_SM * device_sm_count() && (int64_t)KC_KEYS * 2 << log_size < ((int64_t)a.max_pages << a.page_shift)) log_size++;
     if (blocks << log_size > 0x7fffffff) { set_error("kv_attend: too many rows in one call"); return -1; }
-    MB_CUDA(launch_kernel(kernel, dim3((unsigned)(blocks << log_size), (unsigned)a.Hkv), dim3(Sh::THREADS), (size_t)Sh::SMEM, st, true, 1 << log_size, k, v, a, box_rows, log_size));
+    CUtensorMap q = k;
+    if (FMT != KV_F32 && !kv_rows_map(&q, a, FMT == KV_BF16)) { set_error("kv_attend: no tensor map of the rows"); return -1; }
+    MB_CUDA(launch_kernel(kernel, dim3((unsigned)(blocks << log_size), (unsigned)a.Hkv), dim3(Sh::THREADS), (size_t)Sh::SMEM, st, true, 1 << log_size, q, k, v, a,
+                          box_rows, log_size));
     note_launch();
     return 0;
 }
