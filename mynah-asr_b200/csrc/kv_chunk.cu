@@ -9,21 +9,22 @@
 //   tensor memory  S0, S1: scores of the two tiles (128 columns each), O0, O1: results; the probabilities, as 16-bit operands, overwrite
 //                  the scores, or have columns of their own where D <= 64 leaves room (then S(i + 1) is computed under the exponentials
 //                  of tile i)
-//   warps          0-3 and 4-7: softmax of tile 0 and 1, a thread per row; 8: TMA; 9: MMA
+//   warps          0-3 (and 4-7): softmax of tile 0 (and 1), a thread per row; then TMA, and MMA
 //   order of MMAs  P0 V(i), S0(i + 1), P1 V(i), S1(i + 1): one tile's exponentials run under the other's products. MMAs run in the
 //                  order of their issue, so S(i + 1) does not overwrite the P(i) that P V(i) reads, and whoever sees S(i + 1) finished
-//                  finds O at rest. With columns of their own for P: S0(i + 1), S1(i + 1), P0 V(i), P1 V(i).
+//                  finds O at rest. With columns of their own for P: S(i + 1) in front of P V(i).
+// A CTA stays and takes block after block (heads of a block side by side, later positions, which see more keys, first): the next block's
+// place, queries and first keys are looked up, fetched and multiplied while the results of the one before are written.
 // The softmax keeps a running maximum per row; O is rescaled only when it has grown by more than 2^8 (what is stale cancels in the
 // final division). F32 rows: queries and probabilities as (hi, lo) f16 pairs, two products each.
 // A call with few blocks is launched as clusters: the CTAs of a cluster take a block's tiles in turn, two at least each, and join their
 // results through distributed shared memory.
 #include "kv.h"
-#include <stdlib.h>
 
 namespace mb {
 
 static constexpr int KC_ROWS = 128, KC_KEYS = 128, KC_HALF = 128 * 128;      // a 128-row x 64-column box of 16-bit values: 16 KB
-static constexpr int KC_HEAD = 1024;
+static constexpr int KC_HEAD = 1024, KC_STAY = 3000;
 static constexpr int KC_PART = 3;                    // P V begins when the first 3 x 32 keys' probabilities are there
 static constexpr float KC_NONE = -1e30f;             // "maximum" of no keys
 
@@ -31,7 +32,10 @@ template <int DP, int FMT> struct ChunkShape {
     static constexpr int HALVES = DP / 64, PLANES = FMT == KV_F32 ? 2 : 1;
     static constexpr int TILES = DP == 64 ? 1 : 2, PER_SM = DP == 64 ? 2 : 1;          // tiles of rows of a CTA, CTAs of an SM
     static constexpr int SOFT = 4 * TILES, W_TMA = SOFT, W_MMA = SOFT + 1;             // warps
-    static constexpr int THREADS = TILES == 2 ? 384 : 192;     // (warps 10 and 11 of twelve lend their registers)
+    // The launch's registers are dealt out anew between the softmax warps and the four warps of TMA and MMA, two of which have no other
+    // work than to lend theirs
+    static constexpr int THREADS = 32 * (SOFT + 4), REGS = TILES == 2 ? 168 : 128, MORE = TILES == 2 ? 208 : 192, LESS = TILES == 2 ? 88 : 64;
+    static_assert(32 * SOFT * MORE + 128 * LESS <= THREADS * REGS, "a share beyond the launch's registers waits for good");
     static constexpr int OPERAND = HALVES * KC_HALF;           // a tile of queries (one plane), of keys, or of values
     static constexpr int Q = TILES * PLANES * OPERAND;
     static constexpr int STAGES = DP == 64 ? 6 - PLANES : PLANES == 1 ? 5 : 3;
@@ -47,7 +51,7 @@ template <int DP, int FMT> struct ChunkShape {
     static_assert(TILES * 128 * (LDO * 4 + 8 + 64) <= Q + STAGES * OPERAND, "parts");
 };
 
-struct KcPlace { int seq, block; KvSeq q; };
+struct KcItem { int seq, block; KvSeq q; };
 
 __device__ __forceinline__ void kc_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
     asm volatile(
@@ -84,11 +88,8 @@ __device__ __forceinline__ void kc_wait_ld32(float *x) {
                    "+f"(x[21]), "+f"(x[22]), "+f"(x[23]), "+f"(x[24]), "+f"(x[25]), "+f"(x[26]), "+f"(x[27]), "+f"(x[28]), "+f"(x[29]), "+f"(x[30]), "+f"(x[31])
                  :: "memory");
 }
-// The registers of the launch, KC_REGS a thread, are dealt out anew: 2 x 128 threads with 208 and 128 with 88 are 384 with 168.
-static constexpr int KC_REGS = 168, KC_REGS_MORE = 208, KC_REGS_LESS = 88;
-static_assert(256 * KC_REGS_MORE + 128 * KC_REGS_LESS <= 384 * KC_REGS, "a share beyond the launch's registers waits for good");
-__device__ __forceinline__ void kc_regs_more() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(KC_REGS_MORE)); }
-__device__ __forceinline__ void kc_regs_less() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(KC_REGS_LESS)); }
+template <int N> __device__ __forceinline__ void kc_regs_more() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N> __device__ __forceinline__ void kc_regs_less() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 // Instruction descriptor: f32 accumulators, A and B both f16 (or both bf16: formats 1 << 7 and 1 << 10), M x N
 __host__ __device__ constexpr uint32_t kc_idesc(bool bf, int N) { return umma_idesc_f16(KC_ROWS, N) | (bf ? (1u << 7) | (1u << 10) : 0u); }
 // B operand [keys][D] with D contiguous: eight-key groups 1024 bytes apart, 64-wide blocks of D one half apart
@@ -96,81 +97,116 @@ __device__ __forceinline__ uint64_t kc_desc_mn(uint32_t addr) {
     return umma_desc_sw128(addr) | ((uint64_t)(KC_HALF >> 4) << 16);
 }
 
-// The block of positions that CTA x of a kv head works on: the call's blocks from the last to the first, since later positions see more
-// keys and what takes longest should begin first. By one warp; false where there is none.
-__device__ __forceinline__ bool kc_place(const KvArgs &a, int x, int per_block, int lane, KcPlace *at) {
-    int total = 0;
-    bool bad = false;
-    KvSeq q = {0, 0, 0};
-    for (int s0 = 0; s0 < a.n_seq; s0 += 32) {
+// Where the TMA warp finds the call's blocks: all their number, and the x-th from the last, since later positions see more keys and
+// what takes longest should begin first. With up to 32 sequences a lane keeps one.
+struct KcFinder {
+    int per_block, total;
+    KvSeq q;
+    __device__ __forceinline__ int blocks() const { return (q.n + per_block - 1) / per_block; }
+    __device__ __forceinline__ void look(const KvArgs &a, int s, bool *bad) {
         q = {0, 0, 0};
-        if (s0 + lane < a.n_seq) bad |= !kv_seq(a.row_off, a.kv_len, s0 + lane, a.n_rows, kv_capacity(a), &q);
-        total += __reduce_add_sync(0xffffffffu, (q.n + per_block - 1) / per_block);
+        if (s < a.n_seq) *bad |= !kv_seq(a.row_off, a.kv_len, s, a.n_rows, kv_capacity(a), &q);
     }
-    if (bad) atomicExch(a.status, ST_PAGE);
-    int nth = total - 1 - x;
-    if (nth < 0) return false;
-    for (int s0 = 0; s0 < a.n_seq; s0 += 32) {
-        if (a.n_seq > 32) {
-            q = {0, 0, 0};
-            if (s0 + lane < a.n_seq) kv_seq(a.row_off, a.kv_len, s0 + lane, a.n_rows, kv_capacity(a), &q);
+    __device__ __forceinline__ void init(const KvArgs &a, int per, int lane) {
+        per_block = per; total = 0;
+        bool bad = false;
+        for (int s0 = 0; s0 < a.n_seq; s0 += 32) {
+            look(a, s0 + lane, &bad);
+            total += __reduce_add_sync(0xffffffffu, blocks());
         }
-        const int n = (q.n + per_block - 1) / per_block;
-        int upto = n;
+        if (bad) atomicExch(a.status, ST_PAGE);
+    }
+    __device__ __forceinline__ void find(const KvArgs &a, int x, int lane, KcItem *at) {
+        int nth = total - 1 - x;
+        at->seq = -1; at->block = 0; at->q = {0, 0, 0};
+        if (nth < 0) return;
+        bool bad = false;
+        for (int s0 = 0; s0 < a.n_seq; s0 += 32) {
+            if (a.n_seq > 32) look(a, s0 + lane, &bad);
+            const int n = blocks();
+            int upto = n;
 #pragma unroll
-        for (int o = 1; o < 32; o *= 2) {
-            const int v = __shfl_up_sync(0xffffffffu, upto, o);
-            if (lane >= o) upto += v;
+            for (int o = 1; o < 32; o *= 2) {
+                const int v = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= o) upto += v;
+            }
+            const unsigned in = __ballot_sync(0xffffffffu, nth < upto);
+            if (in) {
+                const int who = __ffs(in) - 1;
+                at->seq = s0 + who;
+                at->block = nth - __shfl_sync(0xffffffffu, upto - n, who);
+                at->q.begin = __shfl_sync(0xffffffffu, q.begin, who);
+                at->q.n = __shfl_sync(0xffffffffu, q.n, who);
+                at->q.len = __shfl_sync(0xffffffffu, q.len, who);
+                return;
+            }
+            nth -= __shfl_sync(0xffffffffu, upto, 31);
         }
-        const unsigned in = __ballot_sync(0xffffffffu, nth < upto);
-        if (in) {
-            const int who = __ffs(in) - 1;
-            at->seq = s0 + who;
-            at->block = nth - __shfl_sync(0xffffffffu, upto - n, who);
-            at->q.begin = __shfl_sync(0xffffffffu, q.begin, who);
-            at->q.n = __shfl_sync(0xffffffffu, q.n, who);
-            at->q.len = __shfl_sync(0xffffffffu, q.len, who);
-            return true;
-        }
-        nth -= __shfl_sync(0xffffffffu, upto, 31);
     }
-    return false;
-}
+};
+
+// What a block is to those who work on it
+struct KcBlock {
+    KvSeq sq;
+    int seq, kvh, t0, base_pos, last, top, low, n, nt, rank, shares;
+    KvTiles tiles;
+    __device__ __forceinline__ KcBlock(const KvArgs &a, const volatile int *item, int tq, int n_tiles, int size, int rank_) {
+        // (one lane's values for all, so that the compiler keeps them and what follows from them in uniform registers)
+        auto same = [](int v) { return __shfl_sync(0xffffffffu, v, 0); };
+        seq = same(item[0]); kvh = same(item[2]);
+        sq = {same(item[3]), same(item[4]), same(item[5])};
+        t0 = same(item[1]) * n_tiles * tq;                     // first position's place among the sequence's rows
+        base_pos = sq.len - sq.n;
+        last = min(t0 + n_tiles * tq, sq.n) - 1;
+        top = base_pos + last;                                 // last key that any row sees,
+        low = base_pos + t0 - a.window + 1;                    // and first that a window shows
+        tiles = {0, 0, 0};
+        if (seq >= 0) tiles = kv_tiles(base_pos + t0 > 0 ? base_pos + t0 : 0, top, a.window, a.sinks, KC_KEYS);
+        // CTAs that share the block: two tiles each at least, by the block's own tiles
+        rank = rank_;
+        shares = min(size, tiles.count < 4 ? 1 : 1 << (30 - __clz(tiles.count)));
+        n = rank < shares ? (tiles.count - rank + shares - 1) / shares : 0;
+        nt = n_tiles == 2 && t0 + tq <= last ? 2 : 1;          // tiles that have rows
+    }
+    __device__ __forceinline__ int tile_at(int i) const { return tiles.at(rank + i * shares) * KC_KEYS; }       // first key of the CTA's i-th tile
+    // its groups of 32 keys [lo, hi) that some row sees
+    __device__ __forceinline__ void groups(const KvArgs &a, int j0, int *lo, int *hi) const {
+        *lo = 0;
+        *hi = min(4, ((top - j0) >> 5) + 1);
+        if (a.window > 0) {
+            if (j0 + KC_KEYS <= low) *hi = min(*hi, (a.sinks - j0 + 31) >> 5);         // a tile of the first tokens
+            else if (low > j0 && a.sinks <= j0) *lo = (low - j0) >> 5;
+        }
+    }
+};
 
 template <int DP, int FMT>
 __global__ void __launch_bounds__(ChunkShape<DP, FMT>::THREADS, ChunkShape<DP, FMT>::PER_SM)
-kv_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const KvArgs a, int box_rows, int log_size) {
+kv_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const KvArgs a,
+                int box_rows, int log_size) {
     using Sh = ChunkShape<DP, FMT>;
     constexpr bool BF = FMT == KV_BF16, F32 = FMT == KV_F32, OWN_P = Sh::OWN_P;
     constexpr int STAGES = Sh::STAGES, TILES = Sh::TILES;
     extern __shared__ uint8_t kc_raw[];
     uint8_t *head = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(kc_raw) + 1023) & ~uintptr_t(1023));
     uint8_t *qst = head + KC_HEAD, *ring = qst + Sh::Q;
-    uint64_t *full = reinterpret_cast<uint64_t *>(head), *empty = full + STAGES, *q_full = empty + STAGES, *s_full = q_full + 1,
-             *s_free = s_full + 2, *p_part = s_free + 2, *p_full = p_part + 2, *o_full = p_full + 2, *drain = o_full + 2;
+    uint64_t *full = reinterpret_cast<uint64_t *>(head), *empty = full + STAGES, *q_full = empty + STAGES, *q_empty = q_full + 1, *s_full = q_empty + 1,
+             *s_free = s_full + 2, *p_part = s_free + 2, *p_full = p_part + 2, *o_full = p_full + 2, *i_full = o_full + 2, *i_empty = i_full + 2,
+             *drain = i_empty + 2;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(drain + 1);
-    volatile int *place = reinterpret_cast<volatile int *>(tmem_slot + 1);
+    volatile int *items = reinterpret_cast<volatile int *>(tmem_slot + 1);     // two of eight words: sequence, block, kv head, its rows and keys
     const int warp = warp_index(), lane = threadIdx.x & 31;
 
-    chain_trigger();
-    chain_wait();
-    const int tq = KC_ROWS / a.G;                              // positions of a tile
-    const uint32_t inv_g = (65536u + a.G - 1) / a.G;           // x / G = x inv_g / 2^16 for x < 1024, G <= 64
-    auto by_g = [&](int x) { return (int)(((uint32_t)x * inv_g) >> 16); };
-    const int size = 1 << log_size, rank = (int)blockIdx.x & (size - 1);
-    if (warp == 0) {
-        KcPlace at = {-1, 0, {0, 0, 0}};
-        if (!kc_place(a, (int)(blockIdx.x >> log_size), TILES * tq, lane, &at)) at.seq = -1;
-        if (lane == 0) { place[0] = at.seq; place[1] = at.block; place[2] = at.q.begin; place[3] = at.q.n; place[4] = at.q.len; }
-    }
-    if (threadIdx.x == 32) {
+    if (threadIdx.x == 0) {
         tma_prefetch_desc(&tmK); tma_prefetch_desc(&tmV);
+        if (!F32) tma_prefetch_desc(&tmQ);
         for (int s = 0; s < STAGES; s++) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
-        mbar_init(q_full, F32 ? Sh::SOFT : 1);
+        mbar_init(q_full, F32 ? Sh::SOFT : 1); mbar_init(q_empty, 1);
         for (int t = 0; t < TILES; t++) {
             mbar_init(&s_full[t], 1); mbar_init(&o_full[t], 1);
             mbar_init(&s_free[t], 4); mbar_init(&p_part[t], 4); mbar_init(&p_full[t], 4);
         }
+        for (int i = 0; i < 2; i++) { mbar_init(&i_full[i], 1); mbar_init(&i_empty[i], Sh::SOFT + 1); }
         mbar_init(drain, 1);
         mbar_fence_init();
     }
@@ -178,85 +214,97 @@ kv_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
+    chain_trigger();
+    chain_wait();
     const uint32_t tmem = *tmem_slot;
-    // (one lane's values for all, so that the compiler keeps them and what follows from them in uniform registers)
-    auto same = [](int v) { return __shfl_sync(0xffffffffu, v, 0); };
-    const int seq = same(place[0]), block = same(place[1]);
-    const KvSeq sq = {same(place[2]), same(place[3]), same(place[4])};
-    const int kvh = blockIdx.y, t0 = block * TILES * tq;          // first position's place among the sequence's rows
-    const int base_pos = sq.len - sq.n;
-    const int last = min(t0 + TILES * tq, sq.n) - 1;
-    const int top = base_pos + last, low = base_pos + t0 - a.window + 1;     // last key that any row sees; first that a window shows
-    KvTiles tiles = {0, 0, 0};
-    if (seq >= 0) tiles = kv_tiles(base_pos + t0 > 0 ? base_pos + t0 : 0, top, a.window, a.sinks, KC_KEYS);
-    // CTAs that share the block: two tiles each at least, by the block's own tiles
-    const int shares = min(size, tiles.count < 4 ? 1 : 1 << (30 - __clz(tiles.count)));
-    const int n = rank < shares ? (tiles.count - rank + shares - 1) / shares : 0;
-    const int nt = TILES == 2 && t0 + tq <= last ? 2 : 1;                    // tiles that have rows
-    auto tile_at = [&](int i) { return tiles.at(rank + i * shares) * KC_KEYS; };       // first key of this CTA's i-th tile
-    // its groups of 32 keys [lo, hi) that some row sees
-    auto groups = [&](int j0, int *lo, int *hi) {
-        *lo = 0;
-        *hi = min(4, ((top - j0) >> 5) + 1);
-        if (a.window > 0) {
-            if (j0 + KC_KEYS <= low) *hi = min(*hi, (a.sinks - j0 + 31) >> 5);         // a tile of the first tokens
-            else if (low > j0 && a.sinks <= j0) *lo = (low - j0) >> 5;
-        }
+    const int tq = KC_ROWS / a.G;                              // positions of a tile
+    const uint32_t inv_g = (65536u + a.G - 1) / a.G;           // x / G = x inv_g / 2^16 for x < 256, G <= 64
+    auto by_g = [&](int x) { return (int)(((uint32_t)x * inv_g) >> 16); };
+    const int size = 1 << log_size, rank = (int)blockIdx.x & (size - 1);
+    const bool once = log_size > 0;                            // a cluster's CTAs work on one block and join their results
+    // Everybody but the TMA warp: the CTA's j-th block, -1 as its sequence behind the last one, and -2 where it does not come
+    auto next_block = [&](int j) {
+        const bool got = mbar_wait_warp(&i_full[j & 1], (uint32_t)((j >> 1) & 1));
+        KcBlock b(a, items + (j & 1) * 8, tq, TILES, size, rank);
+        if (!got) { b.seq = -2; b.n = 0; }
+        return b;
     };
-
+    auto leave_block = [&](int j) {                            // its words are not needed any more
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&i_empty[j & 1]);
+    };
     // row of a softmax thread, in tile t
     const int t = TILES == 2 ? (warp >> 2) & 1 : 0, r = (warp & 3) * 32 + lane;
-    const int tok = t0 + t * tq + by_g(r);
     const bool soft = warp < Sh::SOFT;
     const uint32_t trow = tmem + ((uint32_t)((warp & 3) * 32) << 16), s_at = trow + Sh::COL_S + t * 128, p_at = trow + Sh::COL_P + t * Sh::STEP_P,
                    o_at = trow + Sh::COL_O + t * DP;
     float m = KC_NONE, l = 0.f;                                // of the row: running maximum and sum
+
     if (!soft) {
-    if (TILES == 2) kc_regs_less();                            // (one instruction for the four warps)
+    kc_regs_less<Sh::LESS>();                                  // (one instruction for the four warps)
     if (warp == Sh::W_TMA) {
         // ---- lane = one box of a tile: 64 of the D columns, the slots of one page. Item 2 i of the ring is K(i), 2 i + 1 V(i).
         const int shift = a.page_shift, boxes = KC_KEYS / box_rows * Sh::HALVES;
         const int b_half = lane % Sh::HALVES, b_sub = lane / Sh::HALVES;
         const uint32_t b_at = b_half * KC_HALF + b_sub * box_rows * 128;
-        auto seen = [&](int j) { return j <= top && (a.window <= 0 || j + box_rows - 1 >= low || j < a.sinks); };
-        auto entry_of = [&](int i) -> int {
-            const int j = tile_at(i) + b_sub * box_rows;
-            return lane < boxes && i < n && seen(j) ? a.table[(size_t)seq * a.max_pages + (j >> shift)] : -1;
-        };
-        int entry = entry_of(0), s = 0, ph = 0, r = 0;
+        KcFinder finder;
+        finder.init(a, TILES * tq, lane);
+        int s = 0, ph = 0, r = 0, queries = 0;                 // place in the ring, its parity, requests; blocks with queries so far
         bool ok = true;
-        if (!F32 && n > 0) {                                   // 16-bit queries: rows as they lie are the tile's rows
-            if (lane == 0) mbar_expect_tx(q_full, (uint32_t)(nt * Sh::HALVES * 128 * tq * a.G));
+        for (int j = 0, x = (int)(blockIdx.x >> log_size); ok; j++, x += (int)gridDim.x) {
+            if (j >= 2 && !mbar_wait_warp(&i_empty[j & 1], (uint32_t)(((j >> 1) & 1) ^ 1))) { ok = false; break; }
+            volatile int *item = items + (j & 1) * 8;
+            KcItem at;
+            finder.find(a, x / a.Hkv, lane, &at);
+            if (lane == 0) {
+                item[0] = at.seq; item[1] = at.block; item[2] = x % a.Hkv; item[3] = at.q.begin; item[4] = at.q.n; item[5] = at.q.len;
+                mbar_arrive(&i_full[j & 1]);
+            }
             __syncwarp();
-            if (lane < nt * Sh::HALVES)
-                kc_load_3d(qst + (lane / Sh::HALVES) * Sh::OPERAND + (lane % Sh::HALVES) * KC_HALF, &tmQ, (lane % Sh::HALVES) * 64, kvh * a.G,
-                           sq.begin + t0 + lane / Sh::HALVES * tq, q_full);
-        }
-        for (int i = 0; i < n && ok; i++) {
-            const int next = entry_of(i + 1);
-            const int j = tile_at(i) + b_sub * box_rows;
-            if (lane < boxes && (unsigned)entry >= (unsigned)a.n_pages) {
-                if (seen(j)) atomicExch(a.status, ST_PAGE);
-                entry = 0;                                     // any finite rows do
-            }
-            const int y = (int)kv_row(a, entry, kvh, j & ((1 << shift) - 1));
-#pragma unroll
-            for (int kv = 0; kv < 2; kv++) {
-                if (r >= STAGES && !mbar_wait_warp(&empty[s], (uint32_t)(ph ^ 1))) { ok = false; break; }
-                if (lane == 0) mbar_expect_tx(&full[s], Sh::OPERAND);
+            const KcBlock b(a, item, tq, TILES, size, rank);
+            if (b.seq < 0) break;
+            auto seen = [&](int j) { return j <= b.top && (a.window <= 0 || j + box_rows - 1 >= b.low || j < a.sinks); };
+            auto entry_of = [&](int i) -> int {
+                const int j = b.tile_at(i) + b_sub * box_rows;
+                return lane < boxes && i < b.n && seen(j) ? a.table[(size_t)b.seq * a.max_pages + (j >> shift)] : -1;
+            };
+            int entry = entry_of(0);
+            if (!F32 && b.n > 0) {                             // 16-bit queries: rows as they lie are the tile's rows
+                if (queries > 0 && !mbar_wait_warp(q_empty, (uint32_t)((queries - 1) & 1))) { ok = false; break; }
+                if (lane == 0) mbar_expect_tx(q_full, (uint32_t)(b.nt * Sh::HALVES * 128 * tq * a.G));
                 __syncwarp();
-                if (lane < boxes) tma_load_2d(ring + s * Sh::OPERAND + b_at, kv ? &tmV : &tmK, b_half * 64, y, &full[s]);
-                r++;
-                if (++s == STAGES) { s = 0; ph ^= 1; }
+                if (lane < b.nt * Sh::HALVES)
+                    kc_load_3d(qst + (lane / Sh::HALVES) * Sh::OPERAND + (lane % Sh::HALVES) * KC_HALF, &tmQ, (lane % Sh::HALVES) * 64, b.kvh * a.G,
+                               b.sq.begin + b.t0 + lane / Sh::HALVES * tq, q_full);
+                queries++;
             }
-            entry = next;
+            for (int i = 0; i < b.n && ok; i++) {
+                const int next = entry_of(i + 1);
+                const int j = b.tile_at(i) + b_sub * box_rows;
+                if (lane < boxes && (unsigned)entry >= (unsigned)a.n_pages) {
+                    if (seen(j)) atomicExch(a.status, ST_PAGE);
+                    entry = 0;                                 // any finite rows do
+                }
+                const int y = (int)kv_row(a, entry, b.kvh, j & ((1 << shift) - 1));
+#pragma unroll
+                for (int kv = 0; kv < 2; kv++) {
+                    if (r >= STAGES && !mbar_wait_warp(&empty[s], (uint32_t)(ph ^ 1))) { ok = false; break; }
+                    if (lane == 0) mbar_expect_tx(&full[s], Sh::OPERAND);
+                    __syncwarp();
+                    if (lane < boxes) tma_load_2d(ring + s * Sh::OPERAND + b_at, kv ? &tmV : &tmK, b_half * 64, y, &full[s]);
+                    if (r < STAGES) r++;
+                    if (++s == STAGES) { s = 0; ph ^= 1; }
+                }
+                entry = next;
+            }
+            if (once) break;
         }
         if (!ok && lane == 0) atomicExch(a.status, ST_TIMEOUT_PRODUCER);
-        for (int t = 0; t < STAGES && t < r; t++) {            // what was asked for has to land before the CTA leaves
+        for (int u = 0; u < STAGES && u < r; u++) {            // what was asked for has to land before the CTA leaves
             if (s == 0) { s = STAGES; ph ^= 1; }
             if (!mbar_wait_warp(&full[--s], (uint32_t)ph)) break;
         }
-        if (!F32 && n > 0) mbar_wait_warp(q_full, 0);
+        if (!F32 && queries > 0) mbar_wait_warp(q_full, (uint32_t)((queries - 1) & 1));
     } else if (warp == Sh::W_MMA) {
         const uint32_t idesc_o = kc_idesc(BF, a.D) | (1u << 16);       // V: MN-major
         const uint64_t qdesc = umma_desc_sw128(smem_u32(qst)), kdesc = umma_desc_sw128(smem_u32(ring)), vdesc = kc_desc_mn(smem_u32(ring));
@@ -294,55 +342,73 @@ kv_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
             if (++s == STAGES) { s = 0; ph ^= 1; }
             return got;
         };
-        bool ok = n > 0 ? mbar_wait_warp(q_full, 0) : true;
-        int sk = 0, sv = 0, lo = 0, hi = 4;
-        if (n > 0) groups(tile_at(0), &lo, &hi);
-        if (ok && n > 0 && (ok = take(&sk))) {
-            tc_fence_after();
-            if (elect_one()) {
-                for (int t = 0; t < nt; t++) { issue_s(t, sk, hi); tc_commit(&s_full[t]); }
-                tc_commit(&empty[sk]);
-            }
-            __syncwarp();
-            ok = take(&sv);
-        }
-        // An issued product keeps the pipe busy for 60 clocks, a wait that has come true costs as much: the waits stand where
-        // products are still under way.
-        for (int i = 0; i < n && ok; i++) {
-            const bool more = i + 1 < n;
-            const int v = sv, start = i == 0 ? lo : -1;
-            int lo2 = 0, hi2 = 4;
-            if (more) groups(tile_at(i + 1), &lo2, &hi2);
-            if (OWN_P && more) {
-                ok = take(&sk);
-                for (int t = 0; t < nt && ok; t++) {
-                    if (!mbar_wait_warp(&s_free[t], (uint32_t)(i & 1))) { ok = false; break; }
+        int done0 = 0, done1 = 0, queries = 0;                 // tiles of keys behind each tile of rows; blocks with queries so far
+        bool ok = true;
+        for (int j = 0; ok; j++) {
+            const KcBlock b = next_block(j);
+            if (b.seq < 0) { ok = b.seq == -1; break; }
+            leave_block(j);
+            const int n = b.n, nt = b.nt;
+            if (n > 0) {
+                int sk = 0, sv = 0, lo, hi;
+                b.groups(a, b.tile_at(0), &lo, &hi);
+                ok = mbar_wait_warp(q_full, (uint32_t)(queries & 1)) && take(&sk);
+                queries++;
+                if (ok) {
                     tc_fence_after();
                     if (elect_one()) {
-                        issue_s(t, sk, hi2); tc_commit(&s_full[t]);
-                        if (t == nt - 1) tc_commit(&empty[sk]);
+                        for (int t = 0; t < nt; t++) { issue_s(t, sk, hi); tc_commit(&s_full[t]); }
+                        tc_commit(&empty[sk]);
                     }
                     __syncwarp();
+                    ok = take(&sv);
                 }
-            }
-            for (int t = 0; t < nt && ok; t++) {
-                if (!mbar_wait_warp(&p_part[t], (uint32_t)(i & 1))) { ok = false; break; }
-                tc_fence_after();
-                if (elect_one()) issue_o(t, v, lo, min(hi, KC_PART), start);
-                __syncwarp();
-                if (more && !OWN_P && t == 0 && !take(&sk)) { ok = false; break; }     // K(i + 1)
-                if (more && t == nt - 1 && !take(&sv)) { ok = false; break; }          // V(i + 1)
-                if (!mbar_wait_warp(&p_full[t], (uint32_t)(i & 1))) { ok = false; break; }
-                tc_fence_after();
-                if (elect_one()) {
-                    issue_o(t, v, max(lo, KC_PART), hi, start);
-                    if (OWN_P || !more) tc_commit(&o_full[t]);
-                    if (more && !OWN_P) { issue_s(t, sk, hi2); tc_commit(&s_full[t]); }
-                    if (t == nt - 1) { tc_commit(&empty[v]); if (more && !OWN_P) tc_commit(&empty[sk]); }
+                // An issued product keeps the pipe busy for 60 clocks, a wait that has come true costs as much: the waits stand where
+                // products are still under way.
+                for (int i = 0; i < n && ok; i++) {
+                    const bool more = i + 1 < n;
+                    const int v = sv, start = i == 0 ? lo : -1;
+                    int lo2 = 0, hi2 = 4;
+                    if (more) b.groups(a, b.tile_at(i + 1), &lo2, &hi2);
+                    if (OWN_P && more) {
+                        ok = take(&sk);
+                        for (int t = 0; t < nt && ok; t++) {
+                            if (!mbar_wait_warp(&s_free[t], (uint32_t)(((t ? done1 : done0) + i) & 1))) { ok = false; break; }
+                            tc_fence_after();
+                            if (elect_one()) {
+                                issue_s(t, sk, hi2); tc_commit(&s_full[t]);
+                                if (t == nt - 1) tc_commit(&empty[sk]);
+                            }
+                            __syncwarp();
+                        }
+                    }
+                    for (int t = 0; t < nt && ok; t++) {
+                        if (!mbar_wait_warp(&p_part[t], (uint32_t)(((t ? done1 : done0) + i) & 1))) { ok = false; break; }
+                        tc_fence_after();
+                        if (elect_one()) issue_o(t, v, lo, min(hi, KC_PART), start);
+                        __syncwarp();
+                        if (more && !OWN_P && t == 0 && !take(&sk)) { ok = false; break; }     // K(i + 1)
+                        if (more && t == nt - 1 && !take(&sv)) { ok = false; break; }          // V(i + 1)
+                        if (!mbar_wait_warp(&p_full[t], (uint32_t)(((t ? done1 : done0) + i) & 1))) { ok = false; break; }
+                        tc_fence_after();
+                        if (elect_one()) {
+                            issue_o(t, v, max(lo, KC_PART), hi, start);
+                            if (OWN_P || !more) tc_commit(&o_full[t]);
+                            if (more && !OWN_P) { issue_s(t, sk, hi2); tc_commit(&s_full[t]); }
+                            if (t == nt - 1) {
+                                tc_commit(&empty[v]);
+                                if (more && !OWN_P) tc_commit(&empty[sk]);
+                                if (!more) tc_commit(q_empty);
+                            }
+                        }
+                        __syncwarp();
+                    }
+                    lo = lo2; hi = hi2;
                 }
-                __syncwarp();
+                done0 += n;
+                if (nt == 2) done1 += n;
             }
-            lo = lo2; hi = hi2;
+            if (once) break;
         }
         if (!ok) {                                             // nothing may run on when tensor memory is given back
             if (lane == 0) atomicExch(a.status, ST_TIMEOUT_MMA);
@@ -353,285 +419,316 @@ kv_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
     }
     } else {
     // ---- softmax: thread = row
-    if (TILES == 2) kc_regs_more();
-    if (F32 && n > 0) {
-        // the warp's 32 rows, neighbouring lanes on neighbouring pieces of eight values
-        constexpr int PIECES = DP / 8, ROWS = 32 / PIECES, ROUNDS = 32 / ROWS, BATCH = 8;
-        uint8_t *qt = qst + t * Sh::PLANES * Sh::OPERAND;
-        const int c = lane % PIECES;
-        bool bad = false;
-        if (t < nt) {
+    kc_regs_more<Sh::MORE>();
+    const float sc = a.scale * 1.4426950408889634f;
+    bool ok = true;
+    int done = 0, blocks = 0;                                  // tiles of keys, and blocks, behind this tile of rows
+    for (int j = 0; ok; j++) {
+        const KcBlock b = next_block(j);
+        if (b.seq < 0) { ok = b.seq == -1; break; }
+        const int n = b.n, tok = b.t0 + t * tq + by_g(r);
+        if (F32 && n > 0) {
+                // the warp's 32 rows, neighbouring lanes on neighbouring pieces of eight values
+                constexpr int PIECES = DP / 8, ROWS = 32 / PIECES, ROUNDS = 32 / ROWS, BATCH = 8;
+                uint8_t *qt = qst + t * Sh::PLANES * Sh::OPERAND;
+                const int c = lane % PIECES;
+                bool bad = false;
+                if (t < b.nt) {
 #pragma unroll 1
-            for (int b = 0; b < ROUNDS; b += BATCH) {
-                float4 in[BATCH][2];
+                    for (int u = 0; u < ROUNDS; u += BATCH) {
+                        float4 in[BATCH][2];
 #pragma unroll
-                for (int i = 0; i < BATCH; i++) {
-                    const int row = (warp & 3) * 32 + (b + i) * ROWS + lane / PIECES, pl = by_g(row), at = t0 + t * tq + pl;
-                    in[i][0] = in[i][1] = make_float4(0.f, 0.f, 0.f, 0.f);
-                    if (row < tq * a.G && at < sq.n && c * 8 < a.D) {
-                        const float4 *p = reinterpret_cast<const float4 *>(static_cast<const float *>(a.q) + (int64_t)(sq.begin + at) * a.ldq +
-                                                                           (int64_t)(kvh * a.G + row - pl * a.G) * a.D + c * 8);
-                        in[i][0] = p[0]; in[i][1] = p[1];
+                        for (int i = 0; i < BATCH; i++) {
+                            const int row = (warp & 3) * 32 + (u + i) * ROWS + lane / PIECES, pl = by_g(row), at = b.t0 + t * tq + pl;
+                            in[i][0] = in[i][1] = make_float4(0.f, 0.f, 0.f, 0.f);
+                            if (row < tq * a.G && at < b.sq.n && c * 8 < a.D) {
+                                const float4 *p = reinterpret_cast<const float4 *>(static_cast<const float *>(a.q) + (int64_t)(b.sq.begin + at) * a.ldq +
+                                                                                   (int64_t)(b.kvh * a.G + row - pl * a.G) * a.D + c * 8);
+                                in[i][0] = p[0]; in[i][1] = p[1];
+                            }
+                        }
+#pragma unroll
+                        for (int i = 0; i < BATCH; i++) {
+                            const int row = (warp & 3) * 32 + (u + i) * ROWS + lane / PIECES;
+                            uint8_t *to = qt + (c >> 3) * KC_HALF + row * 128 + (((c & 7) ^ (row & 7)) << 4);
+                            const float *f = reinterpret_cast<const float *>(in[i]);
+                            uint4 hi, lo;
+#pragma unroll
+                            for (int e = 0; e < 8; e++) bad |= !(fabsf(f[e]) < H16_MAX);
+                            kv_split(f[0], f[1], hi.x, lo.x); kv_split(f[2], f[3], hi.y, lo.y); kv_split(f[4], f[5], hi.z, lo.z); kv_split(f[6], f[7], hi.w, lo.w);
+                            *reinterpret_cast<uint4 *>(to) = hi;
+                            *reinterpret_cast<uint4 *>(to + Sh::OPERAND) = lo;
+                        }
                     }
+                    if (bad) atomicExch(a.status, ST_RANGE);
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");       // generic-proxy stores -> visible to the tensor core
                 }
-#pragma unroll
-                for (int i = 0; i < BATCH; i++) {
-                    const int row = (warp & 3) * 32 + (b + i) * ROWS + lane / PIECES;
-                    uint8_t *to = qt + (c >> 3) * KC_HALF + row * 128 + (((c & 7) ^ (row & 7)) << 4);
-                    const float *f = reinterpret_cast<const float *>(in[i]);
-                    uint4 hi, lo;
-#pragma unroll
-                    for (int e = 0; e < 8; e++) bad |= !(fabsf(f[e]) < H16_MAX);
-                    kv_split(f[0], f[1], hi.x, lo.x); kv_split(f[2], f[3], hi.y, lo.y); kv_split(f[4], f[5], hi.z, lo.z); kv_split(f[6], f[7], hi.w, lo.w);
-                    *reinterpret_cast<uint4 *>(to) = hi;
-                    *reinterpret_cast<uint4 *>(to + Sh::OPERAND) = lo;
-                }
-            }
-            if (bad) atomicExch(a.status, ST_RANGE);
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");       // generic-proxy stores -> visible to the tensor core
+            __syncwarp();
+            if (lane == 0) mbar_arrive(q_full);
         }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(q_full);
-    }
-    if (t < nt) {
-        bool ok = true;
-        // rows that do not exist take the last one's position, so that they need no mask of their own
-        const int pos = base_pos + min(r < tq * a.G ? tok : t0 + t * tq, sq.n - 1);
-        const float sc = a.scale * 1.4426950408889634f;
-        float2 l2[2] = {{0.f, 0.f}, {0.f, 0.f}};
-        for (int i = 0; i < n && ok; i++) {
-            if (!mbar_wait_warp(&s_full[t], (uint32_t)(i & 1))) { ok = false; break; }
-            tc_fence_after();
-            float x[KC_KEYS];
-            tc_ld32(s_at, x);
-            tc_ld32(s_at + 32, x + 32);
-            kc_wait_ld32(x); kc_wait_ld32(x + 32);
-            tc_ld32(s_at + 64, x + 64);
-            tc_ld32(s_at + 96, x + 96);
-            float m4[4] = {x[0], x[1], x[2], x[3]};
-#pragma unroll
-            for (int c = 4; c < 60; c += 8)
-#pragma unroll
-                for (int e = 0; e < 4; e++) m4[e] = fmaxf(m4[e], fmaxf(x[c + e], x[c + 4 + e]));
-#pragma unroll
-            for (int e = 0; e < 4; e++) m4[e] = fmaxf(m4[e], x[60 + e]);
-            kc_wait_ld32(x + 64); kc_wait_ld32(x + 96);
-            if (OWN_P) {                                       // the scores are in registers
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&s_free[t]);
-            }
-#pragma unroll
-            for (int c = 64; c < 128; c += 8)
-#pragma unroll
-                for (int e = 0; e < 4; e++) m4[e] = fmaxf(m4[e], fmaxf(x[c + e], x[c + 4 + e]));
-            const int j0 = tile_at(i), d = pos - j0;
-            const bool whole = d >= KC_KEYS - 1 && (a.window <= 0 || d < a.window || j0 + KC_KEYS - 1 < a.sinks);
-            const bool all = __all_sync(0xffffffffu, whole);
-            if (!all) {                                        // (columns that have no scores are hidden, too)
-                // 32 columns at a time, where some row of the warp does not see them all: a bit per column, visible up to d, above
-                // `under`, or below `keep`
-                const int under = a.window > 0 ? d - a.window : -1, keep = a.sinks - j0;
-                auto upto = [](int c) -> uint32_t { return c < 0 ? 0u : c >= 31 ? 0xffffffffu : (2u << c) - 1u; };      // bits 0 to c
-                m4[0] = m4[1] = m4[2] = m4[3] = -INFINITY;
-#pragma unroll
-                for (int w = 0; w < 4; w++) {
-                    const uint32_t see = upto(d - 32 * w) & (~upto(under - 32 * w) | upto(keep - 1 - 32 * w));
-                    if (!__all_sync(0xffffffffu, see == 0xffffffffu)) {
-#pragma unroll
-                        for (int c = 0; c < 32; c++)
-                            if (!(see >> c & 1)) x[32 * w + c] = -INFINITY;
-                    }
-#pragma unroll
-                    for (int c = 0; c < 32; c += 8)
-#pragma unroll
-                        for (int e = 0; e < 4; e++) m4[e] = fmaxf(m4[e], fmaxf(x[32 * w + c + e], x[32 * w + c + 4 + e]));
-                }
-            }
-            const float mt = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * sc;
-            if (OWN_P && i > 0) {                              // P(i - 1) has been read, and O is at rest
-                if (!mbar_wait_warp(&o_full[t], (uint32_t)((i - 1) & 1))) { ok = false; break; }
+        m = KC_NONE; l = 0.f;
+        if (t < b.nt) {
+            // rows that do not exist take the last one's position, so that they need no mask of their own
+            const int pos = b.base_pos + min(r < tq * a.G ? tok : b.t0 + t * tq, b.sq.n - 1);
+            float2 l2[2] = {{0.f, 0.f}, {0.f, 0.f}};
+            for (int i = 0; i < n && ok; i++) {
+                if (!mbar_wait_warp(&s_full[t], (uint32_t)((done + i) & 1))) { ok = false; break; }
                 tc_fence_after();
-            }
-            const bool grow = mt > m + 8.f;
-            if (__any_sync(0xffffffffu, grow)) {
-                const float alpha = grow ? kv_ex2(m - mt) : 1.f;
-                if (grow) m = mt;
-                l2[0].x *= alpha; l2[0].y *= alpha; l2[1].x *= alpha; l2[1].y *= alpha;
-                if (i > 0) {
-#pragma unroll 1
-                    for (int c = 0; c < DP / 16; c++) {
-                        float o[16];
-                        tc_ld16(o_at + 16 * c, o);
-                        tc_wait_ld();
+                float x[KC_KEYS];
+                tc_ld32(s_at, x);
+                tc_ld32(s_at + 32, x + 32);
+                kc_wait_ld32(x); kc_wait_ld32(x + 32);
+                tc_ld32(s_at + 64, x + 64);
+                tc_ld32(s_at + 96, x + 96);
+                float m4[4] = {x[0], x[1], x[2], x[3]};
 #pragma unroll
-                        for (int e = 0; e < 16; e++) o[e] *= alpha;
-                        kc_st16(o_at + 16 * c, reinterpret_cast<const uint32_t *>(o));
+                for (int c = 4; c < 60; c += 8)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) m4[e] = fmaxf(m4[e], fmaxf(x[c + e], x[c + 4 + e]));
+#pragma unroll
+                for (int e = 0; e < 4; e++) m4[e] = fmaxf(m4[e], x[60 + e]);
+                kc_wait_ld32(x + 64); kc_wait_ld32(x + 96);
+                if (OWN_P) {                                       // the scores are in registers
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&s_free[t]);
+                }
+#pragma unroll
+                for (int c = 64; c < 128; c += 8)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) m4[e] = fmaxf(m4[e], fmaxf(x[c + e], x[c + 4 + e]));
+                const int j0 = b.tile_at(i), d = pos - j0;
+                const bool whole = d >= KC_KEYS - 1 && (a.window <= 0 || d < a.window || j0 + KC_KEYS - 1 < a.sinks);
+                const bool all = __all_sync(0xffffffffu, whole);
+                if (!all) {                                        // (columns that have no scores are hidden, too)
+                    // 32 columns at a time, where some row of the warp does not see them all: a bit per column, visible up to d, above
+                    // `under`, or below `keep`
+                    const int under = a.window > 0 ? d - a.window : -1, keep = a.sinks - j0;
+                    auto upto = [](int c) -> uint32_t { return c < 0 ? 0u : c >= 31 ? 0xffffffffu : (2u << c) - 1u; };      // bits 0 to c
+                    m4[0] = m4[1] = m4[2] = m4[3] = -INFINITY;
+#pragma unroll
+                    for (int w = 0; w < 4; w++) {
+                        const uint32_t see = upto(d - 32 * w) & (~upto(under - 32 * w) | upto(keep - 1 - 32 * w));
+                        if (!__all_sync(0xffffffffu, see == 0xffffffffu)) {
+#pragma unroll
+                            for (int c = 0; c < 32; c++)
+                                if (!(see >> c & 1)) x[32 * w + c] = -INFINITY;
+                        }
+#pragma unroll
+                        for (int c = 0; c < 32; c += 8)
+#pragma unroll
+                            for (int e = 0; e < 4; e++) m4[e] = fmaxf(m4[e], fmaxf(x[32 * w + c + e], x[32 * w + c + 4 + e]));
                     }
                 }
-            }
-            const float2 sc2 = make_float2(sc, sc), neg = make_float2(-m, -m);
-            auto open = [&](int c) {                           // the exponentials of 16 keys, in place
-#pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    float *v = x + c * 16 + 2 * e;
-                    const float2 y = kv_fma2(make_float2(v[0], v[1]), sc2, neg);
-                    v[0] = kv_ex2(y.x); v[1] = kv_ex2(y.y);
+                const float mt = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * sc;
+                if (OWN_P && i > 0) {                              // P(i - 1) has been read, and O is at rest
+                    if (!mbar_wait_warp(&o_full[t], (uint32_t)((done + i - 1) & 1))) { ok = false; break; }
+                    tc_fence_after();
                 }
-            };
-            auto close = [&](int c) {                          // summed, packed and stored
-                uint32_t hi[8], lo[F32 ? 8 : 1];
-#pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    const float *v = x + c * 16 + 2 * e;
-                    l2[e & 1] = kv_add2(l2[e & 1], make_float2(v[0], v[1]));
-                    if (F32) kv_split(v[0], v[1], hi[e], lo[F32 ? e : 0]);
-                    else hi[e] = kv_pack<BF>(v[0], v[1]);
-                }
-                kc_st8(p_at + 8 * c, hi);
-                if (F32) kc_st8(p_at + 64 + 8 * c, lo);
-            };
-            auto ready = [&](uint64_t *bar) {
-                kc_wait_st();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(bar);
-            };
-            // some keys' exponentials are under way while those before are summed, packed and stored
-            if (Sh::WHOLE && all) {
-#pragma unroll
-                for (int c = 0; c <= 8; c++) {
-                    if (c < 8) open(c);
-                    if (c > 0) close(c - 1);
-                    if (c == 2 * KC_PART) ready(&p_part[t]);
-                }
-            } else {
-                int lo, hi;
-                groups(j0, &lo, &hi);
-#pragma unroll
-                for (int c = 0; c <= 4; c++) {
-                    if (c < 4 && c >= lo && c < hi) { open(2 * c); open(2 * c + 1); }
-                    if (c > 0 && c > lo && c <= hi) { close(2 * c - 2); close(2 * c - 1); }
-                    if (c == KC_PART) ready(&p_part[t]);
-                }
-            }
-            ready(&p_full[t]);
-        }
-        if (n > 0 && ok) ok = mbar_wait_warp(&o_full[t], (uint32_t)(OWN_P ? (n - 1) & 1 : 0));
-        if (!ok && lane == 0) atomicExch(a.status, ST_TIMEOUT_EPILOGUE);
-        tc_fence_after();
-        l = (l2[0].x + l2[0].y) + (l2[1].x + l2[1].y);
-    }
-    }
-    if (shares == 1) {
-        // through shared memory, where the tile's queries were (its products are done): a warp's 32 rows in pieces of 16 bytes, turned by
-        // the row so that both sides touch all banks, and out in whole rows
-        if (soft && rank == 0 && t < nt) {
-            constexpr int PIECE = F32 ? 4 : 8, PIECES = DP / PIECE;            // values of 16 bytes; pieces of a row
-            uint8_t *stage = qst + t * Sh::PLANES * Sh::OPERAND + (warp & 3) * (32 * PIECES * 16);
-            const float inv = l != 0.f ? 1.f / l : 0.f;
+                const bool grow = mt > m + 8.f;
+                if (__any_sync(0xffffffffu, grow)) {
+                    const float alpha = grow ? kv_ex2(m - mt) : 1.f;
+                    if (grow) m = mt;
+                    l2[0].x *= alpha; l2[0].y *= alpha; l2[1].x *= alpha; l2[1].y *= alpha;
+                    if (i > 0) {
 #pragma unroll 1
-            for (int c = 0; c < DP / 32; c++) {
-                float o[32];
-                if (n > 0) {
+                        for (int c = 0; c < DP / 16; c++) {
+                            float o[16];
+                            tc_ld16(o_at + 16 * c, o);
+                            tc_wait_ld();
+#pragma unroll
+                            for (int e = 0; e < 16; e++) o[e] *= alpha;
+                            kc_st16(o_at + 16 * c, reinterpret_cast<const uint32_t *>(o));
+                        }
+                    }
+                }
+                const float2 sc2 = make_float2(sc, sc), neg = make_float2(-m, -m);
+                auto open = [&](int c) {                           // the exponentials of 16 keys, in place
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        float *v = x + c * 16 + 2 * e;
+                        const float2 y = kv_fma2(make_float2(v[0], v[1]), sc2, neg);
+                        v[0] = kv_ex2(y.x); v[1] = kv_ex2(y.y);
+                    }
+                };
+                auto close = [&](int c) {                          // summed, packed and stored
+                    uint32_t hi[8], lo[F32 ? 8 : 1];
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        const float *v = x + c * 16 + 2 * e;
+                        l2[e & 1] = kv_add2(l2[e & 1], make_float2(v[0], v[1]));
+                        if (F32) kv_split(v[0], v[1], hi[e], lo[F32 ? e : 0]);
+                        else hi[e] = kv_pack<BF>(v[0], v[1]);
+                    }
+                    kc_st8(p_at + 8 * c, hi);
+                    if (F32) kc_st8(p_at + 64 + 8 * c, lo);
+                };
+                auto ready = [&](uint64_t *bar) {
+                    kc_wait_st();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(bar);
+                };
+                // some keys' exponentials are under way while those before are summed, packed and stored
+                if (Sh::WHOLE && all) {
+#pragma unroll
+                    for (int c = 0; c <= 8; c++) {
+                        if (c < 8) open(c);
+                        if (c > 0) close(c - 1);
+                        if (c == 2 * KC_PART) ready(&p_part[t]);
+                    }
+                } else {
+                    int lo, hi;
+                    b.groups(a, j0, &lo, &hi);
+#pragma unroll
+                    for (int c = 0; c <= 4; c++) {
+                        if (c < 4 && c >= lo && c < hi) { open(2 * c); open(2 * c + 1); }
+                        if (c > 0 && c > lo && c <= hi) { close(2 * c - 2); close(2 * c - 1); }
+                        if (c == KC_PART) ready(&p_part[t]);
+                    }
+                }
+                ready(&p_full[t]);
+            }
+            if (n > 0 && ok) ok = mbar_wait_warp(&o_full[t], (uint32_t)(OWN_P ? (done + n - 1) & 1 : blocks & 1));
+            if (n > 0) { done += n; blocks++; }
+            tc_fence_after();
+            l = (l2[0].x + l2[0].y) + (l2[1].x + l2[1].y);
+            // (what the results need of the block is read again, so that it takes no registers above)
+            const KcBlock e(a, items + (j & 1) * 8, tq, TILES, size, rank);
+            if (e.shares == 1 && rank == 0 && ok) {
+                const int tok = e.t0 + t * tq + by_g(r);
+                const float inv = l != 0.f ? 1.f / l : 0.f;
+                const bool valid = r < tq * a.G && tok < e.sq.n;
+                const int64_t to = (int64_t)(e.sq.begin + tok) * a.ldo + (int64_t)(e.kvh * a.G + r - by_g(r) * a.G) * a.D;
+#pragma unroll 1
+                for (int c = 0; c < DP / 32; c++) {
+                    float o[32];
+                    if (n > 0) {
+                        tc_ld32(o_at + 32 * c, o);
+                        kc_wait_ld32(o);
+                    }
+#pragma unroll
+                    for (int u = 0; u < 32; u++) o[u] = inv != 0.f ? o[u] * inv : 0.f;
+                    if (valid) {
+#pragma unroll
+                        for (int u = 0; u < 32; u += 8) {
+                            if (c * 32 + u >= a.D) continue;
+                            if (F32) {
+                                float4 *p = reinterpret_cast<float4 *>(static_cast<float *>(a.out) + to + c * 32 + u);
+                                p[0] = make_float4(o[u], o[u + 1], o[u + 2], o[u + 3]);
+                                p[1] = make_float4(o[u + 4], o[u + 5], o[u + 6], o[u + 7]);
+                            } else {
+                                *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(a.out) + to + c * 32 + u) =
+                                    make_uint4(kv_pack<BF>(o[u], o[u + 1]), kv_pack<BF>(o[u + 2], o[u + 3]), kv_pack<BF>(o[u + 4], o[u + 5]), kv_pack<BF>(o[u + 6], o[u + 7]));
+                            }
+                        }
+                    }
+                    __syncwarp();
+                }
+                tc_fence_before();                             // (the next block's products are ordered behind these loads by its P)
+            }
+        }
+        leave_block(j);
+        if (once) break;
+    }
+    if (!ok && lane == 0) atomicExch(a.status, ST_TIMEOUT_EPILOGUE);
+    }
+    __syncwarp();
+    if (once) {
+        __syncthreads();                                       // (the TMA warp has written the block's words)
+        const KcBlock b(a, items, tq, TILES, size, rank);
+        if (b.shares > 1) {
+            // parts of the rows' results and (maximum, sum) of each, where queries and tiles were; then the weights of the parts, and their sum
+            // by all CTAs of the cluster, each for its rows
+            float *part = reinterpret_cast<float *>(qst), *weight = part + TILES * 128 * (Sh::LDO + 2);
+            float2 *ml = reinterpret_cast<float2 *>(part + TILES * 128 * Sh::LDO);
+            __syncthreads();                                       // (both tiles' products have been waited for)
+            if (soft && t < b.nt && b.n > 0) {
+                float *row = part + (t * 128 + r) * Sh::LDO;
+#pragma unroll 1
+                for (int c = 0; c < DP / 32; c++) {
+                    float o[32];
                     tc_ld32(o_at + 32 * c, o);
                     tc_wait_ld();
+#pragma unroll
+                    for (int e = 0; e < 32; e += 4) *reinterpret_cast<float4 *>(row + c * 32 + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                }
+                ml[t * 128 + r] = make_float2(m, l);
+            }
+            kv_cluster_sync();
+            const uint32_t part0 = smem_u32(part), ml0 = smem_u32(ml);
+            const int per_tile = tq * a.G, rows = min((b.last - b.t0 + 1) * a.G, b.nt * per_tile), share = (rows + size - 1) >> log_size;
+            const int v0 = rank * share, mine = max(0, min(share, rows - v0)), quads = a.D / 4;
+            auto place_of = [&](int v) { return v < per_tile ? v : 128 + v - per_tile; };
+            for (int v = threadIdx.x; v < mine; v += Sh::THREADS) {
+                const int at = place_of(v0 + v);
+                float2 e[16];
+                float top_m = KC_NONE, total = 0.f;
+#pragma unroll
+                for (int p = 0; p < 16; p++) {
+                    e[p] = make_float2(KC_NONE, 0.f);
+                    if (p < b.shares) e[p] = kv_peer2(kv_peer(ml0 + at * 8, p));
                 }
 #pragma unroll
-                for (int e = 0; e < 32; e++) o[e] = inv != 0.f ? o[e] * inv : 0.f;
+                for (int p = 0; p < 16; p++) top_m = fmaxf(top_m, e[p].x);
 #pragma unroll
-                for (int e = 0; e < 32; e += PIECE) {
-                    const int k = c * (32 / PIECE) + e / PIECE;
-                    uint4 v;
-                    if (F32) v = make_uint4(__float_as_uint(o[e]), __float_as_uint(o[e + 1]), __float_as_uint(o[e + 2]), __float_as_uint(o[e + 3]));
-                    else v = make_uint4(kv_pack<BF>(o[e], o[e + 1]), kv_pack<BF>(o[e + 2], o[e + 3]), kv_pack<BF>(o[e + (F32 ? 0 : 4)], o[e + (F32 ? 0 : 5)]), kv_pack<BF>(o[e + (F32 ? 0 : 6)], o[e + (F32 ? 0 : 7)]));
-                    *reinterpret_cast<uint4 *>(stage + (lane * PIECES + (k ^ (lane & 7))) * 16) = v;
+                for (int p = 0; p < 16; p++) {
+                    e[p].x = kv_ex2(e[p].x - top_m);
+                    total = fmaf(e[p].x, e[p].y, total);
                 }
+                const float inv = total != 0.f ? 1.f / total : 0.f;
+#pragma unroll
+                for (int p = 0; p < 16; p++)
+                    if (p < b.shares) weight[v * 16 + p] = e[p].x * inv;
             }
-            __syncwarp();
-            const int k = lane % PIECES;
-#pragma unroll 4
-            for (int i = 0; i < PIECES; i++) {                 // 32 / PIECES rows each
-                const int row = i * (32 / PIECES) + lane / PIECES, rt = (warp & 3) * 32 + row, pl = by_g(rt), at = t0 + t * tq + pl;
-                if (rt < tq * a.G && at < sq.n && k * PIECE < a.D) {
-                    const uint4 v = *reinterpret_cast<const uint4 *>(stage + (row * PIECES + (k ^ (row & 7))) * 16);
-                    const int64_t to = (int64_t)(sq.begin + at) * a.ldo + (int64_t)(kvh * a.G + rt - pl * a.G) * a.D + k * PIECE;
-                    *reinterpret_cast<uint4 *>(static_cast<uint8_t *>(a.out) + to * (F32 ? 4 : 2)) = v;
-                }
-            }
-        }
-    } else {
-        // parts of the rows' results and (maximum, sum) of each, where queries and tiles were; then the weights of the parts, and their sum
-        // by all CTAs of the cluster, each for its rows
-        float *part = reinterpret_cast<float *>(qst), *weight = part + TILES * 128 * (Sh::LDO + 2);
-        float2 *ml = reinterpret_cast<float2 *>(part + TILES * 128 * Sh::LDO);
-        __syncthreads();                                       // (both tiles' products have been waited for)
-        if (soft && t < nt && n > 0) {
-            float *row = part + (t * 128 + r) * Sh::LDO;
-#pragma unroll 1
-            for (int c = 0; c < DP / 32; c++) {
-                float o[32];
-                tc_ld32(o_at + 32 * c, o);
-                tc_wait_ld();
+            __syncthreads();
+            for (int u = threadIdx.x; u < mine * quads; u += Sh::THREADS) {
+                const int v = u / quads, c = (u - v * quads) * 4, at = place_of(v0 + v);
+                float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+                for (int p0 = 0; p0 < b.shares; p0 += 4) {
+                    float4 o[4];
 #pragma unroll
-                for (int e = 0; e < 32; e += 4) *reinterpret_cast<float4 *>(row + c * 32 + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
-            }
-            ml[t * 128 + r] = make_float2(m, l);
-        }
-        kv_cluster_sync();
-        const uint32_t part0 = smem_u32(part), ml0 = smem_u32(ml);
-        const int per_tile = tq * a.G, rows = min((last - t0 + 1) * a.G, nt * per_tile), share = (rows + size - 1) >> log_size;
-        const int v0 = rank * share, mine = max(0, min(share, rows - v0)), quads = a.D / 4;
-        auto place_of = [&](int v) { return v < per_tile ? v : 128 + v - per_tile; };
-        for (int v = threadIdx.x; v < mine; v += Sh::THREADS) {
-            const int at = place_of(v0 + v);
-            float2 e[16];
-            float top_m = KC_NONE, total = 0.f;
-#pragma unroll
-            for (int p = 0; p < 16; p++) {
-                e[p] = make_float2(KC_NONE, 0.f);
-                if (p < shares) e[p] = kv_peer2(kv_peer(ml0 + at * 8, p));
-            }
-#pragma unroll
-            for (int p = 0; p < 16; p++) top_m = fmaxf(top_m, e[p].x);
-#pragma unroll
-            for (int p = 0; p < 16; p++) {
-                e[p].x = kv_ex2(e[p].x - top_m);
-                total = fmaf(e[p].x, e[p].y, total);
-            }
-            const float inv = total != 0.f ? 1.f / total : 0.f;
-#pragma unroll
-            for (int p = 0; p < 16; p++)
-                if (p < shares) weight[v * 16 + p] = e[p].x * inv;
-        }
-        __syncthreads();
-        for (int u = threadIdx.x; u < mine * quads; u += Sh::THREADS) {
-            const int v = u / quads, c = (u - v * quads) * 4, at = place_of(v0 + v);
-            float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-            for (int p0 = 0; p0 < shares; p0 += 4) {
-                float4 o[4];
-#pragma unroll
-                for (int p = 0; p < 4; p++) {
-                    o[p] = make_float4(0.f, 0.f, 0.f, 0.f);
-                    if (p0 + p < shares) o[p] = kv_peer4(kv_peer(part0 + (at * Sh::LDO + c) * 4, p0 + p));
-                }
-#pragma unroll
-                for (int p = 0; p < 4; p++)
-                    if (p0 + p < shares) {
-                        const float w = weight[v * 16 + p0 + p];
-                        sum.x = fmaf(w, o[p].x, sum.x); sum.y = fmaf(w, o[p].y, sum.y); sum.z = fmaf(w, o[p].z, sum.z); sum.w = fmaf(w, o[p].w, sum.w);
+                    for (int p = 0; p < 4; p++) {
+                        o[p] = make_float4(0.f, 0.f, 0.f, 0.f);
+                        if (p0 + p < b.shares) o[p] = kv_peer4(kv_peer(part0 + (at * Sh::LDO + c) * 4, p0 + p));
                     }
+#pragma unroll
+                    for (int p = 0; p < 4; p++)
+                        if (p0 + p < b.shares) {
+                            const float w = weight[v * 16 + p0 + p];
+                            sum.x = fmaf(w, o[p].x, sum.x); sum.y = fmaf(w, o[p].y, sum.y); sum.z = fmaf(w, o[p].z, sum.z); sum.w = fmaf(w, o[p].w, sum.w);
+                        }
+                }
+                const int pl = by_g(v0 + v);
+                const int64_t to = (int64_t)(b.sq.begin + b.t0 + pl) * a.ldo + (int64_t)(b.kvh * a.G + v0 + v - pl * a.G) * a.D + c;
+                if (F32) *reinterpret_cast<float4 *>(static_cast<float *>(a.out) + to) = sum;
+                else *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(a.out) + to) = make_uint2(kv_pack<BF>(sum.x, sum.y), kv_pack<BF>(sum.z, sum.w));
             }
-            const int pl = by_g(v0 + v);
-            const int64_t to = (int64_t)(sq.begin + t0 + pl) * a.ldo + (int64_t)(kvh * a.G + v0 + v - pl * a.G) * a.D + c;
-            if (F32) *reinterpret_cast<float4 *>(static_cast<float *>(a.out) + to) = sum;
-            else *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(a.out) + to) = make_uint2(kv_pack<BF>(sum.x, sum.y), kv_pack<BF>(sum.z, sum.w));
+            kv_cluster_sync();                                     // nobody leaves while its part is being read
         }
-        kv_cluster_sync();                                     // nobody leaves while its part is being read
     }
     tc_fence_before();
     __syncthreads();
     if (warp == Sh::W_MMA) tc_dealloc(tmem, Sh::TMEM);
+}
+
+// Clusters of 2^k CTAs that run at a time on the current device with a CTA per SM; -1 with the error set
+template <int DP, int FMT>
+static int most_clusters(int k) {
+    using Sh = ChunkShape<DP, FMT>;
+    static PerDevice known[5] = {};                            // (the number and one)
+    int dev = 0;
+    if (!known[k].below(1, &dev)) return (int)known[k].v[dev] - 1;
+    cudaLaunchConfig_t lc = {};
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = 1u << k; at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    lc.gridDim = dim3(1u << k); lc.blockDim = dim3(Sh::THREADS); lc.dynamicSmemBytes = Sh::SMEM;
+    lc.attrs = at; lc.numAttrs = 1;
+    int n = 0;
+    MB_CUDA(cudaOccupancyMaxActiveClusters(&n, kv_chunk_kernel<DP, FMT>, &lc));
+    known[k].record(dev, (size_t)n + 1);
+    return n;
 }
 
 template <int DP, int FMT>
@@ -643,24 +740,33 @@ static int chunk_launch(const CUtensorMap &k, const CUtensorMap &v, const KvArgs
     if (configured.below((size_t)Sh::SMEM, &dev)) {
         cudaFuncAttributes at;
         MB_CUDA(cudaFuncGetAttributes(&at, kernel));
-        if (Sh::TILES == 2 && at.numRegs != KC_REGS) { set_error("kv_attend: the kernel was built with %d registers, not %d", at.numRegs, KC_REGS); return -1; }
+        if (at.numRegs < Sh::REGS) { set_error("kv_attend: the kernel was built with %d registers, not %d", at.numRegs, Sh::REGS); return -1; }
         MB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::SMEM));
         MB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
         configured.record(dev, (size_t)Sh::SMEM);
     }
     const int per_block = Sh::TILES * (KC_ROWS / a.G);
     const int64_t full = ((int64_t)a.n_rows + per_block - 1) / per_block, seqs = a.n_seq < a.n_rows ? a.n_seq : a.n_rows;
-    const int64_t blocks = a.n_rows / per_block + seqs;        // the last block of each sequence may be short
-    // Clusters where the blocks that are likely (whole ones, or one per sequence) leave SMs without work, as large as those fill
+    const int64_t blocks = (a.n_rows / per_block + seqs) * a.Hkv;              // the last block of each sequence may be short
+    // Clusters where the blocks that are likely (whole ones, or one per sequence) leave SMs without work: the largest of which as many
+    // run at a time (with one CTA per SM a GPU of 148 has room for fewer than eight clusters of 16)
     const int64_t likely = (full > seqs ? full : seqs) * a.Hkv;
     int log_size = 0;
-    if (const char *e = getenv("KV_S")) log_size = atoi(e);
-    else while (log_size < 4 && likely << (log_size + 1) <= Sh::PER_SM * device_sm_count() && (int64_t)KC_KEYS * 2 << log_size < ((int64_t)a.max_pages << a.page_shift)) log_size++;
+    for (int k = 1; k <= 4 && (int64_t)KC_KEYS << k < ((int64_t)a.max_pages << a.page_shift); k++) {
+        const int most = most_clusters<DP, FMT>(k);
+        if (most < 0) return -1;
+        if (likely <= (int64_t)Sh::PER_SM * most) log_size = k;
+    }
     if (blocks << log_size > 0x7fffffff) { set_error("kv_attend: too many rows in one call"); return -1; }
+    // Where blocks are short, as many CTAs as fit take one after the other; where they are long, the hardware deals them out better than a
+    // fixed order (32 and 8 heads of 128, us, that way and with a CTA per block: 8 x 500 rows 49, 52, 4 x 2000 162, 175; 8000 490, 454)
+    const int64_t keys = (int64_t)a.max_pages << a.page_shift, seen = (int64_t)a.window + a.sinks + per_block;
+    const bool stay = (a.window > 0 && seen < keys ? seen : keys) <= KC_STAY;
+    const int64_t room = (int64_t)Sh::PER_SM * device_sm_count();
+    const int64_t ctas = log_size ? blocks << log_size : stay && blocks > room ? room : blocks;
     CUtensorMap q = k;
     if (FMT != KV_F32 && !kv_rows_map(&q, a, FMT == KV_BF16)) { set_error("kv_attend: no tensor map of the rows"); return -1; }
-    MB_CUDA(launch_kernel(kernel, dim3((unsigned)(blocks << log_size), (unsigned)a.Hkv), dim3(Sh::THREADS), (size_t)Sh::SMEM, st, true, 1 << log_size, q, k, v, a,
-                          box_rows, log_size));
+    MB_CUDA(launch_kernel(kernel, dim3((unsigned)ctas), dim3(Sh::THREADS), (size_t)Sh::SMEM, st, true, 1 << log_size, q, k, v, a, box_rows, log_size));
     note_launch();
     return 0;
 }

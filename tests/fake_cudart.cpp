@@ -145,6 +145,7 @@ cudaError_t cudaGetLastError() { const cudaError_t e = last_error; last_error = 
 const char *cudaGetErrorString(cudaError_t) { return "an error of the fake runtime"; }
 cudaError_t cudaGetSymbolAddress(void **p, const void *) { *p = nullptr; return cudaErrorInvalidSymbol; }
 cudaError_t cudaFuncSetAttribute(const void *, cudaFuncAttribute, int) { return cudaSuccess; }
+cudaError_t cudaOccupancyMaxActiveClusters(int *n, const void *, const cudaLaunchConfig_t *c) { *n = 148 / (int)c->attrs[0].val.clusterDim.x; return cudaSuccess; }
 cudaError_t cudaFuncGetAttributes(cudaFuncAttributes *a, const void *) { memset(a, 0, sizeof(*a)); a->numRegs = 168; return cudaSuccess; }
 cudaError_t cudaOccupancyMaxActiveBlocksPerMultiprocessorWithFlags(int *n, const void *, int, size_t, unsigned) { *n = 1; return cudaSuccess; }
 cudaError_t cudaGetDriverEntryPoint(const char *, void **p, unsigned long long, cudaDriverEntryPointQueryResult *q) {

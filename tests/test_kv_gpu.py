@@ -467,7 +467,7 @@ def test_two_graphs_and_streams_at_once(gpu_pkg, rows):
 
 
 def test_same_bits_every_time_and_beside_others(gpu_pkg):
-    """No atomics in sums: a call gives its bits again, from any stream and thread, and a sequence of rows gives the same bits alone."""
+    """No atomics in sums: a call gives its bits again, from any stream and thread, and a sequence gives the same bits beside others."""
     from concurrent.futures import ThreadPoolExecutor
     for rows in (None, [30, 129, 300]):
         lay = P.Layout([900, 2000, 333], 16, rows)
@@ -490,13 +490,24 @@ def test_same_bits_every_time_and_beside_others(gpu_pkg):
         torch.cuda.synchronize()
         with ThreadPoolExecutor(4) as pool:
             assert all(pool.map(one, range(8)))
-        if rows:
-            begin = 30
-            alone = torch.zeros(129, 512, device="cuda")
-            b = cache.batch(lay.len_dev[1:2].contiguous(), lay.table_dev[1:2].contiguous(), row_off=torch.tensor([0, 129], dtype=torch.int32).cuda(), n_rows=129)
-            cache.attend(b, q[begin:begin + 129], alone, stream=here())
-            cache.sync(here())
-            assert torch.equal(alone, first[begin:begin + 129])
+        # beside other sequences, in a call of as many rows and sequences: how a sequence is cut does not depend on the others
+        order, other = [2, 1, 0], P.Layout([333, 2000, 7], 16, [300, 129, 7] if rows else None, seed=5)
+        table = other.table.clone()
+        table[:, :] = -1
+        for to, (at, keep) in enumerate(((2, True), (1, True), (0, False))):
+            n = min(table.shape[1], lay.table.shape[1])
+            table[to, :n] = lay.table[at, :n] if keep else lay.table[0, :n]
+        n_rows = lay.n_rows
+        q2 = torch.zeros(n_rows, 512, device="cuda")
+        begin2 = other.begin
+        for to, at in enumerate(order[:2]):
+            q2[begin2[to]:begin2[to] + lay.rows[at]] = q[lay.begin[at]:lay.begin[at] + lay.rows[at]]
+        out2 = torch.zeros_like(q2)
+        b2 = cache.batch(other.len_dev, table.cuda(), row_off=other.off_dev, n_rows=n_rows)
+        cache.attend(b2, q2, out2, stream=here())
+        cache.sync(here())
+        for to, at in enumerate(order[:2]):
+            assert torch.equal(out2[begin2[to]:begin2[to] + lay.rows[at]], first[lay.begin[at]:lay.begin[at] + lay.rows[at]])
 
 
 def test_offsets_beyond_32_bits(gpu_pkg):
