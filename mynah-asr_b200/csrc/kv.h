@@ -14,7 +14,7 @@ struct KvArgs {
     int H, Hkv, G, D;                                // G = H / Hkv query heads share a kv head
     int page_shift, n_pages;
     int window, sinks;
-    float scale;
+    float scale2;                                    // of scores, for powers of two
     uint16_t *k, *v;                                 // pools
     int *status;
     // the call

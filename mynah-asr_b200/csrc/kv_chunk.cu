@@ -30,23 +30,28 @@ static constexpr float KC_NONE = -1e30f;             // "maximum" of no keys
 
 template <int DP, int FMT> struct ChunkShape {
     static constexpr int HALVES = DP / 64, PLANES = FMT == KV_F32 ? 2 : 1;
-    static constexpr int TILES = DP == 64 ? 1 : 2, PER_SM = DP == 64 ? 2 : 1;          // tiles of rows of a CTA, CTAs of an SM
+    // F32 rows: the tensor cores cut every sum toward zero, which over 1000 keys costs 5e-6 of a result; so a tile's P V is a sum of its
+    // own, in columns F, that the softmax warps add to O
+    static constexpr bool FRESH = FMT == KV_F32;
+    static constexpr int TILES = DP == 64 || FRESH ? 1 : 2, PER_SM = DP == 64 ? 2 : 1;         // tiles of rows of a CTA, CTAs of an SM
     static constexpr int SOFT = 4 * TILES, W_TMA = SOFT, W_MMA = SOFT + 1;             // warps
     // The launch's registers are dealt out anew between the softmax warps and the four warps of TMA and MMA, two of which have no other
     // work than to lend theirs
+    static constexpr bool DEAL = TILES == 2 || PER_SM == 2;
     static constexpr int THREADS = 32 * (SOFT + 4), REGS = TILES == 2 ? 168 : 128, MORE = TILES == 2 ? 208 : 192, LESS = TILES == 2 ? 88 : 64;
-    static_assert(32 * SOFT * MORE + 128 * LESS <= THREADS * REGS, "a share beyond the launch's registers waits for good");
+    static_assert(!DEAL || 32 * SOFT * MORE + 128 * LESS <= THREADS * REGS, "a share beyond the launch's registers waits for good");
     static constexpr int OPERAND = HALVES * KC_HALF;           // a tile of queries (one plane), of keys, or of values
     static constexpr int Q = TILES * PLANES * OPERAND;
-    static constexpr int STAGES = DP == 64 ? 6 - PLANES : PLANES == 1 ? 5 : 3;
+    static constexpr int STAGES = DP == 64 ? 6 - PLANES : 5;
     static constexpr int SMEM = KC_HEAD + Q + STAGES * OPERAND + 1024;
     static_assert(PER_SM * (SMEM + 1024) <= 233472, "shared memory");
-    static constexpr bool OWN_P = DP == 64 && PLANES == 1;     // columns of their own for the probabilities
+    static constexpr bool OWN_P = TILES == 1 && (DP == 64) == (PLANES == 1);   // columns of their own for the probabilities
     // a path of its own for tiles that all rows see: more code, which pays where most tiles are such
     static constexpr bool WHOLE = DP == 128 && PLANES == 1;
-    static constexpr int COL_S = 0, COL_P = OWN_P ? 128 * TILES : 0, STEP_P = OWN_P ? 64 : 128, COL_O = 128 * TILES + (OWN_P ? 64 * TILES : 0);
+    static constexpr int COL_S = 0, COL_P = OWN_P ? 128 * TILES : 0, STEP_P = OWN_P ? 64 * PLANES : 128, COL_O = 128 * TILES + (OWN_P ? STEP_P * TILES : 0);
+    static constexpr int COL_F = COL_O + (FRESH ? TILES * DP : 0);     // where P V goes
     static constexpr int TMEM = 512 / PER_SM;
-    static_assert(COL_O + TILES * DP <= TMEM, "tensor memory");
+    static_assert(COL_F + TILES * DP <= TMEM, "tensor memory");
     static constexpr int LDO = DP + 4;                         // a part of a row's result in shared memory
     static_assert(TILES * 128 * (LDO * 4 + 8 + 64) <= Q + STAGES * OPERAND, "parts");
 };
@@ -237,11 +242,22 @@ kv_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
     const int t = TILES == 2 ? (warp >> 2) & 1 : 0, r = (warp & 3) * 32 + lane;
     const bool soft = warp < Sh::SOFT;
     const uint32_t trow = tmem + ((uint32_t)((warp & 3) * 32) << 16), s_at = trow + Sh::COL_S + t * 128, p_at = trow + Sh::COL_P + t * Sh::STEP_P,
-                   o_at = trow + Sh::COL_O + t * DP;
+                   o_at = trow + Sh::COL_O + t * DP, f_at = trow + Sh::COL_F + t * DP;
     float m = KC_NONE, l = 0.f;                                // of the row: running maximum and sum
+    auto result = [&](int n, int c, float *o) {                // 32 columns of the row's result over n tiles
+        tc_ld32(f_at + 32 * c, o);
+        kc_wait_ld32(o);
+        if (Sh::FRESH && n > 1) {
+            float more[32];
+            tc_ld32(o_at + 32 * c, more);
+            kc_wait_ld32(more);
+#pragma unroll
+            for (int e = 0; e < 32; e++) o[e] += more[e];
+        }
+    };
 
     if (!soft) {
-    kc_regs_less<Sh::LESS>();                                  // (one instruction for the four warps)
+    if (Sh::DEAL) kc_regs_less<Sh::LESS>();                    // (one instruction for the four warps)
     if (warp == Sh::W_TMA) {
         // ---- lane = one box of a tile: 64 of the D columns, the slots of one page. Item 2 i of the ring is K(i), 2 i + 1 V(i).
         const int shift = a.page_shift, boxes = KC_KEYS / box_rows * Sh::HALVES;
@@ -313,27 +329,26 @@ kv_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
             const uint64_t kd = kdesc + (uint64_t)((s * Sh::OPERAND) >> 4);
             const uint32_t idesc = kc_idesc(BF, 32 * hi);
 #pragma unroll
-            for (int plane = 0; plane < Sh::PLANES; plane++) {
+            for (int plane = Sh::PLANES - 1; plane >= 0; plane--) {            // (the small products first: every sum is cut to the accumulator's bits)
                 const uint64_t qd = qdesc + (uint64_t)(((t * Sh::PLANES + plane) * Sh::OPERAND) >> 4);
 #pragma unroll
                 for (int kk = 0; kk < DP / 16; kk++) {
                     const uint64_t ko = (uint64_t)(((kk >> 2) * KC_HALF + (kk & 3) * 32) >> 4);
-                    if (kk < steps) tc_mma_f16(tmem + Sh::COL_S + t * 128, qd + ko, kd + ko, idesc, (kk | plane) != 0);
+                    if (kk < steps) tc_mma_f16(tmem + Sh::COL_S + t * 128, qd + ko, kd + ko, idesc, kk != 0 || plane != Sh::PLANES - 1);
                 }
             }
         };
-        // groups [k0, k1) of P V; group `start` of the first tile begins the sum
+        // groups [k0, k1) of P V, again the small products first; group `start` begins the sum
         auto issue_o = [&](int t, int s, int k0, int k1, int start) {
             const uint64_t vd = vdesc + (uint64_t)((s * Sh::OPERAND) >> 4);
-            for (int k = k0; k < k1; k++) {
 #pragma unroll
-                for (int b = 0; b < 2; b++) {
+            for (int plane = Sh::PLANES - 1; plane >= 0; plane--)
+                for (int k = k0; k < k1; k++) {
 #pragma unroll
-                    for (int plane = 0; plane < Sh::PLANES; plane++)
-                        kc_mma_ts(tmem + Sh::COL_O + t * DP, tmem + Sh::COL_P + t * Sh::STEP_P + plane * 64 + 16 * k + 8 * b,
-                                  vd + (uint64_t)((k * 4096 + b * 2048) >> 4), idesc_o, k != start || b != 0 || plane != 0);
+                    for (int b = 0; b < 2; b++)
+                        kc_mma_ts(tmem + Sh::COL_F + t * DP, tmem + Sh::COL_P + t * Sh::STEP_P + plane * 64 + 16 * k + 8 * b,
+                                  vd + (uint64_t)((k * 4096 + b * 2048) >> 4), idesc_o, k != start || b != 0 || plane != Sh::PLANES - 1);
                 }
-            }
         };
         int s = 0, ph = 0;                                     // ring place of the next item
         auto take = [&](int *at) {                             // waits for the next item
@@ -367,7 +382,7 @@ kv_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                 // products are still under way.
                 for (int i = 0; i < n && ok; i++) {
                     const bool more = i + 1 < n;
-                    const int v = sv, start = i == 0 ? lo : -1;
+                    const int v = sv, start = i == 0 || Sh::FRESH ? lo : -1;
                     int lo2 = 0, hi2 = 4;
                     if (more) b.groups(a, b.tile_at(i + 1), &lo2, &hi2);
                     if (OWN_P && more) {
@@ -419,8 +434,8 @@ kv_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
     }
     } else {
     // ---- softmax: thread = row
-    kc_regs_more<Sh::MORE>();
-    const float sc = a.scale * 1.4426950408889634f;
+    if (Sh::DEAL) kc_regs_more<Sh::MORE>();
+    const float sc = a.scale2;
     bool ok = true;
     int done = 0, blocks = 0;                                  // tiles of keys, and blocks, behind this tile of rows
     for (int j = 0; ok; j++) {
@@ -470,10 +485,22 @@ kv_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
         if (t < b.nt) {
             // rows that do not exist take the last one's position, so that they need no mask of their own
             const int pos = b.base_pos + min(r < tq * a.G ? tok : b.t0 + t * tq, b.sq.n - 1);
-            float2 l2[2] = {{0.f, 0.f}, {0.f, 0.f}};
+            auto gather = [&](int i, float alpha) {                // O = (O + P(i - 1) V) alpha
+#pragma unroll 1
+                for (int c = 0; c < DP / 16; c++) {
+                    float f[32];                                   // 16 columns of F, and of O
+                    tc_ld16(f_at + 16 * c, f);
+                    tc_ld16(i > 1 ? o_at + 16 * c : f_at, f + 16);
+                    kc_wait_ld32(f);
+#pragma unroll
+                    for (int e = 0; e < 16; e++) f[e] = (i > 1 ? f[e] + f[e + 16] : f[e]) * alpha;
+                    kc_st16(o_at + 16 * c, reinterpret_cast<const uint32_t *>(f));
+                }
+            };
             for (int i = 0; i < n && ok; i++) {
                 if (!mbar_wait_warp(&s_full[t], (uint32_t)((done + i) & 1))) { ok = false; break; }
                 tc_fence_after();
+                if (Sh::FRESH && !OWN_P && i > 0) gather(i, 1.f);  // (while the scores take no registers)
                 float x[KC_KEYS];
                 tc_ld32(s_at, x);
                 tc_ld32(s_at + 32, x + 32);
@@ -526,11 +553,15 @@ kv_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                     tc_fence_after();
                 }
                 const bool grow = mt > m + 8.f;
-                if (__any_sync(0xffffffffu, grow)) {
+                const bool any = __any_sync(0xffffffffu, grow);
+                if (any || (Sh::FRESH && OWN_P)) {
                     const float alpha = grow ? kv_ex2(m - mt) : 1.f;
                     if (grow) m = mt;
-                    l2[0].x *= alpha; l2[0].y *= alpha; l2[1].x *= alpha; l2[1].y *= alpha;
-                    if (i > 0) {
+                    l *= alpha;
+                    if (Sh::FRESH && OWN_P && i > 0) {
+                        gather(i, alpha);
+                    } else if (i > 0) {
+                        if (Sh::FRESH) kc_wait_st();
 #pragma unroll 1
                         for (int c = 0; c < DP / 16; c++) {
                             float o[16];
@@ -543,6 +574,7 @@ kv_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                     }
                 }
                 const float2 sc2 = make_float2(sc, sc), neg = make_float2(-m, -m);
+                float2 l2[2] = {{0.f, 0.f}, {0.f, 0.f}};           // the tile's sum: small terms are not lost one by one in a large l
                 auto open = [&](int c) {                           // the exponentials of 16 keys, in place
 #pragma unroll
                     for (int e = 0; e < 8; e++) {
@@ -588,11 +620,11 @@ kv_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                     }
                 }
                 ready(&p_full[t]);
+                l += (l2[0].x + l2[0].y) + (l2[1].x + l2[1].y);
             }
             if (n > 0 && ok) ok = mbar_wait_warp(&o_full[t], (uint32_t)(OWN_P ? (done + n - 1) & 1 : blocks & 1));
             if (n > 0) { done += n; blocks++; }
             tc_fence_after();
-            l = (l2[0].x + l2[0].y) + (l2[1].x + l2[1].y);
             // (what the results need of the block is read again, so that it takes no registers above)
             const KcBlock e(a, items + (j & 1) * 8, tq, TILES, size, rank);
             if (e.shares == 1 && rank == 0 && ok) {
@@ -603,10 +635,7 @@ kv_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
 #pragma unroll 1
                 for (int c = 0; c < DP / 32; c++) {
                     float o[32];
-                    if (n > 0) {
-                        tc_ld32(o_at + 32 * c, o);
-                        kc_wait_ld32(o);
-                    }
+                    if (n > 0) result(n, c, o);
 #pragma unroll
                     for (int u = 0; u < 32; u++) o[u] = inv != 0.f ? o[u] * inv : 0.f;
                     if (valid) {
@@ -648,8 +677,7 @@ kv_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
 #pragma unroll 1
                 for (int c = 0; c < DP / 32; c++) {
                     float o[32];
-                    tc_ld32(o_at + 32 * c, o);
-                    tc_wait_ld();
+                    result(b.n, c, o);
 #pragma unroll
                     for (int e = 0; e < 32; e += 4) *reinterpret_cast<float4 *>(row + c * 32 + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
                 }

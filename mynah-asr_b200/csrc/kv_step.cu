@@ -215,7 +215,7 @@ kv_step_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
             m[nt][0] = m[nt][1] = KS_NONE;
             l[nt][0] = l[nt][1] = 0.f;
         }
-        const float sc = a.scale * 1.4426950408889634f;
+        const float sc = a.scale2;
         const int g = lane >> 3, rr = lane & 7;                // ldmatrix: lane group = 8 x 8 matrix, row in it
         const uint32_t base = smem_u32(smem) + warp * OWN * 128;
         const uint32_t k_row = ((g & 1) * 8 + rr) * 128, v_row = ((g >> 1) * 8 + rr) * 128;
@@ -313,20 +313,38 @@ kv_step_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
                     }
                 }
                 // ---- values: rows = D (V transposed on its way out of shared memory), columns = heads
+                // F32 rows: the tensor cores cut sums toward zero, which over 1000 keys costs 5e-6 of a result, so each tile's sum is one of its
+                // own, the small products first, and added here
+                auto values = [&](int dt, int mt, auto &&sum) {
+                    uint32_t v4[4];
+                    ks_ldsm_t(vt + (dt >> 2) * (TILE * 128) + mt * 2048 + v_row + ((((dt & 3) * 2 + (g & 1)) ^ rr) << 4), v4);
 #pragma unroll
-                for (int mt = 0; mt < MT; mt++)
+                    for (int nt = 0; nt < NT; nt++) sum(nt, v4);
+                };
+                if (F32) {
 #pragma unroll
                     for (int dt = 0; dt < DP / 16; dt++) {
                         if (dt * 16 < a.D) {
-                            uint32_t v4[4];
-                            ks_ldsm_t(vt + (dt >> 2) * (TILE * 128) + mt * 2048 + v_row + ((((dt & 3) * 2 + (g & 1)) ^ rr) << 4), v4);
+                            float f[NT][4] = {};
 #pragma unroll
-                            for (int nt = 0; nt < NT; nt++) {
-                                ks_mma<BF>(o[nt][dt], v4, pb[nt][mt][0], pb[nt][mt][1]);
-                                if (F32) ks_mma<BF>(o[nt][dt], v4, pl[F32 ? nt : 0][F32 ? mt : 0][0], pl[F32 ? nt : 0][F32 ? mt : 0][1]);
-                            }
+                            for (int mt = 0; mt < MT; mt++)
+                                values(dt, mt, [&](int nt, const uint32_t *v4) {
+                                    ks_mma<BF>(f[nt], v4, pl[F32 ? nt : 0][F32 ? mt : 0][0], pl[F32 ? nt : 0][F32 ? mt : 0][1]);
+                                    ks_mma<BF>(f[nt], v4, pb[nt][mt][0], pb[nt][mt][1]);
+                                });
+#pragma unroll
+                            for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                                for (int e = 0; e < 4; e++) o[nt][dt][e] += f[nt][e];
                         }
                     }
+                } else {
+#pragma unroll
+                    for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+                        for (int dt = 0; dt < DP / 16; dt++)
+                            if (dt * 16 < a.D) values(dt, mt, [&](int nt, const uint32_t *v4) { ks_mma<BF>(o[nt][dt], v4, pb[nt][mt][0], pb[nt][mt][1]); });
+                }
             }
             __syncwarp();                                      // every lane has read the stage
             if (lane == 0) mbar_arrive(&empty[s]);

@@ -570,3 +570,30 @@ def test_refusals(gpu_pkg):
     cache.attend(cache.batch(lay.len_dev[:0], lay.table_dev[:0]), q, out, stream=here())      # no sequences: nothing happens
     cache.sync(here())
     assert (out == 0).all()
+
+
+@pytest.mark.parametrize("kind,dim", [("chunk", 128), ("chunk", 64), ("chunk", 48), ("step", 128), ("step", 64)])
+def test_long_sums_of_f32_rows(pkg, kind, dim):
+    # Values that share a mean, so that their sum grows with every key. A product's sum is cut, not rounded: a loss of 2^-23 at most and of
+    # half as much on average, and half of that again while the sum grows to its end. With at most 10 such cuts (8 of 16 keys, and two small
+    # products between them) before a sum is put away: 10 * 2^-23 / 4 = 3e-7. Scores of |s| <= 4 that are off by D / 16 cuts each on their way
+    # up, 8 * 2^-24 * 4 / 2 = 1e-6 of a weight at most, average over the keys; 32-bit sums of 64 tiles: 2^-24 * sqrt(64). Together below 1e-6; a
+    # sum that stays in the tensor core for 8192 keys loses 512 * 2 * 2^-25 = 3e-5.
+    lay = P.Layout([8192, 8190], 64, [400, 150]) if kind == "chunk" else P.Layout([8192] * 40, 64)
+    heads = 40 if kind == "chunk" else 4                  # (so many that no kernel splits the keys)
+    cache, k, v = filled(pkg, lay, heads, heads, dim, "f32")
+    v.copy_((1 + randn(7, *v.shape)).to(v.dtype))
+    q = 0.5 * randn(3, lay.n_rows, heads * dim)
+    out = torch.zeros_like(q)
+    cache.attend(lay.batch(cache), q, out, stream=here())
+    cache.sync(here())
+    some = [0, heads // 2, heads - 1]
+    for s in range(0, len(lay.lens), 13):
+        n, m, at = lay.lens[s], lay.rows[s], lay.begin[s]
+        keys, values = (P.keys_of(p, lay, s, list(range(n)))[:, some].transpose(0, 1) for p in (k, v))
+        pick = slice(at, at + m)
+        scores = q[pick].double().reshape(m, heads, dim)[:, some].transpose(0, 1) @ keys.transpose(1, 2) / dim ** 0.5
+        scores.masked_fill_(torch.arange(n, device="cuda") > torch.arange(n - m, n, device="cuda")[:, None], -float("inf"))
+        want = (torch.softmax(scores, -1) @ values).transpose(0, 1)
+        got = out[pick].double().reshape(m, heads, dim)[:, some]
+        assert (got - want).norm() <= 1e-6 * want.norm()
