@@ -6,6 +6,8 @@
     python mynah-asr_b200/kernel_case.py qgemv --T 1 --n 65536 --k 4096 --fmt q4_0 [--iters 3]
     python mynah-asr_b200/kernel_case.py attention --T 750 --batch 16 [--heads 8] [--impl 0] [--iters 3]
     python mynah-asr_b200/kernel_case.py aed --batch 32 --T 250 [--positions 64] [--launches] [--iters 3]
+    python mynah-asr_b200/kernel_case.py kv --batch 64 --T 1 --keys 4000 [--heads 32 --kv-heads 8 --dim 128] [--rows bf16]
+                                            [--page 16] [--window 0 --sinks 0] [--iters 3]
 
 gemm : the tcgen05 contraction on resident fp16 planes (large T); with --fmt q8n --a8 the integer contraction
        (tcgen05 kind::i8) on reference-native int8 weights and int8 activation rows.
@@ -15,6 +17,9 @@ qgemv: the weight-streaming small-T kernel on the stored blocks; sizes above the
 aed  : all positions of a Canary-1B-shaped decoder behind a tiny encoder, as the persistent few-row kernel (Q8_0 weights) or,
        with --launches, as few-row contractions, single-query self- and cross-attention and the turn between positions (f32
        weights, which have no tiles for that kernel): a profiler target that holds < 1 GB.
+kv   : one layer's paged cache: `batch` sequences bring T new rows each (1: single tokens) behind keys - T cached ones; their
+       append (rotation, rows to their pages) and their attention over the pages, each timed by device events on three caches
+       in turn, so that what a call reads has not just been read.
 attention: the rel-pos self-attention kernel inside a one-layer encoder (d = 128 x heads) over a packed batch of
        `batch` segments of T frames; the time is that of the attention launches alone (device events around
        them), the flops are 6 T^2 d per segment: content scores, the needed half of the position band, P.V.
@@ -108,13 +113,70 @@ def aed_case(pkg, a, rng):
     m.close()
 
 
+def kv_case(pkg, a):
+    import torch
+    rows = {"f32": (pkg.F32, torch.float32), "f16": (pkg.F16, torch.float16), "bf16": (pkg.BF16, torch.bfloat16)}[a.rows]
+    T, n, H, Hkv, D = a.T or 1, a.batch, a.heads, a.kv_heads, a.dim
+    if not 1 <= T <= a.keys:
+        raise SystemExit("kv: --keys counts the new rows too")
+    per = (a.keys + a.page - 1) // a.page
+    off = None if T == 1 else torch.arange(0, n * T + 1, T, dtype=torch.int32, device="cuda")
+    lens = torch.full((n,), a.keys, dtype=torch.int32, device="cuda")
+    sets = []
+    for i in range(3):
+        cache = pkg.KvCache(H, Hkv, D, a.page, n * per, fmt=rows[0], rotary_dim=D, window=a.window, n_sinks=a.sinks)
+        for p in cache.pages():
+            t = torch.as_tensor(p, device="cuda")
+            t.view(torch.bfloat16 if a.rows == "bf16" else torch.float16).normal_()
+        table = torch.randperm(n * per, device="cuda").to(torch.int32).reshape(n, per)
+        q, out = (torch.randn(n * T, H * D, device="cuda").to(rows[1]) for _ in range(2))
+        k, v = (torch.randn(n * T, Hkv * D, device="cuda").to(rows[1]) for _ in range(2))
+        sets.append((cache, cache.batch(lens, table, row_off=off, n_rows=n * T), q, k, v, out))
+    stream = torch.cuda.Stream()
+    torch.cuda.synchronize()
+
+    def timed(call):
+        ms = []
+        with torch.cuda.stream(stream):
+            for i in range(3 + 3 * a.iters):
+                e = [torch.cuda.Event(enable_timing=True) for _ in range(2)]
+                e[0].record(); call(*sets[i % 3]); e[1].record()
+                ms.append(e)
+        stream.synchronize()
+        return sorted(x.elapsed_time(y) for x, y in ms[3:])[(3 * a.iters) // 2]
+
+    append = timed(lambda c, b, q, k, v, o: c.append(b, q, k, v, q, stream=stream.cuda_stream))
+    attend = timed(lambda c, b, q, k, v, o: c.attend(b, q, o, stream=stream.cuda_stream))
+    for s in sets:
+        s[0].sync()
+    item = 4 if a.rows == "f32" else 2
+    seen = [min(p + 1, a.window + min(a.sinks, max(p + 1 - a.window, 0))) if a.window else p + 1 for p in range(a.keys - T, a.keys)]
+    read = min(a.keys, a.window + T - 1 + a.sinks) if a.window else a.keys      # keys of a sequence that some row sees
+    sizes = {"append": n * T * D * (2 * H * item + 2 * Hkv * (item + 2)),
+             "attend": n * (2 * read * Hkv * D * 2 + 2 * T * H * D * item)}
+    flops = 4.0 * n * H * D * sum(seen)
+    print(json.dumps({"kernel": "kv", "rows": a.rows, "batch": n, "T": T, "keys": a.keys, "heads": H, "kv_heads": Hkv, "dim": D, "page": a.page,
+                      "window": a.window, "sinks": a.sinks, "append_ms": append, "append_bytes": sizes["append"],
+                      "append_gbs": sizes["append"] / append / 1e6, "attend_ms": attend, "attend_bytes": sizes["attend"], "attend_flops": flops,
+                      "attend_gbs": sizes["attend"] / attend / 1e6, "attend_tflops": flops / attend / 1e9}))
+    for s in sets:
+        s[0].close()
+
+
 def main():
     ap = argparse.ArgumentParser()
-    ap.add_argument("kernel", choices=["gemm", "qgemv", "attention", "aed"])
+    ap.add_argument("kernel", choices=["gemm", "qgemv", "attention", "aed", "kv"])
     ap.add_argument("--positions", type=int, default=64, help="aed: decode positions per call (prompt of 5 included)")
     ap.add_argument("--launches", action="store_true", help="aed: weights whose positions are chained launches")
     ap.add_argument("--batch", type=int, default=16)
-    ap.add_argument("--heads", type=int, default=8)
+    ap.add_argument("--heads", type=int, default=8, help="attention, kv: (query) heads")
+    ap.add_argument("--kv-heads", type=int, default=8, help="kv: key/value heads")
+    ap.add_argument("--dim", type=int, default=128, help="kv: head dimension")
+    ap.add_argument("--keys", type=int, default=1000, help="kv: keys of each sequence, its new rows included")
+    ap.add_argument("--page", type=int, default=16, help="kv: positions of a page")
+    ap.add_argument("--window", type=int, default=0, help="kv: keys that a row sees (0: all)")
+    ap.add_argument("--sinks", type=int, default=0, help="kv: first keys that a windowed row sees all the same")
+    ap.add_argument("--rows", default="bf16", choices=["f32", "f16", "bf16"], help="kv: type of the rows")
     ap.add_argument("--impl", type=int, default=0, help="attention: 0 default (tcgen05 where eligible), 2 warp-level tiled kernel")
     ap.add_argument("--T", type=int, default=0)
     ap.add_argument("--n", type=int, default=4096)
@@ -132,6 +194,8 @@ def main():
         return attention_case(pkg, a, rng)
     if a.kernel == "aed":
         return aed_case(pkg, a, rng)
+    if a.kernel == "kv":
+        return kv_case(pkg, a)
     T = a.T or (16384 if a.kernel == "gemm" else 1)
     if a.fmt == "q8n":
         wq = rng.integers(-127, 128, (a.n, a.k), dtype=np.int8)
