@@ -358,7 +358,7 @@ typedef struct {
     const int *row_off;                  /* [n_seq + 1], not decreasing, or NULL */
     const int *kv_len;                   /* [n_seq] */
     const int *page_table;               /* [n_seq][max_pages] */
-    int max_pages;
+    int max_pages;                       /* max_pages x page_size is at most 2^26 */
 } mynah_b200_kv_batch;
 
 /* Both calls below: rows of n_heads (n_kv_heads) x head_dim values on the handle's device, ld* the stride from row to row
@@ -375,7 +375,11 @@ typedef struct {
 int mynah_b200_kv_append(mynah_b200_kv *h, const mynah_b200_kv_batch *b, const void *q, long long ldq, const void *k, long long ldk,
                          const void *v, long long ldv, void *q_out, long long ldqo, void *stream);
 /* attend: out = softmax over the visible keys of scale q . k, times their values; 0 for a row that sees none. q as
- * append left it in q_out. */
+ * append left it in q_out; out may be q itself with the same stride. How the keys of a sequence are cut into parts that
+ * are summed and joined depends on n_seq, n_rows and max_pages and on the sequence itself, never on the others, and no
+ * sum on what ran first: the same call gives the same bits. F32 rows: queries are kept to 2^-25 absolutely or 2^-22
+ * relatively, whichever is more, and lie below 65504. F16 / BF16 rows: values are summed by the tensor cores, which
+ * cut each sum toward zero; that adds up to 2e-8 of a result per 16 keys (2e-5 over 16000). */
 int mynah_b200_kv_attend(mynah_b200_kv *h, const mynah_b200_kv_batch *b, const void *q, long long ldq, void *out, long long ldo,
                          void *stream);
 /* waits for `stream` (NULL: the handle's own) and reports, once, what the handle's calls have found since the last sync:

@@ -120,7 +120,7 @@ int take_batch(const char *what, const mynah_b200_kv *h, const mynah_b200_kv_bat
     if (b->n_seq < 0 || b->n_rows < 0) no = "a negative count";
     else if (b->n_seq == 0 || b->n_rows == 0) return 1;
     else if (!b->kv_len || !b->page_table) no = "a null table";
-    else if (b->max_pages < 1 || (int64_t)b->max_pages * c.page_size > 0x7fffffffll) no = "max_pages x page_size is from 1 page to 2^31 - 1 positions";
+    else if (b->max_pages < 1 || (int64_t)b->max_pages * c.page_size > KV_MOST) no = "max_pages x page_size is from 1 page to 2^26 positions";
     else if (!b->row_off && b->n_rows < b->n_seq) no = "fewer rows than sequences";
     else if (((uintptr_t)b->kv_len | (uintptr_t)b->page_table | (uintptr_t)b->row_off) & 3) no = "a misaligned table";
     else if (!reachable(b->kv_len, h->device) || !reachable(b->page_table, h->device) || (b->row_off && !reachable(b->row_off, h->device)))
@@ -128,7 +128,7 @@ int take_batch(const char *what, const mynah_b200_kv *h, const mynah_b200_kv_bat
     if (no) { set_error("%s: %s", what, no); return -1; }
     a->H = c.n_heads; a->Hkv = c.n_kv_heads; a->G = c.n_heads / c.n_kv_heads; a->D = c.head_dim;
     a->page_shift = __builtin_ctz((unsigned)c.page_size); a->n_pages = c.n_pages;
-    a->window = c.window; a->sinks = c.n_sinks;
+    a->window = c.window < KV_MOST ? c.window : KV_MOST; a->sinks = c.n_sinks < KV_MOST ? c.n_sinks : KV_MOST;
     // Products' sums are cut toward zero, not rounded, at each of their D / 16 instructions: measured with F32 rows, a score of D = 128 is
     // short of 1.2e-7 of itself on average, one of D = 64 of 0.8e-7. The factor gives back the mean.
     const double scale = c.scale > 0 ? (double)c.scale : 1 / sqrt((double)c.head_dim);

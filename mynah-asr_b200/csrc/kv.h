@@ -9,6 +9,9 @@ namespace mb {
 
 enum { KV_F32 = 0, KV_F16 = 1, KV_BF16 = 2 };       // rows; the cache holds f16 for the first two, bf16 for the third
 
+// Positions of a sequence: sums with a window, a tile or a page stay in 32 bits, and a block's work within the kernels' limit on waits
+static constexpr int KV_MOST = 1 << 26;
+
 // Pools are [page][kv head][slot][D], 16 bits a value: the keys of one head in one page are one run of memory.
 struct KvArgs {
     int H, Hkv, G, D;                                // G = H / Hkv query heads share a kv head

@@ -1,6 +1,10 @@
 """The paged key/value cache on the GPU: append and attend against their definitions in 64 bits (kv_plain), at the sizes, masks and
 tables where they can go wrong. Bounds are those of the arithmetic, worked out in kv_plain."""
+import json
 import math
+import os
+import subprocess
+import sys
 
 import numpy as np
 import pytest
@@ -573,7 +577,7 @@ def test_refusals(gpu_pkg):
 
 
 @pytest.mark.parametrize("kind,dim", [("chunk", 128), ("chunk", 64), ("chunk", 48), ("step", 128), ("step", 64)])
-def test_long_sums_of_f32_rows(pkg, kind, dim):
+def test_long_sums_of_f32_rows(gpu_pkg, kind, dim):
     # Values that share a mean, so that their sum grows with every key. A product's sum is cut, not rounded: a loss of 2^-23 at most and of
     # half as much on average, and half of that again while the sum grows to its end. With at most 10 such cuts (8 of 16 keys, and two small
     # products between them) before a sum is put away: 10 * 2^-23 / 4 = 3e-7. Scores of |s| <= 4 that are off by D / 16 cuts each on their way
@@ -581,7 +585,7 @@ def test_long_sums_of_f32_rows(pkg, kind, dim):
     # sum that stays in the tensor core for 8192 keys loses 512 * 2 * 2^-25 = 3e-5.
     lay = P.Layout([8192, 8190], 64, [400, 150]) if kind == "chunk" else P.Layout([8192] * 40, 64)
     heads = 40 if kind == "chunk" else 4                  # (so many that no kernel splits the keys)
-    cache, k, v = filled(pkg, lay, heads, heads, dim, "f32")
+    cache, k, v = filled(gpu_pkg, lay, heads, heads, dim, "f32")
     v.copy_((1 + randn(7, *v.shape)).to(v.dtype))
     q = 0.5 * randn(3, lay.n_rows, heads * dim)
     out = torch.zeros_like(q)
@@ -597,3 +601,71 @@ def test_long_sums_of_f32_rows(pkg, kind, dim):
         want = (torch.softmax(scores, -1) @ values).transpose(0, 1)
         got = out[pick].double().reshape(m, heads, dim)[:, some]
         assert (got - want).norm() <= 1e-6 * want.norm()
+
+
+@pytest.mark.parametrize("more", [["--T", "1"], ["--T", "70", "--rows", "f32", "--kv-heads", "2"], ["--T", "5", "--rows", "f16", "--dim", "64", "--window", "100", "--sinks", "3"]])
+def test_kernel_case(gpu_pkg, more):
+    got = subprocess.run([sys.executable, os.path.join(os.path.dirname(gpu_pkg.__file__), "kernel_case.py"), "kv", "--batch", "3", "--keys", "333", "--iters", "1"] + more,
+                         capture_output=True, text=True, timeout=300)
+    assert got.returncode == 0, got.stderr
+    said = json.loads(got.stdout)
+    assert said["kernel"] == "kv" and 0 < said["append_ms"] < 100 and 0 < said["attend_ms"] < 100
+
+
+# ------------------------------------------------------------------------------------------------------------ the ends of what is allowed
+MOST = 2 ** 31 - 1
+
+
+@pytest.mark.parametrize("rows", [None, [200, 300, 1]])
+@pytest.mark.parametrize("window,sinks", [(MOST, 0), (MOST, MOST), (1, MOST), (1, MOST - 31), (2, 2 ** 26 + 1), (1, 0)])
+def test_largest_windows_and_sinks(gpu_pkg, rows, window, sinks):
+    lay = P.Layout([200, 700, 1], 16, rows)
+    for dim, fmt in ((64, "bf16"), (128, "f32")):
+        _, q, got = attend_case(gpu_pkg, lay, 4, 2, dim, fmt, window=window, n_sinks=sinks)
+        if window + sinks > 700:                          # everything in front is seen, as without a window
+            cache, _, _ = filled(gpu_pkg, lay, 4, 2, dim, fmt)
+            plain = torch.full_like(q, 7.0)
+            cache.attend(lay.batch(cache), q, plain, stream=here())
+            cache.sync(here())
+            assert torch.allclose(plain.float(), got.float(), rtol=0.02, atol=0.02)
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("lens,rows", [([5000, 40, 0], None), ([300] * 60, None), ([3000, 40], [130, 40]), ([800, 700, 900], [700, 650, 900])])
+def test_attend_in_place(gpu_pkg, fmt, lens, rows):
+    """out may be q: with few blocks, whose parts several CTAs share, and with many."""
+    lay = P.Layout(lens, 16, rows, extra_rows=3)
+    for heads, kv_heads, dim in ((8, 2, 64), (32, 8, 128), (40, 1, 128)):
+        cache, _, _ = filled(gpu_pkg, lay, heads, kv_heads, dim, fmt)
+        q = randn(3, lay.n_rows, heads * dim).to(P.ROWS[fmt])
+        out, same = torch.zeros_like(q), q.clone()
+        out[lay.real:] = q[lay.real:]
+        cache.attend(lay.batch(cache), q, out, stream=here())
+        cache.attend(lay.batch(cache), same, same, stream=here())
+        cache.sync(here())
+        assert torch.equal(out, same)
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("dim,heads", [(128, 1), (128, 4), (64, 1), (32, 8)])
+def test_chunk_clusters_of_many_sequences(gpu_pkg, fmt, dim, heads):
+    """More sequences than lanes, few blocks: clusters, whose CTAs share long blocks and leave short ones to the first of them."""
+    rows = [(i * 5) % 9 for i in range(37)]
+    lens = [r + (0 if i % 3 else 1700 + 90 * i) for i, r in enumerate(rows)]
+    attend_case(gpu_pkg, P.Layout(lens, 16, rows, extra_rows=5), heads, 1, dim, fmt)
+    attend_case(gpu_pkg, P.Layout(lens, 16, rows), heads, 1, dim, fmt, window=700, n_sinks=150)
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("rows", [None, [150, 300]])
+def test_rows_far_apart(gpu_pkg, fmt, rows):
+    """Rows of a wider tensor, in and out: what lies between them stays."""
+    lay = P.Layout([400, 310], 16, rows)
+    cache, k, v = filled(gpu_pkg, lay, 6, 2, 48, fmt)
+    wide = randn(3, lay.n_rows, 288 * 3 + 8).to(P.ROWS[fmt])
+    q, out = wide[:, 288:576], torch.full_like(wide, 7.0)
+    cache.attend(lay.batch(cache), q, out[:, 576:864], stream=here())
+    cache.sync(here())
+    want, bound = P.attend(lay, q.contiguous(), k, v, 2, fmt=fmt)
+    P.check(out[:, 576:864], want, bound)
+    assert (out[:, :576] == 7).all() and (out[:, 864:] == 7).all()
