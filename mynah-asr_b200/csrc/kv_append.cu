@@ -36,8 +36,9 @@ __device__ __forceinline__ typename KaQuad<FMT>::type ka_close(const float *v) {
 }
 
 static constexpr int KA_WARPS = 8;
-// The largest magnitude that a cache value may have: beyond it a bf16 would round to infinity; f16 as the operand planes
-static constexpr float KA_BF16_MAX = 3.3895313e38f;
+// Below what a cache value lies: from (2 - 2^-8) 2^127 on, halfway behind the largest bf16, it would round to infinity; f16 as the operand
+// planes
+static constexpr float KA_BF16_MAX = 0x1.ffp127f;
 
 enum { KA_Q, KA_K, KA_V };
 // What a lane knows of its row: where its quads begin, cosines and sines of its pairs, the row's slot

@@ -136,7 +136,8 @@ def kv_refuses(pkg, fake):
     good = dict(kv_len=lens, page_table=table)
     call = lambda b, q=rows, ldq=256, out=rows, ldo=256: L.mynah_b200_kv_attend(h, C.addressof(b), q, ldq, out, ldo, None)  # noqa: E731
     host = np.zeros(4096, np.float32)
-    for b in (dict(good, n_seq=-1), dict(good, n_rows=-1), dict(good, kv_len=None), dict(good, page_table=None), dict(good, max_pages=0),
+    for b in (dict(good, n_seq=-1), dict(good, n_rows=-1), dict(good, n_rows=2 ** 30 + 1), dict(good, n_seq=2 ** 31 - 1, n_rows=2 ** 31 - 1, row_off=off),
+              dict(good, max_pages=2 ** 22 + 1), dict(good, kv_len=None), dict(good, page_table=None), dict(good, max_pages=0),
               dict(good, max_pages=2 ** 28), dict(good, n_seq=3), dict(good, kv_len=lens + 2), dict(good, row_off=off + 1),
               dict(good, kv_len=host.ctypes.data), dict(good, page_table=host.ctypes.data), dict(good, row_off=host.ctypes.data)):
         assert call(_batch(pkg, **b)) == -1, b

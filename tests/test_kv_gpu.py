@@ -669,3 +669,56 @@ def test_rows_far_apart(gpu_pkg, fmt, rows):
     want, bound = P.attend(lay, q.contiguous(), k, v, 2, fmt=fmt)
     P.check(out[:, 576:864], want, bound)
     assert (out[:, :576] == 7).all() and (out[:, 864:] == 7).all()
+
+
+def test_largest_values(gpu_pkg):
+    """The largest finite numbers of the rows' type go into the cache as they are (f16: below 65504)."""
+    for fmt, top in (("bf16", torch.finfo(torch.bfloat16).max), ("f16", 65472.0), ("f32", 65472.0)):
+        lay = P.Layout([3], 8, [3])
+        cache, k, v = filled(gpu_pkg, lay, 2, 2, 16, fmt)
+        x = torch.tensor([top, -top, 0.0, 1.0], device="cuda").repeat(8)[None].repeat(3, 1).to(P.ROWS[fmt])
+        out = torch.zeros_like(x)
+        cache.append(lay.batch(cache), x, x, x, out, stream=here())
+        cache.sync(here())
+        assert torch.equal(out, x)
+        for pool in (k, v):
+            assert torch.equal(P.keys_of(pool, lay, 0, [0, 1, 2]).reshape(3, 32), x.double())
+
+
+FIRST = """
+import importlib.util, os, sys
+spec = importlib.util.spec_from_file_location("mynah_asr_b200", sys.argv[1], submodule_search_locations=[os.path.dirname(sys.argv[1])])
+pkg = importlib.util.module_from_spec(spec); sys.modules["mynah_asr_b200"] = pkg; spec.loader.exec_module(pkg)
+import torch
+for fmt, t in ((pkg.F32, torch.float32), (pkg.BF16, torch.bfloat16)):
+    for dim in (64, 128):
+        cache = pkg.KvCache(4, 2, dim, 16, 64, fmt=fmt)
+        table = torch.arange(64, dtype=torch.int32, device="cuda").reshape(2, 32)
+        lens = torch.full((2,), 300, dtype=torch.int32, device="cuda")
+        off = torch.tensor([0, 40, 80], dtype=torch.int32, device="cuda")
+        x = torch.randn(80, 8 * dim, device="cuda").to(t)
+        q, k, v = x[:, :4 * dim], x[:, 4 * dim:6 * dim], x[:, 6 * dim:]
+        turned, a, b = (torch.zeros(80, 4 * dim, device="cuda", dtype=t) for _ in range(3))
+        batch, step = cache.batch(lens, table, row_off=off, n_rows=80), cache.batch(lens, table)
+        def calls(out):
+            s = torch.cuda.current_stream().cuda_stream
+            cache.append(batch, q, k, v, turned, stream=s)
+            cache.attend(batch, turned, out, stream=s)
+            cache.attend(step, turned, out, stream=s)
+        graph = torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph):
+            calls(a)
+        graph.replay()
+        torch.cuda.synchronize()
+        calls(b)
+        torch.cuda.synchronize()
+        cache.sync()
+        assert torch.equal(a, b) and a.abs().sum() > 0
+print("same")
+"""
+
+
+def test_first_calls_of_a_process_are_captured(gpu_pkg):
+    got = subprocess.run([sys.executable, "-c", FIRST, gpu_pkg.__file__], capture_output=True, text=True, timeout=300)
+    assert got.returncode == 0 and "same" in got.stdout, got.stderr
