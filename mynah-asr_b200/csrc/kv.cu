@@ -18,8 +18,8 @@ struct mynah_b200_kv {
     uint8_t *block = nullptr;
     double *turns = nullptr;
     float *q_norm = nullptr, *k_norm = nullptr;
-    CUtensorMap map_k, map_v;
-    int box = 0;
+    CUtensorMap map_k, map_v, chunk_k, chunk_v;                // for single tokens, for prompts
+    int chunk_box = 0;
     int *status() const { return reinterpret_cast<int *>(block); }
     ~mynah_b200_kv() {
         cudaFree(k); cudaFree(v); cudaFree(block);              // (waits for the handle's work)
@@ -196,8 +196,10 @@ mynah_b200_kv *mynah_b200_kv_create(const mynah_b200_kv_config *cfg) {
         delete h;
         return nullptr;
     }
-    h->box = kv_box(D, cfg->page_size);
-    if (!pool_map(&h->map_k, h->k, *cfg, h->box) || !pool_map(&h->map_v, h->v, *cfg, h->box)) {
+    const int box = kv_box(D, cfg->page_size);
+    h->chunk_box = cfg->page_size < 32 ? cfg->page_size : 32;
+    if (!pool_map(&h->map_k, h->k, *cfg, box) || !pool_map(&h->map_v, h->v, *cfg, box) || !pool_map(&h->chunk_k, h->k, *cfg, h->chunk_box) ||
+        !pool_map(&h->chunk_v, h->v, *cfg, h->chunk_box)) {
         set_error("kv_create: no tensor map of the pools");
         delete h;
         return nullptr;
@@ -250,7 +252,7 @@ int mynah_b200_kv_attend(mynah_b200_kv *h, const mynah_b200_kv_batch *b, const v
     if (no) { set_error("kv_attend: %s", no); return -1; }
     a.q = q; a.ldq = ldq; a.out = out; a.ldo = ldo;
     const cudaStream_t st = stream ? (cudaStream_t)stream : h->stream;
-    return a.row_off ? kv_chunk(h->map_k, h->map_v, a, h->box, h->fmt, st) : kv_step(h->map_k, h->map_v, a, h->fmt, st);
+    return a.row_off ? kv_chunk(h->chunk_k, h->chunk_v, a, h->chunk_box, h->fmt, st) : kv_step(h->map_k, h->map_v, a, h->fmt, st);
 }
 
 int mynah_b200_kv_sync(mynah_b200_kv *h, void *stream) {

@@ -139,7 +139,8 @@ __device__ __forceinline__ void kv_look_over(const KvArgs &a, int lane) {
 #endif
 
 int kv_append(const KvAppendArgs &a, int fmt, cudaStream_t st);
-// Attention of one row per sequence, and of many. Maps of the two pools as [rows][D] with boxes of 64 columns and kv_box slots.
+// Attention of one row per sequence, and of many. Maps of the two pools as [rows][D] with boxes of 64 columns and kv_box slots (prompts:
+// box_rows, a page or 32 of them).
 int kv_box(int D, int page_size);
 int kv_step(const CUtensorMap &k, const CUtensorMap &v, const KvArgs &a, int fmt, cudaStream_t st);
 // 16-bit query rows as [rows][H][D]: boxes of 64 columns, G heads and 128 / G rows

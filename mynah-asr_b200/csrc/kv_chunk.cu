@@ -4,8 +4,7 @@
 // Bound by the tensor cores and, as much, by the exponentials (4 D operations and one exponential per pair of row and key). A CTA
 // owns one kv head and two tiles of 128 rows: the G query heads of 128 / G positions each (row r is head r % G of position r / G), so
 // that short pieces fill a tile and all heads share the keys' tiles. Keys and values come in tiles of 128 by TMA, from their pages
-// straight into the swizzled operand layout; of a tile at the edge of what is visible only the groups of 32 keys that some row sees
-// are computed.
+// straight into the swizzled operand layout: groups of 32 keys, those that some row sees, side by side (KvGroups).
 //   tensor memory  S0, S1: scores of the two tiles (128 columns each), O0, O1: results; the probabilities, as 16-bit operands, overwrite
 //                  the scores, or have columns of their own where D <= 64 leaves room (then S(i + 1) is computed under the exponentials
 //                  of tile i)
@@ -154,7 +153,7 @@ struct KcFinder {
 struct KcBlock {
     KvSeq sq;
     int seq, kvh, t0, base_pos, last, top, low, n, nt, rank, shares;
-    KvTiles tiles;
+    KvGroups keys;
     __device__ __forceinline__ KcBlock(const KvArgs &a, const volatile int *item, int tq, int n_tiles, int size, int rank_) {
         // (one lane's values for all, so that the compiler keeps them and what follows from them in uniform registers)
         auto same = [](int v) { return __shfl_sync(0xffffffffu, v, 0); };
@@ -165,24 +164,17 @@ struct KcBlock {
         last = min(t0 + n_tiles * tq, sq.n) - 1;
         top = base_pos + last;                                 // last key that any row sees,
         low = base_pos + t0 - a.window + 1;                    // and first that a window shows
-        tiles = {0, 0, 0};
-        if (seq >= 0) tiles = kv_tiles(base_pos + t0 > 0 ? base_pos + t0 : 0, top, a.window, a.sinks, KC_KEYS);
+        keys = {0, 0, 0};
+        if (seq >= 0) keys = kv_groups(base_pos + t0 > 0 ? base_pos + t0 : 0, top, a.window, a.sinks);
+        const int tiles = (keys.count + 3) / 4;
         // CTAs that share the block: two tiles each at least, by the block's own tiles
         rank = rank_;
-        shares = min(size, tiles.count < 4 ? 1 : 1 << (30 - __clz(tiles.count)));
-        n = rank < shares ? (tiles.count - rank + shares - 1) / shares : 0;
+        shares = min(size, tiles < 4 ? 1 : 1 << (30 - __clz(tiles)));
+        n = rank < shares ? (tiles - rank + shares - 1) / shares : 0;
         nt = n_tiles == 2 && t0 + tq <= last ? 2 : 1;          // tiles that have rows
     }
-    __device__ __forceinline__ int tile_at(int i) const { return tiles.at(rank + i * shares) * KC_KEYS; }       // first key of the CTA's i-th tile
-    // its groups of 32 keys [lo, hi) that some row sees
-    __device__ __forceinline__ void groups(const KvArgs &a, int j0, int *lo, int *hi) const {
-        *lo = 0;
-        *hi = min(4, ((top - j0) >> 5) + 1);
-        if (a.window > 0) {
-            if (j0 + KC_KEYS <= low) *hi = min(*hi, (a.sinks - j0 + 31) >> 5);         // a tile of the first tokens
-            else if (low > j0 && a.sinks <= j0) *lo = (low - j0) >> 5;
-        }
-    }
+    __device__ __forceinline__ int tile_at(int i) const { return 4 * (rank + i * shares); }        // first group of the CTA's i-th tile,
+    __device__ __forceinline__ int groups(int g0) const { return min(4, keys.count - g0); }        // and how many it has
 };
 
 template <int DP, int FMT>
@@ -280,8 +272,9 @@ kv_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
             const KcBlock b(a, item, tq, TILES, size, rank);
             if (b.seq < 0) break;
             auto seen = [&](int j) { return j <= b.top && (a.window <= 0 || j + box_rows - 1 >= b.low || j < a.sinks); };
+            auto key_of = [&](int i) { return b.keys.at(b.tile_at(i) + (b_sub * box_rows >> 5)) + (b_sub * box_rows & 31); };
             auto entry_of = [&](int i) -> int {
-                const int j = b.tile_at(i) + b_sub * box_rows;
+                const int j = key_of(i);
                 return lane < boxes && i < b.n && seen(j) ? a.table[(size_t)b.seq * a.max_pages + (j >> shift)] : -1;
             };
             int entry = entry_of(0);
@@ -296,7 +289,7 @@ kv_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
             }
             for (int i = 0; i < b.n && ok; i++) {
                 const int next = entry_of(i + 1);
-                const int j = b.tile_at(i) + b_sub * box_rows;
+                const int j = key_of(i);
                 if (lane < boxes && (unsigned)entry >= (unsigned)a.n_pages) {
                     if (seen(j)) atomicExch(a.status, ST_PAGE);
                     entry = 0;                                 // any finite rows do
@@ -338,8 +331,8 @@ kv_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                 }
             }
         };
-        // groups [k0, k1) of P V, again the small products first; group `start` begins the sum
-        auto issue_o = [&](int t, int s, int k0, int k1, int start) {
+        // groups [k0, k1) of P V, again the small products first; the first one begins the sum
+        auto issue_o = [&](int t, int s, int k0, int k1, bool begins) {
             const uint64_t vd = vdesc + (uint64_t)((s * Sh::OPERAND) >> 4);
 #pragma unroll
             for (int plane = Sh::PLANES - 1; plane >= 0; plane--)
@@ -347,7 +340,7 @@ kv_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
 #pragma unroll
                     for (int b = 0; b < 2; b++)
                         kc_mma_ts(tmem + Sh::COL_F + t * DP, tmem + Sh::COL_P + t * Sh::STEP_P + plane * 64 + 16 * k + 8 * b,
-                                  vd + (uint64_t)((k * 4096 + b * 2048) >> 4), idesc_o, k != start || b != 0 || plane != Sh::PLANES - 1);
+                                  vd + (uint64_t)((k * 4096 + b * 2048) >> 4), idesc_o, !begins || k != 0 || b != 0 || plane != Sh::PLANES - 1);
                 }
         };
         int s = 0, ph = 0;                                     // ring place of the next item
@@ -365,8 +358,7 @@ kv_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
             leave_block(j);
             const int n = b.n, nt = b.nt;
             if (n > 0) {
-                int sk = 0, sv = 0, lo, hi;
-                b.groups(a, b.tile_at(0), &lo, &hi);
+                int sk = 0, sv = 0, hi = b.groups(b.tile_at(0));
                 ok = mbar_wait_warp(q_full, (uint32_t)(queries & 1)) && take(&sk);
                 queries++;
                 if (ok) {
@@ -382,9 +374,8 @@ kv_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                 // products are still under way.
                 for (int i = 0; i < n && ok; i++) {
                     const bool more = i + 1 < n;
-                    const int v = sv, start = i == 0 || Sh::FRESH ? lo : -1;
-                    int lo2 = 0, hi2 = 4;
-                    if (more) b.groups(a, b.tile_at(i + 1), &lo2, &hi2);
+                    const int v = sv, hi2 = more ? b.groups(b.tile_at(i + 1)) : 4;
+                    const bool begins = i == 0 || Sh::FRESH;
                     if (OWN_P && more) {
                         ok = take(&sk);
                         for (int t = 0; t < nt && ok; t++) {
@@ -400,14 +391,14 @@ kv_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                     for (int t = 0; t < nt && ok; t++) {
                         if (!mbar_wait_warp(&p_part[t], (uint32_t)(((t ? done1 : done0) + i) & 1))) { ok = false; break; }
                         tc_fence_after();
-                        if (elect_one()) issue_o(t, v, lo, min(hi, KC_PART), start);
+                        if (elect_one()) issue_o(t, v, 0, min(hi, KC_PART), begins);
                         __syncwarp();
                         if (more && !OWN_P && t == 0 && !take(&sk)) { ok = false; break; }     // K(i + 1)
                         if (more && t == nt - 1 && !take(&sv)) { ok = false; break; }          // V(i + 1)
                         if (!mbar_wait_warp(&p_full[t], (uint32_t)(((t ? done1 : done0) + i) & 1))) { ok = false; break; }
                         tc_fence_after();
                         if (elect_one()) {
-                            issue_o(t, v, max(lo, KC_PART), hi, start);
+                            issue_o(t, v, KC_PART, hi, begins);
                             if (OWN_P || !more) tc_commit(&o_full[t]);
                             if (more && !OWN_P) { issue_s(t, sk, hi2); tc_commit(&s_full[t]); }
                             if (t == nt - 1) {
@@ -418,7 +409,7 @@ kv_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                         }
                         __syncwarp();
                     }
-                    lo = lo2; hi = hi2;
+                    hi = hi2;
                 }
                 done0 += n;
                 if (nt == 2) done1 += n;
@@ -524,18 +515,18 @@ kv_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                 for (int c = 64; c < 128; c += 8)
 #pragma unroll
                     for (int e = 0; e < 4; e++) m4[e] = fmaxf(m4[e], fmaxf(x[c + e], x[c + 4 + e]));
-                const int j0 = b.tile_at(i), d = pos - j0;
-                const bool whole = d >= KC_KEYS - 1 && (a.window <= 0 || d < a.window || j0 + KC_KEYS - 1 < a.sinks);
+                const int g0 = b.tile_at(i), j0 = b.keys.at(g0), d = pos - j0;
+                const bool whole = d >= KC_KEYS - 1 && (a.window <= 0 || (d < a.window && (g0 >= b.keys.first || g0 + 4 <= b.keys.first)) || j0 + KC_KEYS - 1 < a.sinks);
                 const bool all = __all_sync(0xffffffffu, whole);
                 if (!all) {                                        // (columns that have no scores are hidden, too)
                     // 32 columns at a time, where some row of the warp does not see them all: a bit per column, visible up to d, above
                     // `under`, or below `keep`
-                    const int under = a.window > 0 ? d - a.window : -1, keep = a.sinks - j0;
                     auto upto = [](int c) -> uint32_t { return c < 0 ? 0u : c >= 31 ? 0xffffffffu : (2u << c) - 1u; };      // bits 0 to c
                     m4[0] = m4[1] = m4[2] = m4[3] = -INFINITY;
 #pragma unroll
                     for (int w = 0; w < 4; w++) {
-                        const uint32_t see = upto(d - 32 * w) & (~upto(under - 32 * w) | upto(keep - 1 - 32 * w));
+                        const int jw = b.keys.at(g0 + w), dw = pos - jw;
+                        const uint32_t see = upto(dw) & (~upto(a.window > 0 ? dw - a.window : -1) | upto(a.sinks - 1 - jw));
                         if (!__all_sync(0xffffffffu, see == 0xffffffffu)) {
 #pragma unroll
                             for (int c = 0; c < 32; c++)
@@ -610,12 +601,11 @@ kv_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                         if (c == 2 * KC_PART) ready(&p_part[t]);
                     }
                 } else {
-                    int lo, hi;
-                    b.groups(a, j0, &lo, &hi);
+                    const int hi = b.groups(g0);
 #pragma unroll
                     for (int c = 0; c <= 4; c++) {
-                        if (c < 4 && c >= lo && c < hi) { open(2 * c); open(2 * c + 1); }
-                        if (c > 0 && c > lo && c <= hi) { close(2 * c - 2); close(2 * c - 1); }
+                        if (c < 4 && c < hi) { open(2 * c); open(2 * c + 1); }
+                        if (c > 0 && c <= hi) { close(2 * c - 2); close(2 * c - 1); }
                         if (c == KC_PART) ready(&p_part[t]);
                     }
                 }

@@ -57,4 +57,26 @@ MB_HD KvTiles kv_tiles(int pos0, int pos1, int window, int sinks, int tile) {
     return t;
 }
 
+// The same in groups of 32 keys: groups [0, first) of the first tokens, then those from the position `start` on. Tiles are cut from the
+// row of groups, so that a few first tokens take no tile of their own, and a window's first tile begins where the window does.
+struct KvGroups {
+    int first, start, count;
+    MB_HD int at(int g) const { return g < first ? 32 * g : start + 32 * (g - first); }     // first position of group g
+};
+MB_HD KvGroups kv_groups(int pos0, int pos1, int window, int sinks) {
+    KvGroups t = {0, 0, 0};
+    if (pos1 < 0) return t;
+    if (window > 0) {
+        const int64_t low = (int64_t)pos0 - window + 1;
+        if (low > 0) {
+            const int s = sinks < pos1 + 1 ? sinks : pos1 + 1;
+            t.start = (int)(low < pos1 ? low : pos1) & ~31;
+            t.first = s > 0 ? (s - 1) / 32 + 1 : 0;
+            if (t.first >= t.start / 32) { t.first = 0; t.start = 0; }             // the two meet
+        }
+    }
+    t.count = t.first + (pos1 - t.start) / 32 + 1;
+    return t;
+}
+
 }  // namespace mb

@@ -26,6 +26,11 @@ int tiles(int p0, int p1, int window, int sinks, int tile, int *out, int cap) {
     for (int i = 0; i < t.count && i < cap; i++) out[i] = t.at(i);
     return t.count;
 }
+int groups(int p0, int p1, int window, int sinks, int *out, int cap) {
+    const KvGroups t = kv_groups(p0, p1, window, sinks);
+    for (int i = 0; i < t.count && i < cap; i++) out[i] = t.at(i);
+    return t.count;
+}
 }
 """
 
@@ -78,6 +83,25 @@ def test_tiles_cover_what_is_seen(index, tile):
     top = 2 ** 31 - 1
     assert index.tiles(top - 5, top - 1, 64, 4, tile, out, 4096) in (2, 3, 4)
     assert index.tiles(top - 5, top - 1, 64, top, tile, out, 4096) == (top - 1) // tile + 1
+
+
+def test_groups_cover_what_is_seen(index):
+    """The groups of 32 keys of rows at [p0, p1]: in order, none twice, every visible key in one, and none that no row sees."""
+    out = (C.c_int * 4096)()
+    for window in (0, 1, 5, 31, 32, 33, 128, 391, 2 ** 26):
+        for sinks in ((0, 1, 32, 33, 160, 2 ** 26) if window else (0,)):
+            for p0 in (-7, -1, 0, 1, 31, 32, 33, 127, 128, 515, 2560):
+                for more in (0, 1, 31, 32, 127, 261):
+                    p1 = p0 + more
+                    n = index.groups(p0, p1, window, sinks, out, 4096)
+                    got = list(out[:n])
+                    need = {j // 32 * 32 for p in range(max(p0, 0), p1 + 1) for j in ([*range(min(sinks, p + 1)), *range(max(p - window + 1, 0), p + 1)] if window else range(p + 1))}
+                    assert got == sorted(set(got)) and need <= set(got), (window, sinks, p0, p1, got)
+                    assert all(j % 32 == 0 and 0 <= j <= max(p1, 0) for j in got)
+                    if p0 >= 0:                               # (the group between the first tokens and the window may come too, where they meet)
+                        assert len(set(got) - need) <= 1
+    top = 2 ** 26 - 1
+    assert index.groups(top - 5, top, 64, 4, out, 4096) in (3, 4) and index.groups(0, top, 2 ** 26, 2 ** 26, out, 4096) == 2 ** 21
 
 
 # ------------------------------------------------------------------------------------------- in the child process
