@@ -45,8 +45,6 @@ template <int DP, int FMT> struct ChunkShape {
     static constexpr int SMEM = KC_HEAD + Q + STAGES * OPERAND + 1024;
     static_assert(PER_SM * (SMEM + 1024) <= 233472, "shared memory");
     static constexpr bool OWN_P = TILES == 1 && (DP == 64) == (PLANES == 1);   // columns of their own for the probabilities
-    // a path of its own for tiles that all rows see: more code, which pays where most tiles are such
-    static constexpr bool WHOLE = DP == 128 && PLANES == 1;
     static constexpr int COL_S = 0, COL_P = OWN_P ? 128 * TILES : 0, STEP_P = OWN_P ? 64 * PLANES : 128, COL_O = 128 * TILES + (OWN_P ? STEP_P * TILES : 0);
     static constexpr int COL_F = COL_O + (FRESH ? TILES * DP : 0);     // where P V goes
     static constexpr int TMEM = 512 / PER_SM;
@@ -593,7 +591,8 @@ kv_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                     if (lane == 0) mbar_arrive(bar);
                 };
                 // some keys' exponentials are under way while those before are summed, packed and stored
-                if (Sh::WHOLE && all) {
+                const int hi = b.groups(g0);
+                if (hi == 4) {
 #pragma unroll
                     for (int c = 0; c <= 8; c++) {
                         if (c < 8) open(c);
@@ -601,7 +600,6 @@ kv_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                         if (c == 2 * KC_PART) ready(&p_part[t]);
                     }
                 } else {
-                    const int hi = b.groups(g0);
 #pragma unroll
                     for (int c = 0; c <= 4; c++) {
                         if (c < 4 && c < hi) { open(2 * c); open(2 * c + 1); }
