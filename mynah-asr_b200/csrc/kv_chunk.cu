@@ -37,7 +37,7 @@ template <int DP, int FMT> struct ChunkShape {
     // The launch's registers are dealt out anew between the softmax warps and the four warps of TMA and MMA, two of which have no other
     // work than to lend theirs
     static constexpr bool DEAL = TILES == 2 || PER_SM == 2;
-    static constexpr int THREADS = 32 * (SOFT + 4), REGS = TILES == 2 ? 168 : 128, MORE = TILES == 2 ? 208 : 192, LESS = TILES == 2 ? 88 : 64;
+    static constexpr int THREADS = 32 * (SOFT + 4), REGS = TILES == 2 ? 168 : 128, MORE = TILES == 2 ? 208 : 200, LESS = TILES == 2 ? 88 : 56;
     static_assert(!DEAL || 32 * SOFT * MORE + 128 * LESS <= THREADS * REGS, "a share beyond the launch's registers waits for good");
     static constexpr int OPERAND = HALVES * KC_HALF;           // a tile of queries (one plane), of keys, or of values
     static constexpr int Q = TILES * PLANES * OPERAND;
@@ -52,8 +52,6 @@ template <int DP, int FMT> struct ChunkShape {
     static constexpr int LDO = DP + 4;                         // a part of a row's result in shared memory
     static_assert(TILES * 128 * (LDO * 4 + 8 + 64) <= Q + STAGES * OPERAND, "parts");
 };
-
-struct KcItem { int seq, block; KvSeq q; };
 
 __device__ __forceinline__ void kc_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
     asm volatile(
@@ -118,9 +116,9 @@ struct KcFinder {
         }
         if (bad) atomicExch(a.status, ST_PAGE);
     }
-    __device__ __forceinline__ void find(const KvArgs &a, int x, int lane, KcItem *at) {
+    __device__ __forceinline__ void find(const KvArgs &a, int x, int lane, int *seq, int *block, KvSeq *at) {
         int nth = total - 1 - x;
-        at->seq = -1; at->block = 0; at->q = {0, 0, 0};
+        *seq = -1; *block = 0; *at = {0, 0, 0};
         if (nth < 0) return;
         bool bad = false;
         for (int s0 = 0; s0 < a.n_seq; s0 += 32) {
@@ -135,11 +133,11 @@ struct KcFinder {
             const unsigned in = __ballot_sync(0xffffffffu, nth < upto);
             if (in) {
                 const int who = __ffs(in) - 1;
-                at->seq = s0 + who;
-                at->block = nth - __shfl_sync(0xffffffffu, upto - n, who);
-                at->q.begin = __shfl_sync(0xffffffffu, q.begin, who);
-                at->q.n = __shfl_sync(0xffffffffu, q.n, who);
-                at->q.len = __shfl_sync(0xffffffffu, q.len, who);
+                *seq = s0 + who;
+                *block = nth - __shfl_sync(0xffffffffu, upto - n, who);
+                at->begin = __shfl_sync(0xffffffffu, q.begin, who);
+                at->n = __shfl_sync(0xffffffffu, q.n, who);
+                at->len = __shfl_sync(0xffffffffu, q.len, who);
                 return;
             }
             nth -= __shfl_sync(0xffffffffu, upto, 31);
@@ -147,33 +145,60 @@ struct KcFinder {
     }
 };
 
-// What a block is to those who work on it
+// What a block is to those who work on it. The TMA warp finds it out and leaves it as words in shared memory.
 struct KcBlock {
-    KvSeq sq;
-    int seq, kvh, t0, base_pos, last, top, low, n, nt, rank, shares;
+    static constexpr int WORDS = 12;
+    int seq, kvh, begin, rows, t0, base_pos;         // its sequence (-1: no block, -2: the wait for one ran out), head, the sequence's rows; the block's
+                                                     // first one among them, the position of row 0 of the sequence
+    int n, nt, rank, shares;                         // tiles of keys of this CTA, tiles that have rows, CTAs that share the block
     KvGroups keys;
-    __device__ __forceinline__ KcBlock(const KvArgs &a, const volatile int *item, int tq, int n_tiles, int size, int rank_) {
-        // (one lane's values for all, so that the compiler keeps them and what follows from them in uniform registers)
-        auto same = [](int v) { return __shfl_sync(0xffffffffu, v, 0); };
-        seq = same(item[0]); kvh = same(item[2]);
-        sq = {same(item[3]), same(item[4]), same(item[5])};
-        t0 = same(item[1]) * n_tiles * tq;                     // first position's place among the sequence's rows
-        base_pos = sq.len - sq.n;
-        last = min(t0 + n_tiles * tq, sq.n) - 1;
-        top = base_pos + last;                                 // last key that any row sees,
-        low = base_pos + t0 - a.window + 1;                    // and first that a window shows
+    __device__ __forceinline__ void make(const KvArgs &a, int seq_, int block, int kvh_, const KvSeq &q, int tq, int n_tiles, int size, int rank_) {
+        seq = seq_; kvh = kvh_; begin = q.begin; rows = q.n;
+        t0 = block * n_tiles * tq;
+        base_pos = q.len - q.n;
         keys = {0, 0, 0};
-        if (seq >= 0) keys = kv_groups(base_pos + t0 > 0 ? base_pos + t0 : 0, top, a.window, a.sinks);
-        const int tiles = (keys.count + 3) / 4;
+        if (seq >= 0) keys = kv_groups(base_pos + t0 > 0 ? base_pos + t0 : 0, top(tq, n_tiles), a.window, a.sinks);
         // CTAs that share the block: two tiles each at least, by the block's own tiles
+        const int tiles = (keys.count + 3) / 4, log_shares = min(31 - __clz(size), tiles < 4 ? 0 : 30 - __clz(tiles));
+        rank = rank_; shares = 1 << log_shares;
+        n = rank < shares ? (tiles - rank + shares - 1) >> log_shares : 0;
+        nt = n_tiles == 2 && t0 + tq < rows ? 2 : 1;
+    }
+    __device__ __forceinline__ int top(int tq, int n_tiles) const { return base_pos + min(t0 + n_tiles * tq, rows) - 1; }      // last key that any row sees
+    __device__ __forceinline__ void write(volatile int *w) const {
+        w[0] = seq; w[1] = kvh; w[2] = begin; w[3] = rows; w[4] = t0; w[5] = base_pos; w[6] = n; w[7] = nt; w[8] = shares;
+        w[9] = keys.first; w[10] = keys.start; w[11] = keys.count;
+    }
+    __device__ __forceinline__ void read(const volatile int *w, int lane, int rank_) {
+        // (one lane's values for all, so that the compiler keeps them and what follows from them in uniform registers)
+        const int v = w[lane < WORDS ? lane : 0];
+        auto word = [&](int i) { return __shfl_sync(0xffffffffu, v, i); };
+        seq = word(0); kvh = word(1); begin = word(2); rows = word(3); t0 = word(4); base_pos = word(5); n = word(6); nt = word(7); shares = word(8);
+        keys.first = word(9); keys.start = word(10); keys.count = word(11);
         rank = rank_;
-        shares = min(size, tiles < 4 ? 1 : 1 << (30 - __clz(tiles)));
-        n = rank < shares ? (tiles - rank + shares - 1) / shares : 0;
-        nt = n_tiles == 2 && t0 + tq <= last ? 2 : 1;          // tiles that have rows
     }
     __device__ __forceinline__ int tile_at(int i) const { return 4 * (rank + i * shares); }        // first group of the CTA's i-th tile,
     __device__ __forceinline__ int groups(int g0) const { return min(4, keys.count - g0); }        // and how many it has
 };
+
+// Four lanes' 16 words each, turned so that a lane's words 4 k to 4 k + 3 are its quarter of the words of the four lanes' k-th: lane q of
+// the four gets words 4 q ... of lane k. Stores of rows then touch eight lines an instruction instead of 32.
+__device__ __forceinline__ void kc_quads(uint32_t *w, int lane) {
+#pragma unroll
+    for (int step = 1; step < 4; step *= 2) {
+        const bool up = lane & step;
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+            if (!(k & step)) {
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    uint32_t &lo = w[4 * k + e], &hi = w[4 * (k + step) + e];
+                    const uint32_t got = __shfl_xor_sync(0xffffffffu, up ? lo : hi, step);
+                    if (up) lo = got; else hi = got;
+                }
+            }
+    }
+}
 
 template <int DP, int FMT>
 __global__ void __launch_bounds__(ChunkShape<DP, FMT>::THREADS, ChunkShape<DP, FMT>::PER_SM)
@@ -189,7 +214,7 @@ kv_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
              *s_free = s_full + 2, *p_part = s_free + 2, *p_full = p_part + 2, *o_full = p_full + 2, *i_full = o_full + 2, *i_empty = i_full + 2,
              *drain = i_empty + 2;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(drain + 1);
-    volatile int *items = reinterpret_cast<volatile int *>(tmem_slot + 1);     // two of eight words: sequence, block, kv head, its rows and keys
+    volatile int *items = reinterpret_cast<volatile int *>(tmem_slot + 1);     // two blocks' words
     const int warp = warp_index(), lane = threadIdx.x & 31;
 
     if (threadIdx.x == 0) {
@@ -220,7 +245,8 @@ kv_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
     // Everybody but the TMA warp: the CTA's j-th block, -1 as its sequence behind the last one, and -2 where it does not come
     auto next_block = [&](int j) {
         const bool got = mbar_wait_warp(&i_full[j & 1], (uint32_t)((j >> 1) & 1));
-        KcBlock b(a, items + (j & 1) * 8, tq, TILES, size, rank);
+        KcBlock b;
+        b.read(items + (j & 1) * KcBlock::WORDS, lane, rank);
         if (!got) { b.seq = -2; b.n = 0; }
         return b;
     };
@@ -234,15 +260,18 @@ kv_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
     const uint32_t trow = tmem + ((uint32_t)((warp & 3) * 32) << 16), s_at = trow + Sh::COL_S + t * 128, p_at = trow + Sh::COL_P + t * Sh::STEP_P,
                    o_at = trow + Sh::COL_O + t * DP, f_at = trow + Sh::COL_F + t * DP;
     float m = KC_NONE, l = 0.f;                                // of the row: running maximum and sum
-    auto result = [&](int n, int c, float *o) {                // 32 columns of the row's result over n tiles
-        tc_ld32(f_at + 32 * c, o);
-        kc_wait_ld32(o);
-        if (Sh::FRESH && n > 1) {
-            float more[32];
-            tc_ld32(o_at + 32 * c, more);
-            kc_wait_ld32(more);
+    constexpr int COLS = F32 ? 16 : 32;                        // columns in 16 words
+    auto result = [&](int n, int c, float *o) {                // COLS columns of the row's result over n tiles
+        if constexpr (F32) {
+            float f[32];
+            tc_ld16(f_at + c, f);
+            tc_ld16(n > 1 ? o_at + c : f_at + c, f + 16);
+            kc_wait_ld32(f);
 #pragma unroll
-            for (int e = 0; e < 32; e++) o[e] += more[e];
+            for (int e = 0; e < 16; e++) o[e] = n > 1 ? f[e] + f[e + 16] : f[e];
+        } else {
+            tc_ld32(f_at + c, o);
+            kc_wait_ld32(o);
         }
     };
 
@@ -259,17 +288,20 @@ kv_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
         bool ok = true;
         for (int j = 0, x = (int)(blockIdx.x >> log_size); ok; j++, x += (int)gridDim.x) {
             if (j >= 2 && !mbar_wait_warp(&i_empty[j & 1], (uint32_t)(((j >> 1) & 1) ^ 1))) { ok = false; break; }
-            volatile int *item = items + (j & 1) * 8;
-            KcItem at;
-            finder.find(a, x / a.Hkv, lane, &at);
+            const int nth = x / a.Hkv;
+            int seq, block;
+            KvSeq sq;
+            finder.find(a, nth, lane, &seq, &block, &sq);
+            KcBlock b;
+            b.make(a, seq, block, x - nth * a.Hkv, sq, tq, TILES, size, rank);
             if (lane == 0) {
-                item[0] = at.seq; item[1] = at.block; item[2] = x % a.Hkv; item[3] = at.q.begin; item[4] = at.q.n; item[5] = at.q.len;
+                b.write(items + (j & 1) * KcBlock::WORDS);
                 mbar_arrive(&i_full[j & 1]);
             }
             __syncwarp();
-            const KcBlock b(a, item, tq, TILES, size, rank);
             if (b.seq < 0) break;
-            auto seen = [&](int j) { return j <= b.top && (a.window <= 0 || j + box_rows - 1 >= b.low || j < a.sinks); };
+            const int top = b.top(tq, TILES), low = b.base_pos + b.t0 - a.window + 1;       // last key that any row sees, and first that a window shows
+            auto seen = [&](int j) { return j <= top && (a.window <= 0 || j + box_rows - 1 >= low || j < a.sinks); };
             auto key_of = [&](int i) { return b.keys.at(b.tile_at(i) + (b_sub * box_rows >> 5)) + (b_sub * box_rows & 31); };
             auto entry_of = [&](int i) -> int {
                 const int j = key_of(i);
@@ -282,7 +314,7 @@ kv_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                 __syncwarp();
                 if (lane < b.nt * Sh::HALVES)
                     kc_load_3d(qst + (lane / Sh::HALVES) * Sh::OPERAND + (lane % Sh::HALVES) * KC_HALF, &tmQ, (lane % Sh::HALVES) * 64, b.kvh * a.G,
-                               b.sq.begin + b.t0 + lane / Sh::HALVES * tq, q_full);
+                               b.begin + b.t0 + lane / Sh::HALVES * tq, q_full);
                 queries++;
             }
             for (int i = 0; i < b.n && ok; i++) {
@@ -445,8 +477,8 @@ kv_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                         for (int i = 0; i < BATCH; i++) {
                             const int row = (warp & 3) * 32 + (u + i) * ROWS + lane / PIECES, pl = by_g(row), at = b.t0 + t * tq + pl;
                             in[i][0] = in[i][1] = make_float4(0.f, 0.f, 0.f, 0.f);
-                            if (row < tq * a.G && at < b.sq.n && c * 8 < a.D) {
-                                const float4 *p = reinterpret_cast<const float4 *>(static_cast<const float *>(a.q) + (int64_t)(b.sq.begin + at) * a.ldq +
+                            if (row < tq * a.G && at < b.rows && c * 8 < a.D) {
+                                const float4 *p = reinterpret_cast<const float4 *>(static_cast<const float *>(a.q) + (int64_t)(b.begin + at) * a.ldq +
                                                                                    (int64_t)(b.kvh * a.G + row - pl * a.G) * a.D + c * 8);
                                 in[i][0] = p[0]; in[i][1] = p[1];
                             }
@@ -473,17 +505,18 @@ kv_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
         m = KC_NONE; l = 0.f;
         if (t < b.nt) {
             // rows that do not exist take the last one's position, so that they need no mask of their own
-            const int pos = b.base_pos + min(r < tq * a.G ? tok : b.t0 + t * tq, b.sq.n - 1);
+            const int pos = b.base_pos + min(r < tq * a.G ? tok : b.t0 + t * tq, b.rows - 1);
             auto gather = [&](int i, float alpha) {                // O = (O + P(i - 1) V) alpha
 #pragma unroll 1
-                for (int c = 0; c < DP / 16; c++) {
-                    float f[32];                                   // 16 columns of F, and of O
-                    tc_ld16(f_at + 16 * c, f);
-                    tc_ld16(i > 1 ? o_at + 16 * c : f_at, f + 16);
-                    kc_wait_ld32(f);
+                for (int c = 0; c < DP / 32; c++) {
+                    float f[32], o[32];
+                    tc_ld32(f_at + 32 * c, f);
+                    tc_ld32(i > 1 ? o_at + 32 * c : f_at + 32 * c, o);
+                    kc_wait_ld32(f); kc_wait_ld32(o);
 #pragma unroll
-                    for (int e = 0; e < 16; e++) f[e] = (i > 1 ? f[e] + f[e + 16] : f[e]) * alpha;
-                    kc_st16(o_at + 16 * c, reinterpret_cast<const uint32_t *>(f));
+                    for (int e = 0; e < 32; e++) f[e] = (i > 1 ? f[e] + o[e] : f[e]) * alpha;
+                    kc_st16(o_at + 32 * c, reinterpret_cast<const uint32_t *>(f));
+                    kc_st16(o_at + 32 * c + 16, reinterpret_cast<const uint32_t *>(f + 16));
                 }
             };
             for (int i = 0; i < n && ok; i++) {
@@ -614,33 +647,34 @@ kv_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
             if (n > 0) { done += n; blocks++; }
             tc_fence_after();
             // (what the results need of the block is read again, so that it takes no registers above)
-            const KcBlock e(a, items + (j & 1) * 8, tq, TILES, size, rank);
-            if (e.shares == 1 && rank == 0 && ok) {
-                const int tok = e.t0 + t * tq + by_g(r);
+            const volatile int *w = items + (j & 1) * KcBlock::WORDS;
+            if (w[8] == 1 && rank == 0 && ok) {
                 const float inv = l != 0.f ? 1.f / l : 0.f;
-                const bool valid = r < tq * a.G && tok < e.sq.n;
-                const int64_t to = (int64_t)(e.sq.begin + tok) * a.ldo + (int64_t)(e.kvh * a.G + r - by_g(r) * a.G) * a.D;
+                // after the turn a lane stores a quarter of 16 words of each of the four rows of its lanes: where they lie, -1 for rows that are not
+                const int begin = w[2], last = w[3] - w[4] - t * tq, kvh = w[1];       // (rows of the tile: below last)
+                const int64_t first = (int64_t)(begin + w[4] + t * tq) * a.ldo + (int64_t)kvh * a.G * a.D;
+                int64_t to[4];
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    const int row = (r & ~3) + k, pl = by_g(row);
+                    to[k] = row < tq * a.G && pl < last ? first + pl * a.ldo + (row - pl * a.G) * a.D : -1;
+                }
 #pragma unroll 1
-                for (int c = 0; c < DP / 32; c++) {
-                    float o[32];
-                    if (n > 0) result(n, c, o);
+                for (int c = 0; c < DP / COLS; c++) {
+                    float o[COLS];
+                    if (n > 0) result(n, c * COLS, o);
+                    uint32_t v[16];
 #pragma unroll
-                    for (int u = 0; u < 32; u++) o[u] = inv != 0.f ? o[u] * inv : 0.f;
-                    if (valid) {
-#pragma unroll
-                        for (int u = 0; u < 32; u += 8) {
-                            if (c * 32 + u >= a.D) continue;
-                            if (F32) {
-                                float4 *p = reinterpret_cast<float4 *>(static_cast<float *>(a.out) + to + c * 32 + u);
-                                p[0] = make_float4(o[u], o[u + 1], o[u + 2], o[u + 3]);
-                                p[1] = make_float4(o[u + 4], o[u + 5], o[u + 6], o[u + 7]);
-                            } else {
-                                *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(a.out) + to + c * 32 + u) =
-                                    make_uint4(kv_pack<BF>(o[u], o[u + 1]), kv_pack<BF>(o[u + 2], o[u + 3]), kv_pack<BF>(o[u + 4], o[u + 5]), kv_pack<BF>(o[u + 6], o[u + 7]));
-                            }
-                        }
+                    for (int u = 0; u < 16; u++) {
+                        if (F32) v[u] = __float_as_uint(inv != 0.f ? o[u] * inv : 0.f);
+                        else v[u] = inv != 0.f ? kv_pack<BF>(o[2 * u] * inv, o[2 * u + 1] * inv) : 0u;
                     }
-                    __syncwarp();
+                    kc_quads(v, lane);
+                    const int col = c * COLS + (lane & 3) * (COLS / 4);
+#pragma unroll
+                    for (int k = 0; k < 4; k++)
+                        if (to[k] >= 0 && col < a.D)
+                            *reinterpret_cast<uint4 *>(static_cast<uint8_t *>(a.out) + (to[k] + col) * (F32 ? 4 : 2)) = make_uint4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
                 }
                 tc_fence_before();                             // (the next block's products are ordered behind these loads by its P)
             }
@@ -653,7 +687,8 @@ kv_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
     __syncwarp();
     if (once) {
         __syncthreads();                                       // (the TMA warp has written the block's words)
-        const KcBlock b(a, items, tq, TILES, size, rank);
+        KcBlock b;
+        b.read(items, lane, rank);
         if (b.shares > 1) {
             // parts of the rows' results and (maximum, sum) of each, where queries and tiles were; then the weights of the parts, and their sum
             // by all CTAs of the cluster, each for its rows
@@ -663,17 +698,17 @@ kv_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
             if (soft && t < b.nt && b.n > 0) {
                 float *row = part + (t * 128 + r) * Sh::LDO;
 #pragma unroll 1
-                for (int c = 0; c < DP / 32; c++) {
-                    float o[32];
+                for (int c = 0; c < DP; c += COLS) {
+                    float o[COLS];
                     result(b.n, c, o);
 #pragma unroll
-                    for (int e = 0; e < 32; e += 4) *reinterpret_cast<float4 *>(row + c * 32 + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                    for (int e = 0; e < COLS; e += 4) *reinterpret_cast<float4 *>(row + c + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
                 }
                 ml[t * 128 + r] = make_float2(m, l);
             }
             kv_cluster_sync();
             const uint32_t part0 = smem_u32(part), ml0 = smem_u32(ml);
-            const int per_tile = tq * a.G, rows = min((b.last - b.t0 + 1) * a.G, b.nt * per_tile), share = (rows + size - 1) >> log_size;
+            const int per_tile = tq * a.G, rows = min((min(b.t0 + TILES * tq, b.rows) - b.t0) * a.G, b.nt * per_tile), share = (rows + size - 1) >> log_size;
             const int v0 = rank * share, mine = max(0, min(share, rows - v0)), quads = a.D / 4;
             auto place_of = [&](int v) { return v < per_tile ? v : 128 + v - per_tile; };
             for (int v = threadIdx.x; v < mine; v += Sh::THREADS) {
@@ -716,7 +751,7 @@ kv_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                         }
                 }
                 const int pl = by_g(v0 + v);
-                const int64_t to = (int64_t)(b.sq.begin + b.t0 + pl) * a.ldo + (int64_t)(b.kvh * a.G + v0 + v - pl * a.G) * a.D + c;
+                const int64_t to = (int64_t)(b.begin + b.t0 + pl) * a.ldo + (int64_t)(b.kvh * a.G + v0 + v - pl * a.G) * a.D + c;
                 if (F32) *reinterpret_cast<float4 *>(static_cast<float *>(a.out) + to) = sum;
                 else *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(a.out) + to) = make_uint2(kv_pack<BF>(sum.x, sum.y), kv_pack<BF>(sum.z, sum.w));
             }
