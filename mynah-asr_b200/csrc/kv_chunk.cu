@@ -42,16 +42,18 @@ template <int DP, int FMT> struct ChunkShape {
     // own, in columns F, that the softmax warps add to O
     static constexpr bool FRESH = FMT == KV_F32;
     static constexpr int TILES = DP == 64 || FRESH ? 1 : 2, PER_SM = DP == 64 ? 2 : 1;         // tiles of rows of a CTA, CTAs of an SM
-    static constexpr int SOFT = 4 * TILES, W_TMA = SOFT, W_MMA = SOFT + 1;             // warps
+    // two threads a row, 64 of a tile's keys and half of O each, where the SM has no other softmax warps
+    static constexpr int SPLIT = TILES * PER_SM == 1 ? 2 : 1, OWN = KC_KEYS / SPLIT;
+    static constexpr int SOFT = 4 * TILES * SPLIT, W_TMA = SOFT, W_MMA = SOFT + 1;             // warps
     // The launch's registers are dealt out anew between the softmax warps and the four warps of TMA and MMA, two of which have no other
     // work than to lend theirs
-    static constexpr bool DEAL = TILES == 2 || PER_SM == 2;
-    static constexpr int THREADS = 32 * (SOFT + 4), REGS = TILES == 2 ? 168 : 128, MORE = TILES == 2 ? 208 : 200, LESS = TILES == 2 ? 88 : 56;
-    static_assert(!DEAL || 32 * SOFT * MORE + 128 * LESS <= THREADS * REGS, "a share beyond the launch's registers waits for good");
+    static constexpr int THREADS = 32 * (SOFT + 4), REGS = SOFT == 8 ? 168 : 128, MORE = SOFT == 8 ? 208 : 200, LESS = SOFT == 8 ? 88 : 56;
+    static_assert(32 * SOFT * MORE + 128 * LESS <= THREADS * REGS, "a share beyond the launch's registers waits for good");
     static constexpr int OPERAND = HALVES * KC_HALF;           // a tile of queries (one plane), of keys, or of values
     static constexpr int Q = TILES * PLANES * OPERAND;
-    static constexpr int STAGES = DP == 64 ? 6 - PLANES : 5;
-    static constexpr int SMEM = KC_HEAD + Q + STAGES * OPERAND + 1024;
+    static constexpr int STAGES = 6 - PLANES;
+    static constexpr int HEAD = KC_HEAD + (SPLIT == 2 ? 2048 : 0);     // barriers, blocks' words; what the two threads of a row tell one another
+    static constexpr int SMEM = HEAD + Q + STAGES * OPERAND + 1024;
     static_assert(PER_SM * (SMEM + 1024) <= 233472, "shared memory");
     static constexpr bool OWN_P = TILES == 1 && (DP == 64) == (PLANES == 1);   // columns of their own for the probabilities
     static constexpr int COL_S = 0, COL_P = OWN_P ? 128 * TILES : 0, STEP_P = OWN_P ? 64 * PLANES : 128, COL_O = 128 * TILES + (OWN_P ? STEP_P * TILES : 0);
@@ -215,14 +217,14 @@ kv_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                 int box_rows, int log_size) {
     using Sh = ChunkShape<DP, FMT>;
     constexpr bool BF = FMT == KV_BF16, F32 = FMT == KV_F32, OWN_P = Sh::OWN_P;
-    constexpr int STAGES = Sh::STAGES, TILES = Sh::TILES;
+    constexpr int STAGES = Sh::STAGES, TILES = Sh::TILES, SPLIT = Sh::SPLIT, OWN = Sh::OWN, GROUPS = OWN / 32;
     extern __shared__ uint8_t kc_raw[];
     uint8_t *head = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(kc_raw) + 1023) & ~uintptr_t(1023));
-    uint8_t *qst = head + KC_HEAD, *ring = qst + Sh::Q;
+    uint8_t *qst = head + Sh::HEAD, *ring = qst + Sh::Q;
     uint64_t *full = reinterpret_cast<uint64_t *>(head), *empty = full + STAGES, *q_full = empty + STAGES, *q_empty = q_full + 1, *s_full = q_empty + 1,
              *s_free = s_full + 2, *p_part = s_free + 2, *p_full = p_part + 2, *o_full = p_full + 2, *i_full = o_full + 2, *i_empty = i_full + 2,
-             *drain = i_empty + 2;
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(drain + 1);
+             *drain = i_empty + 2, *pair = drain + 1;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(pair + 4);
     volatile int *items = reinterpret_cast<volatile int *>(tmem_slot + 1);     // two blocks' words
     const int warp = warp_index(), lane = threadIdx.x & 31;
 
@@ -233,8 +235,9 @@ kv_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
         mbar_init(q_full, F32 ? Sh::SOFT : 1); mbar_init(q_empty, 1);
         for (int t = 0; t < TILES; t++) {
             mbar_init(&s_full[t], 1); mbar_init(&o_full[t], 1);
-            mbar_init(&s_free[t], 4); mbar_init(&p_part[t], 4); mbar_init(&p_full[t], 4);
+            mbar_init(&s_free[t], 4 * SPLIT); mbar_init(&p_part[t], 4 * SPLIT); mbar_init(&p_full[t], 4 * SPLIT);
         }
+        if (SPLIT == 2) for (int i = 0; i < 4; i++) mbar_init(&pair[i], 2);
         for (int i = 0; i < 2; i++) { mbar_init(&i_full[i], 1); mbar_init(&i_empty[i], Sh::SOFT + 1); }
         mbar_init(drain, 1);
         mbar_fence_init();
@@ -263,8 +266,8 @@ kv_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
         __syncwarp();
         if (lane == 0) mbar_arrive(&i_empty[j & 1]);
     };
-    // row of a softmax thread, in tile t
-    const int t = TILES == 2 ? (warp >> 2) & 1 : 0, r = (warp & 3) * 32 + lane;
+    // row of a softmax thread, in tile t; its keys and columns of a tile are those from half * OWN (half * DP / SPLIT) on
+    const int t = TILES == 2 ? (warp >> 2) & 1 : 0, half = SPLIT == 2 ? (warp >> 2) & 1 : 0, r = (warp & 3) * 32 + lane;
     const bool soft = warp < Sh::SOFT;
     const uint32_t trow = tmem + ((uint32_t)((warp & 3) * 32) << 16), s_at = trow + Sh::COL_S + t * 128, p_at = trow + Sh::COL_P + t * Sh::STEP_P,
                    o_at = trow + Sh::COL_O + t * DP, f_at = trow + Sh::COL_F + t * DP;
@@ -285,7 +288,7 @@ kv_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
     };
 
     if (!soft) {
-    if (Sh::DEAL) kc_regs_less<Sh::LESS>();                    // (one instruction for the four warps)
+    kc_regs_less<Sh::LESS>();                                  // (one instruction for the four warps)
     if (warp == Sh::W_TMA) {
         // ---- lane = one box of a tile: 64 of the D columns, the slots of one page. Item 2 i of the ring is K(i), 2 i + 1 V(i).
         const int shift = a.page_shift, boxes = KC_KEYS / box_rows * Sh::HALVES;
@@ -464,19 +467,32 @@ kv_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
     }
     } else {
     // ---- softmax: thread = row
-    if (Sh::DEAL) kc_regs_more<Sh::MORE>();
+    kc_regs_more<Sh::MORE>();
     const float sc = a.scale2;
     bool ok = true;
     int done = 0, blocks = 0;                                  // tiles of keys, and blocks, behind this tile of rows
+    // The two threads of a row exchange a value; false where the other one's does not come
+    float *told = reinterpret_cast<float *>(head + KC_HEAD);
+    int turn = 0;
+    auto exchange = [&](float mine, float *other) {
+        float *at = told + (turn & 1) * 256 + r;
+        at[half * 128] = mine;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&pair[warp & 3]);
+        const bool got = mbar_wait_warp(&pair[warp & 3], (uint32_t)(turn & 1));
+        *other = at[(half ^ 1) * 128];
+        turn++;
+        return got;
+    };
     for (int j = 0; ok; j++) {
         const KcBlock b = next_block(j);
         if (b.seq < 0) { ok = b.seq == -1; break; }
         const int n = b.n, tok = b.t0 + t * tq + by_g(r);
         if (F32 && n > 0) {
-                // the warp's 32 rows, neighbouring lanes on neighbouring pieces of eight values
-                constexpr int PIECES = DP / 8, ROWS = 32 / PIECES, ROUNDS = 32 / ROWS, BATCH = 8;
+                // the warp's 32 (or 16) rows, neighbouring lanes on neighbouring pieces of eight values
+                constexpr int PIECES = DP / 8, ROWS = 32 / PIECES, ROUNDS = 32 / SPLIT / ROWS, BATCH = 8;
                 uint8_t *qt = qst + t * Sh::PLANES * Sh::OPERAND;
-                const int c = lane % PIECES;
+                const int c = lane % PIECES, row0 = (warp & 3) * 32 + half * (32 / SPLIT);
                 bool bad = false;
                 if (t < b.nt) {
 #pragma unroll 1
@@ -484,7 +500,7 @@ kv_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                         float4 in[BATCH][2];
 #pragma unroll
                         for (int i = 0; i < BATCH; i++) {
-                            const int row = (warp & 3) * 32 + (u + i) * ROWS + lane / PIECES, pl = by_g(row), at = b.t0 + t * tq + pl;
+                            const int row = row0 + (u + i) * ROWS + lane / PIECES, pl = by_g(row), at = b.t0 + t * tq + pl;
                             in[i][0] = in[i][1] = make_float4(0.f, 0.f, 0.f, 0.f);
                             if (row < tq * a.G && at < b.rows && c * 8 < a.D) {
                                 const float4 *p = reinterpret_cast<const float4 *>(static_cast<const float *>(a.q) + (int64_t)(b.begin + at) * a.ldq +
@@ -494,7 +510,7 @@ kv_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                         }
 #pragma unroll
                         for (int i = 0; i < BATCH; i++) {
-                            const int row = (warp & 3) * 32 + (u + i) * ROWS + lane / PIECES;
+                            const int row = row0 + (u + i) * ROWS + lane / PIECES;
                             uint8_t *to = qt + (c >> 3) * KC_HALF + row * 128 + (((c & 7) ^ (row & 7)) << 4);
                             const float *f = reinterpret_cast<const float *>(in[i]);
                             uint4 hi, lo;
@@ -517,7 +533,7 @@ kv_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
             const int pos = b.base_pos + min(r < tq * a.G ? tok : b.t0 + t * tq, b.rows - 1);
             auto gather = [&](int i, float alpha) {                // O = (O + P(i - 1) V) alpha
 #pragma unroll 1
-                for (int c = 0; c < DP / 32; c++) {
+                for (int c = half * (DP / 32 / SPLIT); c < (half + 1) * (DP / 32 / SPLIT); c++) {
                     float f[32], o[32];
                     tc_ld32(f_at + 32 * c, f);
                     tc_ld32(i > 1 ? o_at + 32 * c : f_at + 32 * c, o);
@@ -532,27 +548,28 @@ kv_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                 if (!mbar_wait_warp(&s_full[t], (uint32_t)((done + i) & 1))) { ok = false; break; }
                 tc_fence_after();
                 if (Sh::FRESH && !OWN_P && i > 0) gather(i, 1.f);  // (while the scores take no registers)
-                float x[KC_KEYS];
-                tc_ld32(s_at, x);
-                tc_ld32(s_at + 32, x + 32);
+                float x[OWN], m4[4];
+                const uint32_t x_at = s_at + half * OWN;
+                tc_ld32(x_at, x);
+                tc_ld32(x_at + 32, x + 32);
                 kc_wait_ld32(x); kc_wait_ld32(x + 32);
-                tc_ld32(s_at + 64, x + 64);
-                tc_ld32(s_at + 96, x + 96);
-                float m4[4] = {x[0], x[1], x[2], x[3]};
+                if (OWN == 128) { tc_ld32(x_at + 64, x + OWN - 64); tc_ld32(x_at + 96, x + OWN - 32); }
+#pragma unroll
+                for (int e = 0; e < 4; e++) m4[e] = x[e];
 #pragma unroll
                 for (int c = 4; c < 60; c += 8)
 #pragma unroll
                     for (int e = 0; e < 4; e++) m4[e] = fmaxf(m4[e], fmaxf(x[c + e], x[c + 4 + e]));
 #pragma unroll
                 for (int e = 0; e < 4; e++) m4[e] = fmaxf(m4[e], x[60 + e]);
-                kc_wait_ld32(x + 64); kc_wait_ld32(x + 96);
+                if (OWN == 128) { kc_wait_ld32(x + OWN - 64); kc_wait_ld32(x + OWN - 32); }
                 if (OWN_P) {                                       // the scores are in registers
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&s_free[t]);
                 }
 #pragma unroll
-                for (int c = 64; c < 128; c += 8)
+                for (int c = 64; c < OWN; c += 8)
 #pragma unroll
                     for (int e = 0; e < 4; e++) m4[e] = fmaxf(m4[e], fmaxf(x[c + e], x[c + 4 + e]));
                 const int g0 = b.tile_at(i), j0 = b.keys.at(g0), d = pos - j0;
@@ -564,8 +581,8 @@ kv_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                     auto upto = [](int c) -> uint32_t { return c < 0 ? 0u : c >= 31 ? 0xffffffffu : (2u << c) - 1u; };      // bits 0 to c
                     m4[0] = m4[1] = m4[2] = m4[3] = -INFINITY;
 #pragma unroll
-                    for (int w = 0; w < 4; w++) {
-                        const int jw = b.keys.at(g0 + w), dw = pos - jw;
+                    for (int w = 0; w < GROUPS; w++) {
+                        const int jw = b.keys.at(g0 + half * GROUPS + w), dw = pos - jw;
                         const uint32_t see = upto(dw) & (~upto(a.window > 0 ? dw - a.window : -1) | upto(a.sinks - 1 - jw));
                         if (!__all_sync(0xffffffffu, see == 0xffffffffu)) {
 #pragma unroll
@@ -578,7 +595,13 @@ kv_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                             for (int e = 0; e < 4; e++) m4[e] = fmaxf(m4[e], fmaxf(x[32 * w + c + e], x[32 * w + c + 4 + e]));
                     }
                 }
-                const float mt = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * sc;
+                float mt = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+                if (SPLIT == 2) {
+                    float other;
+                    if (!exchange(mt, &other)) { ok = false; break; }
+                    mt = fmaxf(mt, other);
+                }
+                mt *= sc;
                 if (OWN_P && i > 0) {                              // P(i - 1) has been read, and O is at rest
                     if (!mbar_wait_warp(&o_full[t], (uint32_t)((done + i - 1) & 1))) { ok = false; break; }
                     tc_fence_after();
@@ -623,8 +646,8 @@ kv_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                         if (F32) kv_split(v[0], v[1], hi[e], lo[F32 ? e : 0]);
                         else hi[e] = kv_pack<BF>(v[0], v[1]);
                     }
-                    kc_st8(p_at + 8 * c, hi);
-                    if (F32) kc_st8(p_at + 64 + 8 * c, lo);
+                    kc_st8(p_at + half * (OWN / 2) + 8 * c, hi);
+                    if (F32) kc_st8(p_at + 64 + half * (OWN / 2) + 8 * c, lo);
                 };
                 auto ready = [&](uint64_t *bar) {
                     kc_wait_st();
@@ -633,20 +656,20 @@ kv_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                     if (lane == 0) mbar_arrive(bar);
                 };
                 // some keys' exponentials are under way while those before are summed, packed and stored
-                const int hi = b.groups(g0);
-                if (hi == 4) {
+                const int hi = b.groups(g0) - half * GROUPS, part = KC_PART - half * GROUPS;      // of the thread's groups: those with keys; the first signal's
+                if (hi >= GROUPS) {
 #pragma unroll
-                    for (int c = 0; c <= 8; c++) {
-                        if (c < 8) open(c);
+                    for (int c = 0; c <= 2 * GROUPS; c++) {
+                        if (c < 2 * GROUPS) open(c);
                         if (c > 0) close(c - 1);
-                        if (c == 2 * KC_PART) ready(&p_part[t]);
+                        if (c == 2 * min(part, GROUPS)) ready(&p_part[t]);
                     }
                 } else {
 #pragma unroll
-                    for (int c = 0; c <= 4; c++) {
-                        if (c < 4 && c < hi) { open(2 * c); open(2 * c + 1); }
+                    for (int c = 0; c <= GROUPS; c++) {
+                        if (c < GROUPS && c < hi) { open(2 * c); open(2 * c + 1); }
                         if (c > 0 && c <= hi) { close(2 * c - 2); close(2 * c - 1); }
-                        if (c == KC_PART) ready(&p_part[t]);
+                        if (c == min(part, GROUPS)) ready(&p_part[t]);
                     }
                 }
                 ready(&p_full[t]);
@@ -655,6 +678,11 @@ kv_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
             if (n > 0 && ok) ok = mbar_wait_warp(&o_full[t], (uint32_t)(OWN_P ? (done + n - 1) & 1 : blocks & 1));
             if (n > 0) { done += n; blocks++; }
             tc_fence_after();
+            if (SPLIT == 2 && n > 0 && ok) {
+                float other;
+                ok = exchange(l, &other);
+                l += other;
+            }
             // (what the results need of the block is read again, so that it takes no registers above)
             const volatile int *w = items + (j & 1) * KcBlock::WORDS;
             if (w[8] == 1 && rank == 0 && ok) {
@@ -669,7 +697,7 @@ kv_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                     to[k] = row < tq * a.G && pl < last ? first + pl * a.ldo + (row - pl * a.G) * a.D : -1;
                 }
 #pragma unroll 1
-                for (int c = 0; c < DP / COLS; c++) {
+                for (int c = half * (DP / COLS / SPLIT); c < (half + 1) * (DP / COLS / SPLIT); c++) {
                     float o[COLS];
                     if (n > 0) result(n, c * COLS, o);
                     uint32_t v[16];
@@ -707,13 +735,13 @@ kv_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
             if (soft && t < b.nt && b.n > 0) {
                 float *row = part + (t * 128 + r) * Sh::LDO;
 #pragma unroll 1
-                for (int c = 0; c < DP; c += COLS) {
+                for (int c = half * (DP / SPLIT); c < (half + 1) * (DP / SPLIT); c += COLS) {
                     float o[COLS];
                     result(b.n, c, o);
 #pragma unroll
                     for (int e = 0; e < COLS; e += 4) *reinterpret_cast<float4 *>(row + c + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
                 }
-                ml[t * 128 + r] = make_float2(m, l);
+                if (half == 0) ml[t * 128 + r] = make_float2(m, l);
             }
             kv_cluster_sync();
             const uint32_t part0 = smem_u32(part), ml0 = smem_u32(ml);
