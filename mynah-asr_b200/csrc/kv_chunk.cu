@@ -5,7 +5,7 @@
 // both take about 1024 clocks of an SM for 128 rows and 128 keys). A CTA owns one kv head and one or two tiles of 128 rows: the G query
 // heads of 128 / G positions each (row r is head r % G of position r / G), so that short pieces fill a tile and all heads share the
 // keys' tiles. Keys and values come in tiles of 128 by TMA, from their pages straight into the swizzled operand layout: groups of 32
-// keys, those that some row sees, side by side (KvGroups; a tile of their own for a window's first tokens took 86 us where now 71 do).
+// keys, those that some row sees, side by side (KvGroups; with a tile of their own for a window's first tokens the third case below took 75 us instead of 63).
 //   tensor memory  16-bit rows: scores S (128 columns a tile) and results O. D > 64: two tiles of rows, whose probabilities P overwrite
 //                  their scores. D <= 64: one tile, two CTAs an SM, columns of their own for P, so that S(i + 1) is computed under the
 //                  exponentials of tile i. F32 rows: one tile, and F, the products of one tile of keys (see ChunkShape)
@@ -13,8 +13,8 @@
 //   order of MMAs  P0 V(i), S0(i + 1), P1 V(i), S1(i + 1): one tile's exponentials run under the other's products. MMAs run in the
 //                  order of their issue, so S(i + 1) does not overwrite the P(i) that P V(i) reads, and whoever sees S(i + 1) finished
 //                  finds O at rest. With columns of their own for P: S(i + 1) in front of P V(i).
-// A CTA stays and takes block after block (heads of a block side by side, later positions, which see more keys, first): the next block's
-// place, queries and first keys are looked up, fetched and multiplied while the results of the one before are written.
+// A CTA stays and takes block after block (heads of a block side by side, long blocks first, KcFinder): the next block's place, queries
+// and first keys are looked up, fetched and multiplied while the results of the one before are written.
 // The softmax keeps a running maximum per row; O is rescaled only when it has grown by more than 2^8 (what is stale cancels in the
 // final division). F32 rows: queries and probabilities as (hi, lo) f16 pairs, two products each.
 // A call with few blocks is launched as clusters: the CTAs of a cluster take a block's tiles in turn, two at least each, and join their
@@ -22,7 +22,7 @@
 //
 // Measured (us): 16384 rows of 32 query and 8 kv heads of 128, bf16, 2000 = 1.1 PFLOP/s under the power cap (1.72 GHz; a library's
 // product of matrices holds 1.42 there); 4 pieces of 5 to 61 rows behind 300 to 1500 keys 14.0; 7 prompts of 301 to 4000 rows, 16 and 4
-// heads of 64, f16, window 512, 63.5; 9 of 40 to 1300 F32 rows, 8 heads of 128, 48.1. A tile of D = 128 goes through 1190 clocks of
+// heads of 64, f16, window 512, 58.8; 9 of 40 to 1300 F32 rows, 8 heads of 128, 37.6. A tile of D = 128 goes through 1190 clocks of
 // waiting for its scores, 245 + 220 of their maximum, 1550 of exponentials and packing, 250 of signals; the other tile's take turns with
 // it. Tensor cores and exponential units are busy half of the time each. What was tried against that: steps of 64 keys with two score
 // buffers, so that no softmax waits (2210: products 64 columns wide take as long as 128 wide ones), a part of the exponentials as
@@ -109,7 +109,9 @@ __device__ __forceinline__ uint64_t kc_desc_mn(uint32_t addr) {
 }
 
 // Where the TMA warp finds the call's blocks: all their number, and the x-th from the last, since later positions see more keys and
-// what takes longest should begin first. With up to 32 sequences a lane keeps one.
+// what takes longest should begin first. With up to 32 sequences a lane keeps one, and the x-th longest is found, too: by bisection of
+// the length that more than x blocks have (with it the third and fourth case above take 58.8 and 37.6 us, with the order of the sequences
+// 63.4 and 46.2).
 struct KcFinder {
     int per_block, total;
     KvSeq q;
@@ -126,6 +128,35 @@ struct KcFinder {
             total += __reduce_add_sync(0xffffffffu, blocks());
         }
         if (bad) atomicExch(a.status, ST_PAGE);
+    }
+    // Blocks of the lane's sequence with `tiles` tiles of keys at least: those from some place on (a window bounds all alike)
+    __device__ __forceinline__ int as_long(const KvArgs &a, int tiles) const {
+        const int need = (tiles - 1) * KC_KEYS + 1 - (q.len - q.n);            // rows that the block's last one has in front of it, and itself
+        if (need > q.n || (a.window > 0 && (tiles - 1) * KC_KEYS >= a.window + a.sinks + per_block)) return 0;
+        return blocks() - (need <= per_block ? 0 : (need + per_block - 1) / per_block - 1);
+    }
+    __device__ __forceinline__ void find_longest(const KvArgs &a, int x, int lane, int *seq, int *block, KvSeq *at) {
+        *seq = -1; *block = 0; *at = {0, 0, 0};
+        if (x >= total) return;
+        int lo = 0, hi = __reduce_max_sync(0xffffffffu, q.n > 0 ? (max(q.len, 0) + KC_KEYS - 1) / KC_KEYS : 0) + 1;         // x < blocks of lo tiles, not of hi
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (__reduce_add_sync(0xffffffffu, as_long(a, mid)) > x) lo = mid; else hi = mid;
+        }
+        const int longer = as_long(a, lo + 1), some = lo > 0 ? as_long(a, lo) : blocks(), n = some - longer;
+        int nth = x - __reduce_add_sync(0xffffffffu, longer), upto = n;
+#pragma unroll
+        for (int o = 1; o < 32; o *= 2) {
+            const int v = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += v;
+        }
+        const int who = __ffs(__ballot_sync(0xffffffffu, nth < upto)) - 1;
+        if (who < 0) return;
+        *seq = who;
+        *block = __shfl_sync(0xffffffffu, blocks() - some - (upto - n), who) + nth;
+        at->begin = __shfl_sync(0xffffffffu, q.begin, who);
+        at->n = __shfl_sync(0xffffffffu, q.n, who);
+        at->len = __shfl_sync(0xffffffffu, q.len, who);
     }
     __device__ __forceinline__ void find(const KvArgs &a, int x, int lane, int *seq, int *block, KvSeq *at) {
         int nth = total - 1 - x;
@@ -214,7 +245,7 @@ __device__ __forceinline__ void kc_quads(uint32_t *w, int lane) {
 template <int DP, int FMT>
 __global__ void __launch_bounds__(ChunkShape<DP, FMT>::THREADS, ChunkShape<DP, FMT>::PER_SM)
 kv_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const KvArgs a,
-                int box_rows, int log_size) {
+                int box_rows, int log_size, int longest_first) {
     using Sh = ChunkShape<DP, FMT>;
     constexpr bool BF = FMT == KV_BF16, F32 = FMT == KV_F32, OWN_P = Sh::OWN_P;
     constexpr int STAGES = Sh::STAGES, TILES = Sh::TILES, SPLIT = Sh::SPLIT, OWN = Sh::OWN, GROUPS = OWN / 32;
@@ -298,12 +329,15 @@ kv_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
         finder.init(a, TILES * tq, lane);
         int s = 0, ph = 0, r = 0, queries = 0;                 // place in the ring, its parity, requests; blocks with queries so far
         bool ok = true;
-        for (int j = 0, x = (int)(blockIdx.x >> log_size); ok; j++, x += (int)gridDim.x) {
+        for (int j = 0, x0 = 0; ok; j++, x0 += (int)gridDim.x) {
+            // (there and back: a CTA whose block was the longest of its round gets the shortest of the next)
+            const int x = x0 + (longest_first && (j & 1) ? (int)(gridDim.x - 1 - blockIdx.x) : (int)(blockIdx.x >> log_size));
             if (j >= 2 && !mbar_wait_warp(&i_empty[j & 1], (uint32_t)(((j >> 1) & 1) ^ 1))) { ok = false; break; }
             const int nth = x / a.Hkv;
             int seq, block;
             KvSeq sq;
-            finder.find(a, nth, lane, &seq, &block, &sq);
+            if (longest_first) finder.find_longest(a, nth, lane, &seq, &block, &sq);
+            else finder.find(a, nth, lane, &seq, &block, &sq);
             KcBlock b;
             b.make(a, seq, block, x - nth * a.Hkv, sq, tq, TILES, size, rank);
             if (lane == 0) {
@@ -845,16 +879,18 @@ static int chunk_launch(const CUtensorMap &k, const CUtensorMap &v, const KvArgs
         if (most < 0) return -1;
         if (likely <= (int64_t)Sh::PER_SM * most) log_size = k;
     }
-    if (blocks << log_size > 0x7fffffff) { set_error("kv_attend: too many rows in one call"); return -1; }
+    if (blocks << log_size > 0x3fffffff) { set_error("kv_attend: too many rows in one call"); return -1; }
     // Where blocks are short, as many CTAs as fit take one after the other; where they are long, the hardware deals them out better than a
     // fixed order (32 and 8 heads of 128, us, that way and with a CTA per block: 8 x 500 rows 49, 52, 4 x 2000 162, 175; 8000 490, 454)
     const int64_t keys = (int64_t)a.max_pages << a.page_shift, seen = (int64_t)a.window + a.sinks + per_block;
     const bool stay = (a.window > 0 && seen < keys ? seen : keys) <= KC_STAY;
     const int64_t room = (int64_t)Sh::PER_SM * device_sm_count();
     const int64_t ctas = log_size ? blocks << log_size : stay && blocks > room ? room : blocks;
+    // Which order: the sequences' blocks from the last on, or, where there is more than one round of them, the longest first
+    const bool longest_first = blocks > room && a.n_seq > 1 && a.n_seq <= 32;
     CUtensorMap q = k;
     if (FMT != KV_F32 && !kv_rows_map(&q, a, FMT == KV_BF16)) { set_error("kv_attend: no tensor map of the rows"); return -1; }
-    MB_CUDA(launch_kernel(kernel, dim3((unsigned)ctas), dim3(Sh::THREADS), (size_t)Sh::SMEM, st, true, 1 << log_size, q, k, v, a, box_rows, log_size));
+    MB_CUDA(launch_kernel(kernel, dim3((unsigned)ctas), dim3(Sh::THREADS), (size_t)Sh::SMEM, st, true, 1 << log_size, q, k, v, a, box_rows, log_size, longest_first ? 1 : 0));
     note_launch();
     return 0;
 }

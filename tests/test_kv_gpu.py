@@ -722,3 +722,13 @@ print("same")
 def test_first_calls_of_a_process_are_captured(gpu_pkg):
     got = subprocess.run([sys.executable, "-c", FIRST, gpu_pkg.__file__], capture_output=True, text=True, timeout=300)
     assert got.returncode == 0 and "same" in got.stdout, got.stderr
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("dim,window,sinks", [(64, 0, 0), (128, 0, 0), (64, 200, 5), (128, 333, 70)])
+def test_chunk_more_blocks_than_places(gpu_pkg, fmt, dim, window, sinks):
+    """More blocks than run at a time: the longest first, then there and back. Sequences without rows, with more rows than keys, alike ones."""
+    rows = [640, 1, 0, 640, 129, 900, 700, 640, 128, 64, 257, 500, 0, 333, 640]
+    lens = [640, 700, 50, 640, 2000, 900, 300, 800, 1500, 64, 1280, 500, 0, 0, 640]
+    attend_case(gpu_pkg, P.Layout(lens, 32, rows, extra_rows=9), 16, 16, dim, fmt, window=window, n_sinks=sinks)
+    attend_case(gpu_pkg, P.Layout(lens[::-1], 32, rows[::-1]), 20, 5, dim, fmt, window=window, n_sinks=sinks)
