@@ -21,8 +21,8 @@
 // results through distributed shared memory.
 //
 // Measured (us): 16384 rows of 32 query and 8 kv heads of 128, bf16, 2000 = 1.1 PFLOP/s under the power cap (1.72 GHz; a library's
-// product of matrices holds 1.42 there); 4 pieces of 5 to 61 rows behind 300 to 1500 keys 14.0; 7 prompts of 301 to 4000 rows, 16 and 4
-// heads of 64, f16, window 512, 58.8; 9 of 40 to 1300 F32 rows, 8 heads of 128, 37.6. A tile of D = 128 goes through 1190 clocks of
+// product of matrices holds 1.42 there); 4 pieces of 5 to 61 rows behind 300 to 1500 keys 13.6; 7 prompts of 301 to 4000 rows, 16 and 4
+// heads of 64, f16, window 512, 57.4; 9 of 40 to 1300 F32 rows, 8 heads of 128, 36.9. A tile of D = 128 goes through 1190 clocks of
 // waiting for its scores, 245 + 220 of their maximum, 1550 of exponentials and packing, 250 of signals; the other tile's take turns with
 // it. Tensor cores and exponential units are busy half of the time each. What was tried against that: steps of 64 keys with two score
 // buffers, so that no softmax waits (2210: products 64 columns wide take as long as 128 wide ones), a part of the exponentials as
@@ -110,22 +110,22 @@ __device__ __forceinline__ uint64_t kc_desc_mn(uint32_t addr) {
 
 // Where the TMA warp finds the call's blocks: all their number, and the x-th from the last, since later positions see more keys and
 // what takes longest should begin first. With up to 32 sequences a lane keeps one, and the x-th longest is found, too: by bisection of
-// the length that more than x blocks have (with it the third and fourth case above take 58.8 and 37.6 us, with the order of the sequences
+// the length that more than x blocks have (with it the third and fourth case above took 58.8 and 37.6 us, with the order of the sequences
 // 63.4 and 46.2).
 struct KcFinder {
-    int per_block, total;
+    int per_block, total, mine;                      // rows of a block, blocks of the call, blocks of the lane's sequence
     KvSeq q;
-    __device__ __forceinline__ int blocks() const { return (q.n + per_block - 1) / per_block; }
     __device__ __forceinline__ void look(const KvArgs &a, int s, bool *bad) {
         q = {0, 0, 0};
         if (s < a.n_seq) *bad |= !kv_seq(a.row_off, a.kv_len, s, a.n_rows, kv_capacity(a), &q);
+        mine = (q.n + per_block - 1) / per_block;
     }
     __device__ __forceinline__ void init(const KvArgs &a, int per, int lane) {
         per_block = per; total = 0;
         bool bad = false;
         for (int s0 = 0; s0 < a.n_seq; s0 += 32) {
             look(a, s0 + lane, &bad);
-            total += __reduce_add_sync(0xffffffffu, blocks());
+            total += __reduce_add_sync(0xffffffffu, mine);
         }
         if (bad) atomicExch(a.status, ST_PAGE);
     }
@@ -133,7 +133,7 @@ struct KcFinder {
     __device__ __forceinline__ int as_long(const KvArgs &a, int tiles) const {
         const int need = (tiles - 1) * KC_KEYS + 1 - (q.len - q.n);            // rows that the block's last one has in front of it, and itself
         if (need > q.n || (a.window > 0 && (tiles - 1) * KC_KEYS >= a.window + a.sinks + per_block)) return 0;
-        return blocks() - (need <= per_block ? 0 : (need + per_block - 1) / per_block - 1);
+        return mine - (need <= per_block ? 0 : (need + per_block - 1) / per_block - 1);
     }
     __device__ __forceinline__ void find_longest(const KvArgs &a, int x, int lane, int *seq, int *block, KvSeq *at) {
         *seq = -1; *block = 0; *at = {0, 0, 0};
@@ -143,7 +143,7 @@ struct KcFinder {
             const int mid = (lo + hi) >> 1;
             if (__reduce_add_sync(0xffffffffu, as_long(a, mid)) > x) lo = mid; else hi = mid;
         }
-        const int longer = as_long(a, lo + 1), some = lo > 0 ? as_long(a, lo) : blocks(), n = some - longer;
+        const int longer = as_long(a, lo + 1), some = lo > 0 ? as_long(a, lo) : mine, n = some - longer;
         int nth = x - __reduce_add_sync(0xffffffffu, longer), upto = n;
 #pragma unroll
         for (int o = 1; o < 32; o *= 2) {
@@ -153,7 +153,7 @@ struct KcFinder {
         const int who = __ffs(__ballot_sync(0xffffffffu, nth < upto)) - 1;
         if (who < 0) return;
         *seq = who;
-        *block = __shfl_sync(0xffffffffu, blocks() - some - (upto - n), who) + nth;
+        *block = __shfl_sync(0xffffffffu, mine - some - (upto - n), who) + nth;
         at->begin = __shfl_sync(0xffffffffu, q.begin, who);
         at->n = __shfl_sync(0xffffffffu, q.n, who);
         at->len = __shfl_sync(0xffffffffu, q.len, who);
@@ -165,7 +165,7 @@ struct KcFinder {
         bool bad = false;
         for (int s0 = 0; s0 < a.n_seq; s0 += 32) {
             if (a.n_seq > 32) look(a, s0 + lane, &bad);
-            const int n = blocks();
+            const int n = mine;
             int upto = n;
 #pragma unroll
             for (int o = 1; o < 32; o *= 2) {
@@ -245,7 +245,7 @@ __device__ __forceinline__ void kc_quads(uint32_t *w, int lane) {
 template <int DP, int FMT>
 __global__ void __launch_bounds__(ChunkShape<DP, FMT>::THREADS, ChunkShape<DP, FMT>::PER_SM)
 kv_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const KvArgs a,
-                int box_rows, int log_size, int longest_first) {
+                int box_rows, int log_size, int longest_first, int tq, uint32_t inv_g) {
     using Sh = ChunkShape<DP, FMT>;
     constexpr bool BF = FMT == KV_BF16, F32 = FMT == KV_F32, OWN_P = Sh::OWN_P;
     constexpr int STAGES = Sh::STAGES, TILES = Sh::TILES, SPLIT = Sh::SPLIT, OWN = Sh::OWN, GROUPS = OWN / 32;
@@ -280,8 +280,6 @@ kv_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
     chain_trigger();
     chain_wait();
     const uint32_t tmem = *tmem_slot;
-    const int tq = KC_ROWS / a.G;                              // positions of a tile
-    const uint32_t inv_g = (65536u + a.G - 1) / a.G;           // x / G = x inv_g / 2^16 for x < 256, G <= 64
     auto by_g = [&](int x) { return (int)(((uint32_t)x * inv_g) >> 16); };
     const int size = 1 << log_size, rank = (int)blockIdx.x & (size - 1);
     const bool once = log_size > 0;                            // a cluster's CTAs work on one block and join their results
@@ -322,18 +320,16 @@ kv_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
     kc_regs_less<Sh::LESS>();                                  // (one instruction for the four warps)
     if (warp == Sh::W_TMA) {
         // ---- lane = one box of a tile: 64 of the D columns, the slots of one page. Item 2 i of the ring is K(i), 2 i + 1 V(i).
-        const int shift = a.page_shift, boxes = KC_KEYS / box_rows * Sh::HALVES;
+        const int shift = a.page_shift, boxes = (KC_KEYS >> (__ffs(box_rows) - 1)) * Sh::HALVES;
         const int b_half = lane % Sh::HALVES, b_sub = lane / Sh::HALVES;
         const uint32_t b_at = b_half * KC_HALF + b_sub * box_rows * 128;
+        int x = (int)(blockIdx.x >> log_size), nth = x / a.Hkv;
         KcFinder finder;
         finder.init(a, TILES * tq, lane);
         int s = 0, ph = 0, r = 0, queries = 0;                 // place in the ring, its parity, requests; blocks with queries so far
         bool ok = true;
-        for (int j = 0, x0 = 0; ok; j++, x0 += (int)gridDim.x) {
-            // (there and back: a CTA whose block was the longest of its round gets the shortest of the next)
-            const int x = x0 + (longest_first && (j & 1) ? (int)(gridDim.x - 1 - blockIdx.x) : (int)(blockIdx.x >> log_size));
+        for (int j = 0, x0 = 0; ok; j++) {
             if (j >= 2 && !mbar_wait_warp(&i_empty[j & 1], (uint32_t)(((j >> 1) & 1) ^ 1))) { ok = false; break; }
-            const int nth = x / a.Hkv;
             int seq, block;
             KvSeq sq;
             if (longest_first) finder.find_longest(a, nth, lane, &seq, &block, &sq);
@@ -383,6 +379,10 @@ kv_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                 entry = next;
             }
             if (once) break;
+            // (there and back: a CTA whose block was the longest of its round gets the shortest of the next)
+            x0 += (int)gridDim.x;
+            x = x0 + (longest_first && !(j & 1) ? (int)(gridDim.x - 1 - blockIdx.x) : (int)blockIdx.x);
+            nth = x / a.Hkv;
         }
         if (!ok && lane == 0) atomicExch(a.status, ST_TIMEOUT_PRODUCER);
         for (int u = 0; u < STAGES && u < r; u++) {            // what was asked for has to land before the CTA leaves
@@ -867,7 +867,8 @@ static int chunk_launch(const CUtensorMap &k, const CUtensorMap &v, const KvArgs
         MB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
         configured.record(dev, (size_t)Sh::SMEM);
     }
-    const int per_block = Sh::TILES * (KC_ROWS / a.G);
+    const int tq = KC_ROWS / a.G, per_block = Sh::TILES * tq;                  // positions of a tile of rows, of a block
+    const uint32_t inv_g = (65536u + a.G - 1) / a.G;           // x / G = x inv_g / 2^16 for x < 256, G <= 64
     const int64_t full = ((int64_t)a.n_rows + per_block - 1) / per_block, seqs = a.n_seq < a.n_rows ? a.n_seq : a.n_rows;
     const int64_t blocks = (a.n_rows / per_block + seqs) * a.Hkv;              // the last block of each sequence may be short
     // Clusters where the blocks that are likely (whole ones, or one per sequence) leave SMs without work: the largest of which as many
@@ -890,7 +891,8 @@ static int chunk_launch(const CUtensorMap &k, const CUtensorMap &v, const KvArgs
     const bool longest_first = blocks > room && a.n_seq > 1 && a.n_seq <= 32;
     CUtensorMap q = k;
     if (FMT != KV_F32 && !kv_rows_map(&q, a, FMT == KV_BF16)) { set_error("kv_attend: no tensor map of the rows"); return -1; }
-    MB_CUDA(launch_kernel(kernel, dim3((unsigned)ctas), dim3(Sh::THREADS), (size_t)Sh::SMEM, st, true, 1 << log_size, q, k, v, a, box_rows, log_size, longest_first ? 1 : 0));
+    MB_CUDA(launch_kernel(kernel, dim3((unsigned)ctas), dim3(Sh::THREADS), (size_t)Sh::SMEM, st, true, 1 << log_size, q, k, v, a, box_rows, log_size, longest_first ? 1 : 0,
+                          tq, inv_g));
     note_launch();
     return 0;
 }
