@@ -12,7 +12,8 @@
 // pace hides. The partial results are joined in shared memory, then in the cluster's distributed shared memory, in a fixed order,
 // each CTA for its slice of the values: no workspace, no second launch, no atomics.
 // Measured (32 query and 8 kv heads of 128, bf16): 131071 keys 99 us = 5.4 TB/s (128 CTAs of 148 SMs: a cluster has at most 16), 60
-// ragged sequences of 40 to 9000 keys 76 us = 5.9 TB/s, 700 keys (16 query heads) 7.4 us. A warp that asks for its own tiles took
+// ragged sequences of 40 to 9000 keys 76 us = 5.9 TB/s, 700 keys (16 query heads) 7.4 us; 200 sequences of F32 rows, 8 heads of 64, window 1000, 64 us = 5.6 TB/s
+// (61 without any arithmetic, as are 98 of the 99: what is left is the pace of the copies). A warp that asks for its own tiles took
 // 128 us for the first (each TMA instruction of a diverged lane waits for its operands, in front of the products), query heads as the
 // 16 rows of the products 192 us.
 #include "kv.h"
@@ -108,8 +109,11 @@ __device__ __forceinline__ bool ks_place(const KvArgs &a, const StepPlan &p, int
     return true;
 }
 
+// CTAs that the registers leave room for on an SM
+template <int DP, int FMT, int NT> struct StepRoom { static constexpr int CTAS = NT == 1 && (FMT != KV_F32 || DP == 64) ? 3 : 2; };
+
 template <int DP, int FMT, int NT>
-__global__ void __launch_bounds__(KS_THREADS, NT == 1 && FMT != KV_F32 ? 3 : 2)
+__global__ void __launch_bounds__(KS_THREADS, StepRoom<DP, FMT, NT>::CTAS)
 kv_step_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const KvArgs a, int log_size, int log_even,
                int stages, int head_tiles) {
     using Sh = StepShape<DP>;
@@ -461,8 +465,10 @@ static int step_launch(const CUtensorMap &k, const CUtensorMap &v, const KvArgs 
     while (log_even < 4 && units << (log_even + 1) <= 2 * sms && 1 << log_even < most_tiles) log_even++;
     log_size = log_even;
     while (log_size < 4 && log_size < log_even + 2 && KS_CHUNK << log_size < most_tiles) log_size++;
-    // Tiles ahead: two, so that three CTAs fit an SM; three where no SM has more than one CTA, or registers leave room for two
-    const int stages = FMT == KV_F32 || NT == 2 || units << log_size <= sms ? 3 : 2;
+    // Tiles ahead: two, so that three CTAs fit an SM, where there are more than two for each; three otherwise. us, with two and with three tiles
+    // ahead: 20 sequences of 2000 keys (16 and 8 heads of 64, f16) 18.6, 16.3, 18 of 500 (32 and 8 of 128, bf16) 11.9, 10.9; 60 of 100 to
+    // 4230 (8 heads of 64, F32 rows) 51, 60, 200 under a window of 1000 64, 68
+    const int stages = StepRoom<DP, FMT, NT>::CTAS == 2 || units << log_size <= 2 * sms ? 3 : 2;
     if (units << log_size > 0x7fffffff) { set_error("kv_attend: too many sequences in one call"); return -1; }
     const size_t smem = (size_t)stages * Sh::STAGE + KS_HEAD + 1024;
     MB_CUDA(launch_kernel(kernel, dim3((unsigned)(units << log_size)), dim3(KS_THREADS), smem, st, true, 1 << log_size, k, v, a, log_size, log_even, stages, head_tiles));
