@@ -881,14 +881,14 @@ static int chunk_launch(const CUtensorMap &k, const CUtensorMap &v, const KvArgs
         if (likely <= (int64_t)Sh::PER_SM * most) log_size = k;
     }
     if (blocks << log_size > 0x3fffffff) { set_error("kv_attend: too many rows in one call"); return -1; }
-    // Where blocks are short, as many CTAs as fit take one after the other; where they are long, the hardware deals them out better than a
-    // fixed order (32 and 8 heads of 128, us, that way and with a CTA per block: 8 x 500 rows 49, 52, 4 x 2000 162, 175; 8000 490, 454)
+    // As many CTAs as fit take one block after the other, the longest first (us, that way and with a CTA per block, heads of 128: 4 x 2000 rows
+    // 141, 172, 2 x 4000 237, 270, 8000 440, 460, 9 of 300 to 8000 550, 640). With more sequences than lanes, where the lengths are not
+    // put in order, only blocks that are short: the hardware deals out long ones better (40 of 100 to 8000 F32 rows 1723, 1645)
     const int64_t keys = (int64_t)a.max_pages << a.page_shift, seen = (int64_t)a.window + a.sinks + per_block;
-    const bool stay = (a.window > 0 && seen < keys ? seen : keys) <= KC_STAY;
+    const bool stay = a.n_seq <= 32 || (a.window > 0 && seen < keys ? seen : keys) <= KC_STAY;
     const int64_t room = (int64_t)Sh::PER_SM * device_sm_count();
     const int64_t ctas = log_size ? blocks << log_size : stay && blocks > room ? room : blocks;
-    // Which order: the sequences' blocks from the last on, or, where there is more than one round of them, the longest first
-    const bool longest_first = blocks > room && a.n_seq > 1 && a.n_seq <= 32;
+    const bool longest_first = blocks > room && a.n_seq <= 32;
     CUtensorMap q = k;
     if (FMT != KV_F32 && !kv_rows_map(&q, a, FMT == KV_BF16)) { set_error("kv_attend: no tensor map of the rows"); return -1; }
     MB_CUDA(launch_kernel(kernel, dim3((unsigned)ctas), dim3(Sh::THREADS), (size_t)Sh::SMEM, st, true, 1 << log_size, q, k, v, a, box_rows, log_size, longest_first ? 1 : 0,
