@@ -428,7 +428,7 @@ class KvBatch:
 
 class KvCache:
     """Paged key/value cache of one decoder layer on the current device (mynah_b200_kv). Tensors are anything with torch's
-    data_ptr, shape, stride, dtype and device; row tensors are [rows, heads * head_dim], a row's values side by side."""
+    data_ptr, shape, stride, dtype, device and is_cuda; row tensors are [rows, heads * head_dim], a row's values side by side."""
 
     def __init__(self, n_heads, n_kv_heads, head_dim, page_size, n_pages, fmt=F32, rotary_dim=0, interleaved=False, rope_theta=10000.0,
                  inv_freq=None, q_norm=None, k_norm=None, norm_eps=1e-6, window=0, n_sinks=0, scale=0.0):
@@ -472,26 +472,32 @@ class KvCache:
         return KvBatch(kv_len, page_table, row_off, n_rows)
 
     def _rows(self, t, width, batch, what):
-        """Address and row stride of a row tensor, as the library takes them."""
-        if isinstance(self._dtype, str) and str(t.dtype) == self._dtype:
+        """Address and row stride of a row tensor, as the library takes them (which looks whose memory it is)."""
+        shape = t.shape
+        if t.dtype is self._dtype and t.is_cuda and len(shape) == 2 and shape[1] == width and shape[0] >= batch.n_rows:
+            ld, one = t.stride()
+            if one == 1 or width == 1:
+                return t.data_ptr(), ld if shape[0] > 1 else width
+        elif isinstance(self._dtype, str) and str(t.dtype) == self._dtype:
             self._dtype = t.dtype                        # from now on without the text
-        shape, stride = t.shape, t.stride()
-        if t.dtype != self._dtype or len(shape) != 2 or shape[1] != width or shape[0] < batch.n_rows or (stride[1] != 1 and width > 1) or t.device != batch.device:
-            raise ValueError(f"{what} is a {self._dtype} tensor [at least {batch.n_rows} rows, {width}] on the batch's device, each row's values side by side")
-        return t.data_ptr(), stride[0] if shape[0] > 1 else width
+            return self._rows(t, width, batch, what)
+        raise ValueError(f"{what} is a {self._dtype} tensor [at least {batch.n_rows} rows, {width}] on the batch's device, each row's values side by side")
 
     def append(self, batch, q, k, v, q_out, stream=None):
         """Norm and rotation of the rows; q to q_out, k and v to their slots. stream: an integer handle as torch gives it (0: the
         legacy default stream), or None for the handle's own. Asynchronous."""
-        a, b, c = self._rows(q, self._q_width, batch, "q"), self._rows(k, self._kv_width, batch, "k"), self._rows(v, self._kv_width, batch, "v")
-        o = self._rows(q_out, self._q_width, batch, "q_out")
-        if self._append(self.h, batch.at, *a, *b, *c, *o, 1 if stream == 0 else stream) != 0:
+        a, lda = self._rows(q, self._q_width, batch, "q")
+        b, ldb = self._rows(k, self._kv_width, batch, "k")
+        c, ldc = self._rows(v, self._kv_width, batch, "v")
+        o, ldo = self._rows(q_out, self._q_width, batch, "q_out")
+        if self._append(self.h, batch.at, a, lda, b, ldb, c, ldc, o, ldo, 1 if stream == 0 else stream):
             raise BackendError("kv_append: " + _err())
 
     def attend(self, batch, q, out, stream=None):
         """Attention of the batch's rows over the visible keys of their sequences, into out. Asynchronous, as append."""
-        a, o = self._rows(q, self._q_width, batch, "q"), self._rows(out, self._q_width, batch, "out")
-        if self._attend(self.h, batch.at, *a, *o, 1 if stream == 0 else stream) != 0:
+        a, lda = self._rows(q, self._q_width, batch, "q")
+        o, ldo = self._rows(out, self._q_width, batch, "out")
+        if self._attend(self.h, batch.at, a, lda, o, ldo, 1 if stream == 0 else stream):
             raise BackendError("kv_attend: " + _err())
 
     def sync(self, stream=None):
