@@ -12,7 +12,7 @@
 // pace hides. The partial results are joined in shared memory, then in the cluster's distributed shared memory, in a fixed order,
 // each CTA for its slice of the values: no workspace, no second launch, no atomics.
 // Measured (32 query and 8 kv heads of 128, bf16): 131071 keys 99 us = 5.4 TB/s (128 CTAs of 148 SMs: a cluster has at most 16), 60
-// ragged sequences of 40 to 9000 keys 76 us = 5.9 TB/s, 700 keys (16 query heads) 7.4 us; 200 sequences of F32 rows, 8 heads of 64, window 1000, 64 us = 5.6 TB/s
+// ragged sequences of 40 to 9000 keys 76 us = 5.9 TB/s, 700 keys (16 query heads) 6.2 us; 200 sequences of F32 rows, 8 heads of 64, window 1000, 64 us = 5.6 TB/s
 // (61 without any arithmetic, as are 98 of the 99: what is left is the pace of the copies). A warp that asks for its own tiles took
 // 128 us for the first (each TMA instruction of a diverged lane waits for its operands, in front of the products), query heads as the
 // 16 rows of the products 192 us.
@@ -70,16 +70,18 @@ __device__ __forceinline__ int ks_class(const KvArgs &a, const StepPlan &p, int 
     return max(min(ks_log(t), p.log_even), min(ks_log((t + KS_CHUNK - 1) / KS_CHUNK), p.log_size));
 }
 // What CTA `rank` of cluster v works on: a sequence (-1: nothing), its place among the sequence's units, and k. False for a cluster
-// behind the last one.
+// behind the last one. (All numbers of units are below 2^31.)
 __device__ __forceinline__ bool ks_place(const KvArgs &a, const StepPlan &p, int v, int rank, int tile, int lane, int *seq, int *unit, int *log_parts) {
     if (p.log_size == 0) {                           // a CTA is a unit
-        *seq = v / p.per_seq; *unit = v % p.per_seq; *log_parts = 0;
+        *seq = v / p.per_seq; *unit = v - *seq * p.per_seq; *log_parts = 0;
         return true;
     }
     int count[5] = {0, 0, 0, 0, 0};                  // sequences of each k
+    int first = -1;                                  // k of the lane's one of the first 32
 #pragma unroll 4
     for (int s0 = 0; s0 < a.n_seq; s0 += 32) {
         const int c = s0 + lane < a.n_seq ? ks_class(a, p, s0 + lane, tile) : -1;
+        if (s0 == 0) first = c;
 #pragma unroll
         for (int k = 0; k < 5; k++) count[k] += __popc(__ballot_sync(0xffffffffu, c == k));
     }
@@ -88,17 +90,17 @@ __device__ __forceinline__ bool ks_place(const KvArgs &a, const StepPlan &p, int
     for (int c = 4; c >= 0; c--)
         if (k < 0 && c <= p.log_size) {
             const int share = p.log_size - c;        // a cluster holds 2^share units
-            const int n = (int)(((int64_t)count[c] * p.per_seq + (1 << share) - 1) >> share);
+            const int n = (int)(((unsigned)count[c] * p.per_seq + (1u << share) - 1) >> share);
             if (v < n) { k = c; have = count[c]; } else v -= n;
         }
     if (k < 0) return false;
-    const int64_t u = ((int64_t)v << (p.log_size - k)) + (rank >> k);
-    int nth = (int)(u / p.per_seq);
+    const unsigned u = ((unsigned)v << (p.log_size - k)) + (unsigned)(rank >> k);
+    int nth = (int)(u / (unsigned)p.per_seq);
     *log_parts = k;
-    *unit = (int)(u % p.per_seq);
+    *unit = (int)(u - (unsigned)nth * p.per_seq);
     *seq = -1;
     for (int s0 = 0; nth < have && s0 < a.n_seq; s0 += 32) {
-        const unsigned in = __ballot_sync(0xffffffffu, s0 + lane < a.n_seq && ks_class(a, p, s0 + lane, tile) == k);
+        const unsigned in = __ballot_sync(0xffffffffu, s0 == 0 ? first == k : s0 + lane < a.n_seq && ks_class(a, p, s0 + lane, tile) == k);
         const int c = __popc(in);
         if (nth < c) {
             *seq = s0 + __ffs(__ballot_sync(0xffffffffu, (in >> lane & 1) && __popc(in & ((1u << lane) - 1)) == nth)) - 1;
@@ -417,24 +419,32 @@ kv_step_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
         const int base = rank - part_no;
         for (int q = part_no * KS_THREADS + (int)threadIdx.x; q < rows * quads; q += parts_n * KS_THREADS) {
             const int r = q / quads, c = (q % quads) * 4;
-            float2 e[16];
+            // (eight parts' reads are under way at a time: one after the other, sixteen took 3800 of a short call's 12900 clocks)
             float top = KS_NONE, total = 0.f;
-#pragma unroll
-            for (int p = 0; p < 16; p++) {
-                e[p] = make_float2(KS_NONE, 0.f);
-                if (p < parts_n) e[p] = kv_peer2(kv_peer(at0 + (HEADS * Sh::LDO + 2 * r) * 4, base + p));
-            }
-#pragma unroll
-            for (int p = 0; p < 16; p++) top = fmaxf(top, e[p].x);
             float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+            for (int p0 = 0; p0 < parts_n; p0 += 8) {
+                float2 e[8];
+                float4 v[8];
 #pragma unroll
-            for (int p = 0; p < 16; p++)
-                if (p < parts_n) {
-                    const float4 v4 = kv_peer4(kv_peer(at0 + (r * Sh::LDO + c) * 4, base + p));
-                    const float f = kv_ex2(e[p].x - top);
-                    total = fmaf(f, e[p].y, total);
-                    sum.x = fmaf(f, v4.x, sum.x); sum.y = fmaf(f, v4.y, sum.y); sum.z = fmaf(f, v4.z, sum.z); sum.w = fmaf(f, v4.w, sum.w);
+                for (int p = 0; p < 8; p++) {
+                    const int from = base + min(p0 + p, parts_n - 1);
+                    e[p] = kv_peer2(kv_peer(at0 + (HEADS * Sh::LDO + 2 * r) * 4, from));
+                    v[p] = kv_peer4(kv_peer(at0 + (r * Sh::LDO + c) * 4, from));
                 }
+                float m = top;
+#pragma unroll
+                for (int p = 0; p < 8; p++) m = fmaxf(m, e[p].x);
+                const float old = kv_ex2(top - m);
+                total *= old; sum.x *= old; sum.y *= old; sum.z *= old; sum.w *= old;
+                top = m;
+#pragma unroll
+                for (int p = 0; p < 8; p++) {
+                    const float f = p0 + p < parts_n ? kv_ex2(e[p].x - m) : 0.f;
+                    total = fmaf(f, e[p].y, total);
+                    sum.x = fmaf(f, v[p].x, sum.x); sum.y = fmaf(f, v[p].y, sum.y); sum.z = fmaf(f, v[p].z, sum.z); sum.w = fmaf(f, v[p].w, sum.w);
+                }
+            }
             store(r, c, sum, total);
         }
         kv_cluster_sync();                                     // nobody leaves while its part is being read
