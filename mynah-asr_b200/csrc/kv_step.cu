@@ -111,6 +111,8 @@ __device__ __forceinline__ bool ks_place(const KvArgs &a, const StepPlan &p, int
     return true;
 }
 
+template <int N_> struct KsBatch { static constexpr int N = N_; };
+
 // CTAs that the registers leave room for on an SM
 template <int DP, int FMT, int NT> struct StepRoom { static constexpr int CTAS = NT == 1 && (FMT != KV_F32 || DP == 64) ? 3 : 2; };
 
@@ -417,36 +419,39 @@ kv_step_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
         kv_cluster_sync();
         const uint32_t at0 = smem_u32(mine);
         const int base = rank - part_no;
-        for (int q = part_no * KS_THREADS + (int)threadIdx.x; q < rows * quads; q += parts_n * KS_THREADS) {
-            const int r = q / quads, c = (q % quads) * 4;
-            // (eight parts' reads are under way at a time: one after the other, sixteen took 3800 of a short call's 12900 clocks)
-            float top = KS_NONE, total = 0.f;
-            float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+        // (up to eight parts' reads are under way at a time: one after the other, sixteen took 3800 of a short call's 12900 clocks)
+        auto join = [&](auto at_a_time) {                      // a divisor of parts_n
+            constexpr int N = decltype(at_a_time)::N;
+            for (int q = part_no * KS_THREADS + (int)threadIdx.x; q < rows * quads; q += parts_n * KS_THREADS) {
+                const int r = q / quads, c = (q % quads) * 4;
+                float top = KS_NONE, total = 0.f;
+                float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 1
-            for (int p0 = 0; p0 < parts_n; p0 += 8) {
-                float2 e[8];
-                float4 v[8];
+                for (int p0 = 0; p0 < parts_n; p0 += N) {
+                    float2 e[N];
+                    float4 v[N];
 #pragma unroll
-                for (int p = 0; p < 8; p++) {
-                    const int from = base + min(p0 + p, parts_n - 1);
-                    e[p] = kv_peer2(kv_peer(at0 + (HEADS * Sh::LDO + 2 * r) * 4, from));
-                    v[p] = kv_peer4(kv_peer(at0 + (r * Sh::LDO + c) * 4, from));
+                    for (int p = 0; p < N; p++) {
+                        e[p] = kv_peer2(kv_peer(at0 + (HEADS * Sh::LDO + 2 * r) * 4, base + p0 + p));
+                        v[p] = kv_peer4(kv_peer(at0 + (r * Sh::LDO + c) * 4, base + p0 + p));
+                    }
+                    float m = top;
+#pragma unroll
+                    for (int p = 0; p < N; p++) m = fmaxf(m, e[p].x);
+                    const float old = kv_ex2(top - m);
+                    total *= old; sum.x *= old; sum.y *= old; sum.z *= old; sum.w *= old;
+                    top = m;
+#pragma unroll
+                    for (int p = 0; p < N; p++) {
+                        const float f = kv_ex2(e[p].x - m);
+                        total = fmaf(f, e[p].y, total);
+                        sum.x = fmaf(f, v[p].x, sum.x); sum.y = fmaf(f, v[p].y, sum.y); sum.z = fmaf(f, v[p].z, sum.z); sum.w = fmaf(f, v[p].w, sum.w);
+                    }
                 }
-                float m = top;
-#pragma unroll
-                for (int p = 0; p < 8; p++) m = fmaxf(m, e[p].x);
-                const float old = kv_ex2(top - m);
-                total *= old; sum.x *= old; sum.y *= old; sum.z *= old; sum.w *= old;
-                top = m;
-#pragma unroll
-                for (int p = 0; p < 8; p++) {
-                    const float f = p0 + p < parts_n ? kv_ex2(e[p].x - m) : 0.f;
-                    total = fmaf(f, e[p].y, total);
-                    sum.x = fmaf(f, v[p].x, sum.x); sum.y = fmaf(f, v[p].y, sum.y); sum.z = fmaf(f, v[p].z, sum.z); sum.w = fmaf(f, v[p].w, sum.w);
-                }
+                store(r, c, sum, total);
             }
-            store(r, c, sum, total);
-        }
+        };
+        if (parts_n == 2) join(KsBatch<2>()); else if (parts_n == 4) join(KsBatch<4>()); else join(KsBatch<8>());
         kv_cluster_sync();                                     // nobody leaves while its part is being read
     }
 }
