@@ -100,13 +100,6 @@ __device__ __forceinline__ float2 kv_add2(float2 a, float2 b) {
 
 // ---- tables
 __device__ __forceinline__ int64_t kv_capacity(const KvArgs &a) { return (int64_t)a.max_pages << a.page_shift; }
-// Page of a position whose page index is in range; an entry that names no page is reported and read as page 0
-__device__ __forceinline__ int kv_page(const KvArgs &a, int seq, int page_index) {
-    const int p = a.table[(size_t)seq * a.max_pages + page_index];
-    if ((unsigned)p < (unsigned)a.n_pages) return p;
-    atomicExch(a.status, ST_PAGE);
-    return 0;
-}
 // Index of a cache row (one head at one slot)
 __device__ __forceinline__ size_t kv_row(const KvArgs &a, int page, int head, int slot) {
     return ((((size_t)page * a.Hkv + head) << a.page_shift) + slot);

@@ -608,10 +608,9 @@ kv_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                     for (int e = 0; e < 4; e++) m4[e] = fmaxf(m4[e], fmaxf(x[c + e], x[c + 4 + e]));
                 const int g0 = b.tile_at(i), j0 = b.keys.at(g0), d = pos - j0;
                 const bool whole = d >= KC_KEYS - 1 && (a.window <= 0 || (d < a.window && (g0 >= b.keys.first || g0 + 4 <= b.keys.first)) || j0 + KC_KEYS - 1 < a.sinks);
-                const bool all = __all_sync(0xffffffffu, whole);
-                if (!all) {                                        // (columns that have no scores are hidden, too)
-                    // 32 columns at a time, where some row of the warp does not see them all: a bit per column, visible up to d, above
-                    // `under`, or below `keep`
+                if (!__all_sync(0xffffffffu, whole)) {             // (columns that have no scores are hidden, too)
+                    // 32 columns at a time, where some row of the warp does not see them all: a bit per column, visible up to the row's
+                    // position, and with a window behind its lower end or among the first tokens
                     auto upto = [](int c) -> uint32_t { return c < 0 ? 0u : c >= 31 ? 0xffffffffu : (2u << c) - 1u; };      // bits 0 to c
                     m4[0] = m4[1] = m4[2] = m4[3] = -INFINITY;
 #pragma unroll
