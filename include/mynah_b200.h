@@ -321,7 +321,8 @@ int mynah_b200_stream_step_device(mynah_b200_stream_group *g, const float *mel_d
  *
  * Types: fmt is that of the rows (queries, keys, values, results): F32, F16 or BF16. The cache holds 16 bits a value:
  * bf16 for BF16 rows, else f16. Queries, probabilities and results of F16 / BF16 rows pass through 16 bits, too; for
- * F32 rows they keep f32 accuracy (relative to the stored keys and values).
+ * F32 rows they keep f32 accuracy (relative to the stored keys and values). A probability is held to 2^-22 of itself (F16 rows 2^-11)
+ * or to 2^-39 (F16 rows 2^-32) of the row's largest, whichever is more.
  * Layout: the pools are [n_pages][n_kv_heads][page_size][head_dim]; head h of a row is its values
  * [h head_dim, (h + 1) head_dim); query head h looks at kv head h / (n_heads / n_kv_heads). */
 typedef struct {

@@ -15,8 +15,8 @@
 //                  finds O at rest. With columns of their own for P: S(i + 1) in front of P V(i).
 // A CTA stays and takes block after block (heads of a block side by side, long blocks first, KcFinder): the next block's place, queries
 // and first keys are looked up, fetched and multiplied while the results of the one before are written.
-// The softmax keeps a running maximum per row; O is rescaled only when it has grown by more than 2^8 (what is stale cancels in the
-// final division). F32 rows: queries and probabilities as (hi, lo) f16 pairs, two products each.
+// The softmax keeps a running maximum per row; O is rescaled only when it has grown by more than ChunkTop says (what is stale cancels
+// in the final division). F32 rows: queries and probabilities as (hi, lo) f16 pairs, two products each.
 // A call with few blocks is launched as clusters: the CTAs of a cluster take a block's tiles in turn, two at least each, and join their
 // results through distributed shared memory.
 //
@@ -35,6 +35,14 @@ static constexpr int KC_ROWS = 128, KC_KEYS = 128, KC_HALF = 128 * 128;      // 
 static constexpr int KC_HEAD = 1024, KC_STAY = 3000;
 static constexpr int KC_PART = 3;                    // P V begins when the first 3 x 32 keys' probabilities are there
 static constexpr float KC_NONE = -1e30f;             // "maximum" of no keys
+
+// The maximum of a row may lag by 2^LAG, and a probability is 2^TOP of it, which the final division takes out again: together below f16's 2^16,
+// and what is held of a probability (with F32 rows: of its rest) is 2^-25 / 2^TOP of the largest, where it was 2^-25 without. bf16 has the
+// range. A smaller LAG rescales O more often: f16, 8192 rows of 32 heads of 128, scores spread by 2.5 units: 481 us, with a LAG of 4 518,
+// of 2 540. F32 rows of 128 rescale for every tile in any case; 8 heads of 64 take 41.8 us, with a LAG of 8 40.3.
+template <int FMT> struct ChunkTop {
+    static constexpr float LAG = FMT == KV_F32 ? 1.f : 8.f, TOP = FMT == KV_F32 ? 14.f : FMT == KV_F16 ? 7.f : 0.f;
+};
 
 template <int DP, int FMT> struct ChunkShape {
     static constexpr int HALVES = DP / 64, PLANES = FMT == KV_F32 ? 2 : 1;
@@ -634,12 +642,12 @@ kv_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                     if (!exchange(mt, &other)) { ok = false; break; }
                     mt = fmaxf(mt, other);
                 }
-                mt *= sc;
+                mt = fmaf(mt, sc, -ChunkTop<FMT>::TOP);
                 if (OWN_P && i > 0) {                              // P(i - 1) has been read, and O is at rest
                     if (!mbar_wait_warp(&o_full[t], (uint32_t)((done + i - 1) & 1))) { ok = false; break; }
                     tc_fence_after();
                 }
-                const bool grow = mt > m + 8.f;
+                const bool grow = mt > m + ChunkTop<FMT>::LAG;
                 const bool any = __any_sync(0xffffffffu, grow);
                 if (any || (Sh::FRESH && OWN_P)) {
                     const float alpha = grow ? kv_ex2(m - mt) : 1.f;
