@@ -34,7 +34,6 @@ namespace mb {
 static constexpr int KC_ROWS = 128, KC_KEYS = 128, KC_HALF = 128 * 128;      // a 128-row x 64-column box of 16-bit values: 16 KB
 static constexpr int KC_HEAD = 1024, KC_STAY = 3000;
 static constexpr int KC_PART = 3;                    // P V begins when the first 3 x 32 keys' probabilities are there
-static constexpr float KC_NONE = -1e30f;             // "maximum" of no keys
 
 // The maximum of a row may lag by 2^LAG, and a probability is 2^TOP of it, which the final division takes out again: together below f16's 2^16,
 // and what is held of a probability (with F32 rows: of its rest) is 2^-25 / 2^TOP of the largest, where it was 2^-25 without. bf16 has the
@@ -308,7 +307,7 @@ kv_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
     const bool soft = warp < Sh::SOFT;
     const uint32_t trow = tmem + ((uint32_t)((warp & 3) * 32) << 16), s_at = trow + Sh::COL_S + t * 128, p_at = trow + Sh::COL_P + t * Sh::STEP_P,
                    o_at = trow + Sh::COL_O + t * DP, f_at = trow + Sh::COL_F + t * DP;
-    float m = KC_NONE, l = 0.f;                                // of the row: running maximum and sum
+    float m = -INFINITY, l = 0.f;                              // of the row: running maximum and sum
     constexpr int COLS = F32 ? 16 : 32;                        // columns in 16 words
     auto result = [&](int n, int c, float *o) {                // COLS columns of the row's result over n tiles
         if constexpr (F32) {
@@ -569,7 +568,7 @@ kv_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
             __syncwarp();
             if (lane == 0) mbar_arrive(q_full);
         }
-        m = KC_NONE; l = 0.f;
+        m = -INFINITY; l = 0.f;
         if (t < b.nt) {
             // rows that do not exist take the last one's position, so that they need no mask of their own
             const int pos = b.base_pos + min(r < tq * a.G ? tok : b.t0 + t * tq, b.rows - 1);
@@ -642,15 +641,14 @@ kv_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                     if (!exchange(mt, &other)) { ok = false; break; }
                     mt = fmaxf(mt, other);
                 }
-                mt = fmaf(mt, sc, -ChunkTop<FMT>::TOP);
                 if (OWN_P && i > 0) {                              // P(i - 1) has been read, and O is at rest
                     if (!mbar_wait_warp(&o_full[t], (uint32_t)((done + i - 1) & 1))) { ok = false; break; }
                     tc_fence_after();
                 }
-                const bool grow = mt > m + ChunkTop<FMT>::LAG;
+                const bool grow = (mt - m) * sc > ChunkTop<FMT>::LAG;      // (not where both are -infinity)
                 const bool any = __any_sync(0xffffffffu, grow);
                 if (any || (Sh::FRESH && OWN_P)) {
-                    const float alpha = grow ? kv_ex2(m - mt) : 1.f;
+                    const float alpha = grow ? kv_ex2((m - mt) * sc) : 1.f;
                     if (grow) m = mt;
                     l *= alpha;
                     if (Sh::FRESH && OWN_P && i > 0) {
@@ -668,13 +666,15 @@ kv_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                         }
                     }
                 }
-                const float2 sc2 = make_float2(sc, sc), neg = make_float2(-m, -m);
+                const float2 sc2 = make_float2(sc, sc), top2 = make_float2(ChunkTop<FMT>::TOP, ChunkTop<FMT>::TOP);
+                const float off = m == -INFINITY ? 0.f : -m;       // (no key yet: all are hidden)
+                const float2 off2 = make_float2(off, off);
                 float2 l2[2] = {{0.f, 0.f}, {0.f, 0.f}};           // the tile's sum: small terms are not lost one by one in a large l
                 auto open = [&](int c) {                           // the exponentials of 16 keys, in place
 #pragma unroll
                     for (int e = 0; e < 8; e++) {
                         float *v = x + c * 16 + 2 * e;
-                        const float2 y = kv_fma2(make_float2(v[0], v[1]), sc2, neg);
+                        const float2 y = kv_fma2(kv_add2(make_float2(v[0], v[1]), off2), sc2, top2);
                         v[0] = kv_ex2(y.x); v[1] = kv_ex2(y.y);
                     }
                 };
@@ -792,17 +792,17 @@ kv_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
             for (int v = threadIdx.x; v < mine; v += Sh::THREADS) {
                 const int at = place_of(v0 + v);
                 float2 e[16];
-                float top_m = KC_NONE, total = 0.f;
+                float top_m = -INFINITY, total = 0.f;
 #pragma unroll
                 for (int p = 0; p < 16; p++) {
-                    e[p] = make_float2(KC_NONE, 0.f);
+                    e[p] = make_float2(-INFINITY, 0.f);
                     if (p < b.shares) e[p] = kv_peer2(kv_peer(ml0 + at * 8, p));
                 }
 #pragma unroll
                 for (int p = 0; p < 16; p++) top_m = fmaxf(top_m, e[p].x);
 #pragma unroll
                 for (int p = 0; p < 16; p++) {
-                    e[p].x = kv_ex2(e[p].x - top_m);
+                    e[p].x = kv_weight(e[p].x, top_m, a.scale2);
                     total = fmaf(e[p].x, e[p].y, total);
                 }
                 const float inv = total != 0.f ? 1.f / total : 0.f;

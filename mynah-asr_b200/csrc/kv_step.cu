@@ -20,8 +20,7 @@
 
 namespace mb {
 
-static constexpr float KS_NONE = -1e30f;             // "maximum" of no keys: finite, so that differences of maxima are
-// Probabilities are 2^KS_TOP of the warp's largest, which the final division takes out again: f16 ends at 2^-24, so that what is held of them, and
+// Probabilities are 2^V of the warp's largest, which the final division takes out again: f16 ends at 2^-24, so that what is held of them, and
 // with F32 rows of their rest, is 2^-40 of the largest and not 2^-25 (100 000 keys 17 units below the first one were lost, all but 0.2 %). bf16 has
 // the range.
 template <int FMT> struct StepTop { static constexpr float V = FMT == KV_BF16 ? 0.f : 15.f; };
@@ -224,7 +223,7 @@ kv_step_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
         for (int nt = 0; nt < NT; nt++) {
 #pragma unroll
             for (int i = 0; i < DP / 16; i++) o[nt][i][0] = o[nt][i][1] = o[nt][i][2] = o[nt][i][3] = 0.f;
-            m[nt][0] = m[nt][1] = KS_NONE;
+            m[nt][0] = m[nt][1] = -INFINITY;
             l[nt][0] = l[nt][1] = 0.f;
         }
         const float sc = a.scale2;
@@ -296,20 +295,21 @@ kv_step_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
                         t[0] = fmaxf(t[0], __shfl_xor_sync(0xffffffffu, t[0], w));
                         t[1] = fmaxf(t[1], __shfl_xor_sync(0xffffffffu, t[1], w));
                     }
-                    const float n0 = fmaxf(m[nt][0], fmaf(t[0], sc, -StepTop<FMT>::V)), n1 = fmaxf(m[nt][1], fmaf(t[1], sc, -StepTop<FMT>::V));
+                    const float n0 = fmaxf(m[nt][0], t[0]), n1 = fmaxf(m[nt][1], t[1]);
                     if (__any_sync(0xffffffffu, n0 > m[nt][0] || n1 > m[nt][1])) {
-                        const float a0 = kv_ex2(m[nt][0] - n0), a1 = kv_ex2(m[nt][1] - n1);
+                        const float a0 = kv_weight(m[nt][0], n0, sc), a1 = kv_weight(m[nt][1], n1, sc);
                         l[nt][0] *= a0; l[nt][1] *= a1;
 #pragma unroll
                         for (int d = 0; d < DP / 16; d++) { o[nt][d][0] *= a0; o[nt][d][1] *= a1; o[nt][d][2] *= a0; o[nt][d][3] *= a1; }
                         m[nt][0] = n0; m[nt][1] = n1;
                     }
+                    const float off[2] = {m[nt][0] == -INFINITY ? 0.f : m[nt][0], m[nt][1] == -INFINITY ? 0.f : m[nt][1]};
                     // ---- probabilities, turned from [key][head] to the B operand's layout
 #pragma unroll
                     for (int mt = 0; mt < MT; mt++) {
                         float p[4];
 #pragma unroll
-                        for (int e = 0; e < 4; e++) p[e] = kv_ex2(fmaf(x[nt][mt][e], sc, -m[nt][e & 1]));
+                        for (int e = 0; e < 4; e++) p[e] = kv_ex2(fmaf(x[nt][mt][e] - off[e & 1], sc, StepTop<FMT>::V));
                         l[nt][0] += p[0] + p[2]; l[nt][1] += p[1] + p[3];
 #pragma unroll
                         for (int e = 0; e < 2; e++) {
@@ -397,7 +397,7 @@ kv_step_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
     for (int q = threadIdx.x; q < rows * quads; q += KS_THREADS) {
         const int r = q / quads, c = (q % quads) * 4;
         float2 e[KS_WARPS];
-        float top = KS_NONE, total = 0.f;
+        float top = -INFINITY, total = 0.f;
 #pragma unroll
         for (int w = 0; w < KS_WARPS; w++) {
             e[w] = *reinterpret_cast<const float2 *>(parts + w * PART + HEADS * Sh::LDO + 2 * r);
@@ -407,7 +407,7 @@ kv_step_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
 #pragma unroll
         for (int w = 0; w < KS_WARPS; w++) {
             const float4 v = *reinterpret_cast<const float4 *>(parts + w * PART + r * Sh::LDO + c);
-            const float f = kv_ex2(e[w].x - top);
+            const float f = kv_weight(e[w].x, top, a.scale2);
             total = fmaf(f, e[w].y, total);
             sum.x = fmaf(f, v.x, sum.x); sum.y = fmaf(f, v.y, sum.y); sum.z = fmaf(f, v.z, sum.z); sum.w = fmaf(f, v.w, sum.w);
         }
@@ -428,7 +428,7 @@ kv_step_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
             constexpr int N = decltype(at_a_time)::N;
             for (int q = part_no * KS_THREADS + (int)threadIdx.x; q < rows * quads; q += parts_n * KS_THREADS) {
                 const int r = q / quads, c = (q % quads) * 4;
-                float top = KS_NONE, total = 0.f;
+                float top = -INFINITY, total = 0.f;
                 float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 1
                 for (int p0 = 0; p0 < parts_n; p0 += N) {
@@ -442,12 +442,12 @@ kv_step_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
                     float m = top;
 #pragma unroll
                     for (int p = 0; p < N; p++) m = fmaxf(m, e[p].x);
-                    const float old = kv_ex2(top - m);
+                    const float old = kv_weight(top, m, a.scale2);
                     total *= old; sum.x *= old; sum.y *= old; sum.z *= old; sum.w *= old;
                     top = m;
 #pragma unroll
                     for (int p = 0; p < N; p++) {
-                        const float f = kv_ex2(e[p].x - m);
+                        const float f = kv_weight(e[p].x, m, a.scale2);
                         total = fmaf(f, e[p].y, total);
                         sum.x = fmaf(f, v[p].x, sum.x); sum.y = fmaf(f, v[p].y, sum.y); sum.z = fmaf(f, v[p].z, sum.z); sum.w = fmaf(f, v[p].w, sum.w);
                     }

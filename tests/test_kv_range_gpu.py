@@ -11,6 +11,7 @@ from test_kv_gpu import here, number, randn  # noqa: E402
 
 pytestmark = pytest.mark.gpu
 
+FMTS = ("f32", "f16", "bf16")
 FLOOR = {"f32": 2.0 ** -39, "f16": 2.0 ** -32}            # how finely a probability is held, relative to the largest (the header)
 
 
@@ -58,3 +59,52 @@ def test_small_probabilities(gpu_pkg, fmt, dim, rows):
                     rel = P.PAIR[fmt] + 2.0 ** -22 * (1 + lead + 5 * spread) + (1e-6 if fmt == "f32" else 2e-8 * (n / 16 + 4))
                     bound = wide * rel + FLOOR[fmt] * w.amax(-1, keepdim=True) * ((score > -math.inf).double() @ vv.abs())
                     P.check(out[at:at + m], want, bound + P.HALF_STEP[fmt] * (want.abs() + bound) + 2.0 ** -25 * (fmt == "f16"))
+
+
+def settled(pkg, lay, fmt, heads, dim, scale, q, k_of, seed=5):
+    """Results of all rows, and softmax of the exact scores times the values: k_of(position) gives the first two values of a key, the others are 0."""
+    cache = pkg.KvCache(heads, heads, dim, lay.page, lay.n_pages, fmt=number(pkg, fmt), scale=scale)
+    k, v = P.pools(cache, fmt)
+    v.copy_(1 + 0.25 * randn(seed, *v.shape))
+    for s, n in enumerate(lay.lens):
+        at = torch.arange(n)
+        page, slot = lay.table[s].long()[at // lay.page].cuda(), (at % lay.page).cuda()
+        a, b = k_of(at.double())
+        k[page, :, slot, 0], k[page, :, slot, 1] = (t.cuda()[:, None].expand(n, heads).to(k.dtype) for t in (a, b))
+    rows = torch.zeros(lay.n_rows, heads, dim, device="cuda")
+    rows[..., 0], rows[..., 1] = q
+    rows = rows.reshape(lay.n_rows, heads * dim).to(P.ROWS[fmt])
+    out = torch.zeros_like(rows)
+    cache.attend(lay.batch(cache), rows, out, stream=here())
+    cache.sync(here())
+    for s, (n, m) in enumerate(zip(lay.lens, lay.rows)):
+        kk, vv = (P.keys_of(p, lay, s, list(range(n)))[:, 0] for p in (k, v))
+        x = rows[lay.begin[s], :2].double()
+        score = (scale * (kk[:, 0] * x[0] + kk[:, 1] * x[1])).expand(m, n).clone()
+        score.masked_fill_(torch.arange(n, device="cuda") > torch.arange(n - m, n, device="cuda")[:, None], -math.inf)
+        w = torch.softmax(score, -1)
+        want = w @ vv
+        # weights as in test_small_probabilities, of distances up to 6 units (others are exact or nothing); values all near 1
+        rel = P.PAIR[fmt] + 2.0 ** -22 * 7 + (1e-6 if fmt == "f32" else 2e-8 * (n / 16 + 4))
+        bound = rel * (w @ vv.abs()) + 2.0 ** -32 * n
+        P.check(out[lay.begin[s]:lay.begin[s] + m].double().reshape(m, heads, dim)[:, 0], want, bound + P.HALF_STEP[fmt] * (want.abs() + bound))
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("lens,rows", [([1, 40, 700, 9000], None), ([300] * 80, None), ([1, 40, 3000], [1, 9, 70]), ([700, 900], [700, 333])])
+def test_scores_far_from_zero(gpu_pkg, fmt, dim, lens, rows):
+    lay = P.Layout(lens, 16, rows)
+    top = 1e16 if fmt == "bf16" else 6e4
+    scale = 1.0 if fmt == "bf16" else 1e20
+    flat, heads = torch.zeros_like, 2
+    for sign in (1.0, -1.0):
+        # all alike, 1e30 and more away from 0: the average
+        settled(gpu_pkg, lay, fmt, heads, dim, scale, (top, 0.0), lambda at: (flat(at) + sign * top, flat(at)))
+        # far apart from one another: the largest takes all
+        settled(gpu_pkg, lay, fmt, heads, dim, scale, (top, 0.0), lambda at: (sign * top * (0.25 + (at * 7 % 32) / 64), flat(at)))
+        # small steps on a large common part: 2^22 + {0, 0.5, ... 5}, exact in f32
+        settled(gpu_pkg, lay, fmt, heads, dim, 2.0 ** -7, (32768.0, 64.0), lambda at: (flat(at) + sign * 16384, at * 5 % 11))
+        settled(gpu_pkg, lay, fmt, heads, dim, 2.0 ** -7, (512.0, 64.0), lambda at: (flat(at) + sign * 1024, at * 5 % 11))
+        # rising by more than any distance that a probability survives
+        settled(gpu_pkg, lay, fmt, heads, dim, scale, (top / 64, 0.0), lambda at: (sign * ((at // 64) * 64 - 8192), flat(at)))
