@@ -73,6 +73,17 @@ __device__ __forceinline__ uint32_t kv_pack(float x, float y) {
     const __half2 h = __floats2half2_rn(x, y);
     return *reinterpret_cast<const uint32_t *>(&h);
 }
+// Two results. They are averages, so what rounding has brought beyond the type's largest number is that number (a NaN stays one)
+template <bool BF>
+__device__ __forceinline__ uint32_t kv_pack_result(float x, float y) {
+    constexpr float TOP = BF ? 0x1.fep127f : 65504.f;
+    auto within = [&](float v) {
+        float r;
+        asm("{\n\t.reg .f32 t;\n\tmin.NaN.f32 t, %1, %2;\n\tmax.NaN.f32 %0, t, %3;\n\t}" : "=f"(r) : "f"(v), "f"(TOP), "f"(-TOP));
+        return r;
+    };
+    return kv_pack<BF>(within(x), within(y));
+}
 // x, y as f16 pairs: hi and what it leaves. The rest stays unscaled (it may be subnormal): both products go into one accumulator.
 __device__ __forceinline__ void kv_split(float x, float y, uint32_t &hi, uint32_t &lo) {
     const __half2 h = __floats2half2_rn(x, y);

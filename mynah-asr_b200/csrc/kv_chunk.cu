@@ -37,10 +37,10 @@ static constexpr int KC_PART = 3;                    // P V begins when the firs
 
 // The maximum of a row may lag by 2^LAG, and a probability is 2^TOP of it, which the final division takes out again: together below f16's 2^16,
 // and what is held of a probability (with F32 rows: of its rest) is 2^-25 / 2^TOP of the largest, where it was 2^-25 without. bf16 has the
-// range. A smaller LAG rescales O more often: f16, 8192 rows of 32 heads of 128, scores spread by 2.5 units: 481 us, with a LAG of 4 518,
+// range, but its values end where f32 does: 2^26 of them, the most that a sequence has, do not add up to infinity. A smaller LAG rescales O more often: f16, 8192 rows of 32 heads of 128, scores spread by 2.5 units: 481 us, with a LAG of 4 518,
 // of 2 540. F32 rows of 128 rescale for every tile in any case; 8 heads of 64 take 41.8 us, with a LAG of 8 40.3.
 template <int FMT> struct ChunkTop {
-    static constexpr float LAG = FMT == KV_F32 ? 1.f : 8.f, TOP = FMT == KV_F32 ? 14.f : FMT == KV_F16 ? 7.f : 0.f;
+    static constexpr float LAG = FMT == KV_F32 ? 1.f : 8.f, TOP = FMT == KV_F32 ? 14.f : FMT == KV_F16 ? 7.f : -35.f;
 };
 
 template <int DP, int FMT> struct ChunkShape {
@@ -745,7 +745,7 @@ kv_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
 #pragma unroll
                     for (int u = 0; u < 16; u++) {
                         if (F32) v[u] = __float_as_uint(inv != 0.f ? o[u] * inv : 0.f);
-                        else v[u] = inv != 0.f ? kv_pack<BF>(o[2 * u] * inv, o[2 * u + 1] * inv) : 0u;
+                        else v[u] = inv != 0.f ? kv_pack_result<BF>(o[2 * u] * inv, o[2 * u + 1] * inv) : 0u;
                     }
                     kc_quads(v, lane);
                     const int col = c * COLS + (lane & 3) * (COLS / 4);
@@ -831,7 +831,7 @@ kv_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                 const int pl = by_g(v0 + v);
                 const int64_t to = (int64_t)(b.begin + b.t0 + pl) * a.ldo + (int64_t)(b.kvh * a.G + v0 + v - pl * a.G) * a.D + c;
                 if (F32) *reinterpret_cast<float4 *>(static_cast<float *>(a.out) + to) = sum;
-                else *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(a.out) + to) = make_uint2(kv_pack<BF>(sum.x, sum.y), kv_pack<BF>(sum.z, sum.w));
+                else *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(a.out) + to) = make_uint2(kv_pack_result<BF>(sum.x, sum.y), kv_pack_result<BF>(sum.z, sum.w));
             }
             kv_cluster_sync();                                     // nobody leaves while its part is being read
         }

@@ -22,8 +22,8 @@ namespace mb {
 
 // Probabilities are 2^V of the warp's largest, which the final division takes out again: f16 ends at 2^-24, so that what is held of them, and
 // with F32 rows of their rest, is 2^-40 of the largest and not 2^-25 (100 000 keys 17 units below the first one were lost, all but 0.2 %). bf16 has
-// the range.
-template <int FMT> struct StepTop { static constexpr float V = FMT == KV_BF16 ? 0.f : 15.f; };
+// the range, but its values end where f32 does: 2^26 of them, the most that a sequence has, do not add up to infinity.
+template <int FMT> struct StepTop { static constexpr float V = FMT == KV_BF16 ? -27.f : 15.f; };
 static constexpr int KS_MOST_STAGES = 3, KS_HEAD = 1024;                  // barriers in front of the ring
 static constexpr int KS_WARPS = 4, KS_THREADS = (KS_WARPS + 1) * 32;      // warps that compute, and one that asks for the tiles
 // DP: D rounded up to 64 or 128
@@ -392,7 +392,7 @@ kv_step_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
         const float inv = total != 0.f ? 1.f / total : 0.f;
         const int64_t at = (int64_t)seq * a.ldo + (int64_t)(kvh * a.G + g0 + r) * a.D + c;
         if (F32) *reinterpret_cast<float4 *>(static_cast<float *>(a.out) + at) = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
-        else *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(a.out) + at) = make_uint2(kv_pack<BF>(v.x * inv, v.y * inv), kv_pack<BF>(v.z * inv, v.w * inv));
+        else *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(a.out) + at) = make_uint2(kv_pack_result<BF>(v.x * inv, v.y * inv), kv_pack_result<BF>(v.z * inv, v.w * inv));
     };
     for (int q = threadIdx.x; q < rows * quads; q += KS_THREADS) {
         const int r = q / quads, c = (q % quads) * 4;

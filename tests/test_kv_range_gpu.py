@@ -108,3 +108,25 @@ def test_scores_far_from_zero(gpu_pkg, fmt, dim, lens, rows):
         settled(gpu_pkg, lay, fmt, heads, dim, 2.0 ** -7, (512.0, 64.0), lambda at: (flat(at) + sign * 1024, at * 5 % 11))
         # rising by more than any distance that a probability survives
         settled(gpu_pkg, lay, fmt, heads, dim, scale, (top / 64, 0.0), lambda at: (sign * ((at // 64) * 64 - 8192), flat(at)))
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "f16"])
+@pytest.mark.parametrize("lens,rows", [([1, 2, 3, 40, 700, 9000], None), ([300] * 80, None), ([1, 40, 3000], [1, 9, 70]), ([700, 900], [700, 333])])
+def test_average_of_the_largest_values(gpu_pkg, fmt, lens, rows):
+    """Values that are the largest numbers of the type: no sum of them ends at infinity, and no average beyond them."""
+    top = torch.finfo(P.CACHE[fmt]).max
+    lay = P.Layout(lens, 16, rows)
+    for dim in (64, 128):
+        cache = gpu_pkg.KvCache(4, 2, dim, 16, lay.n_pages, fmt=number(gpu_pkg, fmt))
+        k, v = P.pools(cache, fmt)
+        k.copy_(randn(1, *k.shape))
+        v[..., ::2], v[..., 1::2] = top, -top
+        q = (2 * randn(2, lay.n_rows, 4 * dim)).to(P.ROWS[fmt])
+        out = torch.zeros_like(q)
+        cache.attend(lay.batch(cache), q, out, stream=here())
+        cache.sync(here())
+        want = v[0, 0, 0].double().repeat(4).expand(lay.n_rows, -1)
+        # weights off by one rounding each (the rest of their error is the same in the sum), sums as above; then a rounding
+        rel = P.PAIR[fmt] + 2.0 ** -20 + 2e-8 * (max(lens) / 16 + 4)
+        P.check(out, want, top * (rel + P.HALF_STEP[fmt] * (1 + rel)) * torch.ones_like(want))
+        assert (out.abs() <= top).all()
