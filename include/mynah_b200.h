@@ -367,8 +367,9 @@ typedef struct {
  * device (cudaStreamLegacy for the legacy default stream), or on the handle's own non-blocking stream where NULL. They
  * allocate nothing, use no workspace and can be captured; calls of one handle may overlap on the GPU as long as none
  * writes a slot that another reads or writes. 0, or -1 with mynah_b200_last_error and nothing launched. What only the
- * tables show (a page or length out of range: skipped, or read as page 0) and values that do not fit the cache's 16 bits
- * (not finite, or from 65504 on in f16: stored as 0) are reported by mynah_b200_kv_sync.
+ * tables show (a page or length out of range: skipped, or read as page 0), values that do not fit the cache's 16 bits
+ * (not finite, or from 65504 on in f16: stored as 0) and rows whose scores are not finite (all of them minus infinity: the
+ * result is 0; one NaN or plus infinity: it is NaN) are reported by mynah_b200_kv_sync.
  *
  * append: norm and rotation of q into q_out (which may be q itself with the same stride), of k into the cache, v into the
  * cache as it is. Rows whose position is below 0 (more rows than keys) are skipped. A slot that two rows of a call name

@@ -266,7 +266,7 @@ int mynah_b200_kv_sync(mynah_b200_kv *h, void *stream) {
     if (code == ST_OK) return 0;
     MB_CUDA(cudaMemsetAsync(h->status(), 0, sizeof(int), h->stream));
     MB_CUDA(cudaStreamSynchronize(h->stream));
-    if (code == ST_RANGE) set_error("kv: a value did not fit its 16 bits (f16: |v| >= 65504) or was not finite");
+    if (code == ST_RANGE) set_error("kv: a value did not fit its 16 bits (f16: |v| >= 65504), or a value or a score was not finite");
     else if (code == ST_PAGE) set_error("kv: a table names a page, a length or a row that does not exist");
     else set_error("kv: a bounded wait inside an attention kernel ran out (code %d)", code);
     return -1;

@@ -67,6 +67,8 @@ __device__ __forceinline__ float kv_ex2(float x) {
 // difference of neighbours is exact, where the fused x scale2 - m scale2 has lost its digits for scores of 2^24 and more (16384 bf16 rows:
 // 1 % more time). What was summed under the maximum m counts 2^((m - top) scale2) under a larger one.
 __device__ __forceinline__ float kv_weight(float m, float top, float scale2) { return m == top ? 1.f : kv_ex2((m - top) * scale2); }
+// The sum of a row's probabilities, of which the largest is not small: where it is nothing or no number, the scores were not finite
+__device__ __forceinline__ bool kv_sound(float l) { return l > 0.f && l < INFINITY; }
 template <bool BF>
 __device__ __forceinline__ uint32_t kv_pack(float x, float y) {
     if (BF) { const __nv_bfloat162 h = __floats2bfloat162_rn(x, y); return *reinterpret_cast<const uint32_t *>(&h); }

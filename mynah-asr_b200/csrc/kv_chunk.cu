@@ -556,7 +556,7 @@ kv_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                             const float *f = reinterpret_cast<const float *>(in[i]);
                             uint4 hi, lo;
 #pragma unroll
-                            for (int e = 0; e < 8; e++) bad |= !(fabsf(f[e]) < H16_MAX);
+                            for (int e = 0; e < 8; e++) bad |= !(fabsf(f[e]) < H16_MAX) && b.base_pos + b.t0 + t * tq + by_g(row) >= 0;
                             kv_split(f[0], f[1], hi.x, lo.x); kv_split(f[2], f[3], hi.y, lo.y); kv_split(f[4], f[5], hi.z, lo.z); kv_split(f[6], f[7], hi.w, lo.w);
                             *reinterpret_cast<uint4 *>(to) = hi;
                             *reinterpret_cast<uint4 *>(to + Sh::OPERAND) = lo;
@@ -728,6 +728,8 @@ kv_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
             const volatile int *w = items + (j & 1) * KcBlock::WORDS;
             if (w[8] == 1 && rank == 0 && ok) {
                 const float inv = l != 0.f ? 1.f / l : 0.f;
+                const int mine = w[4] + t * tq + by_g(r);      // the thread's row in its sequence
+                if (r < tq * a.G && mine < w[3] && w[5] + mine >= 0 && !kv_sound(l)) atomicExch(a.status, ST_RANGE);
                 // after the turn a lane stores a quarter of 16 words of each of the four rows of its lanes: where they lie, -1 for rows that are not
                 const int begin = w[2], last = w[3] - w[4] - t * tq, kvh = w[1];       // (rows of the tile: below last)
                 const int64_t first = (int64_t)(begin + w[4] + t * tq) * a.ldo + (int64_t)kvh * a.G * a.D;
@@ -806,6 +808,7 @@ kv_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                     total = fmaf(e[p].x, e[p].y, total);
                 }
                 const float inv = total != 0.f ? 1.f / total : 0.f;
+                if (b.base_pos + b.t0 + by_g(v0 + v) >= 0 && !kv_sound(total)) atomicExch(a.status, ST_RANGE);
 #pragma unroll
                 for (int p = 0; p < 16; p++)
                     if (p < b.shares) weight[v * 16 + p] = e[p].x * inv;

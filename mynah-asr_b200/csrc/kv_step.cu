@@ -393,6 +393,7 @@ kv_step_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
         const int64_t at = (int64_t)seq * a.ldo + (int64_t)(kvh * a.G + g0 + r) * a.D + c;
         if (F32) *reinterpret_cast<float4 *>(static_cast<float *>(a.out) + at) = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
         else *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(a.out) + at) = make_uint2(kv_pack_result<BF>(v.x * inv, v.y * inv), kv_pack_result<BF>(v.z * inv, v.w * inv));
+        if (!kv_sound(total) && c == 0 && pos >= 0) atomicExch(a.status, ST_RANGE);
     };
     for (int q = threadIdx.x; q < rows * quads; q += KS_THREADS) {
         const int r = q / quads, c = (q % quads) * 4;

@@ -130,3 +130,66 @@ def test_average_of_the_largest_values(gpu_pkg, fmt, lens, rows):
         rel = P.PAIR[fmt] + 2.0 ** -20 + 2e-8 * (max(lens) / 16 + 4)
         P.check(out, want, top * (rel + P.HALF_STEP[fmt] * (1 + rel)) * torch.ones_like(want))
         assert (out.abs() <= top).all()
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("heads,kv_heads,dim", [(4, 2, 64), (2, 1, 128)])
+@pytest.mark.parametrize("lens,rows", [([40, 300, 9], None), ([40, 300, 9] * 60, None), ([40, 5000, 9], [9, 70, 9]), ([700, 900, 700] * 3, [700, 333, 600] * 3)])
+def test_scores_that_are_no_numbers_are_reported(gpu_pkg, fmt, heads, kv_heads, dim, lens, rows):
+    """A row whose scores are NaN or infinite is an error of the next sync; the other rows keep their bits, and what no row sees, rows that see no key
+    and rows behind the last sequence are no errors."""
+    lay = P.Layout(lens, 16, rows, extra_rows=3)
+    cache = gpu_pkg.KvCache(heads, kv_heads, dim, 16, lay.n_pages, fmt=number(gpu_pkg, fmt))
+    k, v = P.pools(cache, fmt)
+    k.copy_(randn(1, *k.shape))
+    v.copy_(randn(2, *v.shape))
+    good = randn(3, lay.n_rows, heads * dim).to(P.ROWS[fmt])
+    good[lay.real:] = math.nan
+    out, plain = torch.zeros_like(good), torch.zeros_like(good)
+    batch = lay.batch(cache)
+    cache.attend(batch, good, plain, stream=here())
+    cache.sync(here())
+    at = lay.begin[1] + lay.rows[1] - 1                   # the last row of sequence 1, its last head
+    first = lay.table[1, 0].item()
+    cases = [("nan", math.nan, None), ("inf", math.inf, None)]
+    if fmt == "bf16":                                     # finite numbers whose products are not
+        cases += [("above", 1e30, 1e30), ("below", 1e30, -1e30)]
+    for name, value, key in cases:
+        q = good.clone()
+        q[at, (heads - 1) * dim:] = value
+        kept = k.clone()
+        if key is not None:                               # all keys of sequence 1, or the first one
+            some = lay.table[1] if name == "below" else lay.table[1, :1]
+            k[some[some >= 0].long().cuda(), kv_heads - 1] = key
+        cache.attend(batch, q, out, stream=here())
+        with pytest.raises(gpu_pkg.BackendError, match="finite"):
+            cache.sync(here())
+        cache.sync(here())
+        others = [i for i in range(lay.real) if not lay.begin[1] <= i < lay.begin[1] + lay.rows[1]]
+        assert torch.equal(out[others], plain[others]) and (out[lay.real:] == 0).all()
+        if key is None:
+            assert torch.equal(out[at, :(heads - 1) * dim], plain[at, :(heads - 1) * dim])
+        k.copy_(kept)
+    if fmt == "bf16":                                     # one key at minus infinity among others is none
+        q = good.clone()
+        q[at, (heads - 1) * dim:] = 1e30
+        kept = k.clone()
+        k[:, kv_heads - 1] = 0
+        k[first, kv_heads - 1, 0] = -1e30
+        cache.attend(batch, q, out, stream=here())
+        cache.sync(here())
+        k.copy_(kept)
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+def test_rows_without_keys_are_no_errors(gpu_pkg, fmt):
+    for lens, rows in (([0, 3, 0], None), ([0, 3, 2], [4, 5, 300])):
+        lay = P.Layout(lens, 16, rows)
+        cache = gpu_pkg.KvCache(4, 2, 64, 16, lay.n_pages, fmt=number(gpu_pkg, fmt))
+        q = torch.ones(lay.n_rows, 256, device="cuda").to(P.ROWS[fmt])
+        blind = [lay.begin[s] + i for s, n in enumerate(lay.rows) for i in range(n) if lay.lens[s] - n + i < 0]
+        q[blind] = math.nan
+        out = torch.ones_like(q)
+        cache.attend(lay.batch(cache), q, out, stream=here())
+        cache.sync(here())
+        assert (out == 0).all()
