@@ -1,7 +1,9 @@
 // The paged key/value cache at the C boundary (include/mynah_b200.h): checks of arguments, the handle and its memory.
 #include <math.h>
+#include <stdio.h>
 #include <string.h>
 
+#include <mutex>
 #include <new>
 
 #include "../../include/mynah_b200.h"
@@ -9,7 +11,7 @@
 
 using namespace mb;
 
-// Device memory of a handle: the two pools, and a block [status, 256 B | turns of the rotation | norm weights].
+// Device memory of a handle: the two pools, and a block [status, what a sync took of it, 256 B | turns of the rotation | norm weights].
 struct mynah_b200_kv {
     mynah_b200_kv_config cfg;
     int fmt = KV_BF16, device = 0;
@@ -20,7 +22,10 @@ struct mynah_b200_kv {
     float *q_norm = nullptr, *k_norm = nullptr;
     CUtensorMap map_k, map_v, chunk_k, chunk_v;                // for single tokens, for prompts
     int chunk_box = 0;
+    std::mutex syncing;
+    bool owed = false;                                         // what was taken has not reached the host
     int *status() const { return reinterpret_cast<int *>(block); }
+    int *taken() const { return reinterpret_cast<int *>(block + 128); }
     ~mynah_b200_kv() {
         cudaFree(k); cudaFree(v); cudaFree(block);              // (waits for the handle's work)
         if (stream) cudaStreamDestroy(stream);
@@ -138,6 +143,11 @@ int take_batch(const char *what, const mynah_b200_kv *h, const mynah_b200_kv_bat
     a->n_seq = b->n_seq; a->n_rows = b->n_rows; a->max_pages = b->max_pages;
     a->row_off = b->row_off; a->kv_len = b->kv_len; a->table = b->page_table;
     return 0;
+}
+
+__global__ void kv_take_kernel(int *status, int *taken, int keep) {
+    const int found = atomicExch(status, 0);
+    *taken = keep ? *taken | found : found;
 }
 }  // namespace
 
@@ -260,15 +270,24 @@ int mynah_b200_kv_sync(mynah_b200_kv *h, void *stream) {
     OnDevice on(h->device);
     const cudaStream_t st = stream ? (cudaStream_t)stream : h->stream;
     MB_CUDA(cudaStreamSynchronize(st));
-    int code = 0;
-    MB_CUDA(cudaMemcpyAsync(&code, h->status(), sizeof(int), cudaMemcpyDeviceToHost, h->stream));
+    // Read and cleared in one step: calls on other streams may be reporting at the same time
+    std::lock_guard<std::mutex> one(h->syncing);
+    int found = 0;
+    MB_CUDA(launch_kernel(kv_take_kernel, dim3(1), dim3(1), 0, h->stream, false, 1, h->status(), h->taken(), h->owed ? 1 : 0));
+    h->owed = true;
+    MB_CUDA(cudaMemcpyAsync(&found, h->taken(), sizeof(int), cudaMemcpyDeviceToHost, h->stream));
     MB_CUDA(cudaStreamSynchronize(h->stream));
-    if (code == ST_OK) return 0;
-    MB_CUDA(cudaMemsetAsync(h->status(), 0, sizeof(int), h->stream));
-    MB_CUDA(cudaStreamSynchronize(h->stream));
-    if (code == ST_RANGE) set_error("kv: a value did not fit its 16 bits (f16: |v| >= 65504), or a value or a score was not finite");
-    else if (code == ST_PAGE) set_error("kv: a table names a page, a length or a row that does not exist");
-    else set_error("kv: a bounded wait inside an attention kernel ran out (code %d)", code);
+    h->owed = false;
+    if (found == 0) return 0;
+    const int waits = found & (1 << ST_TIMEOUT_PRODUCER | 1 << ST_TIMEOUT_MMA | 1 << ST_TIMEOUT_EPILOGUE);
+    char text[3][160] = {"", "", ""};
+    if (waits) snprintf(text[0], sizeof(text[0]), " a bounded wait inside an attention kernel ran out (code %d);", __builtin_ctz((unsigned)waits));
+    if (found & 1 << ST_PAGE) snprintf(text[1], sizeof(text[1]), " a table names a page, a length or a row that does not exist;");
+    if (found & 1 << ST_RANGE)
+        snprintf(text[2], sizeof(text[2]), " a value did not fit its 16 bits (f16: |v| >= 65504), or a value or a score was not finite;");
+    char all[480];
+    const int n = snprintf(all, sizeof(all), "%s%s%s", text[0], text[1], text[2]);
+    set_error("kv:%.*s", n - 1, all);
     return -1;
 }
 

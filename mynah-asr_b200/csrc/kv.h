@@ -19,7 +19,7 @@ struct KvArgs {
     int window, sinks;
     float scale2;                                    // of scores, for powers of two
     uint16_t *k, *v;                                 // pools
-    int *status;
+    int *status;                                     // bits 1 << ST_...
     // the call
     int n_seq, n_rows, max_pages;
     const int *row_off, *kv_len, *table;
@@ -115,6 +115,8 @@ __device__ __forceinline__ float2 kv_add2(float2 a, float2 b) {
     return d;
 }
 
+// ---- what a kernel has found: a bit of the handle's word for each code, so that none hides another
+__device__ __forceinline__ void kv_report(const KvArgs &a, int code) { atomicOr(a.status, 1 << code); }
 // ---- tables
 __device__ __forceinline__ int64_t kv_capacity(const KvArgs &a) { return (int64_t)a.max_pages << a.page_shift; }
 // Index of a cache row (one head at one slot)
@@ -144,7 +146,7 @@ __device__ __forceinline__ void kv_look_over(const KvArgs &a, int lane) {
         KvSeq q;
         bad |= !kv_seq(a.row_off, a.kv_len, s, a.n_rows, kv_capacity(a), &q);
     }
-    if (bad) atomicExch(a.status, ST_PAGE);
+    if (bad) kv_report(a, ST_PAGE);
 }
 #endif
 

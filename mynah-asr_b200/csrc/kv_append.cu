@@ -187,7 +187,7 @@ kv_append_kernel(const KvAppendArgs p, int per_part) {
     if (seq < 0) return;                             // behind the last sequence: everything stays as it was
     KvSeq s;
     if (!kv_seq(a.row_off, a.kv_len, seq, a.n_rows, kv_capacity(a), &s) || row < s.begin || row >= s.begin + s.n) {
-        if (lane == 0) atomicExch(a.status, ST_PAGE);
+        if (lane == 0) kv_report(a, ST_PAGE);
         return;
     }
     const int pos = s.len - s.n + (row - s.begin);
@@ -209,7 +209,7 @@ kv_append_kernel(const KvAppendArgs p, int per_part) {
         }
     }
     if ((unsigned)page >= (unsigned)a.n_pages) {
-        if (lane == 0) atomicExch(a.status, ST_PAGE);
+        if (lane == 0) kv_report(a, ST_PAGE);
         return;
     }
     const size_t step = (size_t)a.D << a.page_shift, base = kv_row(a, page, 0, slot) * a.D;
@@ -223,7 +223,7 @@ kv_append_kernel(const KvAppendArgs p, int per_part) {
         fetched = false;
     }
     if (g1 > gq + gk) bad |= ka_heads<FMT, LPH, KA_V>(p, w, v, max(g0 - gq - gk, 0), min(g1 - gq - gk, gk), a.Hkv, a.v + base, step, in, fetched);
-    if (bad) atomicExch(a.status, ST_RANGE);
+    if (bad) kv_report(a, ST_RANGE);
 }
 
 template <int FMT>

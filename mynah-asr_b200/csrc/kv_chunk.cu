@@ -134,7 +134,7 @@ struct KcFinder {
             look(a, s0 + lane, &bad);
             total += __reduce_add_sync(0xffffffffu, mine);
         }
-        if (bad) atomicExch(a.status, ST_PAGE);
+        if (bad) kv_report(a, ST_PAGE);
     }
     // Blocks of the lane's sequence with `tiles` tiles of keys at least: those from some place on (a window bounds all alike)
     __device__ __forceinline__ int as_long(const KvArgs &a, int tiles) const {
@@ -370,7 +370,7 @@ kv_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                 const int next = entry_of(i + 1);
                 const int j = key_of(i);
                 if (lane < boxes && (unsigned)entry >= (unsigned)a.n_pages) {
-                    if (seen(j)) atomicExch(a.status, ST_PAGE);
+                    if (seen(j)) kv_report(a, ST_PAGE);
                     entry = 0;                                 // any finite rows do
                 }
                 const int y = (int)kv_row(a, entry, b.kvh, j & ((1 << shift) - 1));
@@ -391,7 +391,7 @@ kv_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
             x = x0 + (longest_first && !(j & 1) ? (int)(gridDim.x - 1 - blockIdx.x) : (int)blockIdx.x);
             nth = x / a.Hkv;
         }
-        if (!ok && lane == 0) atomicExch(a.status, ST_TIMEOUT_PRODUCER);
+        if (!ok && lane == 0) kv_report(a, ST_TIMEOUT_PRODUCER);
         for (int u = 0; u < STAGES && u < r; u++) {            // what was asked for has to land before the CTA leaves
             if (s == 0) { s = STAGES; ph ^= 1; }
             if (!mbar_wait_warp(&full[--s], (uint32_t)ph)) break;
@@ -500,7 +500,7 @@ kv_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
             if (once) break;
         }
         if (!ok) {                                             // nothing may run on when tensor memory is given back
-            if (lane == 0) atomicExch(a.status, ST_TIMEOUT_MMA);
+            if (lane == 0) kv_report(a, ST_TIMEOUT_MMA);
             if (elect_one()) tc_commit(drain);
             __syncwarp();
             mbar_wait_warp(drain, 0);
@@ -562,7 +562,7 @@ kv_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                             *reinterpret_cast<uint4 *>(to + Sh::OPERAND) = lo;
                         }
                     }
-                    if (bad) atomicExch(a.status, ST_RANGE);
+                    if (bad) kv_report(a, ST_RANGE);
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");       // generic-proxy stores -> visible to the tensor core
                 }
             __syncwarp();
@@ -729,7 +729,7 @@ kv_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
             if (w[8] == 1 && rank == 0 && ok) {
                 const float inv = l != 0.f ? 1.f / l : 0.f;
                 const int mine = w[4] + t * tq + by_g(r);      // the thread's row in its sequence
-                if (r < tq * a.G && mine < w[3] && w[5] + mine >= 0 && !kv_sound(l)) atomicExch(a.status, ST_RANGE);
+                if (r < tq * a.G && mine < w[3] && w[5] + mine >= 0 && !kv_sound(l)) kv_report(a, ST_RANGE);
                 // after the turn a lane stores a quarter of 16 words of each of the four rows of its lanes: where they lie, -1 for rows that are not
                 const int begin = w[2], last = w[3] - w[4] - t * tq, kvh = w[1];       // (rows of the tile: below last)
                 const int64_t first = (int64_t)(begin + w[4] + t * tq) * a.ldo + (int64_t)kvh * a.G * a.D;
@@ -762,7 +762,7 @@ kv_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
         leave_block(j);
         if (once) break;
     }
-    if (!ok && lane == 0) atomicExch(a.status, ST_TIMEOUT_EPILOGUE);
+    if (!ok && lane == 0) kv_report(a, ST_TIMEOUT_EPILOGUE);
     }
     __syncwarp();
     if (once) {
@@ -808,7 +808,7 @@ kv_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                     total = fmaf(e[p].x, e[p].y, total);
                 }
                 const float inv = total != 0.f ? 1.f / total : 0.f;
-                if (b.base_pos + b.t0 + by_g(v0 + v) >= 0 && !kv_sound(total)) atomicExch(a.status, ST_RANGE);
+                if (b.base_pos + b.t0 + by_g(v0 + v) >= 0 && !kv_sound(total)) kv_report(a, ST_RANGE);
 #pragma unroll
                 for (int p = 0; p < 16; p++)
                     if (p < b.shares) weight[v * 16 + p] = e[p].x * inv;

@@ -147,7 +147,7 @@ kv_step_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
     const int g0 = (unit % head_tiles) * HEADS, kvh = unit / head_tiles;
     const int rows = seq < 0 ? 0 : min(HEADS, a.G - g0);
     KvSeq sq = {0, 0, 0};
-    if (seq >= 0 && !kv_seq(nullptr, a.kv_len, seq, a.n_rows, kv_capacity(a), &sq) && threadIdx.x == 0) atomicExch(a.status, ST_PAGE);
+    if (seq >= 0 && !kv_seq(nullptr, a.kv_len, seq, a.n_rows, kv_capacity(a), &sq) && threadIdx.x == 0) kv_report(a, ST_PAGE);
     const int pos = sq.len - 1;
     const KvTiles tiles = kv_tiles(pos, pos, a.window, a.sinks, TILE);
     const int n = part_no < tiles.count ? (tiles.count - part_no + parts_n - 1) >> log_parts : 0;        // tiles of this CTA
@@ -173,7 +173,7 @@ kv_step_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
         for (; i < n; i++) {
             const int next = entry_of(i + 1);
             if (i >= stages && !mbar_wait_warp(&empty[s], (uint32_t)(ph ^ 1))) {
-                if (lane == 0) atomicExch(a.status, ST_TIMEOUT_PRODUCER);
+                if (lane == 0) kv_report(a, ST_TIMEOUT_PRODUCER);
                 break;
             }
             if (lane == 0) mbar_expect_tx(&full[s], Sh::STAGE);
@@ -181,7 +181,7 @@ kv_step_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
             if (lane < boxes) {
                 const int j = key_of(i);
                 if ((unsigned)entry >= (unsigned)a.n_pages) {
-                    if (seen(j)) atomicExch(a.status, ST_PAGE);
+                    if (seen(j)) kv_report(a, ST_PAGE);
                     entry = 0;                                 // any finite rows do
                 }
                 tma_load_2d(smem + s * Sh::STAGE + b_at, map, b_half * 64, (int)kv_row(a, entry, kvh, j & ((1 << shift) - 1)), &full[s]);
@@ -218,7 +218,7 @@ kv_step_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
                         qh[nt][kk][e] = *reinterpret_cast<const uint32_t *>(static_cast<const uint16_t *>(a.q) + at);
                     }
                 }
-        if (bad) atomicExch(a.status, ST_RANGE);
+        if (bad) kv_report(a, ST_RANGE);
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
 #pragma unroll
@@ -234,7 +234,7 @@ kv_step_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
         for (int i = 0; i < n; i++) {
             const int j0 = tiles.at(part_no + (i << log_parts)) * TILE + warp * OWN;
             if (!mbar_wait_warp(&full[s], (uint32_t)ph)) {
-                if (lane == 0) atomicExch(a.status, ST_TIMEOUT_EPILOGUE);
+                if (lane == 0) kv_report(a, ST_TIMEOUT_EPILOGUE);
                 break;
             }
             const uint32_t kt = base + s * Sh::STAGE, vt = kt + Sh::OPERAND;
@@ -393,7 +393,7 @@ kv_step_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
         const int64_t at = (int64_t)seq * a.ldo + (int64_t)(kvh * a.G + g0 + r) * a.D + c;
         if (F32) *reinterpret_cast<float4 *>(static_cast<float *>(a.out) + at) = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
         else *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(a.out) + at) = make_uint2(kv_pack_result<BF>(v.x * inv, v.y * inv), kv_pack_result<BF>(v.z * inv, v.w * inv));
-        if (!kv_sound(total) && c == 0 && pos >= 0) atomicExch(a.status, ST_RANGE);
+        if (!kv_sound(total) && c == 0 && pos >= 0) kv_report(a, ST_RANGE);
     };
     for (int q = threadIdx.x; q < rows * quads; q += KS_THREADS) {
         const int r = q / quads, c = (q % quads) * 4;

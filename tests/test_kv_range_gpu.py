@@ -193,3 +193,49 @@ def test_rows_without_keys_are_no_errors(gpu_pkg, fmt):
         cache.attend(lay.batch(cache), q, out, stream=here())
         cache.sync(here())
         assert (out == 0).all()
+
+
+def test_reports_are_neither_hidden_nor_lost(gpu_pkg):
+    """Two findings before one sync are both named; findings of a stream while another thread syncs a second one are all seen."""
+    import threading
+    import time
+    lay = P.Layout([30, 45], 16)
+    cache = gpu_pkg.KvCache(2, 2, 32, 16, lay.n_pages, fmt=gpu_pkg.F32)
+    good, table = torch.ones(2, 64, device="cuda"), lay.table_dev.clone()
+    large, out = 1e6 * good, torch.zeros_like(good)
+    table[1, 2] = lay.n_pages
+    fine, broken = lay.batch(cache), cache.batch(lay.len_dev, table)
+    calls = {"page": lambda st: cache.append(broken, good, good, good, out, stream=st), "16 bits": lambda st: cache.append(fine, good, large, good, out, stream=st)}
+    for order in (["page", "16 bits"], ["16 bits", "page"], ["page", "page"], ["16 bits"]):
+        for name in order:
+            calls[name](here())
+        with pytest.raises(gpu_pkg.BackendError) as said:
+            cache.sync(here())
+        assert all((name in str(said.value)) == (name in order) for name in calls)
+        cache.sync(here())
+    seen, stop, streams = [], threading.Event(), [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+
+    def look():
+        while not stop.is_set():
+            try:
+                cache.sync(streams[1].cuda_stream)
+            except gpu_pkg.BackendError as e:
+                seen.append(str(e))
+
+    thread = threading.Thread(target=look)
+    thread.start()
+    try:
+        for i in range(300):
+            seen.clear()
+            for name in ("page", "16 bits"):
+                calls[name](streams[0].cuda_stream)
+                until = time.perf_counter() + i % 20 * 5e-6
+                while time.perf_counter() < until:
+                    pass
+            until = time.perf_counter() + 5
+            while not all(any(name in text for text in seen) for name in calls):
+                assert time.perf_counter() < until, "round %d: %s" % (i, seen)
+    finally:
+        stop.set()
+        thread.join()
