@@ -333,7 +333,8 @@ typedef struct {
     int rotary_interleaved;              /* pairs are (2i, 2i + 1) instead of (i, i + rotary_dim / 2) */
     double rope_theta;                   /* pair i turns by theta^(-2i / rotary_dim) per position, */
     const double *inv_freq;              /* or by inv_freq[i] where given [rotary_dim / 2] */
-    const float *q_norm, *k_norm;        /* [head_dim] weights of a root-mean-square norm of every q / k head; NULL: none */
+    const float *q_norm, *k_norm;        /* [head_dim] weights of a root-mean-square norm of every q / k head; NULL: none. The mean of
+                                          * squares with norm_eps has to lie in [2^-126, 2^128) (heads of values from 1e-19 to 1e18) */
     float norm_eps;
     int window, n_sinks;                 /* window > 0: a row at position p sees the keys j with p - window < j <= p, and j < n_sinks */
     float scale;                         /* of the scores, from 1e-20 to 1e20; 0: 1 / sqrt(head_dim) */
@@ -368,7 +369,7 @@ typedef struct {
  * allocate nothing, use no workspace and can be captured; calls of one handle may overlap on the GPU as long as none
  * writes a slot that another reads or writes. 0, or -1 with mynah_b200_last_error and nothing launched. What only the
  * tables show (a page or length out of range: skipped, or read as page 0), values that do not fit the cache's 16 bits
- * (not finite, or from 65504 on in f16: stored as 0) and rows whose scores are not finite (all of them minus infinity: the
+ * (not finite, or from 65504 on in f16: stored as 0; a head whose norm is out of range counts as not finite) and rows whose scores are not finite (all of them minus infinity: the
  * result is 0; one NaN or plus infinity: it is NaN) are reported by mynah_b200_kv_sync.
  *
  * append: norm and rotation of q into q_out (which may be q itself with the same stride), of k into the cache, v into the

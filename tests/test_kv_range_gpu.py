@@ -239,3 +239,44 @@ def test_reports_are_neither_hidden_nor_lost(gpu_pkg):
     finally:
         stop.set()
         thread.join()
+
+
+@pytest.mark.parametrize("fmt", ["f32", "bf16"])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(4, 2, 128), (8, 8, 64), (3, 1, 80), (5, 5, 16)])
+@pytest.mark.parametrize("eps", [1e-6, 0.0])
+def test_norms_of_large_and_small_heads(gpu_pkg, fmt, heads, kv_heads, dim, eps):
+    """Heads whose squares f32 does not hold are reported, and no numbers in q_out, 0 in the cache; those beside them are as they should."""
+    lay = P.Layout([40, 7], 16, [40, 7])
+    w = 1 + 0.3 * randn(5, dim)
+    cache = gpu_pkg.KvCache(heads, kv_heads, dim, 16, lay.n_pages, fmt=number(gpu_pkg, fmt), rotary_dim=dim // 8 * 8, q_norm=w.cpu().numpy(), k_norm=w.cpu().numpy(), norm_eps=eps)
+    k, v = P.pools(cache, fmt)
+    batch = lay.batch(cache)
+    pos = [n - r + i for n, r in zip(lay.lens, lay.rows) for i in range(r)]
+    fine, large, small = [0.0, 1e18, 1.0, 1e9, 1e-3], [3e38, 1e25, 1e20], [1e-38, 1e-25, 1e-30]
+    if eps == 0:
+        fine[0] = 1e-18                                   # (0 / 0 otherwise)
+    for odd in ([], large, small):
+        def rows(seed, n):
+            x = randn(seed, lay.n_rows, n, dim)
+            x = x / x.abs().amax(-1, keepdim=True)        # the largest value of a head is 1
+            power = torch.tensor(fine + odd, device="cuda")
+            which = (torch.arange(lay.n_rows * n, device="cuda") % len(power)).reshape(lay.n_rows, n)
+            return (x * power[which][..., None]).reshape(lay.n_rows, n * dim).to(P.ROWS[fmt]), which >= len(fine)
+
+        (q, odd_q), (kr, odd_k) = rows(1, heads), rows(2, kv_heads)
+        vr, out = randn(3, lay.n_rows, kv_heads * dim).to(P.ROWS[fmt]), torch.zeros_like(q)
+        lost = bool(odd) and (odd is large or eps == 0)
+        cache.append(batch, q, kr, vr, out, stream=here())
+        if lost:
+            with pytest.raises(gpu_pkg.BackendError, match="finite"):
+                cache.sync(here())
+        else:
+            cache.sync(here())
+            odd_q, odd_k = torch.zeros_like(odd_q), torch.zeros_like(odd_k)
+        got_q = out.double().reshape(lay.n_rows, heads, dim)
+        got_k = torch.cat([P.keys_of(k, lay, s, list(range(n - r, n))) for s, (n, r) in enumerate(zip(lay.lens, lay.rows))])
+        assert not got_q[odd_q].isfinite().any() and (got_k[odd_k] == 0).all()
+        for got, x, bad, to in ((got_q, q, odd_q, fmt), (got_k, kr, odd_k, "bf16" if fmt == "bf16" else "f16")):
+            want, bound = P.heads_of(x, dim, w, float(np.float32(eps)), pos, rotary=dim // 8 * 8)
+            # (2^-134: half a step of the smallest bf16 numbers, where a head of 1e-38 turned by a small angle ends up)
+            P.check(got[~bad], want[~bad], P.fits(bound, want, to)[~bad] + 2.0 ** -134)
