@@ -369,7 +369,7 @@ typedef struct {
  * allocate nothing, use no workspace and can be captured; calls of one handle may overlap on the GPU as long as none
  * writes a slot that another reads or writes. 0, or -1 with mynah_b200_last_error and nothing launched. What only the
  * tables show (a page or length out of range: skipped, or read as page 0), values that do not fit the cache's 16 bits
- * (not finite, or from 65504 on in f16: stored as 0; a head whose norm is out of range counts as not finite) and rows whose scores are not finite (all of them minus infinity: the
+ * (not finite, beyond 65504 in F16 rows, from 65504 on in F32 rows: stored as 0; a head whose norm is out of range counts as not finite) and rows whose scores are not finite (all of them minus infinity: the
  * result is 0; one NaN or plus infinity: it is NaN) are reported by mynah_b200_kv_sync.
  *
  * append: norm and rotation of q into q_out (which may be q itself with the same stride), of k into the cache, v into the

@@ -284,7 +284,7 @@ int mynah_b200_kv_sync(mynah_b200_kv *h, void *stream) {
     if (waits) snprintf(text[0], sizeof(text[0]), " a bounded wait inside an attention kernel ran out (code %d);", __builtin_ctz((unsigned)waits));
     if (found & 1 << ST_PAGE) snprintf(text[1], sizeof(text[1]), " a table names a page, a length or a row that does not exist;");
     if (found & 1 << ST_RANGE)
-        snprintf(text[2], sizeof(text[2]), " a value did not fit its 16 bits (f16: |v| >= 65504), or a value or a score was not finite;");
+        snprintf(text[2], sizeof(text[2]), " a value did not fit its 16 bits (f16: 65504), or a value or a score was not finite;");
     char all[480];
     const int n = snprintf(all, sizeof(all), "%s%s%s", text[0], text[1], text[2]);
     set_error("kv:%.*s", n - 1, all);

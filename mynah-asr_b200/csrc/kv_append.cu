@@ -48,9 +48,9 @@ __device__ __forceinline__ float ka_mean(float squares, float inv_d, float eps) 
 }
 
 static constexpr int KA_WARPS = 8;
-// Below what a cache value lies: from (2 - 2^-8) 2^127 on, halfway behind the largest bf16, it would round to infinity; f16 as the operand
-// planes
-static constexpr float KA_BF16_MAX = 0x1.ffp127f;
+// Below what a value lies: from (2 - 2^-8) 2^127 on, halfway behind the largest bf16, and from 65520 on, halfway behind the largest f16, it would
+// round to infinity. F32 rows end where the library's operand planes do.
+static constexpr float KA_BF16_MAX = 0x1.ffp127f, KA_F16_MAX = 65520.f;
 
 enum { KA_Q, KA_K, KA_V };
 // What a lane knows of its row: where its quads begin, cosines and sines of its pairs, the row's slot
@@ -70,7 +70,7 @@ __device__ __forceinline__ bool ka_heads(const KvAppendArgs &p, const KaLane &w,
     constexpr int OUT = KIND == KA_Q ? FMT : FMT == KV_BF16 ? KV_BF16 : KV_F16;
     typedef typename KaQuad<OUT>::type Out;
     const float *norm = KIND == KA_Q ? p.q_norm : KIND == KA_K ? p.k_norm : nullptr;
-    const float top = KIND == KA_Q && FMT == KV_F32 ? INFINITY : FMT == KV_BF16 ? KA_BF16_MAX : H16_MAX;
+    const float top = KIND == KA_Q && FMT == KV_F32 ? INFINITY : FMT == KV_BF16 ? KA_BF16_MAX : FMT == KV_F16 ? KA_F16_MAX : H16_MAX;
     float2 wt[4];
     if (KIND != KA_V && norm && w.on) {
         *reinterpret_cast<float4 *>(wt) = *reinterpret_cast<const float4 *>(norm + w.qa);

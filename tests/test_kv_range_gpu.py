@@ -280,3 +280,30 @@ def test_norms_of_large_and_small_heads(gpu_pkg, fmt, heads, kv_heads, dim, eps)
             want, bound = P.heads_of(x, dim, w, float(np.float32(eps)), pos, rotary=dim // 8 * 8)
             # (2^-134: half a step of the smallest bf16 numbers, where a head of 1e-38 turned by a small angle ends up)
             P.check(got[~bad], want[~bad], P.fits(bound, want, to)[~bad] + 2.0 ** -134)
+
+
+def test_largest_f16_values(gpu_pkg):
+    """65504 is an f16 number: rows of it go into the cache as they are. What norm or rotation brings beyond it is reported."""
+    lay = P.Layout([3], 8, [3])
+    top = 65504.0
+    x = torch.tensor([top, -top, 0.0, 1.0], device="cuda").repeat(8)[None].repeat(3, 1).half()
+    cache = gpu_pkg.KvCache(2, 2, 16, 8, lay.n_pages, fmt=gpu_pkg.F16)
+    out = torch.zeros_like(x)
+    cache.append(lay.batch(cache), x, x, x, out, stream=here())
+    cache.sync(here())
+    assert torch.equal(out, x)
+    for pool in P.pools(cache, "f16"):
+        assert torch.equal(P.keys_of(pool, lay, 0, [0, 1, 2]).reshape(3, 32), x.double())
+    one = torch.ones_like(x)
+    for weight, fits in ((65504.0, True), (65519.0, True), (65521.0, False), (1e6, False)):
+        w = np.full(16, weight, np.float32)               # (a head of ones: the weight itself, off by 2^-22 of it at most)
+        for which in ("q_norm", "k_norm"):
+            cache = gpu_pkg.KvCache(2, 2, 16, 8, lay.n_pages, fmt=gpu_pkg.F16, norm_eps=0.0, **{which: w})
+            cache.append(lay.batch(cache), one, one, one, out, stream=here())
+            if fits:
+                cache.sync(here())
+            else:
+                with pytest.raises(gpu_pkg.BackendError, match="16 bits"):
+                    cache.sync(here())
+            got = out if which == "q_norm" else P.keys_of(P.pools(cache, "f16")[0], lay, 0, [0, 1, 2])
+            assert (got == (top if fits else math.inf if which == "q_norm" else 0.0)).all()
