@@ -307,3 +307,23 @@ def test_largest_f16_values(gpu_pkg):
                     cache.sync(here())
             got = out if which == "q_norm" else P.keys_of(P.pools(cache, "f16")[0], lay, 0, [0, 1, 2])
             assert (got == (top if fits else math.inf if which == "q_norm" else 0.0)).all()
+
+
+@pytest.mark.parametrize("rows", [None, 3])
+def test_scale_of_scores_is_the_one_given(gpu_pkg, rows):
+    # 14 x 0.7419... units between the first key and 64 others, all products exact, the scale to powers of two itself an f32 number (to 3e-12). A tail
+    # probability is off by 2^-25 from its exponent, 2^-22 from the exponential, 2^-22 from its pair; the sum of 64 equal ones by 2^-23 (its hi parts
+    # add up exactly, the cut is that of adding them to the lo parts), that of all probabilities by 2^-23; a rounding: 8e-7
+    scale = 0.7419314384460449
+    lay, cache, k, v, q = led(gpu_pkg, [65], None if rows is None else [rows], 128, "f32", 14.0, 0.0)
+    cache = gpu_pkg.KvCache(1, 1, 128, 256, lay.n_pages, fmt=gpu_pkg.F32, scale=scale)
+    for to, of in zip(P.pools(cache, "f32"), (k, torch.ones_like(v))):
+        to.copy_(of)
+    P.pools(cache, "f32")[1][lay.table[0, 0].item(), :, 0] = 0
+    out = torch.zeros_like(q)
+    cache.attend(lay.batch(cache), q, out, stream=here())
+    cache.sync(here())
+    for i in range(lay.n_rows):
+        tail = (65 - lay.n_rows + i) * math.exp(-14 * scale)
+        want = tail / (1 + tail)
+        assert abs(out[i].double() - want).max() <= 8e-7 * want
