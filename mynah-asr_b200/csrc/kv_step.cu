@@ -61,7 +61,7 @@ __device__ __forceinline__ void ks_mma(float *c, const uint32_t *a, uint32_t b0,
 // kv head, head tile) of one k stand side by side in clusters, those of the largest k first, so that what takes longest begins first;
 // every warp finds its place from the lengths. Ragged batches need the long sequences cut finer than the others: 32 sequences of 100
 // to 16000 keys (8 kv heads of 128) take 72 us this way and 187 with a CTA per unit, 32 of 4096 keys 92 and 83.
-static constexpr int KS_CHUNK = 16;
+static constexpr int KS_CHUNK = 16, KS_MANY = 256;
 struct StepPlan {
     int log_size, log_even, per_seq;                 // CTAs of a cluster, see above, units of a sequence
 };
@@ -484,7 +484,11 @@ static int step_launch(const CUtensorMap &k, const CUtensorMap &v, const KvArgs 
     }
     while (log_even < 4 && units << (log_even + 1) <= 2 * sms && 1 << log_even < most_tiles) log_even++;
     log_size = log_even;
-    while (log_size < 4 && log_size < log_even + 2 && KS_CHUNK << log_size < most_tiles) log_size++;
+    // (Not where the units alone keep the GPU busy, or the lengths that every warp looks through are many: bf16, 4 query heads of 128 per kv head, a
+    // table for 32768 keys, us, cut and not: 32 sequences of 8 kv heads, 100 to 16000 keys 70, 186, 20 to 300 keys 8.4, 7.4; 192 357, 430 and 52, 22;
+    // 256 473, 517 and 77, 28, of 2 kv heads 121, 229 and 22, 11; 2048 with 2 query heads of 64 each 4918, 1643 and 2622, 145.)
+    const bool cut = a.n_seq <= KS_MANY && units <= 12 * sms;
+    while (cut && log_size < 4 && log_size < log_even + 2 && KS_CHUNK << log_size < most_tiles) log_size++;
     // Tiles ahead: two, so that three CTAs fit an SM, where there are more than two for each; three otherwise. us, with two and with three tiles
     // ahead: 20 sequences of 2000 keys (16 and 8 heads of 64, f16) 18.6, 16.3, 18 of 500 (32 and 8 of 128, bf16) 11.9, 10.9; 60 of 100 to
     // 4230 (8 heads of 64, F32 rows) 51, 60, 200 under a window of 1000 64, 68

@@ -327,3 +327,29 @@ def test_scale_of_scores_is_the_one_given(gpu_pkg, rows):
         tail = (65 - lay.n_rows + i) * math.exp(-14 * scale)
         want = tail / (1 + tail)
         assert abs(out[i].double() - want).max() <= 8e-7 * want
+
+
+@pytest.mark.parametrize("n", [257, 600, 3000])
+@pytest.mark.parametrize("fmt,heads,kv_heads,dim", [("bf16", 4, 2, 64), ("f32", 2, 1, 128)])
+def test_many_sequences(gpu_pkg, n, fmt, heads, kv_heads, dim):
+    """Steps and prompts of more sequences than a warp counts through, some of them empty, in a table with room for far longer ones."""
+    lens = [(i * 37) % 90 + (700 if i % 97 == 5 else 0) for i in range(n)]
+    for rows in (None, [min((i * 13) % 7 + (150 if i % 101 == 9 else 0), m) if i % 5 else 0 for i, m in enumerate(lens)]):
+        lay = P.Layout(lens, 16, rows, extra_rows=3, max_pages=400)
+        cache = gpu_pkg.KvCache(heads, kv_heads, dim, 16, lay.n_pages, fmt=number(gpu_pkg, fmt))
+        k, v = P.pools(cache, fmt)
+        k.copy_(randn(1, *k.shape))
+        v.copy_(randn(2, *v.shape))
+        q, kr, vr = (randn(s, lay.n_rows, w * dim).to(P.ROWS[fmt]) for s, w in ((3, heads), (4, kv_heads), (5, kv_heads)))
+        turned, out = torch.full_like(q, 7.0), torch.full_like(q, 7.0)
+        cache.append(lay.batch(cache), q, kr, vr, turned, stream=here())
+        cache.attend(lay.batch(cache), q, out, stream=here())
+        cache.sync(here())
+        full = [i for s, m in enumerate(lay.rows) for i in range(lay.begin[s], lay.begin[s] + m) if lens[s]]
+        assert torch.equal(turned[full], q[full]) and (turned[lay.real:] == 7).all() and (out[lay.real:] == 7).all()
+        want, bound = P.attend(lay, q, k, v, kv_heads, fmt=fmt)
+        P.check(out[:lay.real], want, bound)
+        for s in range(0, n, 41):
+            m = min(lay.rows[s], lens[s])
+            got = P.keys_of(v, lay, s, list(range(lens[s] - m, lens[s])))
+            assert torch.equal(got, vr[lay.begin[s]:lay.begin[s] + m].to(v.dtype).double().reshape(got.shape))
