@@ -356,7 +356,7 @@ int mynah_b200_kv_pages(const mynah_b200_kv *h, void **k, void **v);
  * and no new row needs may hold anything. kv_len[s] = 0 (one row per sequence) is an empty place: nothing is stored, its
  * result is 0. Rows behind the last sequence are left as they are. */
 typedef struct {
-    int n_seq, n_rows;                   /* n_rows: rows that the buffers hold; each at most 2^30 */
+    int n_seq, n_rows;                   /* at most 2^16 sequences, and 2^30 rows that the buffers hold */
     const int *row_off;                  /* [n_seq + 1], not decreasing, or NULL */
     const int *kv_len;                   /* [n_seq] */
     const int *page_table;               /* [n_seq][max_pages] */

@@ -123,7 +123,7 @@ int take_batch(const char *what, const mynah_b200_kv *h, const mynah_b200_kv_bat
     const mynah_b200_kv_config &c = h->cfg;
     const char *no = nullptr;
     if (b->n_seq < 0 || b->n_rows < 0) no = "a negative count";
-    else if (b->n_seq > 1 << 30 || b->n_rows > 1 << 30) no = "at most 2^30 sequences and rows";
+    else if (b->n_seq > KV_MOST_SEQ || b->n_rows > 1 << 30) no = "at most 2^16 sequences and 2^30 rows";
     else if (b->n_seq == 0 || b->n_rows == 0) return 1;
     else if (!b->kv_len || !b->page_table) no = "a null table";
     else if (b->max_pages < 1 || (int64_t)b->max_pages * c.page_size > KV_MOST) no = "max_pages x page_size is from 1 page to 2^26 positions";

@@ -11,6 +11,8 @@ enum { KV_F32 = 0, KV_F16 = 1, KV_BF16 = 2 };       // rows; the cache holds f16
 
 // Positions of a sequence: sums with a window, a tile or a page stay in 32 bits, and a block's work within the kernels' limit on waits
 static constexpr int KV_MOST = 1 << 26;
+// Sequences of a call: what a warp that looks for its work passes over stays within the limit on waits, too
+static constexpr int KV_MOST_SEQ = 1 << 16;
 
 // Pools are [page][kv head][slot][D], 16 bits a value: the keys of one head in one page are one run of memory.
 struct KvArgs {
@@ -139,12 +141,13 @@ __device__ __forceinline__ int kv_find_seq(const KvArgs &a, int r, int lane) {
     }
     return lo < a.n_seq ? lo : -1;
 }
-// Reports sequences whose tables contradict the call (rows are found from the offsets, so a row may miss that they decrease)
-__device__ __forceinline__ void kv_look_over(const KvArgs &a, int lane) {
+// Reports sequences whose tables contradict the call (rows are found from the offsets, so a row may miss that they decrease): the warp's share of
+// them, one of `of`
+__device__ __forceinline__ void kv_look_over(const KvArgs &a, int lane, int which, int of) {
     bool bad = false;
-    for (int s = lane; s < a.n_seq; s += 32) {
+    for (int64_t s = (int64_t)which * 32 + lane; s < a.n_seq; s += (int64_t)of * 32) {
         KvSeq q;
-        bad |= !kv_seq(a.row_off, a.kv_len, s, a.n_rows, kv_capacity(a), &q);
+        bad |= !kv_seq(a.row_off, a.kv_len, (int)s, a.n_rows, kv_capacity(a), &q);
     }
     if (bad) kv_report(a, ST_PAGE);
 }

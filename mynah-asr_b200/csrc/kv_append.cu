@@ -162,7 +162,7 @@ kv_append_kernel(const KvAppendArgs p, int per_part) {
     chain_trigger();
     chain_wait();
     const int row = (int)blockIdx.x * KA_WARPS + (int)(threadIdx.x >> 5);
-    if (row == 0 && blockIdx.y == 0 && a.row_off) kv_look_over(a, lane);
+    if (blockIdx.y == 0 && a.row_off) kv_look_over(a, lane, row, (int)gridDim.x * KA_WARPS);
     if (row >= a.n_rows) return;
     KaLane w;
     const int l = lane % LPH;

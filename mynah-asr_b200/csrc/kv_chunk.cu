@@ -118,7 +118,8 @@ __device__ __forceinline__ uint64_t kc_desc_mn(uint32_t addr) {
 // Where the TMA warp finds the call's blocks: all their number, and the x-th from the last, since later positions see more keys and
 // what takes longest should begin first. With up to 32 sequences a lane keeps one, and the x-th longest is found, too: by bisection of
 // the length that more than x blocks have (with it the third and fourth case above took 58.8 and 37.6 us, with the order of the sequences
-// 63.4 and 46.2).
+// 63.4 and 46.2). Up to 256 are counted through, 32 at a time; with more, see KcMany.
+static constexpr int KC_LANES = 32, KC_COUNT = 256;
 struct KcFinder {
     int per_block, total, mine;                      // rows of a block, blocks of the call, blocks of the lane's sequence
     KvSeq q;
@@ -127,7 +128,8 @@ struct KcFinder {
         if (s < a.n_seq) *bad |= !kv_seq(a.row_off, a.kv_len, s, a.n_rows, kv_capacity(a), &q);
         mine = (q.n + per_block - 1) / per_block;
     }
-    __device__ __forceinline__ void init(const KvArgs &a, int per, int lane) {
+    // most: blocks of tables that are in order. Rows that several sequences claim make no more than that.
+    __device__ __forceinline__ void init(const KvArgs &a, int per, int most, int lane) {
         per_block = per; total = 0;
         bool bad = false;
         for (int s0 = 0; s0 < a.n_seq; s0 += 32) {
@@ -135,6 +137,7 @@ struct KcFinder {
             total += __reduce_add_sync(0xffffffffu, mine);
         }
         if (bad) kv_report(a, ST_PAGE);
+        total = min(total, most);
     }
     // Blocks of the lane's sequence with `tiles` tiles of keys at least: those from some place on (a window bounds all alike)
     __device__ __forceinline__ int as_long(const KvArgs &a, int tiles) const {
@@ -171,7 +174,7 @@ struct KcFinder {
         if (nth < 0) return;
         bool bad = false;
         for (int s0 = 0; s0 < a.n_seq; s0 += 32) {
-            if (a.n_seq > 32) look(a, s0 + lane, &bad);
+            if (a.n_seq > KC_LANES) look(a, s0 + lane, &bad);
             const int n = mine;
             int upto = n;
 #pragma unroll
@@ -193,6 +196,35 @@ struct KcFinder {
         }
     }
 };
+
+// The same where counting takes long: block i of sequence s has the number row_off[s] / per_block + s + i, which no other block has, so a sequence is
+// found by bisection of the offsets, and numbers without a block are passed over. (Sequences of 5 to 40 rows, us, counted through and this
+// way: 300 65, 66, 1000 302, 192, 4000 3600, 740.)
+struct KcMany {
+    int per_block, total;
+    __device__ __forceinline__ void init(const KvArgs &, int per, int most, int) { per_block = per; total = most; }
+    __device__ __forceinline__ void find(const KvArgs &a, int x, int lane, int *seq, int *block, KvSeq *at) const {
+        const int nth = total - 1 - x;
+        *seq = -1; *block = 0; *at = {0, 0, 0};
+        if (nth < 0) return;
+        // the last sequence whose first number is nth at most: each round looks at 32 places of what is left
+        int lo = 0, hi = a.n_seq;
+        while (hi - lo > 1) {
+            const int step = (hi - lo + 31) / 32, place = min(lo + lane * step, hi - 1);
+            const unsigned below = __ballot_sync(0xffffffffu, lo + lane * step < hi && a.row_off[place] / per_block + place <= nth);
+            if (below == 0) return;
+            lo += (31 - __clz(below)) * step;
+            hi = min(hi, lo + step);
+        }
+        KvSeq s;
+        const int i = nth - a.row_off[lo] / per_block - lo;
+        if (!kv_seq(a.row_off, a.kv_len, lo, a.n_rows, kv_capacity(a), &s) || i < 0 || i >= (s.n + per_block - 1) / per_block) return;
+        *seq = lo; *block = i; *at = s;
+    }
+};
+
+template <bool MANY> struct KcFind { typedef KcFinder Type; };
+template <> struct KcFind<true> { typedef KcMany Type; };
 
 // What a block is to those who work on it. The TMA warp finds it out and leaves it as words in shared memory.
 struct KcBlock {
@@ -249,10 +281,10 @@ __device__ __forceinline__ void kc_quads(uint32_t *w, int lane) {
     }
 }
 
-template <int DP, int FMT>
+template <int DP, int FMT, bool MANY>
 __global__ void __launch_bounds__(ChunkShape<DP, FMT>::THREADS, ChunkShape<DP, FMT>::PER_SM)
 kv_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const KvArgs a,
-                int box_rows, int log_size, int longest_first, int tq, uint32_t inv_g) {
+                int box_rows, int log_size, int longest_first, int tq, uint32_t inv_g, int most) {
     using Sh = ChunkShape<DP, FMT>;
     constexpr bool BF = FMT == KV_BF16, F32 = FMT == KV_F32, OWN_P = Sh::OWN_P;
     constexpr int STAGES = Sh::STAGES, TILES = Sh::TILES, SPLIT = Sh::SPLIT, OWN = Sh::OWN, GROUPS = OWN / 32;
@@ -331,15 +363,23 @@ kv_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
         const int b_half = lane % Sh::HALVES, b_sub = lane / Sh::HALVES;
         const uint32_t b_at = b_half * KC_HALF + b_sub * box_rows * 128;
         int x = (int)(blockIdx.x >> log_size), nth = x / a.Hkv;
-        KcFinder finder;
-        finder.init(a, TILES * tq, lane);
+        typename KcFind<MANY>::Type finder;
+        finder.init(a, TILES * tq, most, lane);
         int s = 0, ph = 0, r = 0, queries = 0;                 // place in the ring, its parity, requests; blocks with queries so far
         bool ok = true;
         for (int j = 0, x0 = 0; ok; j++) {
             if (j >= 2 && !mbar_wait_warp(&i_empty[j & 1], (uint32_t)(((j >> 1) & 1) ^ 1))) { ok = false; break; }
             int seq, block;
             KvSeq sq;
-            if (longest_first) finder.find_longest(a, nth, lane, &seq, &block, &sq);
+            if constexpr (MANY) {
+                for (;;) {
+                    finder.find(a, nth, lane, &seq, &block, &sq);
+                    if (seq >= 0 || nth >= most || once) break;
+                    x0 += (int)gridDim.x;                      // a number without a block
+                    x = x0 + (int)blockIdx.x;
+                    nth = x / a.Hkv;
+                }
+            } else if (longest_first) finder.find_longest(a, nth, lane, &seq, &block, &sq);
             else finder.find(a, nth, lane, &seq, &block, &sq);
             KcBlock b;
             b.make(a, seq, block, x - nth * a.Hkv, sq, tq, TILES, size, rank);
@@ -392,6 +432,7 @@ kv_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
             nth = x / a.Hkv;
         }
         if (!ok && lane == 0) kv_report(a, ST_TIMEOUT_PRODUCER);
+        if (MANY) kv_look_over(a, lane, (int)blockIdx.x, (int)gridDim.x);
         for (int u = 0; u < STAGES && u < r; u++) {            // what was asked for has to land before the CTA leaves
             if (s == 0) { s = STAGES; ph ^= 1; }
             if (!mbar_wait_warp(&full[--s], (uint32_t)ph)) break;
@@ -845,7 +886,7 @@ kv_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
 }
 
 // Clusters of 2^k CTAs that run at a time on the current device with a CTA per SM; -1 with the error set
-template <int DP, int FMT>
+template <int DP, int FMT, bool MANY>
 static int most_clusters(int k) {
     using Sh = ChunkShape<DP, FMT>;
     static PerDevice known[5] = {};                            // (the number and one)
@@ -858,15 +899,15 @@ static int most_clusters(int k) {
     lc.gridDim = dim3(1u << k); lc.blockDim = dim3(Sh::THREADS); lc.dynamicSmemBytes = Sh::SMEM;
     lc.attrs = at; lc.numAttrs = 1;
     int n = 0;
-    MB_CUDA(cudaOccupancyMaxActiveClusters(&n, kv_chunk_kernel<DP, FMT>, &lc));
+    MB_CUDA(cudaOccupancyMaxActiveClusters(&n, kv_chunk_kernel<DP, FMT, MANY>, &lc));
     known[k].record(dev, (size_t)n + 1);
     return n;
 }
 
-template <int DP, int FMT>
+template <int DP, int FMT, bool MANY>
 static int chunk_launch(const CUtensorMap &k, const CUtensorMap &v, const KvArgs &a, int box_rows, cudaStream_t st) {
     using Sh = ChunkShape<DP, FMT>;
-    auto kernel = kv_chunk_kernel<DP, FMT>;
+    auto kernel = kv_chunk_kernel<DP, FMT, MANY>;
     static PerDevice configured = {};
     int dev = 0;
     if (configured.below((size_t)Sh::SMEM, &dev)) {
@@ -880,13 +921,13 @@ static int chunk_launch(const CUtensorMap &k, const CUtensorMap &v, const KvArgs
     const int tq = KC_ROWS / a.G, per_block = Sh::TILES * tq;                  // positions of a tile of rows, of a block
     const uint32_t inv_g = (65536u + a.G - 1) / a.G;           // x / G = x inv_g / 2^16 for x < 256, G <= 64
     const int64_t full = ((int64_t)a.n_rows + per_block - 1) / per_block, seqs = a.n_seq < a.n_rows ? a.n_seq : a.n_rows;
-    const int64_t blocks = (a.n_rows / per_block + seqs) * a.Hkv;              // the last block of each sequence may be short
+    const int64_t most = a.n_rows / per_block + (MANY ? a.n_seq : seqs), blocks = most * a.Hkv;      // the last block of each sequence may be short
     // Clusters where the blocks that are likely (whole ones, or one per sequence) leave SMs without work: the largest of which as many
     // run at a time (with one CTA per SM a GPU of 148 has room for fewer than eight clusters of 16)
     const int64_t likely = (full > seqs ? full : seqs) * a.Hkv;
     int log_size = 0;
     for (int k = 1; k <= 4 && (int64_t)KC_KEYS << k < ((int64_t)a.max_pages << a.page_shift); k++) {
-        const int most = most_clusters<DP, FMT>(k);
+        const int most = most_clusters<DP, FMT, MANY>(k);
         if (most < 0) return -1;
         if (likely <= (int64_t)Sh::PER_SM * most) log_size = k;
     }
@@ -895,24 +936,31 @@ static int chunk_launch(const CUtensorMap &k, const CUtensorMap &v, const KvArgs
     // 141, 172, 2 x 4000 237, 270, 8000 440, 460, 9 of 300 to 8000 550, 640). With more sequences than lanes, where the lengths are not
     // put in order, only blocks that are short: the hardware deals out long ones better (40 of 100 to 8000 F32 rows 1723, 1645)
     const int64_t keys = (int64_t)a.max_pages << a.page_shift, seen = (int64_t)a.window + a.sinks + per_block;
-    const bool stay = a.n_seq <= 32 || (a.window > 0 && seen < keys ? seen : keys) <= KC_STAY;
+    const bool stay = a.n_seq <= KC_LANES || (a.window > 0 && seen < keys ? seen : keys) <= KC_STAY;
     const int64_t room = (int64_t)Sh::PER_SM * device_sm_count();
     const int64_t ctas = log_size ? blocks << log_size : stay && blocks > room ? room : blocks;
-    const bool longest_first = blocks > room && a.n_seq <= 32;
+    const bool longest_first = !MANY && blocks > room && a.n_seq <= KC_LANES;
     CUtensorMap q = k;
     if (FMT != KV_F32 && !kv_rows_map(&q, a, FMT == KV_BF16)) { set_error("kv_attend: no tensor map of the rows"); return -1; }
     MB_CUDA(launch_kernel(kernel, dim3((unsigned)ctas), dim3(Sh::THREADS), (size_t)Sh::SMEM, st, true, 1 << log_size, q, k, v, a, box_rows, log_size, longest_first ? 1 : 0,
-                          tq, inv_g));
+                          tq, inv_g, (int)most));
     note_launch();
     return 0;
 }
 
+template <int DP, int FMT>
+static int chunk_find(const CUtensorMap &k, const CUtensorMap &v, const KvArgs &a, int box_rows, cudaStream_t st) {
+    // (up to here 256 sequences that all claim all rows have fewer blocks than 31 bits)
+    const bool many = a.n_seq > KC_COUNT || a.n_rows >= 1 << 22;
+    return many ? chunk_launch<DP, FMT, true>(k, v, a, box_rows, st) : chunk_launch<DP, FMT, false>(k, v, a, box_rows, st);
+}
+
 int kv_chunk(const CUtensorMap &k, const CUtensorMap &v, const KvArgs &a, int box_rows, int fmt, cudaStream_t st) {
     if (a.D <= 64)
-        return fmt == KV_F32 ? chunk_launch<64, KV_F32>(k, v, a, box_rows, st) : fmt == KV_F16 ? chunk_launch<64, KV_F16>(k, v, a, box_rows, st)
-                                                                                          : chunk_launch<64, KV_BF16>(k, v, a, box_rows, st);
-    return fmt == KV_F32 ? chunk_launch<128, KV_F32>(k, v, a, box_rows, st) : fmt == KV_F16 ? chunk_launch<128, KV_F16>(k, v, a, box_rows, st)
-                                                                                       : chunk_launch<128, KV_BF16>(k, v, a, box_rows, st);
+        return fmt == KV_F32 ? chunk_find<64, KV_F32>(k, v, a, box_rows, st) : fmt == KV_F16 ? chunk_find<64, KV_F16>(k, v, a, box_rows, st)
+                                                                                        : chunk_find<64, KV_BF16>(k, v, a, box_rows, st);
+    return fmt == KV_F32 ? chunk_find<128, KV_F32>(k, v, a, box_rows, st) : fmt == KV_F16 ? chunk_find<128, KV_F16>(k, v, a, box_rows, st)
+                                                                                     : chunk_find<128, KV_BF16>(k, v, a, box_rows, st);
 }
 
 }  // namespace mb

@@ -117,6 +117,11 @@ def test_kv_host(fake_runtime, name):  # noqa: F811
     assert r.returncode == 0, r.stdout + r.stderr
 
 
+@pytest.mark.parametrize("name", ["kv_limits"])
+def test_kv_host_limits(fake_runtime, name):  # noqa: F811
+    test_kv_host(fake_runtime, name)
+
+
 def _config(pkg, **more):
     c = pkg.KvConfig()
     pkg.lib().mynah_b200_kv_config_default(C.byref(c))
@@ -244,6 +249,24 @@ def kv_failed_calls(pkg, fake):
         assert call() == 0
     fake.fake_fail(b"cudaMemcpyAsync", 1)
     assert L.mynah_b200_kv_sync(h, None) == -1 and L.mynah_b200_kv_sync(h, None) == 0
+    L.mynah_b200_kv_free(h)
+
+
+@scenario
+def kv_limits(pkg, fake):
+    """As many sequences as a warp can look through within the limit on waits, and not one more."""
+    L = pkg.lib()
+    h = L.mynah_b200_kv_create(C.byref(_config(pkg)))
+    lens, table, off, rows = _dev(4 << 16), _dev(4 << 18), _dev((4 << 16) + 4), _dev(256)
+    seen = []
+    cb = LAUNCH(lambda name, args, recorded: seen.append(name))
+    fake.fake_on_launch(cb)
+    for n, row_off, n_rows, ok in ((1 << 16, off, 1, True), (1 << 16, None, 1 << 16, True), ((1 << 16) + 1, off, 1, False), ((1 << 16) + 1, None, 1 << 17, False)):
+        b, before = _batch(pkg, n_seq=n, n_rows=n_rows, row_off=row_off, kv_len=lens, page_table=table, max_pages=4), len(seen)
+        for call in (lambda: L.mynah_b200_kv_append(h, C.addressof(b), *([rows, 256] * 4), None), lambda: L.mynah_b200_kv_attend(h, C.addressof(b), rows, 256, rows, 256, None)):
+            assert call() == (0 if ok else -1)
+            assert ok or b"sequences" in L.mynah_b200_last_error()
+        assert len(seen) == before + 2 * ok
     L.mynah_b200_kv_free(h)
 
 

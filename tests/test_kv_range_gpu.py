@@ -353,3 +353,45 @@ def test_many_sequences(gpu_pkg, n, fmt, heads, kv_heads, dim):
             m = min(lay.rows[s], lens[s])
             got = P.keys_of(v, lay, s, list(range(lens[s] - m, lens[s])))
             assert torch.equal(got, vr[lay.begin[s]:lay.begin[s] + m].to(v.dtype).double().reshape(got.shape))
+
+
+@pytest.mark.parametrize("n", [6, 30, 200, 300])
+def test_rows_that_many_sequences_claim(gpu_pkg, n):
+    """Offsets that go back and forth, so that every second sequence has all rows: reported, no more work than a table in order has, and the next
+    call as if nothing had been."""
+    lay = P.Layout([500] * n, 16, [1] * n, extra_rows=900)
+    cache = gpu_pkg.KvCache(4, 2, 64, 16, lay.n_pages, fmt=gpu_pkg.BF16)
+    k, v = P.pools(cache, "bf16")
+    k.copy_(randn(1, *k.shape))
+    v.copy_(randn(2, *v.shape))
+    wide = randn(3, lay.n_rows + 40, 256).bfloat16()
+    q, out = wide[20:-20], torch.full_like(wide, 7.0)
+    off = torch.tensor([lay.n_rows * (i % 2) for i in range(n + 1)], dtype=torch.int32, device="cuda")
+    batch = cache.batch(lay.len_dev, lay.table_dev, row_off=off, n_rows=lay.n_rows)
+    cache.attend(batch, q, out[20:-20], stream=here())
+    with pytest.raises(gpu_pkg.BackendError, match="does not exist"):
+        cache.sync(here())
+    assert (out[:20] == 7).all() and (out[-20:] == 7).all()
+    cache.append(batch, q, q[:, :128], q[:, :128], out[20:-20], stream=here())
+    with pytest.raises(gpu_pkg.BackendError, match="does not exist"):
+        cache.sync(here())
+    assert (out[:20] == 7).all() and (out[-20:] == 7).all()
+    cache.attend(lay.batch(cache), q, out[20:-20], stream=here())
+    cache.sync(here())
+    want, bound = P.attend(lay, q, k, v, 2, fmt="bf16")
+    P.check(out[20:20 + lay.real], want, bound)
+
+
+def test_prompts_in_buffers_of_many_rows(gpu_pkg):
+    lay = P.Layout([300, 0, 4000], 16, [300, 0, 700], extra_rows=2 ** 22)
+    cache = gpu_pkg.KvCache(2, 1, 16, 16, lay.n_pages, fmt=gpu_pkg.BF16)
+    k, v = P.pools(cache, "bf16")
+    k.copy_(randn(1, *k.shape))
+    v.copy_(randn(2, *v.shape))
+    q = randn(3, lay.n_rows, 32).bfloat16()
+    out = torch.full_like(q, 7.0)
+    cache.attend(lay.batch(cache), q, out, stream=here())
+    cache.sync(here())
+    want, bound = P.attend(lay, q, k, v, 1, fmt="bf16")
+    P.check(out[:lay.real], want, bound)
+    assert (out[lay.real:] == 7).all()
