@@ -14,6 +14,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import sys
 
 import numpy as np
 
@@ -428,7 +429,10 @@ class KvBatch:
 
 class KvCache:
     """Paged key/value cache of one decoder layer on the current device (mynah_b200_kv). Tensors are anything with torch's
-    data_ptr, shape, stride, dtype, device and is_cuda; row tensors are [rows, heads * head_dim], a row's values side by side."""
+    data_ptr, shape, stride, dtype, device and is_cuda; row tensors are [rows, heads * head_dim], a row's values side by side.
+
+    stream is an integer handle as torch gives it (0: the legacy default stream), or None for torch's current stream of the cache's device, the one
+    that its tensors are written and freed on (without torch: the handle's own, which waits for no other)."""
 
     def __init__(self, n_heads, n_kv_heads, head_dim, page_size, n_pages, fmt=F32, rotary_dim=0, interleaved=False, rope_theta=10000.0,
                  inv_freq=None, q_norm=None, k_norm=None, norm_eps=1e-6, window=0, n_sinks=0, scale=0.0):
@@ -451,6 +455,8 @@ class KvCache:
         self.n_heads, self.n_kv_heads, self.head_dim, self.page_size, self.n_pages, self.fmt = n_heads, n_kv_heads, head_dim, page_size, n_pages, fmt
         self._dtype = {F32: "torch.float32", F16: "torch.float16", BF16: "torch.bfloat16"}[fmt]
         self._q_width, self._kv_width = n_heads * head_dim, n_kv_heads * head_dim
+        torch = sys.modules.get("torch")
+        self._current = None if torch is None else (lambda device=torch.cuda.current_device(): torch.cuda.current_stream(device).cuda_stream)
         self._append, self._attend = lib().mynah_b200_kv_append, lib().mynah_b200_kv_attend
 
     def close(self):
@@ -483,26 +489,30 @@ class KvCache:
             return self._rows(t, width, batch, what)
         raise ValueError(f"{what} is a {self._dtype} tensor [at least {batch.n_rows} rows, {width}] on the batch's device, each row's values side by side")
 
+    def _stream(self, stream):
+        if stream is None and self._current is not None:
+            stream = self._current()
+        return 1 if stream == 0 else stream
+
     def append(self, batch, q, k, v, q_out, stream=None):
-        """Norm and rotation of the rows; q to q_out, k and v to their slots. stream: an integer handle as torch gives it (0: the
-        legacy default stream), or None for the handle's own. Asynchronous."""
+        """Norm and rotation of the rows; q to q_out, k and v to their slots. Asynchronous on `stream`."""
         a, lda = self._rows(q, self._q_width, batch, "q")
         b, ldb = self._rows(k, self._kv_width, batch, "k")
         c, ldc = self._rows(v, self._kv_width, batch, "v")
         o, ldo = self._rows(q_out, self._q_width, batch, "q_out")
-        if self._append(self.h, batch.at, a, lda, b, ldb, c, ldc, o, ldo, 1 if stream == 0 else stream):
+        if self._append(self.h, batch.at, a, lda, b, ldb, c, ldc, o, ldo, stream or self._stream(stream)):
             raise BackendError("kv_append: " + _err())
 
     def attend(self, batch, q, out, stream=None):
-        """Attention of the batch's rows over the visible keys of their sequences, into out. Asynchronous, as append."""
+        """Attention of the batch's rows over the visible keys of their sequences, into out. Asynchronous on `stream`."""
         a, lda = self._rows(q, self._q_width, batch, "q")
         o, ldo = self._rows(out, self._q_width, batch, "out")
-        if self._attend(self.h, batch.at, a, lda, o, ldo, 1 if stream == 0 else stream):
+        if self._attend(self.h, batch.at, a, lda, o, ldo, stream or self._stream(stream)):
             raise BackendError("kv_attend: " + _err())
 
     def sync(self, stream=None):
-        """Waits, and raises for what the calls since the last sync have found."""
-        _check(lib().mynah_b200_kv_sync(self.h, 1 if stream == 0 else stream), "kv_sync")
+        """Waits for `stream`, and raises for what the calls since the last sync have found."""
+        _check(lib().mynah_b200_kv_sync(self.h, stream or self._stream(stream)), "kv_sync")
 
 
 class QMat:

@@ -395,3 +395,39 @@ def test_prompts_in_buffers_of_many_rows(gpu_pkg):
     want, bound = P.attend(lay, q, k, v, 1, fmt="bf16")
     P.check(out[:lay.real], want, bound)
     assert (out[lay.real:] == 7).all()
+
+
+def test_calls_without_a_stream_follow_the_tensors(gpu_pkg):
+    """Without a stream, a call is one of torch's current stream: it waits for what writes its rows, and its results are there for what comes next."""
+    lay = P.Layout([300, 40], 16, [64, 40])
+    cache, side = gpu_pkg.KvCache(4, 2, 64, 16, lay.n_pages, fmt=gpu_pkg.BF16, rotary_dim=64), torch.cuda.Stream()
+    k, v = P.pools(cache, "bf16")
+    k.copy_(randn(1, *k.shape))
+    v.copy_(randn(2, *v.shape))
+    x = randn(3, lay.n_rows, 512).bfloat16()
+    batch, want, turned, out, late = lay.batch(cache), torch.zeros_like(x[:, :256]), torch.zeros_like(x[:, :256]), torch.zeros_like(x[:, :256]), torch.zeros_like(x)
+    cache.append(batch, x[:, :256], x[:, 256:384], x[:, 384:], turned, stream=here())
+    cache.attend(batch, turned, want, stream=here())
+    cache.sync(here())
+    for pool in (k, v):
+        pool[lay.table[1, :3].long().cuda()] = 0
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(20_000_000)                     # 10 ms
+        late.copy_(x)
+        cache.append(batch, late[:, :256], late[:, 256:384], late[:, 384:], turned)
+        cache.attend(batch, turned, out)
+        copy = out.clone()
+        cache.sync()
+        assert torch.equal(out, want)                     # (the sync has waited)
+    assert torch.equal(copy, want)
+    graph = torch.cuda.CUDAGraph()
+    out.zero_()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        cache.attend(batch, turned, out)
+    torch.cuda.synchronize()
+    assert (out == 0).all()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)
