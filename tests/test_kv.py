@@ -104,6 +104,18 @@ def test_groups_cover_what_is_seen(index):
     assert index.groups(top - 5, top, 64, 4, out, 4096) in (3, 4) and index.groups(0, top, 2 ** 26, 2 ** 26, out, 4096) == 2 ** 21
 
 
+def test_integration_example(tmp_path):
+    """The layer shown to hosts is C that compiles against the header, and waits wherever rows pass from one stream to another."""
+    with open(os.path.join(HERE, "..", "INTEGRATION.md")) as f:
+        code = f.read().split("## 4b.")[1].split("```c\n")[1].split("```")[0]
+    (tmp_path / "layer.c").write_text('#include <stdio.h>\n#include "mynah_b200.h"\nvoid layer(const mynah_b200_qmat *w_qkv, const mynah_b200_qmat *w_out, '
+                                      "const float *h, float *x, float *q, float *y, long long ld, int n_seq, int n_rows, const int *row_off, const int *kv_len, "
+                                      "const int *page_table, int max_pages, void *stream) {\n" + code + "}\n")
+    subprocess.run(["gcc", "-std=c11", "-Wall", "-Werror", "-fsyntax-only", "-I", os.path.join(HERE, "..", "include"), str(tmp_path / "layer.c")], check=True)
+    calls = [line.split("mynah_b200_")[1].split("(")[0] for line in code.splitlines() if "bad |" in line or "int bad" in line]
+    assert calls == ["qmat_mul_device", "qmat_sync", "kv_append", "kv_attend", "kv_sync", "qmat_mul_device", "qmat_sync"]
+
+
 # ------------------------------------------------------------------------------------------- in the child process
 def scenario(f):
     SCENARIOS[f.__name__] = f
