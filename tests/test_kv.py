@@ -116,6 +116,22 @@ def test_integration_example(tmp_path):
     assert calls == ["qmat_mul_device", "qmat_sync", "kv_append", "kv_attend", "kv_sync", "qmat_mul_device", "qmat_sync"]
 
 
+def test_registers_are_looked_at_by_the_build():
+    """A compiler that gives the prompts' kernel another number of registers than it deals out is found by the build."""
+    from importlib.util import module_from_spec, spec_from_file_location
+    spec = spec_from_file_location("mynah_build", os.path.join(HERE, "..", "mynah-asr_b200", "build.py"))
+    build = module_from_spec(spec)
+    spec.loader.exec_module(build)
+    report = "".join("ptxas info    : Compiling entry function '_ZN2mb15kv_chunk_kernelILi%dELi%dELb0EEEv' for 'sm_100a'\nptxas info    : Function properties for x\n"
+                     "    0 bytes stack frame\nptxas info    : Used %d registers, used 1 barriers\n" % (d, f, {64: 128, 128: 168}[d]) for d in (64, 128) for f in range(3))
+    assert build.missing_registers("kv_chunk.cu", report) == [] and build.missing_registers("kv.cu", "") == []
+    assert len(build.missing_registers("kv_chunk.cu", report.replace("168", "160", 1))) == 1
+    assert len(build.missing_registers("kv_chunk.cu", report.replace("128 registers", "126 registers"))) == 3
+    assert len(build.missing_registers("kv_chunk.cu", "")) == 2
+    with open(os.path.join(build.CSRC, "kv_chunk.cu")) as f:
+        assert "REGS = SOFT == 8 ? 168 : 128" in f.read()
+
+
 # ------------------------------------------------------------------------------------------- in the child process
 def scenario(f):
     SCENARIOS[f.__name__] = f
