@@ -372,13 +372,13 @@ typedef struct {
  * (not finite, beyond 65504 in F16 rows, from 65504 on in F32 rows: stored as 0; a head whose norm is out of range counts as not finite) and rows whose scores are not finite (all of them minus infinity: the
  * result is 0; one NaN or plus infinity: it is NaN) are reported by mynah_b200_kv_sync.
  *
- * append: norm and rotation of q into q_out (which may be q itself with the same stride), of k into the cache, v into the
+ * append: norm and rotation of q into q_out (which may be q itself with the same stride, and shares no values with k or v), of k into the cache, v into the
  * cache as it is. Rows whose position is below 0 (more rows than keys) are skipped. A slot that two rows of a call name
  * ends up with a mix of the two. */
 int mynah_b200_kv_append(mynah_b200_kv *h, const mynah_b200_kv_batch *b, const void *q, long long ldq, const void *k, long long ldk,
                          const void *v, long long ldv, void *q_out, long long ldqo, void *stream);
 /* attend: out = softmax over the visible keys of scale q . k, times their values; 0 for a row that sees none. q as
- * append left it in q_out; out may be q itself with the same stride. How the keys of a sequence are cut into parts that
+ * append left it in q_out; out may be q itself with the same stride, and shares no values with it otherwise. How the keys of a sequence are cut into parts that
  * are summed and joined depends on n_seq, n_rows and max_pages and on the sequence itself, never on the others, and no
  * sum on what ran first: the same call gives the same bits. F32 rows: queries are kept to 2^-25 absolutely or 2^-22
  * relatively, whichever is more, and lie below 65504; scores are sums that the

@@ -118,6 +118,18 @@ const char *refuse_rows(const mynah_b200_kv *h, const void *p, long long ld, int
     return nullptr;
 }
 
+// Whether rows that are written share values with rows that are read, other than by being the same ones: one row's result would be read as
+// another's input. `n` rows of `width` values, `size` bytes each.
+bool clash(const void *out, long long ldo, int wo, const void *in, long long ldi, int wi, int n, int size) {
+    if (out == in && ldo == ldi) return false;
+    const uintptr_t o = (uintptr_t)out, i = (uintptr_t)in;
+    if (o + ((uintptr_t)(n - 1) * ldo + wo) * size <= i || i + ((uintptr_t)(n - 1) * ldi + wi) * size <= o) return false;
+    if (ldo != ldi) return true;
+    // side by side in wider rows: the columns where those behind begin
+    const uintptr_t ld = (uintptr_t)ldo * size, ahead = (o > i ? o - i : i - o) % ld, first = (uintptr_t)(o > i ? wi : wo) * size, second = (uintptr_t)(o > i ? wo : wi) * size;
+    return ahead < first || ahead + second > ld;
+}
+
 // 1: nothing to do, 0: go on, -1: refused
 int take_batch(const char *what, const mynah_b200_kv *h, const mynah_b200_kv_batch *b, KvArgs *a) {
     const mynah_b200_kv_config &c = h->cfg;
@@ -240,6 +252,10 @@ int mynah_b200_kv_append(mynah_b200_kv *h, const mynah_b200_kv_batch *b, const v
     if (!no) no = refuse_rows(h, k, ldk, p.a.Hkv * D);
     if (!no) no = refuse_rows(h, v, ldv, p.a.Hkv * D);
     if (!no) no = refuse_rows(h, q_out, ldqo, p.a.H * D);
+    const int n = p.a.n_rows, size = row_bytes(h->fmt);
+    if (!no && (clash(q_out, ldqo, p.a.H * D, q, ldq, p.a.H * D, n, size) || clash(q_out, ldqo, p.a.H * D, k, ldk, p.a.Hkv * D, n, size) ||
+                clash(q_out, ldqo, p.a.H * D, v, ldv, p.a.Hkv * D, n, size)))
+        no = "q_out overlaps rows that are read";
     if (no) { set_error("kv_append: %s", no); return -1; }
     p.a.q = q; p.a.ldq = ldq; p.a.out = q_out; p.a.ldo = ldqo;
     p.k_rows = k; p.ldk = ldk; p.v_rows = v; p.ldv = ldv;
@@ -257,6 +273,7 @@ int mynah_b200_kv_attend(mynah_b200_kv *h, const mynah_b200_kv_batch *b, const v
     if (go) return go < 0 ? -1 : 0;
     const char *no = refuse_rows(h, q, ldq, a.H * a.D);
     if (!no) no = refuse_rows(h, out, ldo, a.H * a.D);
+    if (!no && clash(out, ldo, a.H * a.D, q, ldq, a.H * a.D, a.n_rows, row_bytes(h->fmt))) no = "out overlaps rows that are read";
     if (no) { set_error("kv_attend: %s", no); return -1; }
     a.q = q; a.ldq = ldq; a.out = out; a.ldo = ldo;
     const cudaStream_t st = stream ? (cudaStream_t)stream : h->stream;

@@ -145,7 +145,7 @@ def test_kv_host(fake_runtime, name):  # noqa: F811
     assert r.returncode == 0, r.stdout + r.stderr
 
 
-@pytest.mark.parametrize("name", ["kv_limits"])
+@pytest.mark.parametrize("name", ["kv_limits", "kv_overlaps"])
 def test_kv_host_limits(fake_runtime, name):  # noqa: F811
     test_kv_host(fake_runtime, name)
 
@@ -295,6 +295,26 @@ def kv_limits(pkg, fake):
             assert call() == (0 if ok else -1)
             assert ok or b"sequences" in L.mynah_b200_last_error()
         assert len(seen) == before + 2 * ok
+    L.mynah_b200_kv_free(h)
+
+
+@scenario
+def kv_overlaps(pkg, fake):
+    """Results that would be read as other rows' input are refused; the same rows, and columns side by side, are not."""
+    L = pkg.lib()
+    h = L.mynah_b200_kv_create(C.byref(_config(pkg)))                # rows of 256 and 128 f32 values
+    lens, table, at = _dev(64), _dev(256), _dev(1 << 16) + (1 << 14)
+    b = _batch(pkg, n_seq=3, n_rows=3, kv_len=lens, page_table=table)
+    far = _dev(1 << 14)
+    for ld, out, ldo, ok in ((256, at, 256, True), (512, at, 512, True), (512, at + 256 * 4, 512, True), (512, at - 256 * 4, 512, True), (256, at + 3 * 1024, 256, True),
+                             (256, at - 3 * 1024, 256, True), (256, far, 512, True), (512, at + 2 * 2048 + 1024, 256, True),
+                             (256, at + 16, 256, False), (256, at + 1024, 256, False), (256, at - 2048, 256, False), (512, at + 255 * 4 - 12, 512, False),
+                             (512, at + 257 * 4 - 4 + 16, 512, False), (256, at, 512, False), (512, at + 2048, 256, False), (512, at + 2 * 2048 + 1008, 256, False)):
+        assert (L.mynah_b200_kv_attend(h, C.addressof(b), at, ld, out, ldo, None) == 0) == ok, (ld, out - at, ldo)
+        assert ok or b"overlaps" in L.mynah_b200_last_error()
+        assert (L.mynah_b200_kv_append(h, C.addressof(b), at, ld, far, 128, far, 128, out if out != far else far + 8192, ldo, None) == 0) == ok
+    for k, v, ok in ((at + 1024, at + 1536, True), (at + 1024, at + 1008, False), (at + 512, at + 1536, False), (at - 512, at + 1024, True), (at - 496, at + 1024, False)):
+        assert (L.mynah_b200_kv_append(h, C.addressof(b), at, 512, k, 512, v, 512, at, 512, None) == 0) == ok, (k - at, v - at)
     L.mynah_b200_kv_free(h)
 
 
