@@ -439,6 +439,10 @@ class KvCache:
         self.h = None
         c = KvConfig(n_heads, n_kv_heads, head_dim, page_size, n_pages, fmt, rotary_dim, int(interleaved), rope_theta, None, None, None,
                      norm_eps, window, n_sinks, scale)
+        for name, given in (("n_heads", n_heads), ("n_kv_heads", n_kv_heads), ("head_dim", head_dim), ("page_size", page_size), ("n_pages", n_pages),
+                            ("fmt", fmt), ("rotary_dim", rotary_dim), ("window", window), ("n_sinks", n_sinks)):
+            if getattr(c, name) != given:
+                raise ValueError(f"{name} does not fit 32 bits")
         keep = []
         for name, given, kind, n in (("inv_freq", inv_freq, np.float64, rotary_dim // 2), ("q_norm", q_norm, np.float32, head_dim),
                                      ("k_norm", k_norm, np.float32, head_dim)):

@@ -104,6 +104,15 @@ def test_groups_cover_what_is_seen(index):
     assert index.groups(top - 5, top, 64, 4, out, 4096) in (3, 4) and index.groups(0, top, 2 ** 26, 2 ** 26, out, 4096) == 2 ** 21
 
 
+def test_numbers_beyond_32_bits(pkg):
+    """What ctypes would cut to 32 bits is refused: 2^32 + 8 pages are not eight."""
+    good = dict(n_heads=4, n_kv_heads=2, head_dim=64, page_size=16, n_pages=8, window=64, n_sinks=1)
+    for name in good:
+        for more in (2 ** 32, -2 ** 32, 2 ** 40):
+            with pytest.raises(ValueError, match=name):
+                pkg.KvCache(**dict(good, **{name: good[name] + more}))
+
+
 def test_integration_example(tmp_path):
     """The layer shown to hosts is C that compiles against the header, and waits wherever rows pass from one stream to another."""
     with open(os.path.join(HERE, "..", "INTEGRATION.md")) as f:
