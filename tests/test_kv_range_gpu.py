@@ -431,3 +431,34 @@ def test_calls_without_a_stream_follow_the_tensors(gpu_pkg):
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "f16"])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("lens,rows", [([3000] * 4, None), ([3000] * 70, None), ([900, 2100], [40, 300]), ([1500] * 6, [1500] * 6)])
+def test_roundings_of_16_bit_rows(gpu_pkg, fmt, dim, lens, rows):
+    # Two roundings, of each probability and of the result, independent of one another: the mean square of what is off is that of
+    # h^2 / 3 (w . v)^2 over the keys and h^2 / 3 o^2, h half a step relative to the lower end of its binade, times 0.541 for numbers spread evenly over the
+    # logarithm of a binade ((1 - 1 / 4) / (2 ln 2)). Its root may be 10 % above that; one bit less in a probability makes it 58 % more.
+    lay = P.Layout(lens, 16, rows)
+    cache = gpu_pkg.KvCache(4, 2, dim, 16, lay.n_pages, fmt=number(gpu_pkg, fmt))
+    k, v = P.pools(cache, fmt)
+    k.copy_(randn(1, *k.shape))
+    v.copy_(randn(2, *v.shape))
+    q = randn(3, lay.n_rows, 4 * dim).to(P.ROWS[fmt])
+    out = torch.zeros_like(q)
+    cache.attend(lay.batch(cache), q, out, stream=here())
+    cache.sync(here())
+    off, square, count = 0.0, 0.0, 0
+    for s, (n, m) in enumerate(zip(lens, lay.rows)):
+        kk, vv = (P.keys_of(p, lay, s, list(range(n))).transpose(0, 1).repeat_interleave(2, 0) for p in (k, v))
+        rows_of = slice(lay.begin[s], lay.begin[s] + m)
+        score = q[rows_of].double().reshape(m, 4, dim).transpose(0, 1) @ kk.transpose(1, 2) / math.sqrt(dim)
+        score.masked_fill_(torch.arange(n, device="cuda") > torch.arange(n - m, n, device="cuda")[:, None], -math.inf)
+        w = torch.softmax(score, -1)
+        o = w @ vv
+        off += (out[rows_of].double().reshape(m, 4, dim).transpose(0, 1) - o).square().sum().item()
+        square += (w.square() @ vv.square() + o.square()).sum().item()
+        count += o.numel()
+    want = P.HALF_STEP[fmt] * math.sqrt(0.541 / 3 * square / count)
+    assert math.sqrt(off / count) <= 1.1 * want
