@@ -33,15 +33,24 @@ struct mynah_b200_kv {
 };
 
 namespace {
-// The handle's device is the current one while a call runs
+// The handle's device is the current one while a call runs, and its context the calling thread's: a thread that has made no CUDA call yet has a
+// device, but no context, which the encoding of tensor maps asks for.
 struct OnDevice {
+    static thread_local int bound;                             // the device that the thread has been set to
     int before = -1;
     explicit OnDevice(int dev) {
         if (cudaGetDevice(&before) != cudaSuccess) { cudaGetLastError(); before = -1; }
-        if (before != dev) cudaSetDevice(dev); else before = -1;
+        if (before != dev || bound != dev) cudaSetDevice(dev);
+        bound = dev;
+        if (before == dev) before = -1;
     }
-    ~OnDevice() { if (before >= 0) cudaSetDevice(before); }
+    ~OnDevice() {
+        if (before < 0) return;
+        cudaSetDevice(before);
+        bound = before;
+    }
 };
+thread_local int OnDevice::bound = -1;
 
 int row_bytes(int fmt) { return fmt == KV_F32 ? 4 : 2; }
 

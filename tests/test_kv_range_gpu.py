@@ -462,3 +462,29 @@ def test_roundings_of_16_bit_rows(gpu_pkg, fmt, dim, lens, rows):
         count += o.numel()
     want = P.HALF_STEP[fmt] * math.sqrt(0.541 / 3 * square / count)
     assert math.sqrt(off / count) <= 1.1 * want
+
+
+def test_first_call_of_a_thread(gpu_pkg):
+    """A thread that has not touched CUDA before."""
+    import threading
+    for fmt in FMTS:
+        for rows in (None, [30, 129, 300]):
+            lay = P.Layout([900, 2000, 333], 16, rows)
+            cache = gpu_pkg.KvCache(4, 2, 64, 16, lay.n_pages, fmt=number(gpu_pkg, fmt))
+            q = randn(3, lay.n_rows, 256).to(P.ROWS[fmt])
+            kr, turned, out, want, failed = q[:, :128], torch.zeros_like(q), torch.zeros_like(q), torch.zeros_like(q), []
+            batch, stream = lay.batch(cache), torch.cuda.Stream()
+            cache.append(batch, q, kr, kr, turned, stream=here())
+            cache.attend(batch, turned, want, stream=here())
+            cache.sync(here())
+            for call in (lambda: cache.attend(batch, turned, out, stream=stream.cuda_stream), lambda: cache.append(batch, q, kr, kr, turned, stream=stream.cuda_stream),
+                         lambda: cache.sync(stream.cuda_stream)):
+                def run():
+                    try:
+                        call()
+                    except Exception as e:
+                        failed.append(e)
+                thread = threading.Thread(target=run)
+                thread.start()
+                thread.join()
+            assert not failed and torch.equal(out, want)
