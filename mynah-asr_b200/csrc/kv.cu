@@ -292,6 +292,7 @@ int mynah_b200_kv_attend(mynah_b200_kv *h, const mynah_b200_kv_batch *b, const v
 int mynah_b200_kv_sync(mynah_b200_kv *h, void *stream) {
     if (!h) { set_error("kv_sync: null handle"); return -1; }
     OnDevice on(h->device);
+    RelaxedCapture relaxed;                                    // (waits and copies)
     const cudaStream_t st = stream ? (cudaStream_t)stream : h->stream;
     MB_CUDA(cudaStreamSynchronize(st));
     // Read and cleared in one step: calls on other streams may be reporting at the same time

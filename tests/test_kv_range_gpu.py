@@ -488,3 +488,34 @@ def test_first_call_of_a_thread(gpu_pkg):
                 thread.start()
                 thread.join()
             assert not failed and torch.equal(out, want)
+
+
+def test_calls_beside_another_threads_recording(gpu_pkg):
+    """While one thread records, another one calls and syncs on its own stream: neither disturbs the other."""
+    from concurrent.futures import ThreadPoolExecutor
+    for rows in (None, [30, 129, 300]):
+        lay = P.Layout([900, 2000, 333], 16, rows)
+        cache = gpu_pkg.KvCache(6, 3, 48, 16, lay.n_pages, fmt=gpu_pkg.F16)
+        k, v = P.pools(cache, "f16")
+        k.copy_(randn(1, *k.shape))
+        v.copy_(randn(2, *v.shape))
+        q = randn(3, lay.n_rows, 288).half()
+        batch, outs, side = lay.batch(cache), [torch.zeros_like(q) for _ in range(2)], torch.cuda.Stream()
+        torch.cuda.synchronize()
+
+        def other():
+            cache.attend(batch, q, outs[1], stream=side.cuda_stream)
+            cache.sync(side.cuda_stream)
+            return True
+
+        graph = torch.cuda.CUDAGraph()
+        with ThreadPoolExecutor(1) as pool:
+            with torch.cuda.graph(graph):
+                cache.attend(batch, q, outs[0], stream=here())
+                assert pool.submit(other).result()
+                cache.attend(batch, q, outs[0], stream=here())
+        graph.replay()
+        torch.cuda.synchronize()
+        want, bound = P.attend(lay, q, k, v, 3, fmt="f16")
+        for out in outs:
+            P.check(out, want, bound)
