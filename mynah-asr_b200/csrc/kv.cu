@@ -214,10 +214,12 @@ mynah_b200_kv *mynah_b200_kv_create(const mynah_b200_kv_config *cfg) {
         if (cfg->k_norm) h->k_norm = norms + 128;
         // every slot is finite from the start: what a mask hides is multiplied by a probability of 0
         ok = cudaMemsetAsync(h->block, 0, block, h->stream) == cudaSuccess && cudaMemsetAsync(h->k, 0, pool, h->stream) == cudaSuccess &&
-             cudaMemsetAsync(h->v, 0, pool, h->stream) == cudaSuccess && cudaStreamSynchronize(h->stream) == cudaSuccess &&
-             (!rot || cudaMemcpy(h->turns, turns, (size_t)(rot / 2) * sizeof(double), cudaMemcpyHostToDevice) == cudaSuccess) &&
-             (!cfg->q_norm || cudaMemcpy(h->q_norm, cfg->q_norm, (size_t)D * sizeof(float), cudaMemcpyHostToDevice) == cudaSuccess) &&
-             (!cfg->k_norm || cudaMemcpy(h->k_norm, cfg->k_norm, (size_t)D * sizeof(float), cudaMemcpyHostToDevice) == cudaSuccess);
+             cudaMemsetAsync(h->v, 0, pool, h->stream) == cudaSuccess;
+        // (not by the legacy default stream, which may not wait for a stream that another thread records)
+        auto put = [&](void *to, const void *from, size_t n) { return cudaMemcpyAsync(to, from, n, cudaMemcpyHostToDevice, h->stream) == cudaSuccess; };
+        ok = ok && (!rot || put(h->turns, turns, (size_t)(rot / 2) * sizeof(double))) && (!cfg->q_norm || put(h->q_norm, cfg->q_norm, (size_t)D * sizeof(float))) &&
+             (!cfg->k_norm || put(h->k_norm, cfg->k_norm, (size_t)D * sizeof(float)));
+        ok = cudaStreamSynchronize(h->stream) == cudaSuccess && ok;
     }
     if (!ok) {
         const cudaError_t e = cudaGetLastError();

@@ -7,7 +7,7 @@ import pytest
 
 torch = pytest.importorskip("torch")
 import kv_plain as P  # noqa: E402
-from test_kv_gpu import here, number, randn  # noqa: E402
+from test_kv_gpu import attend_case, here, number, randn  # noqa: E402
 
 pytestmark = pytest.mark.gpu
 
@@ -519,3 +519,39 @@ def test_calls_beside_another_threads_recording(gpu_pkg):
         want, bound = P.attend(lay, q, k, v, 3, fmt="f16")
         for out in outs:
             P.check(out, want, bound)
+
+
+@pytest.mark.parametrize("fmt,heads,kv_heads,dim", [("bf16", 4, 2, 64), ("f32", 2, 1, 128), ("f16", 8, 1, 128)])
+def test_few_rows_among_many_sequences(gpu_pkg, fmt, heads, kv_heads, dim):
+    """Nearly all sequences of a prompts' call bring no rows: clusters share the keys of those that do."""
+    n = 700
+    lens = [3000 if i in (0, 13, 350, 698, 699) else i % 5 for i in range(n)]
+    lay = P.Layout(lens, 16, [9 if m == 3000 else 0 for m in lens], extra_rows=3)
+    attend_case(gpu_pkg, lay, heads, kv_heads, dim, fmt)
+
+
+def test_a_cache_made_beside_a_recording(gpu_pkg):
+    """On a stream that waits for the legacy default stream, as cudaStreamCreate makes them."""
+    import ctypes
+    from concurrent.futures import ThreadPoolExecutor
+    runtime = ctypes.CDLL("libcudart.so.12")
+    raw = ctypes.c_void_p()
+    assert runtime.cudaStreamCreate(ctypes.byref(raw)) == 0
+    stream, x, graph = torch.cuda.ExternalStream(raw.value), torch.ones(1000, device="cuda"), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+
+    def make():
+        cache = gpu_pkg.KvCache(2, 2, 16, 16, 8, fmt=gpu_pkg.F16, rotary_dim=16, q_norm=np.ones(16), k_norm=np.ones(16))
+        return cache.close() is None
+
+    with ThreadPoolExecutor(1) as pool:
+        with torch.cuda.graph(graph, stream=stream):
+            x.add_(1)
+            assert pool.submit(make).result()
+            x.add_(1)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert (x == 3).all()
+    del graph
+    torch.cuda.synchronize()
+    assert runtime.cudaStreamDestroy(raw) == 0
