@@ -66,11 +66,15 @@ __device__ __forceinline__ float kv_ex2(float x) {
     return y;
 }
 // A running maximum is that of the scores as the products leave them, -infinity before the first key, and an exponent is (x - m) scale2: the
-// difference of neighbours is exact, where the fused x scale2 - m scale2 has lost its digits for scores of 2^24 and more (16384 bf16 rows:
-// 1 % more time). What was summed under the maximum m counts 2^((m - top) scale2) under a larger one.
+// difference of neighbours is exact, where x scale2 - m scale2 has lost its digits for scores of 2^24 and more. What was summed under the
+// maximum m counts 2^((m - top) scale2) under a larger one.
 __device__ __forceinline__ float kv_weight(float m, float top, float scale2) { return m == top ? 1.f : kv_ex2((m - top) * scale2); }
 // The sum of a row's probabilities, of which the largest is not small: where it is nothing or no number, the scores were not finite
 __device__ __forceinline__ bool kv_sound(float l) { return l > 0.f && l < INFINITY; }
+// Near 0, x scale2 + kv_base(m) is the same in one operation, to 2^-14 of a probability: less than the rounding of 16-bit rows (16384 bf16 rows 2012
+// us, with the difference for all 2044)
+__device__ __forceinline__ float kv_base(float m, float scale2, float up) { return m == -INFINITY ? up : fmaf(-m, scale2, up); }
+__device__ __forceinline__ bool kv_far(float base) { return !(fabsf(base) < 1024.f); }
 template <bool BF>
 __device__ __forceinline__ uint32_t kv_pack(float x, float y) {
     if (BF) { const __nv_bfloat162 h = __floats2bfloat162_rn(x, y); return *reinterpret_cast<const uint32_t *>(&h); }
@@ -80,13 +84,10 @@ __device__ __forceinline__ uint32_t kv_pack(float x, float y) {
 // Two results. They are averages, so what rounding has brought beyond the type's largest number is that number (a NaN stays one)
 template <bool BF>
 __device__ __forceinline__ uint32_t kv_pack_result(float x, float y) {
-    constexpr float TOP = BF ? 0x1.fep127f : 65504.f;
-    auto within = [&](float v) {
-        float r;
-        asm("{\n\t.reg .f32 t;\n\tmin.NaN.f32 t, %1, %2;\n\tmax.NaN.f32 %0, t, %3;\n\t}" : "=f"(r) : "f"(v), "f"(TOP), "f"(-TOP));
-        return r;
-    };
-    return kv_pack<BF>(within(x), within(y));
+    uint32_t r;
+    if (BF) asm("cvt.rn.satfinite.bf16x2.f32 %0, %2, %1;" : "=r"(r) : "f"(x), "f"(y));
+    else asm("cvt.rn.satfinite.f16x2.f32 %0, %2, %1;" : "=r"(r) : "f"(x), "f"(y));
+    return r;
 }
 // x, y as f16 pairs: hi and what it leaves. The rest stays unscaled (it may be subnormal): both products go into one accumulator.
 __device__ __forceinline__ void kv_split(float x, float y, uint32_t &hi, uint32_t &lo) {
@@ -97,6 +98,7 @@ __device__ __forceinline__ void kv_split(float x, float y, uint32_t &hi, uint32_
     lo = *reinterpret_cast<const uint32_t *>(&l);
 }
 // two f32 operations in one instruction
+__device__ __forceinline__ float2 kv_twice(float x) { return make_float2(x, x); }
 __device__ __forceinline__ float2 kv_fma2(float2 a, float2 b, float2 c) {
     float2 d;
     asm("{\n\t.reg .b64 ra, rb, rc, rd;\n\tmov.b64 ra, {%2, %3};\n\tmov.b64 rb, {%4, %5};\n\tmov.b64 rc, {%6, %7};\n\t"

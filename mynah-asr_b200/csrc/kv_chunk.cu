@@ -610,6 +610,8 @@ kv_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
             if (lane == 0) mbar_arrive(q_full);
         }
         m = -INFINITY; l = 0.f;
+        float base = ChunkTop<FMT>::TOP;                       // 16-bit rows: that of m; and whether one of the warp's is far
+        bool far = false;
         if (t < b.nt) {
             // rows that do not exist take the last one's position, so that they need no mask of their own
             const int pos = b.base_pos + min(r < tq * a.G ? tok : b.t0 + t * tq, b.rows - 1);
@@ -692,6 +694,10 @@ kv_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                     const float alpha = grow ? kv_ex2((m - mt) * sc) : 1.f;
                     if (grow) m = mt;
                     l *= alpha;
+                    if (!F32) {
+                        base = kv_base(m, sc, ChunkTop<FMT>::TOP);
+                        far = __any_sync(0xffffffffu, kv_far(base));
+                    }
                     if (Sh::FRESH && OWN_P && i > 0) {
                         gather(i, alpha);
                     } else if (i > 0) {
@@ -707,15 +713,24 @@ kv_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                         }
                     }
                 }
-                const float2 sc2 = make_float2(sc, sc), top2 = make_float2(ChunkTop<FMT>::TOP, ChunkTop<FMT>::TOP);
                 const float off = m == -INFINITY ? 0.f : -m;       // (no key yet: all are hidden)
-                const float2 off2 = make_float2(off, off);
+                const float2 sc2 = kv_twice(sc), off2 = kv_twice(off);
+                float2 top2 = kv_twice(F32 ? ChunkTop<FMT>::TOP : base);
+                if (__builtin_expect(!F32 && far, 0)) {
+                    const float2 o = kv_twice(kv_far(base) ? off : 0.f);
+#pragma unroll
+                    for (int c = 0; c < OWN; c += 2) {
+                        const float2 y = kv_add2(make_float2(x[c], x[c + 1]), o);
+                        x[c] = y.x; x[c + 1] = y.y;
+                    }
+                    if (kv_far(base)) top2 = kv_twice(ChunkTop<FMT>::TOP);
+                }
                 float2 l2[2] = {{0.f, 0.f}, {0.f, 0.f}};           // the tile's sum: small terms are not lost one by one in a large l
                 auto open = [&](int c) {                           // the exponentials of 16 keys, in place
 #pragma unroll
                     for (int e = 0; e < 8; e++) {
                         float *v = x + c * 16 + 2 * e;
-                        const float2 y = kv_fma2(kv_add2(make_float2(v[0], v[1]), off2), sc2, top2);
+                        const float2 y = kv_fma2(F32 ? kv_add2(make_float2(v[0], v[1]), off2) : make_float2(v[0], v[1]), sc2, top2);
                         v[0] = kv_ex2(y.x); v[1] = kv_ex2(y.y);
                     }
                 };
@@ -769,8 +784,10 @@ kv_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
             const volatile int *w = items + (j & 1) * KcBlock::WORDS;
             if (w[8] == 1 && rank == 0 && ok) {
                 const float inv = l != 0.f ? 1.f / l : 0.f;
-                const int mine = w[4] + t * tq + by_g(r);      // the thread's row in its sequence
-                if (r < tq * a.G && mine < w[3] && w[5] + mine >= 0 && !kv_sound(l)) kv_report(a, ST_RANGE);
+                if (!kv_sound(l)) {
+                    const int mine = w[4] + t * tq + by_g(r);  // the thread's row in its sequence
+                    if (r < tq * a.G && mine < w[3] && w[5] + mine >= 0) kv_report(a, ST_RANGE);
+                }
                 // after the turn a lane stores a quarter of 16 words of each of the four rows of its lanes: where they lie, -1 for rows that are not
                 const int begin = w[2], last = w[3] - w[4] - t * tq, kvh = w[1];       // (rows of the tile: below last)
                 const int64_t first = (int64_t)(begin + w[4] + t * tq) * a.ldo + (int64_t)kvh * a.G * a.D;
@@ -849,7 +866,7 @@ kv_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
                     total = fmaf(e[p].x, e[p].y, total);
                 }
                 const float inv = total != 0.f ? 1.f / total : 0.f;
-                if (b.base_pos + b.t0 + by_g(v0 + v) >= 0 && !kv_sound(total)) kv_report(a, ST_RANGE);
+                if (!kv_sound(total) && b.base_pos + b.t0 + by_g(v0 + v) >= 0) kv_report(a, ST_RANGE);
 #pragma unroll
                 for (int p = 0; p < 16; p++)
                     if (p < b.shares) weight[v * 16 + p] = e[p].x * inv;

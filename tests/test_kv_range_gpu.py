@@ -61,7 +61,7 @@ def test_small_probabilities(gpu_pkg, fmt, dim, rows):
                     P.check(out[at:at + m], want, bound + P.HALF_STEP[fmt] * (want.abs() + bound) + 2.0 ** -25 * (fmt == "f16"))
 
 
-def settled(pkg, lay, fmt, heads, dim, scale, q, k_of, seed=5):
+def settled(pkg, lay, fmt, heads, dim, scale, q, k_of, seed=5, more=0.0):
     """Results of all rows, and softmax of the exact scores times the values: k_of(position) gives the first two values of a key, the others are 0."""
     cache = pkg.KvCache(heads, heads, dim, lay.page, lay.n_pages, fmt=number(pkg, fmt), scale=scale)
     k, v = P.pools(cache, fmt)
@@ -85,7 +85,7 @@ def settled(pkg, lay, fmt, heads, dim, scale, q, k_of, seed=5):
         w = torch.softmax(score, -1)
         want = w @ vv
         # weights as in test_small_probabilities, of distances up to 6 units (others are exact or nothing); values all near 1
-        rel = P.PAIR[fmt] + 2.0 ** -22 * 7 + (1e-6 if fmt == "f32" else 2e-8 * (n / 16 + 4))
+        rel = P.PAIR[fmt] + 2.0 ** -22 * 7 + (1e-6 if fmt == "f32" else 2e-8 * (n / 16 + 4) + more)
         bound = rel * (w @ vv.abs()) + 2.0 ** -32 * n
         P.check(out[lay.begin[s]:lay.begin[s] + m].double().reshape(m, heads, dim)[:, 0], want, bound + P.HALF_STEP[fmt] * (want.abs() + bound))
 
@@ -106,6 +106,8 @@ def test_scores_far_from_zero(gpu_pkg, fmt, dim, lens, rows):
         # small steps on a large common part: 2^22 + {0, 0.5, ... 5}, exact in f32
         settled(gpu_pkg, lay, fmt, heads, dim, 2.0 ** -7, (32768.0, 64.0), lambda at: (flat(at) + sign * 16384, at * 5 % 11))
         settled(gpu_pkg, lay, fmt, heads, dim, 2.0 ** -7, (512.0, 64.0), lambda at: (flat(at) + sign * 1024, at * 5 % 11))
+        # rising slowly past the scores from where on 16-bit rows take differences (2^10 to powers of two): an exponent there is off by 2^-14
+        settled(gpu_pkg, lay, fmt, heads, dim, 1 / 8, (8.0, 64.0), lambda at: (at // 64, flat(at) + (87.5 if sign > 0 else -90)), more=2.0 ** -14)
         # rising by more than any distance that a probability survives
         settled(gpu_pkg, lay, fmt, heads, dim, scale, (top / 64, 0.0), lambda at: (sign * ((at // 64) * 64 - 8192), flat(at)))
 
@@ -168,6 +170,7 @@ def test_scores_that_are_no_numbers_are_reported(gpu_pkg, fmt, heads, kv_heads, 
         others = [i for i in range(lay.real) if not lay.begin[1] <= i < lay.begin[1] + lay.rows[1]]
         assert torch.equal(out[others], plain[others]) and (out[lay.real:] == 0).all()
         if key is None:
+            assert out[at, (heads - 1) * dim:].isnan().all()
             assert torch.equal(out[at, :(heads - 1) * dim], plain[at, :(heads - 1) * dim])
         k.copy_(kept)
     if fmt == "bf16":                                     # one key at minus infinity among others is none
