@@ -321,8 +321,8 @@ int mynah_b200_stream_step_device(mynah_b200_stream_group *g, const float *mel_d
  *
  * Types: fmt is that of the rows (queries, keys, values, results): F32, F16 or BF16. The cache holds 16 bits a value:
  * bf16 for BF16 rows, else f16. Queries, probabilities and results of F16 / BF16 rows pass through 16 bits, too; for
- * F32 rows they keep f32 accuracy (relative to the stored keys and values). A probability is held to 2^-22 of itself (F16 rows 2^-11)
- * or to 2^-39 (F16 rows 2^-32) of the row's largest, whichever is more.
+ * F32 rows they keep f32 accuracy (relative to the stored keys and values). A probability is held to 2^-22 of itself (F16
+ * rows 2^-11, BF16 rows 2^-8) or to 2^-39 (F16 rows 2^-32) of the row's largest, whichever is more.
  * Layout: the pools are [n_pages][n_kv_heads][page_size][head_dim]; head h of a row is its values
  * [h head_dim, (h + 1) head_dim); query head h looks at kv head h / (n_heads / n_kv_heads). */
 typedef struct {
@@ -369,25 +369,26 @@ typedef struct {
  * allocate nothing, use no workspace and can be captured; calls of one handle may overlap on the GPU as long as none
  * writes a slot that another reads or writes. 0, or -1 with mynah_b200_last_error and nothing launched. What only the
  * tables show (a page or length out of range: skipped, or read as page 0), values that do not fit the cache's 16 bits
- * (not finite, beyond 65504 in F16 rows, from 65504 on in F32 rows: stored as 0; a head whose norm is out of range counts as not finite) and rows whose scores are not finite (all of them minus infinity: the
- * result is 0; one NaN or plus infinity: it is NaN) are reported by mynah_b200_kv_sync.
+ * (not finite, beyond 65504 in F16 rows, from 65504 on in F32 rows: stored as 0; a head whose norm is out of range counts
+ * as not finite) and rows whose scores are not finite (all of them minus infinity: the result is 0; one NaN or plus
+ * infinity: it is NaN) are reported by mynah_b200_kv_sync.
  *
- * append: norm and rotation of q into q_out (which may be q itself with the same stride, and shares no values with k or v), of k into the cache, v into the
- * cache as it is. Rows whose position is below 0 (more rows than keys) are skipped. A slot that two rows of a call name
+ * append: norm and rotation of q into q_out (which may be q itself with the same stride, and shares no values with k or
+ * v), of k into the cache, v into the cache as it is. Rows whose position is below 0 (more rows than keys) are skipped. A slot that two rows of a call name
  * ends up with a mix of the two. */
 int mynah_b200_kv_append(mynah_b200_kv *h, const mynah_b200_kv_batch *b, const void *q, long long ldq, const void *k, long long ldk,
                          const void *v, long long ldv, void *q_out, long long ldqo, void *stream);
 /* attend: out = softmax over the visible keys of scale q . k, times their values; 0 for a row that sees none. q as
- * append left it in q_out; out may be q itself with the same stride, and shares no values with it otherwise. How the keys of a sequence are cut into parts that
- * are summed and joined depends on n_seq, n_rows and max_pages and on the sequence itself, never on the others, and no
- * sum on what ran first: the same call gives the same bits. F32 rows: queries are kept to 2^-25 absolutely or 2^-22
- * relatively, whichever is more, and lie below 65504; scores are sums that the
- * tensor cores cut toward zero (1e-9 head_dim of themselves on average, measured with head_dim 64 and 128). F16 / BF16 rows: values are summed by the tensor cores, which
+ * append left it in q_out; out may be q itself with the same stride, and shares no values with it otherwise. How the keys
+ * of a sequence are cut into parts that are summed and joined depends on n_seq, n_rows and max_pages and on the sequence
+ * itself, never on the others, and no sum on what ran first: the same call gives the same bits. F32 rows: queries are kept to 2^-25 absolutely or 2^-22
+ * relatively, whichever is more, and lie below 65504; scores are sums that the tensor cores cut toward zero (1e-9 head_dim of
+ * themselves on average, measured with head_dim 64 and 128). F16 / BF16 rows: values are summed by the tensor cores, which
  * cut each sum toward zero; that adds up to 2e-8 of a result per 16 keys (2e-5 over 16000). */
 int mynah_b200_kv_attend(mynah_b200_kv *h, const mynah_b200_kv_batch *b, const void *q, long long ldq, void *out, long long ldo,
                          void *stream);
-/* waits for `stream` (NULL: the handle's own) and reports, once, what the handle's calls have found since the last sync:
- * 0, or -1. Not to be called while the stream is being captured. */
+/* waits for `stream` (NULL: the handle's own) and reports, once, all that the handle's calls have found since the last sync:
+ * 0, or -1. Threads may call it at the same time; it leaves recordings of other threads alone. Not to be called while the stream is being captured. */
 int mynah_b200_kv_sync(mynah_b200_kv *h, void *stream);
 
 /* ---- whole path, resident ------------------------------------------------------- */

@@ -10,8 +10,8 @@
 // registers, and has 2 KB of reads in flight. Sums of squares, norms and rotation are in f32; the angle is formed as turns in
 // f64 and reduced there (a position of 10^6 times a frequency near 1 has no correct digit behind the point in f32), its sine and
 // cosine then in f32.
-// Measured (norm and rotation, 32 query and 8 kv heads of 128, bf16): 32768 rows 164 us = 4.9 TB/s, issue slots 62 % and ALU 55 % taken;
-// 120 rows 4.9 us, one 2.8; 23 sequences of f32 rows, 8 heads of 64, half of each turned, 14.0 us = 3.5 TB/s. With pairs exchanged between
+// Measured (norm and rotation, 32 query and 8 kv heads of 128, bf16): 32768 rows 165 us = 4.9 TB/s, issue slots 62 % and ALU 55 % taken (the
+// 64 registers that 32 warps leave spill 36 bytes); 120 rows 4.9 us, one 2.8; 23 sequences of f32 rows, 8 heads of 64, half of each turned, 14.1 us = 3.5 TB/s. With pairs exchanged between
 // lanes instead, and all kinds of heads in one loop, the first took 441 us.
 #include "kv.h"
 

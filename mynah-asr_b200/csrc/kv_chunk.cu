@@ -20,9 +20,9 @@
 // A call with few blocks is launched as clusters: the CTAs of a cluster take a block's tiles in turn, two at least each, and join their
 // results through distributed shared memory.
 //
-// Measured (us): 16384 rows of 32 query and 8 kv heads of 128, bf16, 2000 = 1.1 PFLOP/s under the power cap (1.72 GHz; a library's
-// product of matrices holds 1.42 there); 4 pieces of 5 to 61 rows behind 300 to 1500 keys 13.6; 7 prompts of 301 to 4000 rows, 16 and 4
-// heads of 64, f16, window 512, 57.4; 9 of 40 to 1300 F32 rows, 8 heads of 128, 36.9. A tile of D = 128 goes through 1190 clocks of
+// Measured (us): 16384 rows of 32 query and 8 kv heads of 128, bf16, 2045 = 1.1 PFLOP/s under the power cap (1.72 GHz; a library's
+// product of matrices holds 1.42 there); 4 pieces of 5 to 61 rows behind 300 to 1500 keys 14.0; 7 prompts of 301 to 4000 rows, 16 and 4
+// heads of 64, f16, window 512, 59.7; 9 of 40 to 1300 F32 rows, 8 heads of 128, 37.4. A tile of D = 128 goes through 1190 clocks of
 // waiting for its scores, 245 + 220 of their maximum, 1550 of exponentials and packing, 250 of signals; the other tile's take turns with
 // it. Tensor cores and exponential units are busy half of the time each. What was tried against that: steps of 64 keys with two score
 // buffers, so that no softmax waits (2210: products 64 columns wide take as long as 128 wide ones), a part of the exponentials as
@@ -37,8 +37,8 @@ static constexpr int KC_PART = 3;                    // P V begins when the firs
 
 // The maximum of a row may lag by 2^LAG, and a probability is 2^TOP of it, which the final division takes out again: together below f16's 2^16,
 // and what is held of a probability (with F32 rows: of its rest) is 2^-25 / 2^TOP of the largest, where it was 2^-25 without. bf16 has the
-// range, but its values end where f32 does: 2^26 of them, the most that a sequence has, do not add up to infinity. A smaller LAG rescales O more often: f16, 8192 rows of 32 heads of 128, scores spread by 2.5 units: 481 us, with a LAG of 4 518,
-// of 2 540. F32 rows of 128 rescale for every tile in any case; 8 heads of 64 take 41.8 us, with a LAG of 8 40.3.
+// range, but its values end where f32 does: 2^26 of them, the most that a sequence has, do not add up to infinity. A smaller LAG rescales O more
+// often: f16, 8192 rows of 32 heads of 128, scores spread by 2.5 units: 481 us, with a LAG of 4 518, of 2 540. F32 rows of 128 rescale for every tile in any case; 8 heads of 64 take 41.8 us, with a LAG of 8 40.3.
 template <int FMT> struct ChunkTop {
     static constexpr float LAG = FMT == KV_F32 ? 1.f : 8.f, TOP = FMT == KV_F32 ? 14.f : FMT == KV_F16 ? 7.f : -35.f;
 };

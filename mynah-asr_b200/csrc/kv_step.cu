@@ -12,7 +12,7 @@
 // pace hides. The partial results are joined in shared memory, then in the cluster's distributed shared memory, in a fixed order,
 // each CTA for its slice of the values: no workspace, no second launch, no atomics.
 // Measured (32 query and 8 kv heads of 128, bf16): 131071 keys 99 us = 5.4 TB/s (128 CTAs of 148 SMs: a cluster has at most 16), 60
-// ragged sequences of 40 to 9000 keys 76 us = 5.9 TB/s, 700 keys (16 query heads) 6.2 us; 200 sequences of F32 rows, 8 heads of 64, window 1000, 64 us = 5.6 TB/s
+// ragged sequences of 40 to 9000 keys 76 us = 5.9 TB/s, 700 keys (16 query heads) 6.4 us; 200 sequences of F32 rows, 8 heads of 64, window 1000, 65 us = 5.6 TB/s
 // (61 without any arithmetic, as are 98 of the 99: what is left is the pace of the copies). A warp that asks for its own tiles took
 // 128 us for the first (each TMA instruction of a diverged lane waits for its operands, in front of the products), query heads as the
 // 16 rows of the products 192 us.
