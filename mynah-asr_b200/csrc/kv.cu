@@ -130,7 +130,7 @@ const char *refuse_rows(const mynah_b200_kv *h, const void *p, long long ld, int
 // Whether rows that are written share values with rows that are read, other than by being the same ones: one row's result would be read as
 // another's input. `n` rows of `width` values, `size` bytes each.
 bool clash(const void *out, long long ldo, int wo, const void *in, long long ldi, int wi, int n, int size) {
-    if (out == in && ldo == ldi) return false;
+    if (out == in && (ldo == ldi || n == 1)) return false;
     const uintptr_t o = (uintptr_t)out, i = (uintptr_t)in;
     if (o + ((uintptr_t)(n - 1) * ldo + wo) * size <= i || i + ((uintptr_t)(n - 1) * ldi + wi) * size <= o) return false;
     if (ldo != ldi) return true;

@@ -322,6 +322,9 @@ def kv_overlaps(pkg, fake):
         assert (L.mynah_b200_kv_attend(h, C.addressof(b), at, ld, out, ldo, None) == 0) == ok, (ld, out - at, ldo)
         assert ok or b"overlaps" in L.mynah_b200_last_error()
         assert (L.mynah_b200_kv_append(h, C.addressof(b), at, ld, far, 128, far, 128, out if out != far else far + 8192, ldo, None) == 0) == ok
+    one = _batch(pkg, n_seq=1, n_rows=1, kv_len=lens, page_table=table)
+    for out, ldo, ok in ((at, 256, True), (at, 512, True), (at + 1024, 256, True), (at + 1008, 512, False), (at - 1008, 256, False)):
+        assert (L.mynah_b200_kv_attend(h, C.addressof(one), at, 260, out, ldo, None) == 0) == ok, (out - at, ldo)
     for k, v, ok in ((at + 1024, at + 1536, True), (at + 1024, at + 1008, False), (at + 512, at + 1536, False), (at - 512, at + 1024, True), (at - 496, at + 1024, False)):
         assert (L.mynah_b200_kv_append(h, C.addressof(b), at, 512, k, 512, v, 512, at, 512, None) == 0) == ok, (k - at, v - at)
     L.mynah_b200_kv_free(h)
