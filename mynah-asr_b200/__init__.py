@@ -460,7 +460,9 @@ class KvCache:
         self._dtype = {F32: "torch.float32", F16: "torch.float16", BF16: "torch.bfloat16"}[fmt]
         self._q_width, self._kv_width = n_heads * head_dim, n_kv_heads * head_dim
         torch = sys.modules.get("torch")
-        self._current = None if torch is None else (lambda device=torch.cuda.current_device(): torch.cuda.current_stream(device).cuda_stream)
+        self._current = None
+        if torch is not None and torch.cuda.is_available():
+            self._current = lambda device=torch.cuda.current_device(): torch.cuda.current_stream(device).cuda_stream
         self._append, self._attend = lib().mynah_b200_kv_append, lib().mynah_b200_kv_attend
 
     def close(self):

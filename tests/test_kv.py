@@ -154,7 +154,7 @@ def test_kv_host(fake_runtime, name):  # noqa: F811
     assert r.returncode == 0, r.stdout + r.stderr
 
 
-@pytest.mark.parametrize("name", ["kv_limits", "kv_overlaps"])
+@pytest.mark.parametrize("name", ["kv_limits", "kv_overlaps", "kv_beside_a_torch_without_cuda"])
 def test_kv_host_limits(fake_runtime, name):  # noqa: F811
     test_kv_host(fake_runtime, name)
 
@@ -328,6 +328,25 @@ def kv_overlaps(pkg, fake):
     for k, v, ok in ((at + 1024, at + 1536, True), (at + 1024, at + 1008, False), (at + 512, at + 1536, False), (at - 512, at + 1024, True), (at - 496, at + 1024, False)):
         assert (L.mynah_b200_kv_append(h, C.addressof(b), at, 512, k, 512, v, 512, at, 512, None) == 0) == ok, (k - at, v - at)
     L.mynah_b200_kv_free(h)
+
+
+@scenario
+def kv_beside_a_torch_without_cuda(pkg, fake):
+    """A process may have a torch that knows no CUDA, or none: the tensors are another library's, the stream is the handle's own."""
+    import types
+
+    def no_cuda():
+        raise AssertionError("Torch not compiled with CUDA enabled")
+
+    stub = types.SimpleNamespace(cuda=types.SimpleNamespace(is_available=lambda: False, current_device=no_cuda, current_stream=no_cuda))
+    for torch in (stub, None):
+        if torch is None:
+            sys.modules.pop("torch", None)
+        else:
+            sys.modules["torch"] = torch
+        cache = pkg.KvCache(4, 2, 64, 16, 8, fmt=pkg.F32)
+        cache.sync()
+        cache.close()
 
 
 if __name__ == "__main__":
