@@ -466,6 +466,7 @@ class KvCache:
         self._append, self._attend = lib().mynah_b200_kv_append, lib().mynah_b200_kv_attend
 
     def close(self):
+        """Waits for the cache's work and frees it. What was made of pages(), and graphs that hold its calls, are not to be used afterwards."""
         if getattr(self, "h", None):
             lib().mynah_b200_kv_free(self.h)
             self.h = None
