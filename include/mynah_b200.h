@@ -381,10 +381,11 @@ int mynah_b200_kv_append(mynah_b200_kv *h, const mynah_b200_kv_batch *b, const v
 /* attend: out = softmax over the visible keys of scale q . k, times their values; 0 for a row that sees none. q as
  * append left it in q_out; out may be q itself with the same stride, and shares no values with it otherwise. How the keys
  * of a sequence are cut into parts that are summed and joined depends on n_seq, n_rows and max_pages and on the sequence
- * itself, never on the others, and no sum on what ran first: the same call gives the same bits. F32 rows: queries are kept to 2^-25 absolutely or 2^-22
- * relatively, whichever is more, and lie below 65504; scores are sums that the tensor cores cut toward zero (1e-9 head_dim of
- * themselves on average, measured with head_dim 64 and 128). F16 / BF16 rows: values are summed by the tensor cores, which
- * cut each sum toward zero; that adds up to 2e-8 of a result per 16 keys (2e-5 over 16000). */
+ * itself, never on the others, and no sum on what ran first: the same call gives the same bits. F32 rows: queries are kept
+ * to 2^-25 absolutely or 2^-22 relatively, whichever is more, and lie below 65504; scores are sums that the tensor cores cut
+ * toward zero (1e-9 head_dim of themselves on average, measured with head_dim 64 and 128). F16 / BF16 rows: values are summed by the tensor cores, which
+ * cut each sum toward zero; that adds up to 2e-8 of a result per 16 keys (2e-5 over 16000). BF16 rows: sums have room for
+ * 2^26 of the largest values, for which values below 1e-30 lose digits. */
 int mynah_b200_kv_attend(mynah_b200_kv *h, const mynah_b200_kv_batch *b, const void *q, long long ldq, void *out, long long ldo,
                          void *stream);
 /* waits for `stream` (NULL: the handle's own) and reports, once, all that the handle's calls have found since the last sync:

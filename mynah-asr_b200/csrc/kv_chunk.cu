@@ -38,7 +38,8 @@ static constexpr int KC_PART = 3;                    // P V begins when the firs
 // The maximum of a row may lag by 2^LAG, and a probability is 2^TOP of it, which the final division takes out again: together below f16's 2^16,
 // and what is held of a probability (with F32 rows: of its rest) is 2^-25 / 2^TOP of the largest, where it was 2^-25 without. bf16 has the
 // range, but its values end where f32 does: 2^26 of them, the most that a sequence has, do not add up to infinity. A smaller LAG rescales O more
-// often: f16, 8192 rows of 32 heads of 128, scores spread by 2.5 units: 481 us, with a LAG of 4 518, of 2 540. F32 rows of 128 rescale for every tile in any case; 8 heads of 64 take 41.8 us, with a LAG of 8 40.3.
+// often: f16, 8192 rows of 32 heads of 128, scores spread by 2.5 units: 481 us, with a LAG of 4 518, of 2 540. F32 rows of
+// 128 rescale for every tile in any case; 8 heads of 64 take 41.8 us, with a LAG of 8 40.3.
 template <int FMT> struct ChunkTop {
     static constexpr float LAG = FMT == KV_F32 ? 1.f : 8.f, TOP = FMT == KV_F32 ? 14.f : FMT == KV_F16 ? 7.f : -35.f;
 };

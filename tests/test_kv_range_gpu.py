@@ -558,3 +558,21 @@ def test_a_cache_made_beside_a_recording(gpu_pkg):
     del graph
     torch.cuda.synchronize()
     assert runtime.cudaStreamDestroy(raw) == 0
+
+
+@pytest.mark.parametrize("rows", [None, [200]])
+def test_small_bf16_values(gpu_pkg, rows):
+    """Values down to 1e-30 come out as exactly as others."""
+    lay = P.Layout([700], 16, rows)
+    for dim in (64, 128):
+        cache = gpu_pkg.KvCache(4, 2, dim, 16, lay.n_pages, fmt=gpu_pkg.BF16)
+        k, v = P.pools(cache, "bf16")
+        k.copy_(randn(1, *k.shape))
+        q = randn(3, lay.n_rows, 4 * dim).bfloat16()
+        out = torch.zeros_like(q)
+        for size in (1.0, 1e-20, 1e-28, 1e-30):
+            v.copy_((1 + 0.1 * randn(5, *v.shape)) * size)
+            cache.attend(lay.batch(cache), q, out, stream=here())
+            cache.sync(here())
+            want, bound = P.attend(lay, q, k, v, 2, fmt="bf16")
+            P.check(out, want, bound)
